@@ -223,8 +223,8 @@ def prepare(case, seed):
     s = dict(case, x=_activation(gen, t, k, case["dtype"]))
     w = torch.randn(experts, n, k, generator=gen, device=DEV) * 0.02
     s["codes"], s["scales"] = _pack(*_quant(w), k)
-    order, _, s["offsets"] = _sorted(ids, experts)
-    s["rows"] = torch.div(order, top, rounding_mode="floor").int()
+    s["order"], s["position"], s["offsets"] = _sorted(ids, experts)
+    s["rows"] = torch.div(s["order"], top, rounding_mode="floor").int()
     # the plain form's padded batch: the most rows of one expert
     s["most"] = max(1, int((s["offsets"][1:] - s["offsets"][:-1]).max()))
     if case["grad"]:
@@ -292,8 +292,7 @@ def _plain_experts(s):
     out = {"y": product(xs, w.transpose(1, 2)).to(dtype)}
     if s["grad"]:
         dxs = product(s["dy"].float(), w)
-        dx = torch.zeros(x.shape, device=x.device).index_add_(0, rows, dxs)
-        out["dx"] = dx.to(dtype)
+        out["dx"] = dxs[s["position"].long()].sum(1).to(dtype)     # (0 where not live)
     return out
 
 
@@ -320,7 +319,8 @@ def _own_route(s):
 
 
 def _own_experts(s):
-    y = _mxfp4().grouped_linear(s["x"], s["codes"], s["scales"], s["offsets"], rows=s["rows"])
+    routing = _moe().Routing(s["order"], s["position"], s["rows"], s["offsets"])
+    y = _mxfp4().grouped_linear(s["x"], s["codes"], s["scales"], routing, gather=True)
     if not s["grad"]:
         return {"y": y}
     dx, = torch.autograd.grad(y, (s["x"],), s["dy"])
