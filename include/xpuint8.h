@@ -526,6 +526,99 @@ int xpuint8_rms_rope_dequant_stream(const void *stream, const int32_t *acc, int6
  * activations apply, for verification. */
 int xpuint8_activation_table(int32_t id, uint16_t *out);
 
+/* ---- MXFP4 --------------------------------------------------------------
+ * Microscaled 4-bit floating point: 32 consecutive values of a row share a
+ * power of two, each one of {0, .5, 1, 1.5, 2, 3, 4, 6} with a sign.  A tensor
+ * [.., K] (K % 32 == 0) is
+ *   codes  [.., K/2]: element 2i in the low half of byte i (code c & 7 counts the
+ *          values above, c & 8 is the sign), and
+ *   scales [.., W], W = xpuint8_mxfp4_scale_width(K) = 16 ceil(K/512): the
+ *          exponent of block k biased by 127 at byte k, 255 for a NaN block; the
+ *          bytes past K/32 are written as 127 and never used.
+ * Quantization of a block: with amax its largest magnitude,
+ *   e = clamp(floor(log2 amax) - 2, -127, 127)  (-127 for amax 0),
+ * each value x / 2^e rounded to nearest even on the grid and saturated at 6; a
+ * block with an infinity or NaN becomes a NaN block.
+ * Element types: 0 bf16, 1 fp16, 2 fp32.  x may have any row stride (elements) and
+ * the alignment of its elements; codes, scales, outputs and work are contiguous and
+ * 16-byte aligned.  No counterpart in the reference. */
+
+/* bytes of a row of scales; -1 for a K that is not a positive multiple of 32 */
+int64_t xpuint8_mxfp4_scale_width(int64_t K);
+
+/* x [M, K] to codes and scales, and what they stand for to out [M, K] (values
+ * beyond fp16's range become infinities) */
+int xpuint8_mxfp4_quantize_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
+                                  uint8_t *codes, uint8_t *scales, int64_t M, int64_t K);
+int xpuint8_mxfp4_dequantize_stream(const void *stream, const uint8_t *codes,
+                                    const uint8_t *scales, void *out, int32_t type, int64_t M,
+                                    int64_t K);
+
+/* y [M, N] = xq wq^T (+ bias [N]): x [M, K] quantized in the call, the weight codes
+ * [N, K/2] and scales [N, W]; fp32 sums, one rounding to y's type, which is x's. */
+int64_t xpuint8_mxfp4_linear_workspace_size(int64_t M, int64_t N, int64_t K);
+int xpuint8_mxfp4_linear_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
+                                const uint8_t *codes, const uint8_t *scales, const void *bias,
+                                int32_t bias_type, void *y, int64_t M, int64_t N, int64_t K,
+                                void *work, int64_t work_bytes);
+
+/* The products of E experts: y[i] = xq[rows[i]] wq[e]^T for offsets[e] <= i <
+ * offsets[e + 1], zeros for the rows past offsets[E]; codes [E, N, K/2], scales
+ * [E, N, W], offsets [E + 1], rows [R] (NULL: x has R rows, row i is its row i)
+ * indexing x's `tokens` rows.  offsets and rows are device data that only the
+ * kernels see: indices out of range are clamped into it.  E <= 1024. */
+int64_t xpuint8_mxfp4_grouped_linear_workspace_size(int64_t R, int64_t tokens, int64_t E,
+                                                    int64_t N, int64_t K);
+int xpuint8_mxfp4_grouped_linear_stream(const void *stream, const void *x, int32_t type,
+                                        int64_t ldx, const int32_t *rows, int64_t tokens,
+                                        const uint8_t *codes, const uint8_t *scales,
+                                        const int32_t *offsets, int64_t E, void *y, int64_t R,
+                                        int64_t N, int64_t K, void *work, int64_t work_bytes);
+
+/* dx [R, K] = dy [R, N] wq, of one weight (offsets NULL) or of the experts' over
+ * their rows, the gradient straight through x's quantization; fp32 sums, one
+ * rounding to dx_type.  work is read for a dy that is not bf16 in whole 16-byte
+ * aligned chunks (N % 8, the row stride % 8), and may then not be NULL. */
+int64_t xpuint8_mxfp4_dx_workspace_size(int32_t type, int64_t R, int64_t N);
+int xpuint8_mxfp4_dx_stream(const void *stream, const void *dy, int32_t type, int64_t ldy,
+                            const uint8_t *codes, const uint8_t *scales, const int32_t *offsets,
+                            int64_t E, void *dx, int32_t dx_type, int64_t R, int64_t N, int64_t K,
+                            void *work, int64_t work_bytes);
+
+/* ---- mixture of experts -------------------------------------------------
+ * T tokens of `top` slots each; slot s = t * top + j holds an expert's index in
+ * [0, E) or anything else for a slot that no expert takes.  E <= 1024.
+ *
+ * Sort the slots by (expert, slot), those without an expert last: order [T*top] the
+ * slot of each row, position [T, top] its inverse, rows[i] = order[i] / top,
+ * offsets [E + 1] the experts' first rows.  ids int32, or int64 (ids_int64 = 1).
+ * No counterpart in the reference. */
+int64_t xpuint8_moe_sort_workspace_size(int64_t T, int64_t top, int64_t E);
+int xpuint8_moe_sort_stream(const void *stream, const void *ids, int32_t ids_int64, int32_t *order,
+                            int32_t *position, int32_t *rows, int32_t *offsets, int64_t T,
+                            int64_t top, int64_t E, void *work, int64_t work_bytes);
+
+/* out [T*top, D]: x's row of each sorted row, zeros for the rows of no expert */
+int xpuint8_moe_dispatch_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
+                                const int32_t *position, const int32_t *offsets, void *out,
+                                int64_t T, int64_t top, int64_t E, int64_t D);
+
+/* out [T, D] = sum_j weights[t, j] * z[position[t, j]] over the slots that an expert
+ * has (weights fp32 [T, top], NULL: ones, which is dispatch's gradient); fp32 sums
+ * in slot order.  out_type is type, or anything for fp32 z without weights. */
+int xpuint8_moe_combine_stream(const void *stream, const void *z, int32_t type, int64_t ldz,
+                               const int32_t *position, const int32_t *offsets,
+                               const float *weights, void *out, int32_t out_type, int64_t T,
+                               int64_t top, int64_t E, int64_t D);
+
+/* the weighted sum's gradients: dz[position[t, j]] = weights[t, j] * dy[t],
+ * dweights[t, j] = <dy[t], z[position[t, j]]> in fp32; zeros where no expert is */
+int xpuint8_moe_combine_grad_stream(const void *stream, const void *dy, int32_t type, int64_t ldy,
+                                    const void *z, int64_t ldz, const int32_t *position,
+                                    const int32_t *offsets, const float *weights, void *dz,
+                                    float *dweights, int64_t T, int64_t top, int64_t E,
+                                    int64_t D);
+
 #ifdef __cplusplus
 }
 #endif

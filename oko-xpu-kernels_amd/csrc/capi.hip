@@ -14,6 +14,7 @@
 #include <string>
 
 #include "activations.hpp"
+#include "capi.hpp"
 #include "kernels.hpp"
 #include "../../include/xpuint8.h"
 
@@ -33,14 +34,14 @@ __device__ uint16_t g_act_tables[kNumTables * kTabSize];
 constexpr size_t kScratchBytes = size_t(64) << 20;
 static __device__ __align__(256) char scratch[kScratchBytes];
 
-namespace {
-
-thread_local std::string t_error;
+static thread_local std::string t_error;
 
 int fail(int code, const std::string& msg) {
     t_error = msg;
     return code;
 }
+
+namespace {
 
 constexpr int kMaxDevices = 64;
 std::mutex g_mutex;
@@ -49,6 +50,8 @@ const uint16_t* g_tab_dev[kMaxDevices] = {};
 char* g_scratch[kMaxDevices] = {};        // device address of `scratch`, per device
 int g_cus[kMaxDevices] = {};
 std::atomic<bool> g_ready[kMaxDevices] = {};
+
+}  // namespace
 
 // Per-device set-up: architecture check and table upload.  Returns 0 or an
 // error code (message set).
@@ -90,6 +93,8 @@ int launched(hipError_t e, const char* what) {
     return 0;
 }
 
+namespace {
+
 // Synchronous wrappers: run on the default stream and wait for it.
 int finish(int rc, const char* what) {
     if (rc != 0) return rc;
@@ -98,10 +103,7 @@ int finish(int rc, const char* what) {
     return 0;
 }
 
-hipStream_t as_stream(const void* s) { return static_cast<hipStream_t>(const_cast<void*>(s)); }
-
 constexpr int64_t kMaxK = 131072;          // 127*127*K < 2^31
-constexpr int64_t kMaxDim = (int64_t(1) << 31) - 1;
 constexpr int64_t kMaxGemmM = int64_t(65535) * 128;   // grid.y limit of the GEMM launch
 
 int check_rows(int64_t M, int64_t K) {
@@ -125,20 +127,6 @@ int check_gemm(int64_t M, int64_t N, int64_t K) {
     if (M > kMaxGemmM || N > kMaxDim) return fail(4, "M must be <= 8388480 and N < 2^31");
     return 0;
 }
-
-// Every buffer is read and written with 16-byte vector accesses.
-#define XPU_NONNULL(p)                                          \
-    if (!(p)) return fail(6, #p " must not be null");           \
-    if (reinterpret_cast<uintptr_t>(p) % 16 != 0)               \
-    return fail(6, #p " must be 16-byte aligned")
-#define XPU_ALIGNED_OPT(p)                                      \
-    if ((p) && reinterpret_cast<uintptr_t>(p) % 16 != 0)        \
-    return fail(6, #p " must be 16-byte aligned")
-#define XPU_TRY(expr)              \
-    do {                           \
-        const int rc_ = (expr);    \
-        if (rc_ != 0) return rc_;  \
-    } while (0)
 
 // The workspace of linear_dx_int8: the row-quantized column-scaled gradient
 // q [M,N] int8 (in the MFMA block layout, or row-major where the quantizer cannot

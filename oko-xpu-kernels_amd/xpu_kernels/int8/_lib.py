@@ -131,6 +131,24 @@ def _signatures():
                                             + [i64] * 7 + [vp, vp] + [i64] * 4
                                             + [ctypes.c_float, i32], c_int),
         "xpuint8_activation_table": ([i32, vp], c_int),
+        "xpuint8_mxfp4_scale_width": ([i64], i64),
+        "xpuint8_mxfp4_quantize_stream": ([vp, vp, i32, i64, vp, vp] + [i64] * 2, c_int),
+        "xpuint8_mxfp4_dequantize_stream": ([vp] * 4 + [i32] + [i64] * 2, c_int),
+        "xpuint8_mxfp4_linear_workspace_size": ([i64] * 3, i64),
+        "xpuint8_mxfp4_linear_stream": ([vp, vp, i32, i64, vp, vp, vp, i32, vp] + [i64] * 3
+                                        + [vp, i64], c_int),
+        "xpuint8_mxfp4_grouped_linear_workspace_size": ([i64] * 5, i64),
+        "xpuint8_mxfp4_grouped_linear_stream": ([vp, vp, i32, i64, vp, i64, vp, vp, vp, i64, vp]
+                                                + [i64] * 3 + [vp, i64], c_int),
+        "xpuint8_mxfp4_dx_workspace_size": ([i32] + [i64] * 2, i64),
+        "xpuint8_mxfp4_dx_stream": ([vp, vp, i32, i64, vp, vp, vp, i64, vp, i32] + [i64] * 3
+                                    + [vp, i64], c_int),
+        "xpuint8_moe_sort_workspace_size": ([i64] * 3, i64),
+        "xpuint8_moe_sort_stream": ([vp, vp, i32] + [vp] * 4 + [i64] * 3 + [vp, i64], c_int),
+        "xpuint8_moe_dispatch_stream": ([vp, vp, i32, i64] + [vp] * 3 + [i64] * 4, c_int),
+        "xpuint8_moe_combine_stream": ([vp, vp, i32, i64] + [vp] * 4 + [i32] + [i64] * 4, c_int),
+        "xpuint8_moe_combine_grad_stream": ([vp, vp, i32, i64, vp, i64] + [vp] * 5 + [i64] * 4,
+                                            c_int),
     }
 
 
