@@ -22,11 +22,11 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 
-// acc += W block (codes w, scale byte I of sw) * X block (codes x, byte I of sx)
-template <int I>
+// acc += W block (codes w, scale byte I of sw) * X block (codes x, byte J of sx)
+template <int I, int J>
 __device__ __forceinline__ v4f mfma4(const v4i& w, int sw, const v4i& x, int sx, const v4f& acc) {
     const v8i a = {w[0], w[1], w[2], w[3], 0, 0, 0, 0}, b = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, I, sw, I, sx);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, I, sw, J, sx);
 }
 
 // ----------------------------------------------------------------- few rows
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(NW * 64) void mx4_skinny_kernel(
         for (int j = 0; j < 4; ++j) {
             const int k = k0 + 128 * j + 32 * g;
             const int b = k < w.K ? int(sw[j] >> (8 * g)) : 127;     // (byte 0 is read)
-            acc = mfma4<0>(wf[j], b, xf[j], xs[j], acc);
+            acc = mfma4<0, 0>(wf[j], b, xf[j], xs[j], acc);
         }
     }
     part[wave][lane] = acc;
@@ -108,144 +108,496 @@ __global__ __launch_bounds__(NW * 64) void mx4_skinny_kernel(
     if (wave != 0 || !has) return;
 #pragma unroll
     for (int i = 1; i < NW; ++i) acc += part[i][lane];
-    store4<T>(out, row, n0 + 4 * g, acc + bias4(out, n0 + 4 * g));
+    const int n = n0 + 4 * g;
+    store4<T>(out, row, n, acc + v4f{bias_at(out, n), bias_at(out, n + 1), bias_at(out, n + 2), bias_at(out, n + 3)});
 }
 
 // -------------------------------------------------------------------- tiles
 // BM x BN tiles of y by a block of 4 waves in 2 x 2, x already quantized.  K in
-// stages of 256 values, 128 bytes of codes a row, which direct global->LDS loads
-// bring two stages deep; the 16 scale bytes of 512 values come every other stage.
-// A stage row's 16-byte chunk c sits at c ^ ((row >> 1) & 7): the 8 lanes that an
-// LDS cycle serves, consecutive rows at one chunk, then cover all banks.  In a
-// stage lane group g holds the chunks 2g and 2g + 1 (one an MFMA), so its two
-// scale bytes are one 16-bit LDS read.
-template <int T, int BM, int BN>
-__global__ __launch_bounds__(256) void mx4_tile_kernel(
+// steps of 128 values, 64 bytes of codes a row and one MFMA of each block, through
+// a ring of four LDS slots that direct global->LDS loads fill four steps ahead.
+// During step t a wave runs its MFMAs on one set of fragments, reads step t + 1's into
+// the other and issues its loads of step t + 4 into the slot of step t, whose last
+// reads the barrier before has seen; the wait and barrier after it see step t + 2
+// land.  So a load has two steps and more to arrive, and a step costs one barrier.
+//
+// Chunk c (16 bytes, one block) of a step's row sits at c ^ ((row >> 1) & 3): a
+// 16-byte LDS read serves the lanes 0-3, 12-15, 20-23 and 24-27 together (and so on),
+// which then cover all 64 banks once.  Lane group g holds chunk g, whose scale in
+// the row's 16 scale bytes of 512 values (four steps) is byte 4t + g.  The MFMA takes
+// its scale from a byte of a register that the instruction names, the same for all
+// lanes, so each 16 bytes are transposed (4 x 4) where they lie in LDS: lane group g
+// then reads one dword, whose byte t is step t's, and shifts it step by step.  That pass also clears the bytes of
+// blocks past K: 2^-127 in both operands, whose products vanish in fp32 (every code is
+// a number, so what the codes there are does not matter: loads past a row's end
+// repeat its last block).  Scales arrive two groups of four steps ahead, and are
+// transposed one ahead.
+//
+// The fragment reads are inline assembly (with the builtins the compiler waits for
+// every direct load before each LDS read); nothing is in flight over a loop edge:
+// each step ends with a wait that redefines what it read.
+__device__ __forceinline__ v4i read16(uint32_t addr, int off) {
+    v4i r;
+    asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "n"(off));
+    return r;
+}
+__device__ __forceinline__ int read4(uint32_t addr, int off) {
+    int r;
+    asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "n"(off));
+    return r;
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// The accumulators of a tile live in the accumulation registers a0 up, named in the
+// instructions: 4 registers an MFMA block, COUNT in all.  As values they were copied
+// at every turn of the loop or spilled (compilers move an MFMA builtin over barriers,
+// and its accumulator with it).  Every such instruction clobbers all of them, so
+// nothing else is kept there.  The compiler neither sees these MFMAs nor places the
+// waits that they need: two wait states between a VALU write and an MFMA that reads it,
+// eighteen between an MFMA and a read of its result by anything but an MFMA on it.
+#define XPU_A10(p) "a" #p "0", "a" #p "1", "a" #p "2", "a" #p "3", "a" #p "4", "a" #p "5", \
+                   "a" #p "6", "a" #p "7", "a" #p "8", "a" #p "9"
+#define XPU_A60 XPU_A10(), XPU_A10(1), XPU_A10(2), XPU_A10(3), XPU_A10(4), XPU_A10(5)
+#define XPU_A64 XPU_A60, "a60", "a61", "a62", "a63"
+#define XPU_A120 XPU_A60, XPU_A10(6), XPU_A10(7), XPU_A10(8), XPU_A10(9), XPU_A10(10), XPU_A10(11)
+#define XPU_A128 XPU_A120, "a120", "a121", "a122", "a123", "a124", "a125", "a126", "a127"
+#define XPU_A256 XPU_A120, XPU_A10(12), XPU_A10(13), XPU_A10(14), XPU_A10(15), XPU_A10(16),     \
+                 XPU_A10(17), XPU_A10(18), XPU_A10(19), XPU_A10(20), XPU_A10(21), XPU_A10(22),  \
+                 XPU_A10(23), XPU_A10(24), "a250", "a251", "a252", "a253", "a254", "a255"
+// blocks B0 .. B3 += W blocks (codes w, scale byte 0 of sw) * one X block
+#define XPU_MFMA4(CLOBBERS)                                                                     \
+    asm volatile(XPU_ONE_MFMA(0, 4, 10, 11) XPU_ONE_MFMA(1, 5, 12, 13)                          \
+                 XPU_ONE_MFMA(2, 6, 14, 15) XPU_ONE_MFMA(3, 7, 16, 17)                          \
+                 ::"v"(w[0]), "v"(w[1]), "v"(w[2]), "v"(w[3]), "v"(sw[0]), "v"(sw[1]),          \
+                 "v"(sw[2]), "v"(sw[3]), "v"(x), "v"(sx), "n"(4 * B0), "n"(4 * B0 + 3),         \
+                 "n"(4 * B1), "n"(4 * B1 + 3), "n"(4 * B2), "n"(4 * B2 + 3), "n"(4 * B3),       \
+                 "n"(4 * B3 + 3)                                                                \
+                 : CLOBBERS)
+#define XPU_ONE_MFMA(W, S, LO, HI)                                                              \
+    "v_mfma_scale_f32_16x16x128_f8f6f4 a[%" #LO ":%" #HI "], %" #W ", %8, a[%" #LO ":%" #HI     \
+    "], %" #S ", %9 op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t"
+template <int COUNT, int B0, int B1, int B2, int B3>
+__device__ __forceinline__ void acc_mfma4(const v4i* w, const int* sw, const v4i& x, int sx) {
+    static_assert(COUNT == 64 || COUNT == 128 || COUNT == 256, "a list of registers");
+    if constexpr (COUNT == 64) XPU_MFMA4(XPU_A64);
+    else if constexpr (COUNT == 128) XPU_MFMA4(XPU_A128);
+    else XPU_MFMA4(XPU_A256);
+}
+// the four registers of block BLOCK = v
+#define XPU_ACC_SET(CLOBBERS)                                                                   \
+    asm volatile("v_accvgpr_write_b32 a[%4], %0\n\tv_accvgpr_write_b32 a[%5], %1\n\t"           \
+                 "v_accvgpr_write_b32 a[%6], %2\n\tv_accvgpr_write_b32 a[%7], %3"               \
+                 ::"v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "n"(4 * BLOCK),                  \
+                 "n"(4 * BLOCK + 1), "n"(4 * BLOCK + 2), "n"(4 * BLOCK + 3)                     \
+                 : CLOBBERS)
+template <int COUNT, int BLOCK>
+__device__ __forceinline__ void acc_set(const v4f& v) {
+    if constexpr (COUNT == 64) XPU_ACC_SET(XPU_A64);
+    else if constexpr (COUNT == 128) XPU_ACC_SET(XPU_A128);
+    else XPU_ACC_SET(XPU_A256);
+}
+template <int BLOCK>
+__device__ __forceinline__ v4f acc_get() {
+    float a, b, c, d;
+    asm volatile("v_accvgpr_read_b32 %0, a[%4]\n\tv_accvgpr_read_b32 %1, a[%5]\n\t"
+                 "v_accvgpr_read_b32 %2, a[%6]\n\tv_accvgpr_read_b32 %3, a[%7]"
+                 : "=v"(a), "=v"(b), "=v"(c), "=v"(d)
+                 : "n"(4 * BLOCK), "n"(4 * BLOCK + 1), "n"(4 * BLOCK + 2), "n"(4 * BLOCK + 3));
+    return v4f{a, b, c, d};
+}
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each(const F& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        each<N, I + 1>(f);
+    }
+}
+template <int N>
+__device__ __forceinline__ void landed(v4i (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+template <int N>
+__device__ __forceinline__ void landed(int (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
+// zeros in the rows of a tile
+template <int BM, int BN>
+__device__ __forceinline__ void zero_rows(const Out& o, int type, const RowTile& t, int n0) {
+    const v4f zero = {0.f, 0.f, 0.f, 0.f};
+    for (int i = threadIdx.x; i < BM * (BN / 4); i += blockDim.x) {
+        const int row = t.row + i / (BN / 4), n = n0 + 4 * (i % (BN / 4));
+        if (row >= t.end) continue;
+        if (type == kBf16) store4<kBf16>(o, row, n, zero);
+        else if (type == kF16) store4<kF16>(o, row, n, zero);
+        else store4<kF32>(o, row, n, zero);
+    }
+}
+
+// One row of COUNT MFMA blocks' results in a 16-bit type, columns n .. n + 16 COUNT (all
+// in the row, 16-byte aligned): lane group g holds the columns 16a + 4g .. + 3 of block a,
+// value(a), and stores 16 bytes: the swap of two blocks' odd and even lane rows
+// (v_permlane16_swap) leaves lane groups 0 and 2 with the columns 0-7 and 8-15 of the
+// one block, 1 and 3 with the other's.  `live`: whether this lane's row is one to write.
+template <int T, int COUNT, class V>
+__device__ __forceinline__ void store_row(const Out& o, int64_t row, bool live, int n, const V& value) {
+    const int g = (threadIdx.x & 63) >> 4;
+    char* const p = o.y + (row * o.N + n + 16 * (g & 1) + 8 * (g >> 1)) * 2;
+    each<COUNT / 2>([&](auto A) {
+        constexpr int a = 2 * decltype(A)::value;
+        const v4f u = value(std::integral_constant<int, a>{});
+        const v4f v = value(std::integral_constant<int, a + 1>{});
+        const auto lo = __builtin_amdgcn_permlane16_swap(pack2<T>(u[0], u[1]), pack2<T>(v[0], v[1]), false, false);
+        const auto hi = __builtin_amdgcn_permlane16_swap(pack2<T>(u[2], u[3]), pack2<T>(v[2], v[3]), false, false);
+        if (live) *reinterpret_cast<uint4*>(p + 32 * a) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+    });
+}
+
+// Tile (tm, tn) of block b.  Blocks go round the 8 XCDs, each with its own L2, so an
+// XCD takes a contiguous eighth of the tiles, walked in bands of 8 row tiles: the
+// blocks of an XCD that run together share few rows of either operand.
+__device__ __forceinline__ bool tile_of(int b, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int tiles = tiles_m * tiles_n, share = (tiles + 7) / 8;
+    const int t = (b % 8) * share + b / 8;
+    if (t >= tiles) return false;
+    const int band = t / (8 * tiles_n), first = band * 8;
+    const int rows = min(tiles_m - first, 8), in = t - band * 8 * tiles_n;
+    tm = first + in % rows;
+    tn = in / rows;
+    return true;
+}
+
+template <int BM, int BN, bool GATHER>
+__global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_kernel(
     const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs, const int* __restrict__ rows,
-    int tokens, Weight w, const int* __restrict__ offsets, int E, Out out, int tiles_n) {
+    int tokens, Weight w, const int* __restrict__ offsets, int E, Out out, int type, int tiles_m,
+    int tiles_n) {
     constexpr int TM = BM / 32, TN = BN / 32;             // MFMA blocks of a wave
     constexpr int ROWS = BM + BN;                         // x rows first
-    constexpr int STAGE = ROWS * 128, SCALES = ROWS * 16;
-    constexpr int PER = ROWS / 32;                        // code loads a wave a stage
-    constexpr int PERS = ROWS / 256;                      // scale loads a wave a stage pair
-    static_assert(ROWS % 256 == 0, "whole scale loads");
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE + 2 * SCALES];
+    constexpr int STEP = ROWS * 64, SCALES = ROWS * 16;
+    constexpr int PX = BM / 64, PW = BN / 64;             // code loads a wave a step
+    constexpr int PL = PX + PW;
+    constexpr int PSX = BM / 64, PS = ROWS / 64;          // scale loads of x, of both, a block
+    constexpr int PER_S = (PS + 3) / 4;
+    constexpr int PER_T = (ROWS + 255) / 256;             // scale rows a thread transposes
+    constexpr int ACC = 4 * TM * TN;                      // block (a, b) is number a * TM + b
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * STEP + 2 * SCALES];
+    __shared__ float bias_of[BN];
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const int wm = wave >> 1, wn = wave & 1;
+    int tm, tn;
+    if (!tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn)) return;
     RowTile t;
-    if (!row_tile<BM>(offsets, E, out.R, blockIdx.x / tiles_n, t)) return;
-    const int n0 = (blockIdx.x % tiles_n) * BN;
+    if (!row_tile<BM>(offsets, E, out.R, tm, t)) return;
+    const int n0 = tn * BN;
     if (t.e == E) {
-        const v4f zero = {0.f, 0.f, 0.f, 0.f};
-        for (int i = threadIdx.x; i < BM * (BN / 4); i += 256) {
-            const int row = t.row + i / (BN / 4);
-            if (row < t.end) store4<T>(out, row, n0 + 4 * (i % (BN / 4)), zero);
-        }
+        zero_rows<BM, BN>(out, type, t, n0);
         return;
     }
     const int K = w.K, KB = K / 2;
-    const int stages = (K + 255) / 256;
-    // the row of the stage that a lane brings: in units of 16 bytes from the
-    // operand's first (32 bits of them reach 64 GB)
-    const uint8_t* const wbase = w.codes + int64_t(t.e) * w.N * KB;
-    const uint8_t* const wsbase = w.scales + int64_t(t.e) * w.N * w.SW;
-    auto source_row = [&](int j) {                        // x row or weight row of stage row j
-        if (j < BM) {
-            int i = min(t.row + j, t.end - 1);
-            if (rows) i = min(max(rows[i], 0), tokens - 1);
-            return i;
-        }
-        return min(n0 + j - BM, w.N - 1);
+    const int steps = (K + 127) / 128, groups = (K + 511) / 512;
+    // Sources: a wave-uniform base and a lane's 32-bit offset from the tile's first
+    // row (a tile spans less than 4 GiB), or, for rows that a list names, the lane's
+    // own address.  Load i of a wave brings 16 rows.
+    const int64_t w0 = int64_t(t.e) * w.N + n0;
+    const uint8_t* const wbase = w.codes + w0 * KB;
+    const uint8_t* const wsbase = w.scales + w0 * w.SW;
+    const uint8_t* const xbase = xc + (GATHER ? 0 : int64_t(t.row) * KB);
+    const uint8_t* const xsbase = xs + (GATHER ? 0 : int64_t(t.row) * w.SW);
+    auto x_row = [&](int j) {                             // the row of tile row j, from xbase
+        const int i = min(t.row + j, t.end - 1);
+        return GATHER ? min(max(rows[i], 0), tokens - 1) : i - t.row;
     };
-    uint32_t at[PER], ats[PERS];
+    auto w_row = [&](int j) { return min(n0 + j, w.N - 1) - n0; };
+    const int lr = lane >> 2;
+    const uint32_t c16 = uint32_t((lane & 3) ^ ((lr >> 1) & 3)) * 16;
+    std::conditional_t<GATHER, const uint8_t*, uint32_t> ax[PX];
+    uint32_t aw[PW];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int j = (wave + 4 * i) * 8 + lane / 8;
-        const int c = (lane & 7) ^ ((j >> 1) & 7);
-        at[i] = uint32_t(source_row(j)) * uint32_t(KB / 16) + c;
+    for (int i = 0; i < PX; ++i) {
+        const int j = (wave + 4 * i) * 16 + lr;
+        if constexpr (GATHER) ax[i] = xbase + int64_t(x_row(j)) * KB + c16;
+        else ax[i] = uint32_t(x_row(j)) * uint32_t(KB) + c16;
     }
 #pragma unroll
-    for (int i = 0; i < PERS; ++i)
-        ats[i] = uint32_t(source_row((wave + 4 * i) * 64 + lane)) * uint32_t(w.SW / 16);
-    auto issue = [&](int s) {
-        uint8_t* const st = smem + (s & 1) * STAGE;
-        const bool tail = (s + 1) * 256 > K;
+    for (int i = 0; i < PW; ++i)
+        aw[i] = uint32_t(w_row((wave + 4 * i) * 16 + lr)) * uint32_t(KB) + c16;
+    uint32_t as[PER_S];                                   // 16-byte units: 64 GiB of scales
+    const uint8_t* sbs[PER_S];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int b = (wave + 4 * i) * 8;             // its first stage row
-            const uint8_t* base = b < BM ? xc : wbase;
-            const uint8_t* p = base + (uint64_t(at[i] + 8u * s) << 4);
-            if (tail) {
-                const int j = b + lane / 8;
-                const int c = (lane & 7) ^ ((j >> 1) & 7);
-                if (s * 256 + c * 32 >= K) p = g_zero_line;
-            }
-            dma16(p, st + b * 128);
+    for (int i = 0; i < PER_S; ++i) {
+        const int b = min(wave + 4 * i, PS - 1);
+        sbs[i] = b < PSX ? xsbase : wsbase;
+        as[i] = uint32_t(b < PSX ? x_row(b * 64 + lane) : w_row((b - PSX) * 64 + lane)) *
+                uint32_t(w.SW / 16);
+    }
+    // load i of this wave's PX + PW (x first) into the slot, from byte k of the rows
+    // less back (for the last step's chunks past the row's end: its last chunk)
+    auto issue_codes = [&](int slot, int64_t k, uint32_t back, int i) {
+        const bool isx = i < PX;
+        const int b = (wave + 4 * (isx ? i : i - PX)) * 16 + (isx ? 0 : BM);
+        const uint8_t* p;
+        if (isx) {
+            if constexpr (GATHER) p = ax[i] + k - back;
+            else p = (xbase + k) + uint64_t(ax[i] - back);
+        } else {
+            p = (wbase + k) + uint64_t(aw[i - PX] - back);
         }
-        if ((s & 1) == 0) {
-            uint8_t* const sc = smem + 2 * STAGE + ((s >> 1) & 1) * SCALES;
+        dma16(p, smem + slot * STEP + b * 64);
+    };
+    auto past_end = [&](int s) {                          // back, of step s
+        const int over = s * 64 + int(c16) + 16 - KB;
+        return over > 0 ? uint32_t(over) : 0u;
+    };
+    auto issue_scales = [&](int q) {
 #pragma unroll
-            for (int i = 0; i < PERS; ++i) {
-                const int b = (wave + 4 * i) * 64;
-                const uint8_t* base = b < BM ? xs : wsbase;
-                dma16(base + (uint64_t(ats[i] + uint32_t(s >> 1)) << 4), sc + b * 16);
-            }
+        for (int i = 0; i < PER_S; ++i) {
+            const int b = wave + 4 * i;
+            if (PS % 4 == 0 || b < PS)
+                dma16(sbs[i] + (uint64_t(as[i] + uint32_t(q)) << 4),
+                      smem + 4 * STEP + (q & 1) * SCALES + b * 1024);
         }
     };
-    v4f acc[TN][TM];
-#pragma unroll
-    for (int a = 0; a < TN; ++a)
-#pragma unroll
-        for (int b = 0; b < TM; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
-    issue(0);
+
     const int xrow = wm * (BM / 2) + r, wrow = BM + wn * (BN / 2) + r;
-    for (int s = 0; s < stages; ++s) {
-        wait_loads();
-        __syncthreads();                                  // stage s landed, s - 1 is read
-        if (s + 1 < stages) issue(s + 1);
-        const uint8_t* const st = smem + (s & 1) * STAGE;
-        const uint8_t* const sc = smem + 2 * STAGE + ((s >> 1) & 1) * SCALES + (s & 1) * 8 + 2 * g;
-        // blocks past K hold zero codes; their scales may be anything
-        const int left = K - s * 256;
-        int sx[TM], sw[TN];
+    const uint32_t sbase = lds_addr(smem);
+    const uint32_t pos = (g ^ ((r >> 1) & 3)) * 16;
+    const uint32_t xat[2] = {sbase + xrow * 64 + pos, sbase + 2 * STEP + xrow * 64 + pos};
+    const uint32_t wat[2] = {sbase + wrow * 64 + pos, sbase + 2 * STEP + wrow * 64 + pos};
+    v4i xf[2][TM], wf[2][TN];                             // of even and odd steps
+    int sx[TM], sw[TN];                                   // byte 0: this step's scale
+    int sr[TM + TN];                                      // the next group's
+    v4i tr[PER_T];                                        // scale rows on their way through
+    auto read_x = [&](auto S, auto Fr, auto I) {
+        constexpr int slot = decltype(S)::value, f = decltype(Fr)::value, i = decltype(I)::value;
+        xf[f][i] = read16(xat[slot >> 1], (slot & 1) * STEP + i * 1024);
+    };
+    auto read_w = [&](auto S, auto Fr, auto I) {
+        constexpr int slot = decltype(S)::value, f = decltype(Fr)::value, i = decltype(I)::value;
+        wf[f][i] = read16(wat[slot >> 1], (slot & 1) * STEP + i * 1024);
+    };
+    auto read_scale = [&](uint32_t at, int i) {           // of block i, x's first
+        sr[i] = i < TM ? read4(at + xrow * 16, i * 256) : read4(at + wrow * 16, (i - TM) * 256);
+    };
+    // the 4 x 4 byte transposition of each row's scales of group q, in place: the
+    // reads, and after they have landed the writes
+    auto scale_row = [&](int q, int i) {
+        return sbase + 4 * STEP + (q & 1) * SCALES + (threadIdx.x + 256 * i) * 16;
+    };
+    const bool tlast = ROWS % 256 == 0 || int(threadIdx.x) + 256 * (PER_T - 1) < ROWS;
+    auto transpose_read = [&](int q) {
+        each<PER_T>([&](auto I) {
+            constexpr int i = decltype(I)::value;
+            tr[i] = read16(i < PER_T - 1 || tlast ? scale_row(q, i) : sbase, 0);
+        });
+    };
+    auto transpose_write = [&](int q) {
+        const int left = K / 32 - q * 16;                 // blocks up to K
 #pragma unroll
-        for (int b = 0; b < TM; ++b) sx[b] = *reinterpret_cast<const uint16_t*>(sc + (xrow + 16 * b) * 16);
+        for (int i = 0; i < PER_T; ++i) {
+            uint32_t d[4];
 #pragma unroll
-        for (int a = 0; a < TN; ++a) sw[a] = *reinterpret_cast<const uint16_t*>(sc + (wrow + 16 * a) * 16);
-        if (left < 256) {
-            const int keep = (64 * g < left ? 0xFF : 0) | (64 * g + 32 < left ? 0xFF00 : 0);
+            for (int c = 0; c < 4; ++c) d[c] = uint32_t(tr[i][c]);
+            if (left < 16) {
 #pragma unroll
-            for (int b = 0; b < TM; ++b) sx[b] &= keep;
-#pragma unroll
-            for (int a = 0; a < TN; ++a) sw[a] &= keep;
+                for (int c = 0; c < 4; ++c) {
+                    const int n = left - 4 * c;           // of the dword's four blocks
+                    d[c] &= n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+                }
+            }
+            const uint32_t lo01 = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u);   // bytes 0, 1 of d0, d1
+            const uint32_t hi01 = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u);   // bytes 2, 3
+            const uint32_t lo23 = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u);
+            const uint32_t hi23 = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
+            const v4i o = {int(__builtin_amdgcn_perm(lo23, lo01, 0x05040100u)),
+                           int(__builtin_amdgcn_perm(lo23, lo01, 0x07060302u)),
+                           int(__builtin_amdgcn_perm(hi23, hi01, 0x05040100u)),
+                           int(__builtin_amdgcn_perm(hi23, hi01, 0x07060302u))};
+            if (i < PER_T - 1 || tlast)
+                asm volatile("ds_write_b128 %0, %1" ::"v"(scale_row(q, i)), "v"(o) : "memory");
         }
-        auto half = [&](auto H) {
-            constexpr int h = decltype(H)::value;
-            v4i xf[TM], wf[TN];
-            const int pos = ((2 * g + h) ^ ((r >> 1) & 7)) * 16;
+    };
+    auto lds_done = [&]() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+    auto barrier = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using C0 = std::integral_constant<int, 0>;
+    using C1 = std::integral_constant<int, 1>;
+    using C2 = std::integral_constant<int, 2>;
+    using C3 = std::integral_constant<int, 3>;
+
+    // the bias of the tile's columns is read ahead of the direct loads (loads complete
+    // in order) and used after them
+    static_assert(BN <= 256, "a column a thread");
+    const float bias_here = bias_at(out, n0 + min(int(threadIdx.x), BN - 1));
+    if (groups > 1) {
+        issue_scales(0);
+        issue_scales(1);
 #pragma unroll
-            for (int b = 0; b < TM; ++b) xf[b] = *reinterpret_cast<const v4i*>(st + (xrow + 16 * b) * 128 + pos);
+        for (int s = 0; s < 4; ++s) {
 #pragma unroll
-            for (int a = 0; a < TN; ++a) wf[a] = *reinterpret_cast<const v4i*>(st + (wrow + 16 * a) * 128 + pos);
+            for (int i = 0; i < PL; ++i) issue_codes(s, s * 64, 0, i);
+        }
+        if (threadIdx.x < BN) bias_of[threadIdx.x] = bias_here;
+    } else {
+        issue_scales(0);
+        for (int s = 0; s < min(steps, 4); ++s) {
+            const uint32_t back = past_end(s);
 #pragma unroll
-            for (int b = 0; b < TM; ++b)
-#pragma unroll
-                for (int a = 0; a < TN; ++a) acc[a][b] = mfma4<h>(wf[a], sw[a], xf[b], sx[b], acc[a][b]);
-        };
-        half(std::integral_constant<int, 0>{});
-        half(std::integral_constant<int, 1>{});
+            for (int i = 0; i < PL; ++i) issue_codes(s, s * 64, back, i);
+        }
+        if (threadIdx.x < BN) bias_of[threadIdx.x] = bias_here;
     }
+    lds_done();
+    // meanwhile the accumulators start from the bias
+    barrier();
+    each<TN>([&](auto A) {
+        constexpr int a = decltype(A)::value;
+        v4i b4 = read16(lds_addr(bias_of) + (wn * (BN / 2) + 4 * g) * 4, a * 64);
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(b4)::"memory");
+        each<TM>([&](auto B) { acc_set<ACC, a * TM + decltype(B)::value>(__builtin_bit_cast(v4f, b4)); });
+    });
+    // (the scales went out first, then the codes step by step: step 0's are in too)
+    if (groups > 1) wait_vm<3 * PL>();
+    else wait_vm<0>();
+    barrier();
+    transpose_read(0);
+    lds_done();
+    landed(tr);
+    transpose_write(0);
+    lds_done();
+    barrier();
+    each<TM + TN>([&](auto I) { read_scale(sbase + 4 * STEP + 4 * g, decltype(I)::value); });
+    each<TM>([&](auto I) { read_x(C0{}, C0{}, I); });
+    each<TN>([&](auto I) { read_w(C0{}, C0{}, I); });
+    lds_done();
+    landed(xf[0]); landed(wf[0]); landed(sr);
 #pragma unroll
-    for (int a = 0; a < TN; ++a) {
-        const int n = n0 + wn * (BN / 2) + 16 * a + 4 * g;
-        const v4f b4 = bias4(out, n);
+    for (int b = 0; b < TM; ++b) sx[b] = sr[b];
 #pragma unroll
-        for (int b = 0; b < TM; ++b) {
+    for (int a = 0; a < TN; ++a) sw[a] = sr[TM + a];
+    if (groups > 1) wait_vm<2 * PL>();                    // step 1 in
+    barrier();                                            // step 0's slot is read
+
+    // step s = 4q + J; FULL: step s + 4 exists and is whole
+    auto step = [&](auto Jc, auto Full, int q) {
+        constexpr int J = decltype(Jc)::value, F = J & 1;
+        constexpr bool FULL = decltype(Full)::value;
+        using Next = std::integral_constant<int, (J + 1) & 3>;
+        using NF = std::integral_constant<int, 1 - F>;
+        const int s = 4 * q + J;
+        const bool more = FULL || s + 4 < steps;
+        const int64_t k = int64_t(s + 4) * 64;
+        const uint32_t back = FULL ? 0u : past_end(s + 4);
+        const uint32_t sat = sbase + 4 * STEP + 4 * g + ((q + 1) & 1) * SCALES;
+        if (J == 0 && q + 2 < groups) issue_scales(q + 2);
+        // (past the last group or step the reads find what was there, and go unused)
+        if constexpr (J == 1) transpose_read(q + 1);
+        if constexpr (J == 2) transpose_write(q + 1);
+        each<TM>([&](auto B) {
+            constexpr int b = decltype(B)::value;
+            constexpr int H = TM / 2;                     // the reads in the step's first half
+            if constexpr (b < H) {
+                each<TM / H>([&](auto I) {
+                    read_x(Next{}, NF{}, std::integral_constant<int, b * (TM / H) + decltype(I)::value>{});
+                });
+                each<TN / H>([&](auto I) {
+                    read_w(Next{}, NF{}, std::integral_constant<int, b * (TN / H) + decltype(I)::value>{});
+                });
+                if constexpr (J == 3)
+                    each<(TM + TN) / H>([&](auto I) { read_scale(sat, b * ((TM + TN) / H) + decltype(I)::value); });
+            }
+            if (more) {
+#pragma unroll
+                for (int i = b * PL / TM; i < (b + 1) * PL / TM; ++i) issue_codes(J, k, back, i);
+            }
+            each<TN / 4>([&](auto A) {
+                constexpr int a = 4 * decltype(A)::value;
+                acc_mfma4<ACC, a * TM + b, (a + 1) * TM + b, (a + 2) * TM + b, (a + 3) * TM + b>(
+                    &wf[F][a], &sw[a], xf[F][b], sx[b]);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        lds_done();
+        landed(xf[1 - F]); landed(wf[1 - F]);
+        if constexpr (J == 1) landed(tr);
+        if constexpr (J == 3) landed(sr);
+#pragma unroll
+        for (int b = 0; b < TM; ++b) sx[b] = J == 3 ? sr[b] : int(uint32_t(sx[b]) >> 8);
+#pragma unroll
+        for (int a = 0; a < TN; ++a) sw[a] = J == 3 ? sr[TM + a] : int(uint32_t(sw[a]) >> 8);
+        // step s + 2 in: of what was issued later, steps s + 3 and s + 4 may be on the way
+        // (a group's scales go out before its first step's codes)
+        if (more) wait_vm<2 * PL>();
+        else if (s + 3 < steps) wait_vm<PL>();
+        else wait_vm<0>();
+        barrier();
+    };
+    const int whole = K / 128;
+    int q = 0;
+#pragma clang loop unroll(disable)
+    for (; 4 * q + 8 <= whole; ++q) {
+        step(C0{}, std::true_type{}, q);
+        step(C1{}, std::true_type{}, q);
+        step(C2{}, std::true_type{}, q);
+        step(C3{}, std::true_type{}, q);
+    }
+#pragma clang loop unroll(disable)
+    for (;; ++q) {
+        step(C0{}, std::false_type{}, q);
+        if (4 * q + 1 >= steps) break;
+        step(C1{}, std::false_type{}, q);
+        if (4 * q + 2 >= steps) break;
+        step(C2{}, std::false_type{}, q);
+        if (4 * q + 3 >= steps) break;
+        step(C3{}, std::false_type{}, q);
+        if (4 * q + 4 >= steps) break;
+    }
+    // the last MFMAs' results before the compiler, which does not see them, reads them
+    asm volatile("s_nop 15\n\ts_nop 15");
+    const int n = n0 + wn * (BN / 2);
+    auto store = [&](auto T) {
+        each<TM>([&](auto B) {
+            constexpr int b = decltype(B)::value;
             const int row = t.row + xrow + 16 * b;
-            if (row < t.end) store4<T>(out, row, n, acc[a][b] + b4);
+            store_row<decltype(T)::value, TN>(out, row, row < t.end, n, [&](auto A) {
+                return acc_get<decltype(A)::value * TM + b>();
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    const bool fast = out.vec8 && n + BN / 2 <= w.N;
+    if (fast && type == kBf16) return store(std::integral_constant<int, kBf16>{});
+    if (fast && type == kF16) return store(std::integral_constant<int, kF16>{});
+    // other types, widths and edges: 16 rows at a time through the wave's own part of
+    // the ring (which nothing reads or fills any more)
+    float* const mine = reinterpret_cast<float*>(smem) + wave * 16 * (BN / 2);
+    each<TM>([&](auto B) {
+        constexpr int b = decltype(B)::value;
+        each<TN>([&](auto A) {
+            constexpr int a = decltype(A)::value;
+            *reinterpret_cast<v4f*>(mine + r * (BN / 2) + 16 * a + 4 * g) = acc_get<a * TM + b>();
+        });
+        lds_done();
+#pragma clang loop unroll(disable)
+        for (int i = lane; i < 16 * (BN / 8); i += 64) {
+            const int rr = i / (BN / 8), c = 4 * (i % (BN / 8));
+            const int row = t.row + wm * (BM / 2) + 16 * b + rr;
+            const v4f v = *reinterpret_cast<const v4f*>(mine + rr * (BN / 2) + c);
+            if (row >= t.end) continue;
+            if (type == kBf16) store4<kBf16>(out, row, n + c, v);
+            else if (type == kF16) store4<kF16>(out, row, n + c, v);
+            else store4<kF32>(out, row, n + c, v);
         }
-    }
+        lds_done();
+    });
 }
 
 }  // namespace
@@ -276,20 +628,52 @@ hipError_t mx4_product_fused(hipStream_t st, const void* x, int type, int64_t ld
     return hipGetLastError();
 }
 
+namespace {
+
+// Whether 256 x 256 tiles (one block a CU, half the operand bytes a product) are
+// faster than 128 x 128 (two blocks a CU, so that one's start and end overlap the
+// other's steps, and finer rounds), by the times that a round of either takes, fitted
+// to both over seven shapes: 8192^3 330 against 430 us, 4096^3 49 against 58; 4096 x 10240
+// x 1280 66 against 51, 32 experts' 16380 x 2816 x 2048 133 against 104.
+bool large_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
+    const double steps = double((K + 127) / 128);
+    auto tiles = [&](int64_t b) {                          // (a group's last tile half full)
+        const int64_t tm = grouped ? R / b + std::min<int64_t>(E, R) / 2 + 1 : (R + b - 1) / b;
+        return tm * ((N + b - 1) / b);
+    };
+    const int64_t cus = device_cus();
+    const int64_t t128 = tiles(128), t256 = tiles(256);
+    const double large = double((t256 + cus - 1) / cus) * (10.0 + 1.13 * steps);
+    const double small = double(t128 / (2 * cus)) * (2.6 + 0.8 * steps) +
+                         (t128 % (2 * cus) > cus ? 2.6 + 0.8 * steps
+                          : t128 % (2 * cus) > 0 ? 2.6 + 0.45 * steps : 0.0);
+    return large < small;
+}
+
+}  // namespace
+
 hipError_t mx4_product(hipStream_t st, const uint8_t* xc, const uint8_t* xs, const int* rows,
                        int64_t tokens, const uint8_t* wc, const uint8_t* ws, const int* offsets,
                        int E, void* y, int type, const void* bias, int bias_type, int64_t R, int N,
                        int K) {
     const Weight w{wc, ws, N, K, int(mx_scale_width(K))};
     const Out o = make_out(y, type, bias, bias_type, R, N);
-    by_type(type, [&](auto T) {
-        constexpr int t = decltype(T)::value;
-        constexpr int BM = 128, BN = 128;
+    auto go = [&](auto M, auto N_) {
+        constexpr int BM = decltype(M)::value, BN = decltype(N_)::value;
         const int tiles_n = (N + BN - 1) / BN;
-        const int64_t tiles = most_tiles(offsets != nullptr, R, E, BM) * tiles_n;
-        hipLaunchKernelGGL((mx4_tile_kernel<t, BM, BN>), dim3(unsigned(tiles)), dim3(256), 0, st,
-                           xc, xs, rows, int(tokens), w, offsets, E, o, tiles_n);
-    });
+        const int tiles_m = int(most_tiles(offsets != nullptr, R, E, BM));
+        const dim3 grid(unsigned((int64_t(tiles_m) * tiles_n + 7) / 8 * 8));
+        if (rows)
+            hipLaunchKernelGGL((mx4_tile_kernel<BM, BN, true>), grid, dim3(256), 0, st, xc, xs,
+                               rows, int(tokens), w, offsets, E, o, type, tiles_m, tiles_n);
+        else
+            hipLaunchKernelGGL((mx4_tile_kernel<BM, BN, false>), grid, dim3(256), 0, st, xc, xs,
+                               rows, int(tokens), w, offsets, E, o, type, tiles_m, tiles_n);
+    };
+    using I128 = std::integral_constant<int, 128>;
+    using I256 = std::integral_constant<int, 256>;
+    if (large_tiles(offsets != nullptr, R, E, N, K)) go(I256{}, I256{});
+    else go(I128{}, I128{});
     return hipGetLastError();
 }
 

@@ -79,19 +79,14 @@ struct Out {
     int bias_type;
     int R, N;
     bool vec;                  // four columns at a time: N % 4 == 0 (and y aligned)
+    bool vec8;                 // eight
 };
-// four columns n .. n + 3 of the bias, 0 past N
-__device__ __forceinline__ v4f bias4(const Out& o, int n) {
-    v4f b = {0.f, 0.f, 0.f, 0.f};
-    if (!o.bias) return b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (n + i >= o.N) break;
-        if (o.bias_type == kF32) b[i] = static_cast<const float*>(o.bias)[n + i];
-        else if (o.bias_type == kBf16) b[i] = bf16_to_f32(static_cast<const uint16_t*>(o.bias)[n + i]);
-        else b[i] = float(static_cast<const _Float16*>(o.bias)[n + i]);
-    }
-    return b;
+// the bias of column n, 0 without one or past N
+__device__ __forceinline__ float bias_at(const Out& o, int n) {
+    if (!o.bias || n >= o.N) return 0.f;
+    if (o.bias_type == kF32) return static_cast<const float*>(o.bias)[n];
+    if (o.bias_type == kBf16) return bf16_to_f32(static_cast<const uint16_t*>(o.bias)[n]);
+    return float(static_cast<const _Float16*>(o.bias)[n]);
 }
 template <int T>
 __device__ __forceinline__ void store4(const Out& o, int64_t row, int n, const v4f& v) {
@@ -148,7 +143,8 @@ void by_type(int type, const F& f) {
 Out make_out(void* y, int type, const void* bias, int bias_type, int64_t R, int N) {
     const int size = type == kF32 ? 4 : 2;
     return Out{static_cast<char*>(y), bias, bias_type, int(R), N,
-               N % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (4 * size) == 0};
+               N % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (4 * size) == 0,
+               N % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0};
 }
 
 }  // namespace

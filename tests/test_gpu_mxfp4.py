@@ -139,6 +139,39 @@ def test_linear(dev, dtype, m, k, n):
     check_linear(dev, x, n, bias=randn(n, seed=2, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype,m,k,n", [(torch.bfloat16, 4090, 8160, 4080),
+                                         (torch.bfloat16, 4001, 8192, 4081),
+                                         (torch.float32, 3890, 7968, 4096)])
+def test_linear_large_tiles(dev, dtype, m, k, n):
+    """Shapes that take the large tiles, ragged in every dimension."""
+    x = randn(m, k, seed=m, dtype=dtype)
+    bias = randn(n, seed=2, dtype=dtype)
+    (codes, scales), wq = weight(n, k, 1, dev)
+    xq, wd = O.dequantize(*O.quantize(x)).to(dev), wq.to(dev)
+    y = mxfp4.linear(x.to(dev), codes, scales, bias.to(dev))
+    b = bias.to(dev).double()
+    assert_close(y, (xq @ wd.t() + b).cpu(), (xq.abs() @ wd.abs().t() + b.abs()).cpu(), k + 1)
+
+
+@pytest.mark.parametrize("gather", [False, True])
+def test_grouped_large_tiles(dev, gather):
+    t, top, e, k, n = 4095, 2, 3, 8160, 3800
+    ids = router(t, top, e, seed=1, dropped=0.02)
+    routing = moe.sort(ids.to(dev), e)
+    w = randn(e, n, k, seed=7, scale=0.05)
+    codes, scales = mxfp4.quantize(w.to(dev))
+    x = randn(t if gather else t * top, k, seed=8, dtype=torch.bfloat16)
+    y = mxfp4.grouped_linear(x.to(dev), codes, scales, routing, gather=gather)
+    xq = O.dequantize(*O.quantize(x)).to(dev)
+    off = routing.offsets.tolist()
+    for i in range(e):
+        r = slice(off[i], off[i + 1])
+        xr = xq[routing.rows[r].long()] if gather else xq[r]
+        wq = O.dequantize(codes[i], scales[i]).to(dev)
+        assert_close(y[r], (xr @ wq.t()).cpu(), (xr.abs() @ wq.abs().t()).cpu(), k)
+    assert (y[off[-1]:] == 0).all()
+
+
 @pytest.mark.parametrize("m", [1, 40, 200])
 @pytest.mark.parametrize("bias_dtype", DTYPES)
 def test_linear_bias_types(dev, m, bias_dtype):
