@@ -3,9 +3,11 @@
 // capi.hip, every check runs before any HIP call.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <string>
 
 #include "capi.hpp"
+#include "kernels.hpp"
 #include "mx4.hpp"
 #include "mx_kernels.hpp"
 #include "../../include/xpuint8.h"
@@ -98,6 +100,14 @@ bool dy_direct(const void* dy, int32_t type, int64_t ldy, int64_t N) {
            reinterpret_cast<uintptr_t>(dy) % 16 == 0;
 }
 
+// Whether dx of one weight goes through the weight as bf16 in the workspace and the
+// bf16 product (gemm_bf16_nn), whose tiles fit more shapes: bf16 of whole 16s, from 128
+// rows on (with the weight's conversion 64 against 96 us at 4096 x 5120 -> 1280, 33 against 39
+// at 256 x 4096 -> 4096; below, the conversion is most of it).
+bool dx_by_bf16(int32_t type, int32_t dx_type, bool grouped, int64_t R, int64_t N, int64_t K) {
+    return type == kBf16 && dx_type == kBf16 && !grouped && N % 16 == 0 && K % 16 == 0 && R >= 128;
+}
+
 }  // namespace
 }  // namespace xpuint8
 
@@ -174,8 +184,12 @@ int xpuint8_mxfp4_grouped_linear_stream(const void* stream, const void* x, int32
                    N, K, work, work_bytes, "mxfp4_grouped_linear");
 }
 
-int64_t xpuint8_mxfp4_dx_workspace_size(int32_t type, int64_t R, int64_t N) {
-    if (type < 0 || type > 2 || R <= 0 || N <= 0 || R > kMaxDim || N > kMaxDim) return -1;
+int64_t xpuint8_mxfp4_dx_workspace_size(int32_t type, int32_t dx_type, int64_t R, int64_t E,
+                                        int64_t N, int64_t K) {
+    if (check_product(R, R, N, K, E > 0, E) != 0 || check_type(type, "type") != 0) return -1;
+    if (dx_by_bf16(type, dx_type, E > 0, R, N, K))
+        return std::max(up(2 * N * K) + up(bf16_dx_work_bytes(int(R), int(N), int(K))),
+                        up(R * mx4_split_width(N) * 2));
     return up(R * mx4_split_width(N) * mx4_split_pieces(type) * 2);
 }
 
@@ -189,11 +203,25 @@ int xpuint8_mxfp4_dx_stream(const void* stream, const void* dy, int32_t type, in
     if (ldy < N) return fail(2, "the row stride must be >= N");
     if (!dy) return fail(6, "dy must not be null");
     XPU_NONNULL(codes); XPU_NONNULL(scales); XPU_NONNULL(dx);
+    const bool grouped = offsets != nullptr;
     const bool direct = dy_direct(dy, type, ldy, N);
+    const int64_t need = xpuint8_mxfp4_dx_workspace_size(type, dx_type, R, grouped ? E : 0, N, K);
+    if (dx_by_bf16(type, dx_type, grouped, R, N, K) && direct && ldy == N) {
+        XPU_NONNULL(work);
+        if (work_bytes < up(2 * N * K))
+            return fail(2, "work must hold xpuint8_mxfp4_dx_workspace_size bytes");
+        XPU_TRY(ensure_device());
+        hipStream_t st = as_stream(stream);
+        char* const wd = static_cast<char*>(work);
+        XPU_TRY(launched(mx4_dequantize(st, codes, scales, wd, kBf16, N, int(K)), "mxfp4_dx (weight)"));
+        return launched(gemm_bf16_nn(st, dy, N, wd, K, dx, K, int(R), int(N), int(K),
+                                     reinterpret_cast<float*>(wd + up(2 * N * K)),
+                                     work_bytes - up(2 * N * K)), "mxfp4_dx (bf16)");
+    }
     if (!direct) {
         XPU_NONNULL(work);
-        if (work_bytes < xpuint8_mxfp4_dx_workspace_size(type, R, N))
-            return fail(2, "work must hold xpuint8_mxfp4_dx_workspace_size(type, R, N) bytes");
+        if (work_bytes < need)
+            return fail(2, "work must hold xpuint8_mxfp4_dx_workspace_size bytes");
         if (R * mx4_split_width(N) > kMaxDim * 256) return fail(4, "dy is too large for one launch");
     }
     XPU_TRY(ensure_device());
@@ -204,7 +232,7 @@ int xpuint8_mxfp4_dx_stream(const void* stream, const void* dy, int32_t type, in
         dy = work;
         ldy = mx4_split_width(N) * pieces;
     }
-    return launched(mx4_dx(st, dy, ldy, pieces, codes, scales, offsets, offsets ? int(E) : 1, dx,
+    return launched(mx4_dx(st, dy, ldy, pieces, codes, scales, offsets, grouped ? int(E) : 1, dx,
                            dx_type, R, int(N), int(K)), "mxfp4_dx");
 }
 

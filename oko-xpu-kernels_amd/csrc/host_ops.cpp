@@ -1,5 +1,6 @@
 // The host path of the Python API's hot calls (xpu_kernels.int8 linear, ffn, the
-// backward's products and the quantizer) as a CPython extension: argument
+// backward's products and the quantizer; xpu_kernels.mxfp4 and moe without gradients) as
+// a CPython extension: argument
 // checks, the packed weight's lookup, allocations and the library call in
 // native code.  In Python these cost more than the small calls' kernels: linear
 // at 16 x 4096 x 4096 took 17.6 us of host time for 8.5 us of GPU work, 6.9 of
@@ -54,8 +55,18 @@ struct Library {
     decltype(&xpuint8_convrot_quantize_stream) quantize;
     decltype(&xpuint8_linear_acc_packed_stream) linear_acc;
     decltype(&xpuint8_linear_dx_int8_reads_packed) dx_reads_packed;
+    decltype(&xpuint8_mxfp4_quantize_stream) mx_quantize;
+    decltype(&xpuint8_mxfp4_dequantize_stream) mx_dequantize;
+    decltype(&xpuint8_mxfp4_linear_workspace_size) mx_linear_size;
+    decltype(&xpuint8_mxfp4_linear_stream) mx_linear;
+    decltype(&xpuint8_mxfp4_grouped_linear_workspace_size) mx_grouped_size;
+    decltype(&xpuint8_mxfp4_grouped_linear_stream) mx_grouped;
+    decltype(&xpuint8_moe_sort_workspace_size) moe_sort_size;
+    decltype(&xpuint8_moe_sort_stream) moe_sort;
+    decltype(&xpuint8_moe_dispatch_stream) moe_dispatch;
+    decltype(&xpuint8_moe_combine_stream) moe_combine;
 };
-constexpr int kEntries = 18;
+constexpr int kEntries = 28;
 static_assert(sizeof(Library) == kEntries * sizeof(void*), "one address per entry");
 
 Library g_lib;
@@ -459,6 +470,237 @@ PyObject* host_quantize(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
+// ------------------------------------------------- MXFP4 and mixture of experts
+// the library's number of a floating element type, -1 for any other
+int32_t type_of(const Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kBFloat16: return 0;
+        case at::kHalf: return 1;
+        case at::kFloat: return 2;
+        default: return -1;
+    }
+}
+const at::ScalarType kTypes[3] = {at::kBFloat16, at::kHalf, at::kFloat};
+
+// a plain tensor (see plain) of bf16, fp16 or fp32
+const Tensor* floating(PyObject* o) {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const Tensor& t = THPVariable_Unpack(o);
+    return t.defined() && type_of(t) >= 0 ? plain(o, t.scalar_type()) : nullptr;
+}
+const Tensor* on(const Tensor* t, const Tensor& like) {
+    return t && t->device() == like.device() ? t : nullptr;
+}
+int64_t scale_width(int64_t k) { return (k + 511) / 512 * 16; }
+
+// codes and scales that belong together
+bool mx_pair(PyObject* c, PyObject* s, const Tensor*& codes, const Tensor*& scales) {
+    codes = plain(c, at::kByte);
+    scales = codes ? on(plain(s, at::kByte), *codes) : nullptr;
+    if (!scales || codes->dim() < 1 || codes->dim() != scales->dim()) return false;
+    const int64_t d = codes->dim() - 1, k = codes->size(d) * 2;
+    return codes->sizes().slice(0, d) == scales->sizes().slice(0, d) && k % 32 == 0 &&
+           scales->size(d) == scale_width(k);
+}
+
+// a moe.Routing (the caller has seen that it is one)
+struct Routing {
+    const Tensor *order, *position, *rows, *offsets;
+};
+bool routing_arg(PyObject* o, const Tensor& like, Routing& r) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+    r.order = on(plain(PyTuple_GET_ITEM(o, 0), at::kInt), like);
+    r.position = on(plain(PyTuple_GET_ITEM(o, 1), at::kInt), like);
+    r.rows = on(plain(PyTuple_GET_ITEM(o, 2), at::kInt), like);
+    r.offsets = on(plain(PyTuple_GET_ITEM(o, 3), at::kInt), like);
+    return r.order && r.position && r.rows && r.offsets && r.position->dim() == 2 &&
+           r.position->numel() == r.order->numel() && r.rows->numel() == r.order->numel() &&
+           r.offsets->numel() >= 2;
+}
+const int32_t* ints(const Tensor* t) { return static_cast<const int32_t*>(t->data_ptr()); }
+int32_t* ints(Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+const uint8_t* bytes(const Tensor* t) { return static_cast<const uint8_t*>(t->data_ptr()); }
+
+// mx_quantize(x): mxfp4.quantize
+PyObject* host_mx_quantize(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 1, [&]() -> PyObject* {
+        const Tensor* x = floating(a[0]);
+        if (!x || x->dim() < 1 || x->size(-1) % 32 != 0) Py_RETURN_NONE;
+        const int64_t k = x->size(-1), m = x->numel() / k;
+        const void* st = current_stream(*x);
+        Tensor c, s;
+        call("mxfp4.quantize", [&] {
+            c = empty(with_last(*x, k / 2), at::kByte, *x);
+            s = empty(with_last(*x, scale_width(k)), at::kByte, *x);
+            return g_lib.mx_quantize(st, x->data_ptr(), type_of(*x), k,
+                                     static_cast<uint8_t*>(c.data_ptr()),
+                                     static_cast<uint8_t*>(s.data_ptr()), m, k);
+        });
+        return pair(c, s);
+    });
+}
+
+// mx_dequantize(codes, scales, type): mxfp4.dequantize
+PyObject* host_mx_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 3, [&]() -> PyObject* {
+        const Tensor *c, *s;
+        const long type = PyLong_AsLong(a[2]);
+        if (type == -1 && PyErr_Occurred()) throw python_error();
+        if (type < 0 || type > 2 || !mx_pair(a[0], a[1], c, s)) Py_RETURN_NONE;
+        const int64_t k = c->size(-1) * 2, m = c->numel() / (k / 2);
+        const void* st = current_stream(*c);
+        Tensor out;
+        call("mxfp4.dequantize", [&] {
+            out = empty(with_last(*c, k), kTypes[type], *c);
+            return g_lib.mx_dequantize(st, bytes(c), bytes(s), out.data_ptr(), int32_t(type), m, k);
+        });
+        return THPVariable_Wrap(out);
+    });
+}
+
+// mx_linear(x, codes, scales, bias): mxfp4.linear without a gradient
+PyObject* host_mx_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 4, [&]() -> PyObject* {
+        const Tensor* x = floating(a[0]);
+        const Tensor *c, *s, *b = nullptr;
+        if (!x || x->dim() < 1 || !mx_pair(a[1], a[2], c, s) || c->dim() != 2 || !on(c, *x))
+            Py_RETURN_NONE;
+        const int64_t n = c->size(0), k = c->size(1) * 2, m = x->numel() / x->size(-1);
+        if (x->size(-1) != k) Py_RETURN_NONE;
+        if (a[3] != Py_None) {
+            b = on(floating(a[3]), *x);
+            if (!b || b->dim() != 1 || b->numel() != n) Py_RETURN_NONE;
+        }
+        const int64_t need = g_lib.mx_linear_size(m, n, k);
+        if (need < 0) fail("mxfp4.linear");
+        const void* st = current_stream(*x);
+        Tensor work, y;
+        call("mxfp4.linear", [&] {
+            if (need > 0) work = workspace(need, *x);
+            y = empty(with_last(*x, n), x->scalar_type(), *x);
+            return g_lib.mx_linear(st, x->data_ptr(), type_of(*x), k, bytes(c), bytes(s),
+                                   b ? b->data_ptr() : nullptr, b ? type_of(*b) : 0, y.data_ptr(),
+                                   m, n, k, need > 0 ? work.data_ptr() : nullptr, need);
+        });
+        return THPVariable_Wrap(y);
+    });
+}
+
+// mx_grouped(x, codes, scales, routing, gather): mxfp4.grouped_linear without a gradient
+PyObject* host_mx_grouped(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 5, [&]() -> PyObject* {
+        const Tensor* x = floating(a[0]);
+        const Tensor *c, *s;
+        Routing r;
+        if (!x || x->dim() != 2 || !mx_pair(a[1], a[2], c, s) || c->dim() != 3 || !on(c, *x) ||
+            !routing_arg(a[3], *x, r))
+            Py_RETURN_NONE;
+        const int gather = PyObject_IsTrue(a[4]);
+        if (gather < 0) throw python_error();
+        const int64_t e = c->size(0), n = c->size(1), k = c->size(2) * 2, t = x->size(0);
+        const int64_t rows = r.order->numel();
+        if (x->size(1) != k || r.offsets->numel() != e + 1 ||
+            t != (gather ? r.position->size(0) : rows))
+            Py_RETURN_NONE;
+        const int64_t need = g_lib.mx_grouped_size(rows, t, e, n, k);
+        if (need < 0) fail("mxfp4.grouped_linear");
+        const void* st = current_stream(*x);
+        Tensor work, y;
+        call("mxfp4.grouped_linear", [&] {
+            if (need > 0) work = workspace(need, *x);
+            y = empty({rows, n}, x->scalar_type(), *x);
+            return g_lib.mx_grouped(st, x->data_ptr(), type_of(*x), k,
+                                    gather ? ints(r.rows) : nullptr, t, bytes(c), bytes(s),
+                                    ints(r.offsets), e, y.data_ptr(), rows, n, k,
+                                    need > 0 ? work.data_ptr() : nullptr, need);
+        });
+        return THPVariable_Wrap(y);
+    });
+}
+
+// moe_sort(ids, n_experts): the four tensors of moe.sort's Routing
+PyObject* host_moe_sort(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 2, [&]() -> PyObject* {
+        const Tensor* ids = plain(a[0], at::kInt);
+        const bool wide = !ids;
+        if (wide) ids = plain(a[0], at::kLong);
+        if (!ids || ids->dim() != 2 || !PyLong_CheckExact(a[1])) Py_RETURN_NONE;
+        const long long e = PyLong_AsLongLong(a[1]);
+        if (e == -1 && PyErr_Occurred()) throw python_error();
+        if (e < 1 || e > 1024) Py_RETURN_NONE;
+        const int64_t t = ids->size(0), top = ids->size(1);
+        const int64_t need = g_lib.moe_sort_size(t, top, e);
+        if (need < 0) fail("moe.sort");
+        const void* st = current_stream(*ids);
+        Tensor work, order, position, rows, offsets;
+        call("moe.sort", [&] {
+            if (need > 0) work = workspace(need, *ids);
+            order = empty({t * top}, at::kInt, *ids);
+            position = empty({t, top}, at::kInt, *ids);
+            rows = empty({t * top}, at::kInt, *ids);
+            offsets = empty({e + 1}, at::kInt, *ids);
+            return g_lib.moe_sort(st, ids->data_ptr(), wide, ints(order), ints(position),
+                                  ints(rows), ints(offsets), t, top, e,
+                                  need > 0 ? work.data_ptr() : nullptr, need);
+        });
+        PyObject* out = PyTuple_New(4);
+        if (!out) throw python_error();
+        const Tensor all[4] = {order, position, rows, offsets};
+        for (int i = 0; i < 4; ++i) {
+            PyObject* o = THPVariable_Wrap(all[i]);
+            if (!o) {
+                Py_DECREF(out);
+                throw python_error();
+            }
+            PyTuple_SET_ITEM(out, i, o);
+        }
+        return out;
+    });
+}
+
+// moe_dispatch(x, routing): moe.dispatch without a gradient
+PyObject* host_moe_dispatch(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 2, [&]() -> PyObject* {
+        const Tensor* x = floating(a[0]);
+        Routing r;
+        if (!x || x->dim() != 2 || !routing_arg(a[1], *x, r) || x->size(0) != r.position->size(0))
+            Py_RETURN_NONE;
+        const int64_t t = x->size(0), d = x->size(1), top = r.position->size(1);
+        const void* st = current_stream(*x);
+        Tensor out;
+        call("moe.dispatch", [&] {
+            out = empty({t * top, d}, x->scalar_type(), *x);
+            return g_lib.moe_dispatch(st, x->data_ptr(), type_of(*x), d, ints(r.position),
+                                      ints(r.offsets), out.data_ptr(), t, top,
+                                      r.offsets->numel() - 1, d);
+        });
+        return THPVariable_Wrap(out);
+    });
+}
+
+// moe_combine(z, routing, weights): moe.combine without a gradient, fp32 weights
+PyObject* host_moe_combine(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 3, [&]() -> PyObject* {
+        const Tensor* z = floating(a[0]);
+        Routing r;
+        if (!z || z->dim() != 2 || !routing_arg(a[1], *z, r)) Py_RETURN_NONE;
+        const Tensor* w = on(plain(a[2], at::kFloat), *z);
+        const int64_t t = r.position->size(0), top = r.position->size(1), d = z->size(1);
+        if (!w || w->dim() != 2 || w->size(0) != t || w->size(1) != top || z->size(0) != t * top)
+            Py_RETURN_NONE;
+        const void* st = current_stream(*z);
+        Tensor out;
+        call("moe.combine", [&] {
+            out = empty({t, d}, z->scalar_type(), *z);
+            return g_lib.moe_combine(st, z->data_ptr(), type_of(*z), d, ints(r.position),
+                                     ints(r.offsets), static_cast<const float*>(w->data_ptr()),
+                                     out.data_ptr(), type_of(*z), t, top,
+                                     r.offsets->numel() - 1, d);
+        });
+        return THPVariable_Wrap(out);
+    });
+}
+
 // bind(addresses, raw_stream, packed): the library's entry points in Library's
 // order, the current-stream accessor and the packed-weight registry
 PyObject* host_bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
@@ -492,6 +734,13 @@ PyMethodDef kMethods[] = {XPU_HOST("bind", host_bind),
                           XPU_HOST("linear_dw", host_linear_dw),
                           XPU_HOST("column_sum", host_column_sum),
                           XPU_HOST("quantize", host_quantize),
+                          XPU_HOST("mx_quantize", host_mx_quantize),
+                          XPU_HOST("mx_dequantize", host_mx_dequantize),
+                          XPU_HOST("mx_linear", host_mx_linear),
+                          XPU_HOST("mx_grouped", host_mx_grouped),
+                          XPU_HOST("moe_sort", host_moe_sort),
+                          XPU_HOST("moe_dispatch", host_moe_dispatch),
+                          XPU_HOST("moe_combine", host_moe_combine),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host",
                        "The int8 API's hot calls in native code (see host_ops.cpp).", -1, kMethods};

@@ -8,14 +8,10 @@
 // bf16, or 2 (fp16) or 3 (fp32) bf16 pieces whose sum is dy exactly (an fp16 value
 // has 11 significant bits, an fp32 one 24, a bf16 one 8; mx4_split): the pieces lie
 // side by side and the contraction runs over the weight's rows once for each.
-#include "mx4_groups.hpp"
+#include "mx4_tiles.hpp"
 
 namespace xpuint8 {
 namespace {
-
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef short v8s __attribute__((ext_vector_type(8)));
 
 // ------------------------------------------------------------------- split
 // dy [R, N] as PIECES bf16 pieces, each of `width` columns (zeros past N)
@@ -48,149 +44,242 @@ __global__ __launch_bounds__(256) void mx4_split_kernel(const char* __restrict__
 }
 
 // ------------------------------------------------------------------- tiles
-// 128 x 128 tiles of dx by a block of 4 waves in 2 x 2, 64 contraction rows a step.
-// dy's 128 bytes of a row come by direct loads (chunk c of row r at c ^ ((r >> 1) & 7));
-// the weight's 64 rows of 4 blocks one block a thread, which writes the 32 values
-// as they lie, 256 bytes a row, for the transposing read ds_read_b64_tr_b16: in each
-// group of 16 lanes lane j gives the address of 4 consecutive bf16 and lane i = 4a + b
-// receives element b of the vectors of lanes a, a + 4, a + 8, a + 12, so that lanes
-// that point at row j / 4, columns 4 (j % 4) of a 4 x 16 block receive its columns.
-// Two such reads are a lane's 8 consecutive n of one k.  The 32-byte slot s of row n
-// sits at s ^ ((n & 3) | ((n >> 3) & 1) << 2): the 16 rows of one read then cover
-// the banks twice, the least for its 512 bytes.
-constexpr int kBM = 128, kBK = 128, kStep = 64;
+// BM x BK tiles of dx by a block of 4 waves in 2 x 2 (a wave every other 16 rows, one
+// half of the columns), 64 contraction rows a stage (two MFMAs of each block), two LDS
+// slots.  While a stage's first half runs, a wave reads the second half's fragments; one
+// wait and barrier then mean that every wave has read the stage, and that the next one
+// is in; while the second half runs, it reads the next stage's first fragments, refills
+// the slot with dy by direct loads, and writes the weight's rows there as bf16, which it
+// has loaded a stage earlier (a thread BK / 4 consecutive values' codes and scales).
+// (A ring of 32-row steps with a load four steps ahead, as the forward product's, is
+// slower at 128 x 128: dy's rows then come in 64-byte pieces, and the L2's requests, not
+// its bytes, bound such tiles; 16380 x 2816 -> 2048 in 32 groups 290 us.)
+//
+// dy's 128 bytes of a row: chunk c (16 bytes) at c ^ ((row >> 1) & 7).  The weight's rows
+// lie as they come, 2 BK bytes each, for the transposing read ds_read_b64_tr_b16: in
+// each group of 16 lanes lane j gives the address of 4 consecutive bf16 and lane i = 4a + b
+// receives element b of the vectors of lanes a, a + 4, a + 8, a + 12, so that lanes which
+// point at row j / 4, columns 4 (j % 4) of a 4 x 16 block receive its columns.  Two such
+// reads are a lane's 8 consecutive n of one k.  The 32-byte piece p of row n sits at
+// p ^ ((n & 3) | ((n >> 3) & 1) << 2): the 16 rows of one read then cover the banks
+// twice, the least for its 512 bytes.
+typedef int v2i __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ int slot_of(int n, int s) { return s ^ ((n & 3) | (((n >> 3) & 1) << 2)); }
-
-__device__ __forceinline__ v4s read_tr(uint32_t at) {
-    v4s v = {};
-#if defined(__HIP_DEVICE_COMPILE__)
-    v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(uintptr_t(at)));
-#endif
-    return v;
+__device__ __forceinline__ v2i read_tr(uint32_t addr, int off) {
+    v2i r;
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "n"(off));
+    return r;
 }
 
-template <int T>
-__global__ __launch_bounds__(256) void mx4_dx_kernel(const uint16_t* __restrict__ dy, int64_t ldy,
-                                                     int pieces, int width, Weight w,
-                                                     const int* __restrict__ offsets, int E,
-                                                     Out out, int tiles_k) {
-    constexpr int DY = kBM * 128, WT = kStep * 256, STAGE = DY + WT;
-    constexpr int TM = 4, TK = 4;
+// blocks B0 .. B3 += W blocks (8 bf16 a lane) * one dy block
+#define XPU_ONE_BF16(W, LO, HI)                                                                 \
+    "v_mfma_f32_16x16x32_bf16 a[%" #LO ":%" #HI "], %" #W ", %4, a[%" #LO ":%" #HI "]\n\t"
+#define XPU_BF16_4(CLOBBERS)                                                                    \
+    asm volatile(XPU_ONE_BF16(0, 5, 6) XPU_ONE_BF16(1, 7, 8) XPU_ONE_BF16(2, 9, 10)             \
+                 XPU_ONE_BF16(3, 11, 12)                                                        \
+                 ::"v"(w0), "v"(w1), "v"(w2), "v"(w3), "v"(x), "n"(4 * B0), "n"(4 * B0 + 3),    \
+                 "n"(4 * B1), "n"(4 * B1 + 3), "n"(4 * B2), "n"(4 * B2 + 3), "n"(4 * B3),       \
+                 "n"(4 * B3 + 3)                                                                \
+                 : CLOBBERS)
+template <int COUNT, int B0, int B1, int B2, int B3>
+__device__ __forceinline__ void acc_bf16_4(const v4i& w0, const v4i& w1, const v4i& w2,
+                                           const v4i& w3, const v4i& x) {
+    static_assert(COUNT == 64 || COUNT == 256, "a list of registers");
+    if constexpr (COUNT == 64) XPU_BF16_4(XPU_A64);
+    else XPU_BF16_4(XPU_A256);
+}
+
+template <int BM, int BK>
+__global__ __launch_bounds__(256, BM * BK > 128 * 128 ? 1 : 2) void mx4_dx_kernel(
+    const uint16_t* __restrict__ dy, int64_t ldy, int pieces, int width, Weight w,
+    const int* __restrict__ offsets, int E, Out out, int type, int tiles_m, int tiles_k) {
+    constexpr int TM = BM / 32, TK = BK / 32;             // MFMA blocks of a wave
+    constexpr int DY = BM * 128, WROW = 2 * BK, WT = 64 * WROW, STAGE = DY + WT;
+    constexpr int PX = BM / 32;                           // dy loads a wave a stage
+    constexpr int NB = BK / 128;                          // weight blocks a thread a stage
+    constexpr int ACC = 4 * TM * TK;                      // block (a, b) is number a * TM + b
     __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const int wm = wave >> 1, wk = wave & 1;
+    int tm, tk;
+    if (!tile_of(blockIdx.x, tiles_m, tiles_k, tm, tk)) return;
     RowTile t;
-    if (!row_tile<kBM>(offsets, E, out.R, blockIdx.x / tiles_k, t)) return;
-    const int k0 = (blockIdx.x % tiles_k) * kBK;
+    if (!row_tile<BM>(offsets, E, out.R, tm, t)) return;
+    const int k0 = tk * BK;
     if (t.e == E) {
-        const v4f zero = {0.f, 0.f, 0.f, 0.f};
-        for (int i = threadIdx.x; i < kBM * (kBK / 4); i += 256) {
-            const int row = t.row + i / (kBK / 4);
-            if (row < t.end) store4<T>(out, row, k0 + 4 * (i % (kBK / 4)), zero);
-        }
+        zero_rows<BM, BK>(out, type, t, k0);
         return;
     }
-    const int steps_piece = (width + kStep - 1) / kStep, steps = steps_piece * pieces;
-    const char* const dyb = reinterpret_cast<const char*>(dy);
-    auto issue_dy = [&](int s) {
+    // contraction stages: a piece's `width` columns of dy against the weight's rows, once
+    // for each piece; in a piece's last stage the weight's rows past N are zeros
+    const int per_piece = (width + 63) / 64, stages = per_piece * pieces;
+    const uint8_t* const dybase = reinterpret_cast<const uint8_t*>(dy + int64_t(t.row) * ldy);
+    const int lr = lane >> 3;
+    const int c8 = ((lane & 7) ^ (((wave * 8 + lr) >> 1) & 7)) * 8;   // the lane's chunk, first column
+    uint64_t ady[PX];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int b = (wave + 4 * i) * 8, j = b + lane / 8;
-            const int c = (lane & 7) ^ ((j >> 1) & 7);
-            const int64_t row = min(t.row + j, t.end - 1);
-            const uint8_t* p = reinterpret_cast<const uint8_t*>(dyb + row * ldy * 2) + int64_t(s) * 128 + c * 16;
-            // past the row's end in its last step (pieces are padded to whole steps)
-            if (pieces == 1 && s * kStep + c * 8 >= width) p = g_zero_line;
-            dma16(p, smem + (s & 1) * STAGE + b * 128);
-        }
+    for (int i = 0; i < PX; ++i)
+        ady[i] = uint64_t(min(t.row + (wave + 4 * i) * 8 + lr, t.end - 1) - t.row) * uint64_t(ldy * 2) +
+                 c8 * 2;
+    // (one piece may end inside a stage: chunks past it come from zeros)
+    const uint8_t* const zeros = scalar(g_zero_line);
+    const int past = pieces == 1 ? width - c8 : 0x7FFFFFFF;
+    auto issue_dy = [&](int slot, int s, int i) {
+        const uint8_t* p = scalar(dybase + int64_t(s) * 128) + ady[i];
+        if (s * 64 >= past) p = zeros;
+        dma16(p, smem + slot * STAGE + (wave + 4 * i) * 1024);
     };
-    const int nr = threadIdx.x >> 2, cb = threadIdx.x & 3;       // this thread's weight block
-    const bool kin = k0 + cb * 32 < w.K;
-    uint4 codes;
-    uint32_t scale;
-    auto load_w = [&](int s) {
-        const int n = (s % steps_piece) * kStep + nr;
-        codes = make_uint4(0, 0, 0, 0);
-        scale = 0;
-        if (n < w.N && kin) {
-            const int64_t row = int64_t(t.e) * w.N + n;
-            codes = *reinterpret_cast<const uint4*>(w.codes + row * (w.K / 2) + k0 / 2 + cb * 16);
-            scale = w.scales[row * w.SW + k0 / 32 + cb];
-        }
-    };
-    auto put_w = [&](int s) {
-        uint8_t* const row = smem + (s & 1) * STAGE + DY + nr * 256;
-        const uint32_t c[4] = {codes.x, codes.y, codes.z, codes.w};
-        const float sc = __uint_as_float(scale << 23);
+    // this thread's part of the weight's rows: NB blocks of row nr
+    const int nr = threadIdx.x >> 2, part = (threadIdx.x & 3) * NB;
+    uint4 codes[NB];
+    uint32_t scale[NB];
+    int un = 0;                                           // the piece's stage that is loaded next
+    const uint8_t* const wbase = w.codes + int64_t(t.e) * w.N * (w.K / 2);
+    const uint8_t* const wsbase = w.scales + int64_t(t.e) * w.N * w.SW;
+    auto load_w = [&]() {
+        const int n = un * 64 + nr;
+        const int64_t row = min(n, w.N - 1);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            uint4 v;
-            v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[q], sc, 0));
-            v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[q], sc, 1));
-            v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[q], sc, 2));
-            v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[q], sc, 3));
-            *reinterpret_cast<uint4*>(row + slot_of(nr, 2 * cb + q / 2) * 32 + (q & 1) * 16) = v;
-        }
-    };
-    v4f acc[TK][TM];
-#pragma unroll
-    for (int a = 0; a < TK; ++a)
-#pragma unroll
-        for (int b = 0; b < TM; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
-    const int drow = wm * 64 + r;
-    issue_dy(0);
-    load_w(0);
-    put_w(0);
-    for (int s = 0; s < steps; ++s) {
-        wait_loads();
-        __syncthreads();                                  // step s is in, s - 1 is read
-        if (s + 1 < steps) {
-            issue_dy(s + 1);
-            load_w(s + 1);
-        }
-        const uint8_t* const st = smem + (s & 1) * STAGE;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            v8s yf[TM];
-            v8bf wf[TK];
-            const int pos = ((4 * h + g) ^ ((r >> 1) & 7)) * 16;
-#pragma unroll
-            for (int b = 0; b < TM; ++b) yf[b] = *reinterpret_cast<const v8s*>(st + (drow + 16 * b) * 128 + pos);
-#pragma unroll
-            for (int a = 0; a < TK; ++a) {
-                v4s part[2];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int n = 32 * h + 8 * g + 4 * q + (r >> 2);
-                    part[q] = read_tr(lds_addr(st + DY + n * 256 + slot_of(n, wk * 4 + a) * 32 + (r & 3) * 8));
-                }
-                const v8s v = {part[0][0], part[0][1], part[0][2], part[0][3],
-                               part[1][0], part[1][1], part[1][2], part[1][3]};
-                wf[a] = __builtin_bit_cast(v8bf, v);
+        for (int i = 0; i < NB; ++i) {
+            const int kb = min(k0 / 32 + part + i, w.K / 32 - 1);     // (columns past K are not stored)
+            codes[i] = *reinterpret_cast<const uint4*>(wbase + row * (w.K / 2) + kb * 16);
+            scale[i] = wsbase[row * w.SW + kb];
+            if (n >= w.N) {
+                codes[i] = make_uint4(0, 0, 0, 0);
+                scale[i] = 0;
             }
-#pragma unroll
-            for (int b = 0; b < TM; ++b)
-#pragma unroll
-                for (int a = 0; a < TK; ++a)
-                    acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        wf[a], __builtin_bit_cast(v8bf, yf[b]), acc[a][b], 0, 0, 0);
         }
-        if (s + 1 < steps) put_w(s + 1);                  // (the slot that step s - 1 had)
+        if (++un == per_piece) un = 0;
+    };
+    const int fn = (nr & 3) | (((nr >> 3) & 1) << 2);
+    const uint32_t sbase = lds_addr(smem);
+    // 8 of the values (dword q of the NB * 4) to the slot at LDS offset `slot`
+    uint32_t wput[NB][2];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            wput[i][h] = sbase + DY + nr * WROW + ((2 * (part + i) + h) ^ fn) * 32;
+    auto put_w = [&](uint32_t slot, int q) {
+        const int i = q >> 2, h = (q >> 1) & 1;
+        const float sc = __uint_as_float(scale[i] << 23);
+        const uint32_t c = (q & 3) == 0 ? codes[i].x : (q & 3) == 1 ? codes[i].y : (q & 3) == 2 ? codes[i].z : codes[i].w;
+        const v4i v = {__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 0)),
+                       __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1)),
+                       __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 2)),
+                       __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 3))};
+        asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(wput[i][h] + slot), "v"(v), "n"(16 * (q & 1)) : "memory");
+    };
+    auto put_all = [&](uint32_t slot) {
+#pragma unroll
+        for (int q = 0; q < 4 * NB; ++q) put_w(slot, q);
+    };
+    // fragments of half H of a stage: 32 contraction rows
+    const uint32_t pos = (g ^ ((r >> 1) & 7)) * 16;       // chunk 4 H + g is at pos ^ (64 H)
+    const uint32_t yat = sbase + (wm * 16 + r) * 128 + pos;
+    const int fr = (r >> 2) | ((g & 1) << 2);             // of the rows that a lane addresses
+    const uint32_t wrow = sbase + DY + (8 * g + (r >> 2)) * WROW + (r & 3) * 8;
+    v4i yf[2][TM];
+    v2i wl[2][TK], wh[2][TK];
+    auto read_y = [&](uint32_t slot, auto H, auto I) {
+        constexpr int h = decltype(H)::value, i = decltype(I)::value;
+        yf[h][i] = read16((yat ^ (64 * h)) + slot, i * 32 * 128);
+    };
+    auto read_w = [&](uint32_t slot, auto H, auto I) {
+        constexpr int h = decltype(H)::value, i = decltype(I)::value;
+        const uint32_t at = wrow + slot + ((wk * TK + i) ^ fr) * 32;
+        wl[h][i] = read_tr(at, h * 32 * WROW);
+        wh[h][i] = read_tr(at, h * 32 * WROW + 4 * WROW);
+    };
+    using H0 = std::integral_constant<int, 0>;
+    using H1 = std::integral_constant<int, 1>;
+    // column b of half h
+    auto column = [&](auto H, auto B, const v4i (&wf)[TK]) {
+        constexpr int h = decltype(H)::value, b = decltype(B)::value;
+        each<TK / 4>([&](auto A) {
+            constexpr int a = 4 * decltype(A)::value;
+            acc_bf16_4<ACC, a * TM + b, (a + 1) * TM + b, (a + 2) * TM + b, (a + 3) * TM + b>(
+                wf[a], wf[a + 1], wf[a + 2], wf[a + 3], yf[h][b]);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    load_w();
+#pragma unroll
+    for (int i = 0; i < PX; ++i) issue_dy(0, 0, i);
+    each<TM * TK>([&](auto I) { acc_set<ACC, decltype(I)::value>(v4f{0.f, 0.f, 0.f, 0.f}); });
+    put_all(0);
+    if (stages > 1) {
+        load_w();
+#pragma unroll
+        for (int i = 0; i < PX; ++i) issue_dy(1, 1, i);
+        put_all(STAGE);
+        load_w();
     }
+    wait_vm<0>();
+    lds_done();
+    block_barrier();
+    each<TM>([&](auto I) { read_y(0, H0{}, I); });
+    each<TK>([&](auto I) { read_w(0, H0{}, I); });
+    lds_done();
+    landed(yf[0]); landed(wl[0]); landed(wh[0]);
+#pragma clang loop unroll(disable)
+    for (int s = 0; s < stages; ++s) {
+        const uint32_t here = (s & 1) * STAGE, next = STAGE - here;
+        {
+            v4i wf[TK];
 #pragma unroll
-    for (int a = 0; a < TK; ++a)
-#pragma unroll
-        for (int b = 0; b < TM; ++b) {
-            const int row = t.row + drow + 16 * b;
-            if (row < t.end) store4<T>(out, row, k0 + wk * 64 + 16 * a + 4 * g, acc[a][b]);
+            for (int a = 0; a < TK; ++a) wf[a] = v4i{wl[0][a][0], wl[0][a][1], wh[0][a][0], wh[0][a][1]};
+            each<TM>([&](auto B) {
+                constexpr int b = decltype(B)::value;
+                read_y(here, H1{}, B);
+                each<TK / TM>([&](auto I) {
+                    read_w(here, H1{}, std::integral_constant<int, b * (TK / TM) + decltype(I)::value>{});
+                });
+                column(H0{}, B, wf);
+            });
         }
+        // the second half's fragments, and the next stage: dy's loads and the weight's
+        // writes of every wave
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        landed(yf[1]); landed(wl[1]); landed(wh[1]);
+        block_barrier();
+        {
+            v4i wf[TK];
+#pragma unroll
+            for (int a = 0; a < TK; ++a) wf[a] = v4i{wl[1][a][0], wl[1][a][1], wh[1][a][0], wh[1][a][1]};
+            const bool more = s + 2 < stages;
+            if (more) {
+                put_all(here);
+                load_w();
+            }
+            // (past the last stage the reads find what the slot held, and go unused)
+            each<TM>([&](auto B) {
+                constexpr int b = decltype(B)::value;
+                read_y(next, H0{}, B);
+                each<TK / TM>([&](auto I) {
+                    read_w(next, H0{}, std::integral_constant<int, b * (TK / TM) + decltype(I)::value>{});
+                });
+                if (more) {
+#pragma unroll
+                    for (int i = b * PX / TM; i < (b + 1) * PX / TM; ++i) issue_dy(s & 1, s + 2, i);
+                }
+                column(H1{}, B, wf);
+            });
+        }
+        lds_done();
+        landed(yf[0]); landed(wl[0]); landed(wh[0]);
+    }
+    wait_vm<0>();                                         // (the last load_w may be on its way)
+    block_barrier();                                      // every wave has read its last stage
+    store_tile<TM, TK>(out, type, t.row + 16 * wm, t.end, k0 + wk * (BK / 2),
+                       reinterpret_cast<float*>(smem) + wave * 16 * (BK / 2));
 }
 
 }  // namespace
 
-int64_t mx4_split_width(int64_t N) { return (N + kStep - 1) / kStep * kStep; }
+int64_t mx4_split_width(int64_t N) { return (N + 63) / 64 * 64; }
 int mx4_split_pieces(int type) { return type == kBf16 ? 1 : type == kF16 ? 2 : 3; }
 
 hipError_t mx4_split(hipStream_t st, const void* dy, int type, int64_t ldy, void* out, int64_t R,
@@ -206,6 +295,28 @@ hipError_t mx4_split(hipStream_t st, const void* dy, int type, int64_t ldy, void
     return hipGetLastError();
 }
 
+namespace {
+
+// Whether 256 x 256 tiles (one block a CU) are faster than 128 x 128 (two), by the
+// times that a round of either takes: 8192^3 1004 against 1140 us, 4096^3 131 against
+// 149; 4096 x 1280 -> 5120 94 against 74, 16380 x 2816 -> 2048 in 32 groups the same.
+bool large_dx_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
+    const double stages = double((N + 63) / 64);
+    auto tiles = [&](int64_t b) {                          // (a group's last tile half full)
+        const int64_t tm = grouped ? R / b + std::min<int64_t>(E, R) / 2 + 1 : (R + b - 1) / b;
+        return tm * ((K + b - 1) / b);
+    };
+    const int64_t cus = device_cus();
+    const int64_t t128 = tiles(128), t256 = tiles(256);
+    const double large = double((t256 + cus - 1) / cus) * (8.0 + 1.95 * stages);
+    const double small = double(t128 / (2 * cus)) * (4.0 + 1.1 * stages) +
+                         (t128 % (2 * cus) > cus ? 4.0 + 1.1 * stages
+                          : t128 % (2 * cus) > 0 ? 4.0 + 0.65 * stages : 0.0);
+    return large < small;
+}
+
+}  // namespace
+
 hipError_t mx4_dx(hipStream_t st, const void* dy, int64_t ldy, int pieces, const uint8_t* wc,
                   const uint8_t* ws, const int* offsets, int E, void* dx, int type, int64_t R,
                   int N, int K) {
@@ -213,14 +324,17 @@ hipError_t mx4_dx(hipStream_t st, const void* dy, int64_t ldy, int pieces, const
     const Out o = make_out(dx, type, nullptr, 0, R, K);
     // pieces lie side by side, mx4_split_width(N) columns each; one piece may end early
     const int width = pieces == 1 ? N : int(mx4_split_width(N));
-    const int tiles_k = (K + kBK - 1) / kBK;
-    const int64_t tiles = most_tiles(offsets != nullptr, R, E, kBM) * tiles_k;
-    by_type(type, [&](auto T) {
-        constexpr int t = decltype(T)::value;
-        hipLaunchKernelGGL((mx4_dx_kernel<t>), dim3(unsigned(tiles)), dim3(256), 0, st,
-                           static_cast<const uint16_t*>(dy), ldy, pieces, width, w, offsets, E, o,
-                           tiles_k);
-    });
+    auto go = [&](auto B) {
+        constexpr int b = decltype(B)::value;
+        const int tiles_k = (K + b - 1) / b;
+        const int tiles_m = int(most_tiles(offsets != nullptr, R, E, b));
+        hipLaunchKernelGGL((mx4_dx_kernel<b, b>),
+                           dim3(unsigned((int64_t(tiles_m) * tiles_k + 7) / 8 * 8)), dim3(256), 0,
+                           st, static_cast<const uint16_t*>(dy), ldy, pieces, width, w, offsets, E,
+                           o, type, tiles_m, tiles_k);
+    };
+    if (large_dx_tiles(offsets != nullptr, R, E, N, K)) go(std::integral_constant<int, 256>{});
+    else go(std::integral_constant<int, 128>{});
     return hipGetLastError();
 }
 

@@ -15,7 +15,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "mx4_groups.hpp"
+#include "mx4_tiles.hpp"
 
 namespace xpuint8 {
 namespace {
@@ -113,7 +113,8 @@ __global__ __launch_bounds__(NW * 64) void mx4_skinny_kernel(
 }
 
 // -------------------------------------------------------------------- tiles
-// BM x BN tiles of y by a block of 4 waves in 2 x 2, x already quantized.  K in
+// BM x BN tiles of y by a block of 4 waves in 2 x 2 (a wave every other 16 rows, one half
+// of the columns), x already quantized.  K in
 // steps of 128 values, 64 bytes of codes a row and one MFMA of each block, through
 // a ring of four LDS slots that direct global->LDS loads fill four steps ahead.
 // During step t a wave runs its MFMAs on one set of fragments, reads step t + 1's into
@@ -136,36 +137,6 @@ __global__ __launch_bounds__(NW * 64) void mx4_skinny_kernel(
 // The fragment reads are inline assembly (with the builtins the compiler waits for
 // every direct load before each LDS read); nothing is in flight over a loop edge:
 // each step ends with a wait that redefines what it read.
-__device__ __forceinline__ v4i read16(uint32_t addr, int off) {
-    v4i r;
-    asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "n"(off));
-    return r;
-}
-__device__ __forceinline__ int read4(uint32_t addr, int off) {
-    int r;
-    asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "n"(off));
-    return r;
-}
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-// The accumulators of a tile live in the accumulation registers a0 up, named in the
-// instructions: 4 registers an MFMA block, COUNT in all.  As values they were copied
-// at every turn of the loop or spilled (compilers move an MFMA builtin over barriers,
-// and its accumulator with it).  Every such instruction clobbers all of them, so
-// nothing else is kept there.  The compiler neither sees these MFMAs nor places the
-// waits that they need: two wait states between a VALU write and an MFMA that reads it,
-// eighteen between an MFMA and a read of its result by anything but an MFMA on it.
-#define XPU_A10(p) "a" #p "0", "a" #p "1", "a" #p "2", "a" #p "3", "a" #p "4", "a" #p "5", \
-                   "a" #p "6", "a" #p "7", "a" #p "8", "a" #p "9"
-#define XPU_A60 XPU_A10(), XPU_A10(1), XPU_A10(2), XPU_A10(3), XPU_A10(4), XPU_A10(5)
-#define XPU_A64 XPU_A60, "a60", "a61", "a62", "a63"
-#define XPU_A120 XPU_A60, XPU_A10(6), XPU_A10(7), XPU_A10(8), XPU_A10(9), XPU_A10(10), XPU_A10(11)
-#define XPU_A128 XPU_A120, "a120", "a121", "a122", "a123", "a124", "a125", "a126", "a127"
-#define XPU_A256 XPU_A120, XPU_A10(12), XPU_A10(13), XPU_A10(14), XPU_A10(15), XPU_A10(16),     \
-                 XPU_A10(17), XPU_A10(18), XPU_A10(19), XPU_A10(20), XPU_A10(21), XPU_A10(22),  \
-                 XPU_A10(23), XPU_A10(24), "a250", "a251", "a252", "a253", "a254", "a255"
 // blocks B0 .. B3 += W blocks (codes w, scale byte 0 of sw) * one X block
 #define XPU_MFMA4(CLOBBERS)                                                                     \
     asm volatile(XPU_ONE_MFMA(0, 4, 10, 11) XPU_ONE_MFMA(1, 5, 12, 13)                          \
@@ -185,92 +156,6 @@ __device__ __forceinline__ void acc_mfma4(const v4i* w, const int* sw, const v4i
     else if constexpr (COUNT == 128) XPU_MFMA4(XPU_A128);
     else XPU_MFMA4(XPU_A256);
 }
-// the four registers of block BLOCK = v
-#define XPU_ACC_SET(CLOBBERS)                                                                   \
-    asm volatile("v_accvgpr_write_b32 a[%4], %0\n\tv_accvgpr_write_b32 a[%5], %1\n\t"           \
-                 "v_accvgpr_write_b32 a[%6], %2\n\tv_accvgpr_write_b32 a[%7], %3"               \
-                 ::"v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "n"(4 * BLOCK),                  \
-                 "n"(4 * BLOCK + 1), "n"(4 * BLOCK + 2), "n"(4 * BLOCK + 3)                     \
-                 : CLOBBERS)
-template <int COUNT, int BLOCK>
-__device__ __forceinline__ void acc_set(const v4f& v) {
-    if constexpr (COUNT == 64) XPU_ACC_SET(XPU_A64);
-    else if constexpr (COUNT == 128) XPU_ACC_SET(XPU_A128);
-    else XPU_ACC_SET(XPU_A256);
-}
-template <int BLOCK>
-__device__ __forceinline__ v4f acc_get() {
-    float a, b, c, d;
-    asm volatile("v_accvgpr_read_b32 %0, a[%4]\n\tv_accvgpr_read_b32 %1, a[%5]\n\t"
-                 "v_accvgpr_read_b32 %2, a[%6]\n\tv_accvgpr_read_b32 %3, a[%7]"
-                 : "=v"(a), "=v"(b), "=v"(c), "=v"(d)
-                 : "n"(4 * BLOCK), "n"(4 * BLOCK + 1), "n"(4 * BLOCK + 2), "n"(4 * BLOCK + 3));
-    return v4f{a, b, c, d};
-}
-template <int N, int I = 0, class F>
-__device__ __forceinline__ void each(const F& f) {
-    if constexpr (I < N) {
-        f(std::integral_constant<int, I>{});
-        each<N, I + 1>(f);
-    }
-}
-template <int N>
-__device__ __forceinline__ void landed(v4i (&f)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
-}
-template <int N>
-__device__ __forceinline__ void landed(int (&f)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
-}
-
-// zeros in the rows of a tile
-template <int BM, int BN>
-__device__ __forceinline__ void zero_rows(const Out& o, int type, const RowTile& t, int n0) {
-    const v4f zero = {0.f, 0.f, 0.f, 0.f};
-    for (int i = threadIdx.x; i < BM * (BN / 4); i += blockDim.x) {
-        const int row = t.row + i / (BN / 4), n = n0 + 4 * (i % (BN / 4));
-        if (row >= t.end) continue;
-        if (type == kBf16) store4<kBf16>(o, row, n, zero);
-        else if (type == kF16) store4<kF16>(o, row, n, zero);
-        else store4<kF32>(o, row, n, zero);
-    }
-}
-
-// One row of COUNT MFMA blocks' results in a 16-bit type, columns n .. n + 16 COUNT (all
-// in the row, 16-byte aligned): lane group g holds the columns 16a + 4g .. + 3 of block a,
-// value(a), and stores 16 bytes: the swap of two blocks' odd and even lane rows
-// (v_permlane16_swap) leaves lane groups 0 and 2 with the columns 0-7 and 8-15 of the
-// one block, 1 and 3 with the other's.  `live`: whether this lane's row is one to write.
-template <int T, int COUNT, class V>
-__device__ __forceinline__ void store_row(const Out& o, int64_t row, bool live, int n, const V& value) {
-    const int g = (threadIdx.x & 63) >> 4;
-    char* const p = o.y + (row * o.N + n + 16 * (g & 1) + 8 * (g >> 1)) * 2;
-    each<COUNT / 2>([&](auto A) {
-        constexpr int a = 2 * decltype(A)::value;
-        const v4f u = value(std::integral_constant<int, a>{});
-        const v4f v = value(std::integral_constant<int, a + 1>{});
-        const auto lo = __builtin_amdgcn_permlane16_swap(pack2<T>(u[0], u[1]), pack2<T>(v[0], v[1]), false, false);
-        const auto hi = __builtin_amdgcn_permlane16_swap(pack2<T>(u[2], u[3]), pack2<T>(v[2], v[3]), false, false);
-        if (live) *reinterpret_cast<uint4*>(p + 32 * a) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
-    });
-}
-
-// Tile (tm, tn) of block b.  Blocks go round the 8 XCDs, each with its own L2, so an
-// XCD takes a contiguous eighth of the tiles, walked in bands of 8 row tiles: the
-// blocks of an XCD that run together share few rows of either operand.
-__device__ __forceinline__ bool tile_of(int b, int tiles_m, int tiles_n, int& tm, int& tn) {
-    const int tiles = tiles_m * tiles_n, share = (tiles + 7) / 8;
-    const int t = (b % 8) * share + b / 8;
-    if (t >= tiles) return false;
-    const int band = t / (8 * tiles_n), first = band * 8;
-    const int rows = min(tiles_m - first, 8), in = t - band * 8 * tiles_n;
-    tm = first + in % rows;
-    tn = in / rows;
-    return true;
-}
-
 template <int BM, int BN, bool GATHER>
 __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_kernel(
     const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs, const int* __restrict__ rows,
@@ -344,9 +229,9 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
         const uint8_t* p;
         if (isx) {
             if constexpr (GATHER) p = ax[i] + k - back;
-            else p = (xbase + k) + uint64_t(ax[i] - back);
+            else p = scalar(xbase + k) + uint64_t(ax[i] - back);
         } else {
-            p = (wbase + k) + uint64_t(aw[i - PX] - back);
+            p = scalar(wbase + k) + uint64_t(aw[i - PX] - back);
         }
         dma16(p, smem + slot * STEP + b * 64);
     };
@@ -364,25 +249,27 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
         }
     };
 
-    const int xrow = wm * (BM / 2) + r, wrow = BM + wn * (BN / 2) + r;
+    const int xrow = wm * 16 + r, wrow = BM + wn * (BN / 2) + r;
     const uint32_t sbase = lds_addr(smem);
     const uint32_t pos = (g ^ ((r >> 1) & 3)) * 16;
     const uint32_t xat[2] = {sbase + xrow * 64 + pos, sbase + 2 * STEP + xrow * 64 + pos};
     const uint32_t wat[2] = {sbase + wrow * 64 + pos, sbase + 2 * STEP + wrow * 64 + pos};
-    v4i xf[2][TM], wf[2][TN];                             // of even and odd steps
+    // fragments of even and odd steps; x's first half is read again as soon as it is used
+    v4i xf[2][TM], wf[2][TN];
+    constexpr int TH = TM / 2;
     int sx[TM], sw[TN];                                   // byte 0: this step's scale
     int sr[TM + TN];                                      // the next group's
     v4i tr[PER_T];                                        // scale rows on their way through
     auto read_x = [&](auto S, auto Fr, auto I) {
         constexpr int slot = decltype(S)::value, f = decltype(Fr)::value, i = decltype(I)::value;
-        xf[f][i] = read16(xat[slot >> 1], (slot & 1) * STEP + i * 1024);
+        xf[i < TH ? 0 : f][i] = read16(xat[slot >> 1], (slot & 1) * STEP + i * 2048);
     };
     auto read_w = [&](auto S, auto Fr, auto I) {
         constexpr int slot = decltype(S)::value, f = decltype(Fr)::value, i = decltype(I)::value;
         wf[f][i] = read16(wat[slot >> 1], (slot & 1) * STEP + i * 1024);
     };
     auto read_scale = [&](uint32_t at, int i) {           // of block i, x's first
-        sr[i] = i < TM ? read4(at + xrow * 16, i * 256) : read4(at + wrow * 16, (i - TM) * 256);
+        sr[i] = i < TM ? read4(at + xrow * 16, i * 512) : read4(at + wrow * 16, (i - TM) * 256);
     };
     // the 4 x 4 byte transposition of each row's scales of group q, in place: the
     // reads, and after they have landed the writes
@@ -422,12 +309,6 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
                 asm volatile("ds_write_b128 %0, %1" ::"v"(scale_row(q, i)), "v"(o) : "memory");
         }
     };
-    auto lds_done = [&]() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
-    auto barrier = [&]() {
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-    };
     using C0 = std::integral_constant<int, 0>;
     using C1 = std::integral_constant<int, 1>;
     using C2 = std::integral_constant<int, 2>;
@@ -457,7 +338,7 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
     }
     lds_done();
     // meanwhile the accumulators start from the bias
-    barrier();
+    block_barrier();
     each<TN>([&](auto A) {
         constexpr int a = decltype(A)::value;
         v4i b4 = read16(lds_addr(bias_of) + (wn * (BN / 2) + 4 * g) * 4, a * 64);
@@ -467,13 +348,13 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
     // (the scales went out first, then the codes step by step: step 0's are in too)
     if (groups > 1) wait_vm<3 * PL>();
     else wait_vm<0>();
-    barrier();
+    block_barrier();
     transpose_read(0);
     lds_done();
     landed(tr);
     transpose_write(0);
     lds_done();
-    barrier();
+    block_barrier();
     each<TM + TN>([&](auto I) { read_scale(sbase + 4 * STEP + 4 * g, decltype(I)::value); });
     each<TM>([&](auto I) { read_x(C0{}, C0{}, I); });
     each<TN>([&](auto I) { read_w(C0{}, C0{}, I); });
@@ -484,7 +365,7 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
 #pragma unroll
     for (int a = 0; a < TN; ++a) sw[a] = sr[TM + a];
     if (groups > 1) wait_vm<2 * PL>();                    // step 1 in
-    barrier();                                            // step 0's slot is read
+    block_barrier();                                            // step 0's slot is read
 
     // step s = 4q + J; FULL: step s + 4 exists and is whole
     auto step = [&](auto Jc, auto Full, int q) {
@@ -503,16 +384,14 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
         if constexpr (J == 2) transpose_write(q + 1);
         each<TM>([&](auto B) {
             constexpr int b = decltype(B)::value;
-            constexpr int H = TM / 2;                     // the reads in the step's first half
-            if constexpr (b < H) {
-                each<TM / H>([&](auto I) {
-                    read_x(Next{}, NF{}, std::integral_constant<int, b * (TM / H) + decltype(I)::value>{});
-                });
-                each<TN / H>([&](auto I) {
-                    read_w(Next{}, NF{}, std::integral_constant<int, b * (TN / H) + decltype(I)::value>{});
+            // the reads in the step's first half
+            if constexpr (b < TH) {
+                read_x(Next{}, NF{}, std::integral_constant<int, TH + b>{});
+                each<TN / TH>([&](auto I) {
+                    read_w(Next{}, NF{}, std::integral_constant<int, b * (TN / TH) + decltype(I)::value>{});
                 });
                 if constexpr (J == 3)
-                    each<(TM + TN) / H>([&](auto I) { read_scale(sat, b * ((TM + TN) / H) + decltype(I)::value); });
+                    each<(TM + TN) / TH>([&](auto I) { read_scale(sat, b * ((TM + TN) / TH) + decltype(I)::value); });
             }
             if (more) {
 #pragma unroll
@@ -521,12 +400,15 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
             each<TN / 4>([&](auto A) {
                 constexpr int a = 4 * decltype(A)::value;
                 acc_mfma4<ACC, a * TM + b, (a + 1) * TM + b, (a + 2) * TM + b, (a + 3) * TM + b>(
-                    &wf[F][a], &sw[a], xf[F][b], sx[b]);
+                    &wf[F][a], &sw[a], xf[b < TH ? 0 : F][b], sx[b]);
             });
+            if constexpr (b < TH) read_x(Next{}, NF{}, B);
             __builtin_amdgcn_sched_barrier(0);
         });
         lds_done();
-        landed(xf[1 - F]); landed(wf[1 - F]);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) asm volatile("" : "+v"(xf[i < TH ? 0 : 1 - F][i]));
+        landed(wf[1 - F]);
         if constexpr (J == 1) landed(tr);
         if constexpr (J == 3) landed(sr);
 #pragma unroll
@@ -538,66 +420,35 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
         if (more) wait_vm<2 * PL>();
         else if (s + 3 < steps) wait_vm<PL>();
         else wait_vm<0>();
-        barrier();
+        block_barrier();
     };
     const int whole = K / 128;
+    using Yes = std::true_type;
+    using No = std::false_type;
     int q = 0;
+    auto whole_groups = [&]() {
 #pragma clang loop unroll(disable)
-    for (; 4 * q + 8 <= whole; ++q) {
-        step(C0{}, std::true_type{}, q);
-        step(C1{}, std::true_type{}, q);
-        step(C2{}, std::true_type{}, q);
-        step(C3{}, std::true_type{}, q);
-    }
+        for (; 4 * q + 8 <= whole; ++q) {
+            step(C0{}, Yes{}, q);
+            step(C1{}, Yes{}, q);
+            step(C2{}, Yes{}, q);
+            step(C3{}, Yes{}, q);
+        }
+    };
+    whole_groups();
 #pragma clang loop unroll(disable)
     for (;; ++q) {
-        step(C0{}, std::false_type{}, q);
+        step(C0{}, No{}, q);
         if (4 * q + 1 >= steps) break;
-        step(C1{}, std::false_type{}, q);
+        step(C1{}, No{}, q);
         if (4 * q + 2 >= steps) break;
-        step(C2{}, std::false_type{}, q);
+        step(C2{}, No{}, q);
         if (4 * q + 3 >= steps) break;
-        step(C3{}, std::false_type{}, q);
+        step(C3{}, No{}, q);
         if (4 * q + 4 >= steps) break;
     }
-    // the last MFMAs' results before the compiler, which does not see them, reads them
-    asm volatile("s_nop 15\n\ts_nop 15");
-    const int n = n0 + wn * (BN / 2);
-    auto store = [&](auto T) {
-        each<TM>([&](auto B) {
-            constexpr int b = decltype(B)::value;
-            const int row = t.row + xrow + 16 * b;
-            store_row<decltype(T)::value, TN>(out, row, row < t.end, n, [&](auto A) {
-                return acc_get<decltype(A)::value * TM + b>();
-            });
-            __builtin_amdgcn_sched_barrier(0);
-        });
-    };
-    const bool fast = out.vec8 && n + BN / 2 <= w.N;
-    if (fast && type == kBf16) return store(std::integral_constant<int, kBf16>{});
-    if (fast && type == kF16) return store(std::integral_constant<int, kF16>{});
-    // other types, widths and edges: 16 rows at a time through the wave's own part of
-    // the ring (which nothing reads or fills any more)
-    float* const mine = reinterpret_cast<float*>(smem) + wave * 16 * (BN / 2);
-    each<TM>([&](auto B) {
-        constexpr int b = decltype(B)::value;
-        each<TN>([&](auto A) {
-            constexpr int a = decltype(A)::value;
-            *reinterpret_cast<v4f*>(mine + r * (BN / 2) + 16 * a + 4 * g) = acc_get<a * TM + b>();
-        });
-        lds_done();
-#pragma clang loop unroll(disable)
-        for (int i = lane; i < 16 * (BN / 8); i += 64) {
-            const int rr = i / (BN / 8), c = 4 * (i % (BN / 8));
-            const int row = t.row + wm * (BM / 2) + 16 * b + rr;
-            const v4f v = *reinterpret_cast<const v4f*>(mine + rr * (BN / 2) + c);
-            if (row >= t.end) continue;
-            if (type == kBf16) store4<kBf16>(out, row, n + c, v);
-            else if (type == kF16) store4<kF16>(out, row, n + c, v);
-            else store4<kF32>(out, row, n + c, v);
-        }
-        lds_done();
-    });
+    store_tile<TM, TN>(out, type, t.row + 16 * wm, t.end, n0 + wn * (BN / 2),
+                       reinterpret_cast<float*>(smem) + wave * 16 * (BN / 2));
 }
 
 }  // namespace

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "kernels.hpp"
 #include "mx4.hpp"
 #include "mx_kernels.hpp"
 

@@ -8,9 +8,6 @@
 
 namespace xpuint8 {
 
-// capi.hip: compute units of the current device
-int device_cus();
-
 // mx4_quant.hip: x [M, K] (row stride ldx) to codes and scales, and back
 hipError_t mx4_quantize(hipStream_t st, const void* x, int type, int64_t ldx, uint8_t* codes,
                         uint8_t* scales, int64_t M, int K);

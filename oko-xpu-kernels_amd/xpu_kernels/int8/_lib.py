@@ -43,7 +43,12 @@ _HOST_ENTRIES = (
     "xpuint8_linear_dw_workspace_size", "xpuint8_linear_dw_work_stream",
     "xpuint8_column_sum_workspace_size", "xpuint8_column_sum_stream",
     "xpuint8_convrot_quantize_stream", "xpuint8_linear_acc_packed_stream",
-    "xpuint8_linear_dx_int8_reads_packed")
+    "xpuint8_linear_dx_int8_reads_packed",
+    "xpuint8_mxfp4_quantize_stream", "xpuint8_mxfp4_dequantize_stream",
+    "xpuint8_mxfp4_linear_workspace_size", "xpuint8_mxfp4_linear_stream",
+    "xpuint8_mxfp4_grouped_linear_workspace_size", "xpuint8_mxfp4_grouped_linear_stream",
+    "xpuint8_moe_sort_workspace_size", "xpuint8_moe_sort_stream",
+    "xpuint8_moe_dispatch_stream", "xpuint8_moe_combine_stream")
 
 
 def _candidate_paths():
@@ -140,7 +145,7 @@ def _signatures():
         "xpuint8_mxfp4_grouped_linear_workspace_size": ([i64] * 5, i64),
         "xpuint8_mxfp4_grouped_linear_stream": ([vp, vp, i32, i64, vp, i64, vp, vp, vp, i64, vp]
                                                 + [i64] * 3 + [vp, i64], c_int),
-        "xpuint8_mxfp4_dx_workspace_size": ([i32] + [i64] * 2, i64),
+        "xpuint8_mxfp4_dx_workspace_size": ([i32] * 2 + [i64] * 4, i64),
         "xpuint8_mxfp4_dx_stream": ([vp, vp, i32, i64, vp, vp, vp, i64, vp, i32] + [i64] * 3
                                     + [vp, i64], c_int),
         "xpuint8_moe_sort_workspace_size": ([i64] * 3, i64),

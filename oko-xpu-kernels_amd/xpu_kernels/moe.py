@@ -22,7 +22,7 @@ import torch
 
 from . import mxfp4
 from .int8 import _lib as L
-from .mxfp4 import TYPES, _check_float, _opt, _rows, _work
+from .mxfp4 import TYPES, _check_float, _opt, _rows, _wants_grad, _work
 
 __all__ = ["Routing", "combine", "dispatch", "ffn", "sort"]
 
@@ -53,6 +53,10 @@ def _check_routing(routing, device):
 
 def sort(expert_ids, n_experts):
     """Sort the slots of ``expert_ids`` [T, top] (int32 or int64) by expert, stably."""
+    if L.HOST is not None:
+        r = L.HOST.moe_sort(expert_ids, n_experts)
+        if r is not None:
+            return Routing._make(r)
     if not isinstance(expert_ids, torch.Tensor) or expert_ids.dtype not in (torch.int32,
                                                                           torch.int64):
         raise TypeError(f"expert_ids must be an int32 or int64 tensor, got "
@@ -159,11 +163,15 @@ def dispatch(x, routing):
     """x [T, D] -> [T*top, D]: each token's row at each of its slots' places, in
     the experts' order; zeros in the rows of no expert.  The gradient sums a
     token's rows in fp32."""
+    if L.HOST is not None and type(routing) is Routing and not _wants_grad(x):
+        r = L.HOST.moe_dispatch(x, routing)
+        if r is not None:
+            return r
     _check_float(x, "x")
     _check_routing(routing, x.device)
     if x.dim() != 2 or x.shape[0] != routing.position.shape[0]:
         raise ValueError(f"x must be [{routing.position.shape[0]}, D], got {tuple(x.shape)}")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _wants_grad(x):
         return _DispatchFn.apply(x, routing)
     return _dispatch(x, routing)
 
@@ -172,6 +180,10 @@ def combine(z, routing, weights):
     """z [T*top, D] in the experts' order -> [T, D]: each token's rows times
     ``weights`` [T, top] (used in fp32), summed in fp32 in slot order.  Gradients
     reach z and weights."""
+    if L.HOST is not None and type(routing) is Routing and not _wants_grad(z, weights):
+        r = L.HOST.moe_combine(z, routing, weights)
+        if r is not None:
+            return r
     _check_float(z, "z")
     _check_routing(routing, z.device)
     t, top = routing.position.shape
@@ -183,7 +195,7 @@ def combine(z, routing, weights):
     if weights.device != z.device:
         raise TypeError(f"weights is on {weights.device} but z is on {z.device}")
     weights = weights.float().contiguous()
-    if torch.is_grad_enabled() and (z.requires_grad or weights.requires_grad):
+    if _wants_grad(z, weights):
         return _CombineFn.apply(z, weights, routing)
     return _combine(z, routing, weights, z.dtype)
 

@@ -62,6 +62,11 @@ def _check_float(t, name):
         raise TypeError(f"expected a GPU (ROCm) tensor, got {t.device}")
 
 
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
+                                           for t in tensors)
+
+
 def _check_pair(codes, scales, lead=None):
     """The K behind codes and scales, both on the GPU and of matching shapes."""
     for t, name in ((codes, "codes"), (scales, "scales")):
@@ -104,6 +109,10 @@ def _opt(t):
 def quantize(x):
     """x [.., K] (bf16, fp16 or fp32) -> (codes uint8 [.., K/2], scales uint8
     [.., scale_width(K)])."""
+    if L.HOST is not None:
+        r = L.HOST.mx_quantize(x)
+        if r is not None:
+            return r
     _check_float(x, "x")
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
@@ -124,6 +133,10 @@ def quantize(x):
 def dequantize(codes, scales, dtype=torch.bfloat16):
     """What codes and scales stand for, [.., K] in ``dtype`` (bf16 and fp32 hold
     every value; fp16 turns what is beyond its range into infinities)."""
+    if L.HOST is not None and dtype in TYPES:
+        r = L.HOST.mx_dequantize(codes, scales, TYPES[dtype])
+        if r is not None:
+            return r
     k = _check_pair(codes, scales)
     if dtype not in TYPES:
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
@@ -176,12 +189,13 @@ def _dx(dy, codes, scales, offsets, out_dtype):
         return dx.zero_()
     if r:
         lib = L._lib()
+        e = 0 if offsets is None else offsets.numel() - 1
         work = None
-        if dy2.dtype != torch.bfloat16 or n % 8 or ld % 8 or dy2.data_ptr() % 16:
-            work = _work(lib.xpuint8_mxfp4_dx_workspace_size(TYPES[dy2.dtype], r, n), dy2)
+        if e == 0 or dy2.dtype != torch.bfloat16 or n % 8 or ld % 8 or dy2.data_ptr() % 16:
+            work = _work(lib.xpuint8_mxfp4_dx_workspace_size(TYPES[dy2.dtype], TYPES[out_dtype],
+                                                             r, e, n, k), dy2)
         if lib.xpuint8_mxfp4_dx_stream(L._stream(dy.device), dy2.data_ptr(), TYPES[dy2.dtype], ld,
-                                       codes.data_ptr(), scales.data_ptr(), _opt(offsets),
-                                       0 if offsets is None else offsets.numel() - 1,
+                                       codes.data_ptr(), scales.data_ptr(), _opt(offsets), e,
                                        dx.data_ptr(), TYPES[out_dtype], r, n, k, _opt(work),
                                        0 if work is None else work.numel()) != 0:
             L._err(lib, "mxfp4 dx")
@@ -212,6 +226,10 @@ def linear(x, codes, scales, bias=None):
     codes [N, K/2] and scales [N, scale_width(K)]; fp32 sums rounded once to x's
     type.  ``bias`` [N] is bf16, fp16 or fp32.  Gradients: dx = dy @ wq, straight
     through x's quantization, and the bias's column sum; the weight has none."""
+    if L.HOST is not None and not _wants_grad(x, bias):
+        r = L.HOST.mx_linear(x, codes, scales, bias)
+        if r is not None:
+            return r
     _check_weight(x, codes, scales, 2)
     codes, scales = L._c(codes), L._c(scales)
     if bias is not None:
@@ -221,7 +239,7 @@ def linear(x, codes, scales, bias=None):
         if bias.device != x.device:
             raise TypeError(f"bias is on {bias.device} but x is on {x.device}")
         bias = bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+    if _wants_grad(x, bias):
         return _LinearFn.apply(x, codes, scales, bias)
     return _linear(x, codes, scales, bias)
 
@@ -274,6 +292,10 @@ def grouped_linear(x, codes, scales, routing, gather=False):
     [T, K], each quantized once and read by every row that is its.  Returns
     [T*top, N] in x's type; the gradient reaches x."""
     from . import moe
+    if L.HOST is not None and type(routing) is moe.Routing and not _wants_grad(x):
+        r = L.HOST.mx_grouped(x, codes, scales, routing, gather)
+        if r is not None:
+            return r
     _check_weight(x, codes, scales, 3)
     moe._check_routing(routing, x.device)
     if routing.offsets.numel() != codes.shape[0] + 1:
@@ -284,6 +306,6 @@ def grouped_linear(x, codes, scales, routing, gather=False):
         raise ValueError(f"x must be [{want}, K] ({'tokens' if gather else 'sorted rows'}), got "
                          f"{tuple(x.shape)}")
     codes, scales = L._c(codes), L._c(scales)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _wants_grad(x):
         return _GroupedFn.apply(x, codes, scales, routing, bool(gather))
     return _grouped(x, codes, scales, routing, gather)

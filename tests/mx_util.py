@@ -1,6 +1,16 @@
 """Shared by the MXFP4 and mixture-of-experts tests: inputs and error bounds."""
 
+import pytest
 import torch
+
+
+@pytest.fixture
+def big_memory():
+    """For a test of several GiB: its memory goes back to the device afterwards, so that
+    no later test's allocation keeps a segment of it."""
+    yield
+    torch.cuda.empty_cache()
+
 
 #: half a unit in the last place, relative (2^-p for p significant bits: 8, 11, 24)
 HALF_ULP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}

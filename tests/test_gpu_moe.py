@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import oracle.mxfp4 as O
-from mx_util import DTYPES, assert_close, randn, router
+from mx_util import DTYPES, assert_close, big_memory, randn, router  # noqa: F401
 from xpu_kernels import moe, mxfp4
 
 pytestmark = pytest.mark.gpu
@@ -150,7 +150,7 @@ def test_empty(dev):
     assert y.shape == (0, 8) and x.grad.shape == (0, 32)
 
 
-def test_rows_past_4_gib(dev):
+def test_rows_past_4_gib(dev, big_memory):
     t, top, d = 70001, 2, 16384                            # 4.6 GB of sorted rows
     ids = router(t, top, 8, seed=1)
     routing = moe.sort(ids.to(dev), 8)

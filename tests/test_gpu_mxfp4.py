@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import oracle.mxfp4 as O
-from mx_util import DTYPES, assert_close, randn, router
+from mx_util import DTYPES, assert_close, big_memory, randn, router  # noqa: F401
 from xpu_kernels import moe, mxfp4
 
 pytestmark = pytest.mark.gpu
@@ -91,7 +91,7 @@ def test_quantize_empty(dev):
     assert mxfp4.dequantize(codes, scales).shape == (0, 64)
 
 
-def test_quantize_past_4_gib(dev):
+def test_quantize_past_4_gib(dev, big_memory):
     m, k = 70001, 32768                                   # 4.6 GB of bf16
     x = torch.empty(m, k, dtype=torch.bfloat16, device=dev).normal_(generator=torch.Generator(dev).manual_seed(1))
     codes, scales = mxfp4.quantize(x)
@@ -142,7 +142,7 @@ def test_linear(dev, dtype, m, k, n):
 @pytest.mark.parametrize("dtype,m,k,n", [(torch.bfloat16, 4090, 8160, 4080),
                                          (torch.bfloat16, 4001, 8192, 4081),
                                          (torch.float32, 3890, 7968, 4096)])
-def test_linear_large_tiles(dev, dtype, m, k, n):
+def test_linear_large_tiles(dev, big_memory, dtype, m, k, n):
     """Shapes that take the large tiles, ragged in every dimension."""
     x = randn(m, k, seed=m, dtype=dtype)
     bias = randn(n, seed=2, dtype=dtype)
@@ -154,7 +154,7 @@ def test_linear_large_tiles(dev, dtype, m, k, n):
 
 
 @pytest.mark.parametrize("gather", [False, True])
-def test_grouped_large_tiles(dev, gather):
+def test_grouped_large_tiles(dev, big_memory, gather):
     t, top, e, k, n = 4095, 2, 3, 8160, 3800
     ids = router(t, top, e, seed=1, dropped=0.02)
     routing = moe.sort(ids.to(dev), e)

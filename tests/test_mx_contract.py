@@ -123,7 +123,8 @@ def test_library_sizes(lib):
     assert lib.xpuint8_mxfp4_linear_workspace_size(4, 8, 48) == -1
     assert lib.xpuint8_mxfp4_linear_workspace_size(1000, 8, 64) >= 1000 * (32 + 16)
     assert lib.xpuint8_mxfp4_grouped_linear_workspace_size(8, 4, 0, 8, 64) == -1
-    assert lib.xpuint8_mxfp4_dx_workspace_size(2, 10, 100) >= 10 * 128 * 3 * 2
+    assert lib.xpuint8_mxfp4_dx_workspace_size(2, 2, 10, 0, 100, 64) >= 10 * 128 * 3 * 2
+    assert lib.xpuint8_mxfp4_dx_workspace_size(0, 0, 10, 0, 100, 48) == -1
     assert lib.xpuint8_moe_sort_workspace_size(4, 2, 4) == 0
 
 
