@@ -16,18 +16,18 @@ namespace xpuint8 {
 namespace {
 
 // ------------------------------------------------------------------- sort
-// A counting sort: a block of 16 waves takes kSortChunk consecutive slots, a wave
-// a run of them, 64 at a time in order.  The lanes of one key are found with one
-// ballot per bit of the key (no atomics, so ranks do not depend on timing); the
-// first of them adds their number to the wave's counter of that key.  With the
-// counters of every wave before it, and those of every block before, a wave
-// knows where its first slot of each key goes, and the second pass hands out the
-// places.  A batch of up to kSortChunk slots is one launch of one block; more
-// slots take a launch of the counts first.  Latency bound: 8 K slots in 64
-// experts 9 us, 64 K 13 us (MI355X).
+// A counting sort: a block of 16 waves takes 1024 KPL consecutive slots, a wave 64 KPL of
+// them, a lane KPL, 64 apart, whose keys it reads once, all together.  The lanes of one
+// key are found with one ballot per bit of the key (no atomics, so ranks do not depend
+// on timing); the first of them adds their number to the wave's counter of that key.
+// With the counters of every wave before it, and those of every block before, a wave
+// knows where its first slot of each key goes, and a second pass over the same
+// registers hands out the places.  Up to 8192 slots are one launch of one block; more
+// take a launch of the counts first, in blocks of 2048 slots (8192 from 128 K on, so
+// that no block reads more than a few dozen others' counts).  Bound by latency: the
+// loads of the keys, some 200 cycles for each 64 of a wave, a store a slot.
 constexpr int kSortWaves = 16;
 constexpr int kSortThreads = kSortWaves * 64;
-constexpr int kSortChunk = 8192;
 constexpr int kMaxExperts = 1024;
 
 template <class I>
@@ -36,7 +36,7 @@ __device__ __forceinline__ int key_of(const I* ids, int64_t s, int E) {
     return v >= 0 && v < I(E) ? int(v) : E;
 }
 
-// the lanes of the wave whose key equals this lane's, among the lanes of `live`
+// the lanes of the wave whose key equals this lane's, among those of `live`
 __device__ __forceinline__ uint64_t peers(int key, int bits, uint64_t live) {
     uint64_t m = live;
     for (int b = 0; b < bits; ++b) {
@@ -47,33 +47,35 @@ __device__ __forceinline__ uint64_t peers(int key, int bits, uint64_t live) {
     return m;
 }
 
-// Counts of each key in each wave's run of the block's chunk, in LDS
-// count[wave * (E + 1) + key] (cleared here).
-template <class I>
-__device__ __forceinline__ void count_keys(const I* ids, int64_t first, int64_t last, int per_wave,
-                                           int E, int bits, int* count) {
+// This lane's keys (-1 past the end) and, in LDS count[wave * (E + 1) + key] (cleared
+// here), the number of each key among the wave's.
+template <int KPL, class I>
+__device__ __forceinline__ void count_keys(const I* ids, int64_t S, int E, int bits,
+                                           int (&key)[KPL], int* count) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t lo = (int64_t(blockIdx.x) * kSortWaves + wave) * (64 * KPL) + lane;
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) key[i] = lo + 64 * i < S ? key_of(ids, lo + 64 * i, E) : -1;
     for (int i = threadIdx.x; i < kSortWaves * (E + 1); i += kSortThreads) count[i] = 0;
     __syncthreads();
     int* mine = count + wave * (E + 1);
-    const int64_t lo = first + int64_t(wave) * per_wave, hi = min(lo + per_wave, last);
-    for (int64_t s0 = lo; s0 < hi; s0 += 64) {
-        const int64_t s = s0 + lane;
-        const bool in = s < hi;
-        const int key = in ? key_of(ids, s, E) : 0;
-        const uint64_t m = peers(key, bits, __builtin_amdgcn_ballot_w64(in));
-        if (in && __builtin_ctzll(m) == lane) mine[key] += __builtin_popcountll(m);
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        const bool in = key[i] >= 0;
+        const uint64_t m = peers(key[i], bits, __builtin_amdgcn_ballot_w64(in));
+        if (in && __builtin_ctzll(m) == lane) mine[key[i]] += __builtin_popcountll(m);
+        __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
 }
 
-template <class I>
+template <int KPL, class I>
 __global__ __launch_bounds__(kSortThreads) void moe_count_kernel(const I* __restrict__ ids,
                                                                  int* __restrict__ counts,
                                                                  int64_t S, int E, int bits) {
     __shared__ int count[kSortWaves * (kMaxExperts + 1)];
-    const int64_t first = int64_t(blockIdx.x) * kSortChunk;
-    count_keys(ids, first, min(first + kSortChunk, S), kSortChunk / kSortWaves, E, bits, count);
+    int key[KPL];
+    count_keys(ids, S, E, bits, key, count);
     for (int k = threadIdx.x; k <= E; k += kSortThreads) {
         int n = 0;
         for (int w = 0; w < kSortWaves; ++w) n += count[w * (E + 1) + k];
@@ -81,33 +83,37 @@ __global__ __launch_bounds__(kSortThreads) void moe_count_kernel(const I* __rest
     }
 }
 
-// counts: the keys' numbers in each of the nb chunks (unused where nb == 1)
-template <class I>
+// counts: the keys' numbers in each block (unused where there is one block)
+template <int KPL, class I>
 __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(
     const I* __restrict__ ids, const int* __restrict__ counts, int* __restrict__ order,
     int* __restrict__ position, int* __restrict__ rows, int* __restrict__ offsets, int64_t S,
-    int top, int E, int bits, int nb, int per_wave) {
+    int top, int E, int bits) {
     __shared__ int count[kSortWaves * (kMaxExperts + 1)];
-    __shared__ int total[kSortThreads + 64];                // (E + 1 <= kSortThreads + 1)
+    __shared__ int total[kMaxExperts + 1];
     __shared__ int wave_sum[kSortWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t first = int64_t(blockIdx.x) * kSortChunk;
-    const int64_t last = min(first + kSortChunk, S);
-    count_keys(ids, first, last, per_wave, E, bits, count);
-    // per key: its number in the blocks before (left in `before`) and in all
-    int before = 0, all = 0;
-    const int k = threadIdx.x;
-    if (k < E) {
-        if (nb == 1) {
-            for (int w = 0; w < kSortWaves; ++w) all += count[w * (E + 1) + k];
-        } else {
-            for (int b = 0; b < nb; ++b) {
-                const int n = counts[int64_t(b) * (E + 1) + k];
-                if (b < int(blockIdx.x)) before += n;
-                all += n;
-            }
+    const int nb = gridDim.x, k = threadIdx.x;
+    // per key: its number in the blocks before and in all; of the slots without an
+    // expert, which follow all others in slot order, the number before
+    int before = 0, all = 0, loose = 0;
+    if (nb > 1 && k <= E) {
+#pragma unroll 8
+        for (int b = 0; b < nb; ++b) {
+            const int n = counts[int64_t(b) * (E + 1) + k];
+            if (b < int(blockIdx.x)) before += n;
+            all += n;
         }
     }
+    if (nb > 1 && k == 0) {
+#pragma unroll 8
+        for (int b = 0; b < int(blockIdx.x); ++b) loose += counts[int64_t(b) * (E + 1) + E];
+    }
+    if (k >= E) before = all = 0;
+    int key[KPL];
+    count_keys(ids, S, E, bits, key, count);
+    if (nb == 1 && k < E)
+        for (int w = 0; w < kSortWaves; ++w) all += count[w * (E + 1) + k];
     // exclusive scan of the numbers over the keys 0 .. E - 1
     int incl = all;
 #pragma unroll
@@ -124,15 +130,10 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(
         offsets[k] = base;
         if (k == E - 1) offsets[E] = base + all;
     }
-    // the slots without an expert follow all others, in slot order: those before
-    // this block are its first slot less the slots with an expert before it
     if (k == 0) {
-        int live = 0, live_before = 0;
+        int live = 0;
         for (int w = 0; w < kSortWaves; ++w) live += wave_sum[w];
-        if (nb > 1) {
-            for (int b = 0; b < int(blockIdx.x); ++b) live_before += counts[int64_t(b) * (E + 1) + E];
-        }
-        total[E] = live + live_before;
+        total[E] = live + loose;
     }
     __syncthreads();
     // each wave's first place of each key, in place of its count
@@ -146,24 +147,31 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(
     }
     __syncthreads();
     int* mine = count + wave * (E + 1);
-    const int64_t lo = first + int64_t(wave) * per_wave, hi = min(lo + per_wave, last);
-    for (int64_t s0 = lo; s0 < hi; s0 += 64) {
-        const int64_t s = s0 + lane;
-        const bool in = s < hi;
-        const int key = in ? key_of(ids, s, E) : 0;
-        const uint64_t m = peers(key, bits, __builtin_amdgcn_ballot_w64(in));
+    const int64_t lo = (int64_t(blockIdx.x) * kSortWaves + wave) * (64 * KPL) + lane;
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        const int s = int(lo) + 64 * i;
+        const bool in = key[i] >= 0;
+        const uint64_t m = peers(key[i], bits, __builtin_amdgcn_ballot_w64(in));
         if (in) {
-            const int at = mine[key] + __builtin_popcountll(m & ((uint64_t(1) << lane) - 1));
-            order[at] = int(s);
+            const int at = mine[key[i]] + __builtin_popcountll(m & ((uint64_t(1) << lane) - 1));
+            order[at] = s;
             position[s] = at;
-            rows[at] = int(s) / top;
+            rows[at] = s / top;
         }
         // every lane has its place before the counter moves on (the wave's LDS
         // accesses are in order)
         __builtin_amdgcn_wave_barrier();
-        if (in && __builtin_ctzll(m) == lane) mine[key] += __builtin_popcountll(m);
+        if (in && __builtin_ctzll(m) == lane) mine[key[i]] += __builtin_popcountll(m);
         __builtin_amdgcn_wave_barrier();
     }
+}
+
+// keys a lane, by the number of slots
+int keys_per_lane(int64_t S) { return S <= 1024 ? 1 : S <= 2048 ? 2 : S <= 8192 ? 8 : S <= 131072 ? 2 : 8; }
+int sort_blocks(int64_t S) {
+    const int64_t chunk = 1024 * keys_per_lane(S);
+    return int((S + chunk - 1) / chunk);
 }
 
 template <class I>
@@ -171,14 +179,19 @@ hipError_t sort_launch(hipStream_t st, const I* ids, int* counts, int* order, in
                        int* rows, int* offsets, int64_t S, int top, int E) {
     int bits = 1;
     while ((1 << bits) < E + 1) ++bits;
-    const int nb = int((S + kSortChunk - 1) / kSortChunk);
-    int per_wave = kSortChunk / kSortWaves;
-    if (nb == 1) per_wave = int((S + kSortThreads - 1) / kSortThreads) * 64;
-    if (nb > 1)
-        hipLaunchKernelGGL((moe_count_kernel<I>), dim3(unsigned(nb)), dim3(kSortThreads), 0, st,
-                           ids, counts, S, E, bits);
-    hipLaunchKernelGGL((moe_sort_kernel<I>), dim3(unsigned(nb)), dim3(kSortThreads), 0, st, ids,
-                       counts, order, position, rows, offsets, S, top, E, bits, nb, per_wave);
+    const int nb = sort_blocks(S);
+    auto go = [&](auto K) {
+        constexpr int kpl = decltype(K)::value;
+        if (nb > 1)
+            hipLaunchKernelGGL((moe_count_kernel<kpl, I>), dim3(unsigned(nb)), dim3(kSortThreads),
+                               0, st, ids, counts, S, E, bits);
+        hipLaunchKernelGGL((moe_sort_kernel<kpl, I>), dim3(unsigned(nb)), dim3(kSortThreads), 0,
+                           st, ids, counts, order, position, rows, offsets, S, top, E, bits);
+    };
+    const int kpl = keys_per_lane(S);
+    if (kpl == 1) go(std::integral_constant<int, 1>{});
+    else if (kpl == 2) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 8>{});
     return hipGetLastError();
 }
 
@@ -286,21 +299,32 @@ __global__ __launch_bounds__(256) void moe_gather_kernel(const char* __restrict_
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[u][i] = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < top; ++j) {
-        const int at = position[p.t * top + j];
-        if (at < 0 || at >= live) continue;
-        const float w = WEIGHTED ? weights[p.t * top + j] : 1.f;
-        const char* src = z + int64_t(at) * ldz * kSize<T>;
+    // four rows are requested together; one that no expert has gives way to row 0 and
+    // is not added
+    for (int j0 = 0; j0 < top; j0 += 4) {
+        float v[4][U][8], w[4];
+        bool has[4];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (p.d + 512 * u < D) {
-                float v[8];
-                load_row8<T, VEC>(src, p.d + 512 * u, D, v);
+        for (int q = 0; q < 4; ++q) {
+            const int64_t slot = p.t * top + min(j0 + q, top - 1);
+            const int at = position[slot];
+            has[q] = j0 + q < top && at >= 0 && at < live;
+            w[q] = WEIGHTED ? weights[slot] : 1.f;
+            const char* src = z + int64_t(has[q] ? at : 0) * ldz * kSize<T>;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (p.d + 512 * u < D) load_row8<T, VEC>(src, p.d + 512 * u, D, v[q][u]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (!has[q]) continue;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    acc[u][i] = WEIGHTED ? __builtin_fmaf(w, v[i], acc[u][i]) : acc[u][i] + v[i];
-            }
+                    acc[u][i] = WEIGHTED ? __builtin_fmaf(w[q], v[q][u][i], acc[u][i])
+                                         : acc[u][i] + v[q][u][i];
+        }
     }
     char* dst = out + p.t * D * kSize<TO>;
 #pragma unroll
@@ -367,15 +391,15 @@ bool vec_rows(const void* p, int64_t ld, int type, int D) {
 }
 
 // calls f with the element type, the vector form and the chunks a wave takes:
-// four once the pieces still give every CU eight waves
-template <class F>
+// MOST once the pieces still give every CU eight waves
+template <int MOST, class F>
 void by_form(int type, bool vec, int64_t tokens, int D, const F& f) {
-    const int64_t pieces4 = tokens * ((D + 2047) / 2048);
+    const int64_t pieces = tokens * ((D + 512 * MOST - 1) / (512 * MOST));
     auto form = [&](auto T) {
         using One = std::integral_constant<int, 1>;
-        using Four = std::integral_constant<int, 4>;
+        using Most = std::integral_constant<int, MOST>;
         if (vec) {
-            if (pieces4 >= 2048) f(T, std::true_type{}, Four{});
+            if (pieces >= 2048) f(T, std::true_type{}, Most{});
             else f(T, std::true_type{}, One{});
         } else {
             f(T, std::false_type{}, One{});
@@ -389,7 +413,7 @@ void by_form(int type, bool vec, int64_t tokens, int D, const F& f) {
 }  // namespace
 
 int64_t moe_sort_work_bytes(int64_t S, int E) {
-    const int64_t nb = (S + kSortChunk - 1) / kSortChunk;
+    const int64_t nb = sort_blocks(S);
     return nb > 1 ? nb * (E + 1) * int64_t(sizeof(int)) : 0;
 }
 
@@ -405,7 +429,7 @@ hipError_t moe_sort(hipStream_t st, const void* ids, bool wide, int* order, int*
 
 hipError_t moe_dispatch(hipStream_t st, const void* x, int type, int64_t ldx, const int* position,
                         const int* offsets, void* out, int64_t tokens, int top, int E, int D) {
-    by_form(type, vec_rows(x, ldx, type, D) && vec_rows(out, D, type, D), tokens, D,
+    by_form<4>(type, vec_rows(x, ldx, type, D) && vec_rows(out, D, type, D), tokens, D,
             [&](auto T, auto V, auto U) {
         constexpr int t = decltype(T)::value, u = decltype(U)::value;
         const int pieces = (D + 512 * u - 1) / (512 * u);
@@ -420,7 +444,7 @@ hipError_t moe_dispatch(hipStream_t st, const void* x, int type, int64_t ldx, co
 hipError_t moe_gather(hipStream_t st, const void* z, int type, int64_t ldz, const int* position,
                       const int* offsets, const float* weights, void* out, int out_type,
                       int64_t tokens, int top, int E, int D) {
-    by_form(type, vec_rows(z, ldz, type, D) && vec_rows(out, D, out_type, D), tokens, D,
+    by_form<1>(type, vec_rows(z, ldz, type, D) && vec_rows(out, D, out_type, D), tokens, D,
             [&](auto T, auto V, auto U) {
         constexpr int t = decltype(T)::value, u = decltype(U)::value;
         constexpr bool v = decltype(V)::value;

@@ -27,6 +27,15 @@ def test_sort(dev, dtype, t, top, experts, dropped):
         assert torch.equal(g.cpu(), w), name
 
 
+@pytest.mark.parametrize("slots", [63, 64, 65, 1023, 1024, 1025, 2047, 2048, 2049, 4097, 8191,
+                                   8192, 8193, 131071, 131072, 131073, 140001])
+@pytest.mark.parametrize("experts", [1, 1023, 1024])
+def test_sort_sizes(dev, slots, experts):
+    _, got, want = routed(slots, 1, experts, dev, seed=slots, dropped=0.03)
+    for g, w, name in zip(got, want, got._fields):
+        assert torch.equal(g.cpu(), w), name
+
+
 def test_sort_ids_out_of_range(dev):
     ids = torch.tensor([[0, 1 << 40], [-(1 << 40), 2], [3, 4], [5, 1 << 32], [-1, 4]])
     for i in (ids, ids.clamp(-(1 << 31), (1 << 31) - 1).int()):
