@@ -74,7 +74,7 @@ int product(const void* stream, const void* x, int32_t type, int64_t ldx, const 
             int64_t E, const void* bias, int32_t bias_type, void* y, int64_t R, int64_t N,
             int64_t K, void* work, int64_t work_bytes, const char* what) {
     const bool grouped = offsets != nullptr;
-    const bool fused = mx4_fused(R, grouped, int(E));
+    const bool fused = mx4_fused(R, grouped, int(E), K);
     if (!fused) {
         if (!work) return fail(6, "work must not be null");
         if (reinterpret_cast<uintptr_t>(work) % 16 != 0)
@@ -145,7 +145,7 @@ int xpuint8_mxfp4_dequantize_stream(const void* stream, const uint8_t* codes,
 
 int64_t xpuint8_mxfp4_linear_workspace_size(int64_t M, int64_t N, int64_t K) {
     if (check_product(M, M, N, K, false, 0) != 0) return -1;
-    return mx4_fused(M, false, 0) ? 0 : quantized_bytes(M, K);
+    return mx4_fused(M, false, 0, K) ? 0 : quantized_bytes(M, K);
 }
 
 int xpuint8_mxfp4_linear_stream(const void* stream, const void* x, int32_t type, int64_t ldx,
@@ -165,7 +165,7 @@ int xpuint8_mxfp4_linear_stream(const void* stream, const void* x, int32_t type,
 int64_t xpuint8_mxfp4_grouped_linear_workspace_size(int64_t R, int64_t tokens, int64_t E,
                                                     int64_t N, int64_t K) {
     if (check_product(R, tokens, N, K, true, E) != 0) return -1;
-    return mx4_fused(R, true, int(E)) ? 0 : quantized_bytes(tokens, K);
+    return mx4_fused(R, true, int(E), K) ? 0 : quantized_bytes(tokens, K);
 }
 
 int xpuint8_mxfp4_grouped_linear_stream(const void* stream, const void* x, int32_t type,

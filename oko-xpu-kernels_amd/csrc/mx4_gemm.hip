@@ -30,86 +30,236 @@ __device__ __forceinline__ v4f mfma4(const v4i& w, int sw, const v4i& x, int sx,
 }
 
 // ----------------------------------------------------------------- few rows
-// Up to 16 rows a tile: the product reads the weight once and is bound by that.
-// A block owns 16 weight rows and all of K, its NW waves every NW-th 512
-// values: lane l takes row l % 16 and the blocks 4j + l / 16 (j = 0..3), so a
-// load instruction covers 64 consecutive bytes of 16 rows, and the row's 16 scale
-// bytes, of which byte l / 16 of dword j belongs to block j.  x is quantized here,
-// in the registers of the lane that multiplies it (a lane's operand is exactly one
-// block), so there is one launch and no quantized copy; the NW partial sums meet
-// in LDS.
+// Up to 16 MB rows of a group: the product reads the weight once and is bound by that and by
+// the latencies around it.  A block takes `nt` consecutive blocks of 16 weight rows and all
+// of K, its NW waves SS groups of 512 values each: lane l takes row l % 16 and the blocks
+// 4j + l / 16 (j = 0..3) of a group, so a load covers 64 consecutive bytes of 16 rows, and
+// the row's 16 scale bytes, of which byte l / 16 of dword j belongs to block j.  x stays in
+// registers for all nt; the next 16 weight rows are requested before this block's are used
+// (three steps ahead measured the same); the NW partial sums meet in LDS (two buffers: one
+// barrier a block).
+//
+// FUSED (MB = 1): x is quantized here, in the registers of the lane that multiplies it (a
+// lane's operand is exactly one block), so there is one launch and no quantized copy.
+// With more rows every block would read all of x in its own type, 2 KB a row and 1024
+// values against 0.5: those take x quantized by a launch before, and so does a K that the
+// waves do not hold at once, which is walked in chunks with x read again for each.
+//
+// MI355X, kernel alone: 1 x 4096 x 4096 5.9 us; 48 x 4096 x 14336 12.9 us (2.4 TB/s of
+// weight); 16 rows of 13 experts of 2048 x 2816 11.2 us (3.6 TB/s).
 template <int T, bool VEC>
-__device__ __forceinline__ void quantize_block(const char* p, v4i& codes, int& scale) {
-    float v[4][8];
+struct Block {                                            // 32 values as they are stored
+    uint4 v[T == kF32 ? 8 : 4];
+    __device__ __forceinline__ void load(const char* p) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) load8<T, VEC>(p + c * 8 * kSize<T>, v[c]);
-    uint32_t m = 0;
+        for (int i = 0; i < (T == kF32 ? 8 : 4); ++i) {
+            if constexpr (VEC) {
+                v[i] = reinterpret_cast<const uint4*>(p)[i];
+            } else {
+                uint32_t d[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (T == kF32) {
+                        d[j] = reinterpret_cast<const uint32_t*>(p)[4 * i + j];
+                    } else {
+                        const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + 8 * i + 2 * j;
+                        d[j] = uint32_t(h[0]) | (uint32_t(h[1]) << 16);
+                    }
+                }
+                v[i] = make_uint4(d[0], d[1], d[2], d[3]);
+            }
+        }
+    }
+    __device__ __forceinline__ void quantize(v4i& codes, int& scale) const {
+        float f[4][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[c][i]));
-    const uint32_t e = mx_scale_byte(m);
+        for (int c = 0; c < 4; ++c) load8<T, true>(v + c * (T == kF32 ? 2 : 1), f[c]);
+        uint32_t m = 0;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) codes[c] = int(mx_encode8(v[c], e));
-    scale = int(e);
-}
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, abs_bits(f[c][i]));
+        const uint32_t e = mx_scale_byte(m);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) codes[c] = int(mx_encode8(f[c], e));
+        scale = int(e);
+    }
+};
 
-template <int T, bool VEC, int NW>
-__global__ __launch_bounds__(NW * 64) void mx4_skinny_kernel(
-    const char* __restrict__ x, int64_t ldx, const int* __restrict__ rows, int tokens, Weight w,
-    const int* __restrict__ offsets, int E, Out out) {
+constexpr int kFewTiles = 64;                             // blocks of weight rows a block takes at most
+
+// x as a kernel of few rows takes it: its own type (FUSED), or codes and scales
+struct Rows {
+    const char* x;
+    int64_t ldx;
+    const uint8_t *codes, *scales;
+    const int* rows;
+    int tokens;
+};
+
+template <int T, bool VEC, bool FUSED, int MB, int NW, int SS, int D, bool CHUNKS>
+__global__ __launch_bounds__(NW * 64) void mx4_few_kernel(Rows x, Weight w,
+                                                          const int* __restrict__ offsets, int E,
+                                                          Out out, int nt) {
+    static_assert(!FUSED || (MB == 1 && !CHUNKS), "one block of rows is quantized in place");
+    static_assert(MB <= NW, "a wave adds up a block of rows");
+    constexpr int kChunk = NW * SS * 512;
+    __shared__ v4f part[2][NW][MB][64];
+    __shared__ v4f bias[kFewTiles][4];
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     RowTile t;
-    if (!row_tile<16>(offsets, E, out.R, blockIdx.y, t)) return;
-    const int n0 = blockIdx.x * 16;
-    const int row = t.row + r;
-    if (t.e == E) {                                    // rows of no group
-        if (wave == 0 && row < t.end)
-            store4<T>(out, row, n0 + 4 * g, v4f{0.f, 0.f, 0.f, 0.f});
+    if (!row_tile<16 * MB>(offsets, E, out.R, blockIdx.y, t)) return;
+    const int tiles = (out.N + 15) / 16, first = blockIdx.x * nt, last = min(first + nt, tiles);
+    if (t.e == E) {                                       // rows of no group
+        for (int i = first; i < last; ++i)
+            for (int b = wave; b < MB; b += NW)
+                if (t.row + 16 * b + r < t.end)
+                    store4<T>(out, t.row + 16 * b + r, 16 * i + 4 * g, v4f{0.f, 0.f, 0.f, 0.f});
         return;
     }
-    __shared__ v4f part[NW][64];
-    const bool has = row < t.end;
-    int src = has ? row : t.row;
-    if (rows) src = min(max(rows[src], 0), tokens - 1);
-    const char* xrow = x + src * ldx * kSize<T>;
-    const int64_t wr = int64_t(t.e) * w.N + min(n0 + r, w.N - 1);
-    const uint8_t* wc = w.codes + wr * (w.K / 2);
-    const uint8_t* ws = w.scales + wr * w.SW;
-    v4f acc = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = wave * 512; k0 < w.K; k0 += NW * 512) {
-        v4i wf[4], xf[4];
-        int xs[4];
-        const uint4 s = *reinterpret_cast<const uint4*>(ws + k0 / 32);
+    const int K = w.K, chunks = CHUNKS ? (K + kChunk - 1) / kChunk : 1;
+    auto k_of = [&](int c, int s, int j) { return c * kChunk + (wave + NW * s) * 512 + 128 * j + 32 * g; };
+    struct Slab {
+        v4i f[SS][4];
+        uint4 s[SS];
+    };
+    const uint8_t* const wc = w.codes + int64_t(t.e) * w.N * (K / 2);
+    const uint8_t* const wsc = w.scales + int64_t(t.e) * w.N * w.SW;
+    // Every load is made, so that the waits can count the loads behind them: past K the
+    // last block again (against zeros of x), past the last step one address for all lanes.
+    auto load = [&](Slab& d, int tile, int c) __attribute__((always_inline)) {
+        const int real = (tile - last) >> 31;             // -1, or 0 past the last step
+        const int64_t row = min(16 * tile + r, w.N - 1) & real;
+        const uint8_t* const code = wc + row * (K / 2);
+        const uint8_t* const scale = wsc + row * w.SW;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = k0 + 128 * j + 32 * g;
-            wf[j] = v4i{0, 0, 0, 0};
-            if (k < w.K) wf[j] = *reinterpret_cast<const v4i*>(wc + k / 2);
+        for (int s = 0; s < SS; ++s) {
+            const int k0 = c * kChunk + (wave + NW * s) * 512;
+            d.s[s] = *reinterpret_cast<const uint4*>(scale + (min(k0 / 32, w.SW - 16) & real));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                d.f[s][j] = *reinterpret_cast<const v4i*>(code + ((min(k_of(c, s, j), K - 32) / 2) & real));
+        }
+    };
+    Slab slab[D];
+    int ahead = first, ca = 0;                            // the next step to request
+    auto request = [&](Slab& d) __attribute__((always_inline)) {
+        load(d, ahead, ca);
+        if constexpr (CHUNKS) ca = ca + 1 < chunks ? ca + 1 : 0;
+        ahead += ca == 0;
+        __builtin_amdgcn_sched_barrier(0);                // the loads stay in this order
+    };
+    v4i xf[MB][SS][4];
+    int xs[MB][SS][4];
+    // the blocks of x, zeros past K and past the last row; `between` runs once the first
+    // of them are requested
+    auto load_x = [&](int c, auto between) __attribute__((always_inline)) {
+        int src[MB];
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            src[m] = min(t.row + 16 * m + r, t.end - 1);
+            if (x.rows) src[m] = min(max(x.rows[src[m]], 0), x.tokens - 1);
+        }
+        if constexpr (FUSED) {
+            const char* const row = x.x + src[0] * x.ldx * kSize<T>;
+#pragma unroll
+            for (int s = 0; s < SS; ++s) {
+                Block<T, VEC> raw[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) raw[j].load(row + min(k_of(c, s, j), K - 32) * kSize<T>);
+                if (s == 0) between();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) raw[j].quantize(xf[0][s][j], xs[0][s][j]);
+            }
+        } else {
+            uint4 sc[MB][SS];
+#pragma unroll
+            for (int m = 0; m < MB; ++m)
+#pragma unroll
+                for (int s = 0; s < SS; ++s) {
+                    const int k0 = c * kChunk + (wave + NW * s) * 512;
+                    sc[m][s] = *reinterpret_cast<const uint4*>(x.scales + int64_t(src[m]) * w.SW +
+                                                               min(k0 / 32, w.SW - 16));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        xf[m][s][j] = *reinterpret_cast<const v4i*>(
+                            x.codes + int64_t(src[m]) * (K / 2) + min(k_of(c, s, j), K - 32) / 2);
+                }
+            between();
+#pragma unroll
+            for (int m = 0; m < MB; ++m)
+#pragma unroll
+                for (int s = 0; s < SS; ++s) {
+                    const uint32_t d[4] = {sc[m][s].x, sc[m][s].y, sc[m][s].z, sc[m][s].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) xs[m][s][j] = int(d[j] >> (8 * g));
+                }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = k0 + 128 * j + 32 * g;
-            xf[j] = v4i{0, 0, 0, 0};
-            xs[j] = 127;
-            if (k < w.K && has) quantize_block<T, VEC>(xrow + k * kSize<T>, xf[j], xs[j]);
-        }
-        const uint32_t sw[4] = {s.x, s.y, s.z, s.w};
+        for (int m = 0; m < MB; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = k0 + 128 * j + 32 * g;
-            const int b = k < w.K ? int(sw[j] >> (8 * g)) : 127;     // (byte 0 is read)
-            acc = mfma4<0, 0>(wf[j], b, xf[j], xs[j], acc);
-        }
-    }
-    part[wave][lane] = acc;
-    __syncthreads();
-    if (wave != 0 || !has) return;
+            for (int s = 0; s < SS; ++s)
 #pragma unroll
-    for (int i = 1; i < NW; ++i) acc += part[i][lane];
-    const int n = n0 + 4 * g;
-    store4<T>(out, row, n, acc + v4f{bias_at(out, n), bias_at(out, n + 1), bias_at(out, n + 2), bias_at(out, n + 3)});
+                for (int j = 0; j < 4; ++j) {
+                    const bool in = k_of(c, s, j) < K && t.row + 16 * m + r < t.end;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) xf[m][s][j][i] = in ? xf[m][s][j][i] : 0;
+                    xs[m][s][j] = in ? xs[m][s][j] : 127;
+                }
+    };
+    if (out.bias)                                         // (a load among the steps would wait for theirs)
+        for (int i = threadIdx.x; i < 16 * (last - first); i += NW * 64)
+            reinterpret_cast<float*>(bias)[i] = bias_at(out, 16 * first + i);
+    v4f acc[MB];
+    auto use = [&](const Slab& d, int tile, int c, int buf) __attribute__((always_inline)) {
+        if (c == 0)
+#pragma unroll
+            for (int m = 0; m < MB; ++m) acc[m] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < SS; ++s) {
+            const uint32_t sw[4] = {d.s[s].x, d.s[s].y, d.s[s].z, d.s[s].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int ws = k_of(c, s, j) < K ? int(sw[j] >> (8 * g)) : 127;  // (byte 0 is read)
+#pragma unroll
+                for (int m = 0; m < MB; ++m) acc[m] = mfma4<0, 0>(d.f[s][j], ws, xf[m][s][j], xs[m][s][j], acc[m]);
+            }
+        }
+        if (c + 1 < chunks) return;
+#pragma unroll
+        for (int m = 0; m < MB; ++m) part[buf][wave][m][lane] = acc[m];
+        __syncthreads();
+        if (wave >= MB || tile >= last) return;
+        const int row = t.row + 16 * wave + r, n = 16 * tile + 4 * g;
+        if (row >= t.end) return;
+        v4f sum = part[buf][0][wave][lane];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) sum += part[buf][i][wave][lane];
+        if (out.bias) sum += bias[tile - first][g];
+        store4<T>(out, row, n, sum);
+    };
+    load_x(0, [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i + 1 < D; ++i) request(slab[i]);
+    });
+    // One step a block of weight rows and chunk of K, requested D - 1 steps ahead.  The loop
+    // ends after D steps only (those past the last store nothing): an exit among them
+    // would join states with different loads under way, and every wait be for all.
+    int tile = first, c = 0, buf = 0;
+    do {
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            request(slab[(i + D - 1) % D]);
+            use(slab[i], tile, c, buf);
+            if constexpr (CHUNKS) c = c + 1 < chunks ? c + 1 : 0;
+            if (c == 0) {
+                buf ^= 1;
+                ++tile;
+            }
+            if constexpr (CHUNKS) load_x(c, [] {});
+        }
+    } while (tile < last);
 }
 
 // -------------------------------------------------------------------- tiles
@@ -453,30 +603,69 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
 
 }  // namespace
 
-// Up to 16 rows a group on average the weight's bytes are the product's time and
-// the quantizer's launch would be most of the rest.
-bool mx4_fused(int64_t R, bool grouped, int E) { return R <= 16 * int64_t(grouped ? E : 1); }
+namespace {
+
+constexpr int64_t kFusedK = 8 * 2 * 512;              // values of a row that the waves hold
+
+// rows of x in their own type or quantized (codes), on the kernel of few rows
+template <int T, bool VEC, bool FUSED, int MB>
+hipError_t few(hipStream_t st, const Rows& x, const Weight& w, const int* offsets, int E,
+               const Out& o) {
+    const int tiles = (o.N + 15) / 16;
+    const int64_t tm = most_tiles(offsets != nullptr, o.R, E, 16 * MB);
+    // Weight blocks a block: as many blocks as the device holds at once (four waves a SIMD
+    // by registers, two with four blocks of rows), since each reads all its rows of x
+    // again.  Of many groups most are empty, or hold one row.
+    const int64_t busy = offsets ? std::min<int64_t>(o.R, E) : tm;
+    const int nw = w.K <= 4 * 512 ? 4 : 8;
+    const int64_t want = int64_t(device_cus()) * (MB == 4 ? 8 : 16) / nw;
+    const int nt = int(std::clamp<int64_t>((tiles * busy + want - 1) / want, 1, kFewTiles));
+    auto go = [&](auto W, auto S, auto D, auto C) {
+        constexpr int nw = decltype(W)::value, ss = decltype(S)::value, d = decltype(D)::value;
+        hipLaunchKernelGGL((mx4_few_kernel<T, VEC, FUSED, MB, nw, ss, d, decltype(C)::value>),
+                           dim3(unsigned((tiles + nt - 1) / nt), unsigned(tm)), dim3(nw * 64), 0, st,
+                           x, w, offsets, E, o, nt);
+        return hipGetLastError();
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    using Four = std::integral_constant<int, 4>;
+    using Eight = std::integral_constant<int, 8>;
+    using Groups = std::integral_constant<int, MB == 1 ? 2 : 1>;
+    auto whole = [&](auto W, auto S) {                   // (one step: nothing to request ahead)
+        if (nt == 1) return go(W, S, One{}, std::false_type{});
+        return go(W, S, Two{}, std::false_type{});
+    };
+    if (nw == 4) return whole(Four{}, One{});
+    if (w.K <= 8 * 512) return whole(Eight{}, One{});
+    if constexpr (FUSED) return whole(Eight{}, Groups{});
+    else return go(Eight{}, Groups{}, Two{}, std::true_type{});
+}
+
+}  // namespace
+
+// Up to 16 rows a group on average the weight's bytes are the product's time and the
+// quantizer's launch (2 to 3 us) would be a third of the rest.
+bool mx4_fused(int64_t R, bool grouped, int E, int64_t K) {
+    return R <= 16 * int64_t(grouped ? E : 1) && K <= kFusedK;
+}
 
 hipError_t mx4_product_fused(hipStream_t st, const void* x, int type, int64_t ldx,
                              const int* rows, int64_t tokens, const uint8_t* wc,
                              const uint8_t* ws, const int* offsets, int E, void* y,
                              const void* bias, int bias_type, int64_t R, int N, int K) {
-    constexpr int NW = 8;
     const Weight w{wc, ws, N, K, int(mx_scale_width(K))};
     const Out o = make_out(y, type, bias, bias_type, R, N);
     const int size = type == kF32 ? 4 : 2;
     const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * size) % 16 == 0;
-    const dim3 grid(unsigned((N + 15) / 16), unsigned(most_tiles(offsets != nullptr, R, E, 16)));
+    const Rows in{static_cast<const char*>(x), ldx, nullptr, nullptr, rows, int(tokens)};
+    hipError_t e = hipSuccess;
     by_type(type, [&](auto T) {
         constexpr int t = decltype(T)::value;
-        if (vec)
-            hipLaunchKernelGGL((mx4_skinny_kernel<t, true, NW>), grid, dim3(NW * 64), 0, st,
-                               static_cast<const char*>(x), ldx, rows, int(tokens), w, offsets, E, o);
-        else
-            hipLaunchKernelGGL((mx4_skinny_kernel<t, false, NW>), grid, dim3(NW * 64), 0, st,
-                               static_cast<const char*>(x), ldx, rows, int(tokens), w, offsets, E, o);
+        e = vec ? few<t, true, true, 1>(st, in, w, offsets, E, o)
+                : few<t, false, true, 1>(st, in, w, offsets, E, o);
     });
-    return hipGetLastError();
+    return e;
 }
 
 namespace {
@@ -509,6 +698,21 @@ hipError_t mx4_product(hipStream_t st, const uint8_t* xc, const uint8_t* xs, con
                        int K) {
     const Weight w{wc, ws, N, K, int(mx_scale_width(K))};
     const Out o = make_out(y, type, bias, bias_type, R, N);
+    // Up to 64 rows the kernel of few rows: 64 x 4096 x 4096 12.5 us with the quantizer against
+    // 17.5 in tiles, 64 x 4096 x 14336 16.1 / 18.2, 48 x 14336 x 4096 27 / 38; 96 rows would
+    // take its block twice, and tiles need 17.5.
+    const int64_t per_group = offsets ? (R + E - 1) / E : R;
+    if (per_group <= 64) {
+        const Rows in{nullptr, 0, xc, xs, rows, int(tokens)};
+        hipError_t e = hipSuccess;
+        by_type(type, [&](auto T) {
+            constexpr int t = decltype(T)::value;
+            e = per_group <= 16   ? few<t, true, false, 1>(st, in, w, offsets, E, o)
+                : per_group <= 32 ? few<t, true, false, 2>(st, in, w, offsets, E, o)
+                                  : few<t, true, false, 4>(st, in, w, offsets, E, o);
+        });
+        return e;
+    }
     auto go = [&](auto M, auto N_) {
         constexpr int BM = decltype(M)::value, BN = decltype(N_)::value;
         const int tiles_n = (N + BN - 1) / BN;

@@ -17,7 +17,7 @@ hipError_t mx4_dequantize(hipStream_t st, const uint8_t* codes, const uint8_t* s
 // mx4_gemm.hip: y [R, N] = xq[rows] wq^T [+ bias] over the groups of offsets [E + 1]
 // (null: one group of all R rows); rows (null: row i is x's row i) indexes the
 // `tokens` rows of x.  mx4_product_fused quantizes x itself (mx4_fused says when).
-bool mx4_fused(int64_t R, bool grouped, int E);
+bool mx4_fused(int64_t R, bool grouped, int E, int64_t K);
 hipError_t mx4_product_fused(hipStream_t st, const void* x, int type, int64_t ldx,
                              const int* rows, int64_t tokens, const uint8_t* wc,
                              const uint8_t* ws, const int* offsets, int E, void* y,

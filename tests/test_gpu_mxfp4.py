@@ -139,6 +139,37 @@ def test_linear(dev, dtype, m, k, n):
     check_linear(dev, x, n, bias=randn(n, seed=2, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype,m,k,n", [
+    (torch.bfloat16, 1, 2048, 8209), (torch.float16, 16, 4096, 8232), (torch.float32, 2, 8192, 8200),
+    (torch.bfloat16, 9, 8224, 40), (torch.float32, 5, 16416, 72), (torch.float16, 3, 4128, 16500),
+    (torch.float16, 32, 2080, 4111), (torch.bfloat16, 33, 2048, 8212), (torch.float32, 17, 8256, 56),
+    (torch.bfloat16, 64, 4128, 4200), (torch.float16, 49, 12320, 4112), (torch.float32, 65, 640, 200)])
+def test_linear_few_rows(dev, dtype, m, k, n):
+    """One to four blocks of 16 rows, K on both sides of what a block's waves hold, weights
+    with several and ragged blocks of rows each."""
+    x = randn(m, k, seed=m, dtype=dtype)
+    x[:, 5::37] *= 30
+    check_linear(dev, x, n, bias=randn(n, seed=2, dtype=dtype))
+
+
+@pytest.mark.parametrize("t,top,experts,k,n,dropped", [
+    (3, 3, 40, 2080, 2056, 0.0), (60, 4, 10, 544, 300, 0.1), (60, 4, 10, 4160, 136, 0.1),
+    (100, 5, 9, 288, 520, 0.05), (70, 6, 8, 4128, 72, 0.0), (31, 2, 4, 8224, 40, 0.2)])
+def test_grouped_few_rows(dev, t, top, experts, k, n, dropped):
+    """Groups of fewer and of more rows than a block takes."""
+    ids = router(t, top, experts, seed=t, dropped=dropped)
+    routing = moe.sort(ids.to(dev), experts)
+    _, _, orows, ooff = O.sort(ids, experts)
+    codes, scales = mxfp4.quantize(randn(experts, n, k, seed=7, scale=0.05).to(dev))
+    wq = O.dequantize(codes.cpu(), scales.cpu())
+    for gather in (False, True):
+        x = randn(t if gather else t * top, k, seed=8, dtype=torch.bfloat16)
+        rows = orows if gather else torch.arange(t * top, dtype=torch.int32)
+        xq = O.dequantize(*O.quantize(x))
+        y = mxfp4.grouped_linear(x.to(dev), codes, scales, routing, gather=gather)
+        assert_close(y, O.grouped(xq, wq, rows, ooff), O.grouped(xq.abs(), wq.abs(), rows, ooff), k)
+
+
 @pytest.mark.parametrize("dtype,m,k,n", [(torch.bfloat16, 4090, 8160, 4080),
                                          (torch.bfloat16, 4001, 8192, 4081),
                                          (torch.float32, 3890, 7968, 4096)])
@@ -256,6 +287,21 @@ def test_linear_gradients(dev, dtype, m, k, n):
     assert dx.dtype == dtype and db.dtype == dtype
     assert_close(dx, d @ wq, d.abs() @ wq.abs(), 3 * n)
     assert_close(db, d.sum(0), d.abs().sum(0), m + 1)
+
+
+@pytest.mark.parametrize("m,k,n", [(127, 96, 64), (128, 96, 64), (129, 1056, 272), (128, 96, 72),
+                                   (700, 2080, 1040)])
+def test_linear_gradient_of_many_rows(dev, m, k, n):
+    """Both sides of the sizes at which dx of a bf16 product is taken from the weight read
+    back, contiguous and strided."""
+    (codes, scales), wq = weight(n, k, 3, dev)
+    x = randn(m, k, seed=m, dtype=torch.bfloat16).to(dev).requires_grad_()
+    y = mxfp4.linear(x, codes, scales)
+    base = randn(m, n + 24, seed=4, dtype=torch.bfloat16).to(dev)
+    for dy in (base[:, :n].contiguous(), base[:, :n], base[:, 3:n + 3], base[:, :1].expand(m, n)):
+        dx, = torch.autograd.grad(y, x, dy, retain_graph=True)
+        d = dy.cpu().double()
+        assert_close(dx, d @ wq, d.abs() @ wq.abs(), 3 * n)
 
 
 def test_linear_gradient_of_strided_dy(dev):
