@@ -14,46 +14,62 @@ namespace xpuint8 {
 namespace {
 
 // ------------------------------------------------------------------- split
-// dy [R, N] as PIECES bf16 pieces, each of `width` columns (zeros past N)
-template <int T, int PIECES>
+// dy [R, N] as PIECES bf16 pieces, each of `width` columns (zeros past N); a thread takes 8
+// columns, in one load where dy's rows are whole, aligned 8s (VEC).  Bound by its bytes.
+template <int T, bool VEC, int PIECES>
 __global__ __launch_bounds__(256) void mx4_split_kernel(const char* __restrict__ dy, int64_t ldy,
                                                         uint16_t* __restrict__ out, int64_t R,
                                                         int N, int width) {
     const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t row = i / width;
-    const int n = int(i - row * width);
+    const int64_t row = i / (width / 8);
+    const int n = int(i - row * (width / 8)) * 8;
     if (row >= R) return;
-    float v = 0.f;
-    if (n < N) {
-        const char* p = dy + (row * ldy + n) * kSize<T>;
-        if constexpr (T == kF32) v = *reinterpret_cast<const float*>(p);
-        else if constexpr (T == kBf16) v = bf16_to_f32(*reinterpret_cast<const uint16_t*>(p));
-        else v = float(*reinterpret_cast<const _Float16*>(p));
+    const char* p = dy + (row * ldy + n) * kSize<T>;
+    float v[8];
+    if (n + 8 <= N) {
+        load8<T, VEC>(p, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = 0.f;
+            if (n + j >= N) continue;
+            if constexpr (T == kF32) v[j] = reinterpret_cast<const float*>(p)[j];
+            else if constexpr (T == kBf16) v[j] = bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[j]);
+            else v[j] = float(reinterpret_cast<const _Float16*>(p)[j]);
+        }
     }
     uint16_t* o = out + row * (int64_t(width) * PIECES) + n;
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
-        // truncated, not rounded: a piece never exceeds what is left, so the largest
-        // values stay finite; what an infinity or NaN leaves is not another one
-        uint32_t u = __float_as_uint(v);
-        uint32_t h = u >> 16;
-        if ((u & 0x7FFFFFFFu) > 0x7F800000u) h |= 0x40u;
-        o[int64_t(q) * width] = uint16_t(h);
-        v = (u & 0x7F800000u) == 0x7F800000u ? 0.f : v - __uint_as_float(h << 16);
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // truncated, not rounded: a piece never exceeds what is left, so the largest
+            // values stay finite; what an infinity or NaN leaves is not another one
+            const uint32_t u = __float_as_uint(v[j]);
+            h[j] = u >> 16;
+            if ((u & 0x7FFFFFFFu) > 0x7F800000u) h[j] |= 0x40u;
+            v[j] = (u & 0x7F800000u) == 0x7F800000u ? 0.f : v[j] - __uint_as_float(h[j] << 16);
+        }
+        *reinterpret_cast<uint4*>(o + int64_t(q) * width) =
+            make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
 }
 
 // ------------------------------------------------------------------- tiles
 // BM x BK tiles of dx by a block of 4 waves in 2 x 2 (a wave every other 16 rows, one
-// half of the columns), 64 contraction rows a stage (two MFMAs of each block), two LDS
-// slots.  While a stage's first half runs, a wave reads the second half's fragments; one
-// wait and barrier then mean that every wave has read the stage, and that the next one
-// is in; while the second half runs, it reads the next stage's first fragments, refills
-// the slot with dy by direct loads, and writes the weight's rows there as bf16, which it
-// has loaded a stage earlier (a thread BK / 4 consecutive values' codes and scales).
-// (A ring of 32-row steps with a load four steps ahead, as the forward product's, is
-// slower at 128 x 128: dy's rows then come in 64-byte pieces, and the L2's requests, not
-// its bytes, bound such tiles; 16380 x 2816 -> 2048 in 32 groups 290 us.)
+// half of the columns), 64 contraction rows a stage (two MFMAs of each block); dy in
+// three LDS slots, the weight in two.  While a stage's first half runs, a wave reads the
+// second half's fragments; one wait and barrier then mean that every wave has read the
+// stage, and that the next one is in; while the second half runs, it reads the next
+// stage's first fragments, requests dy three stages ahead into the slot by direct loads,
+// and writes the weight's rows of two stages ahead as bf16 from the codes and scales that
+// it loaded two stages before (a thread BK / 4 consecutive values).
+// (One slot and one stage less of each: 5 to 13% slower.  A ring of 32-row steps with a
+// load four steps ahead, as the forward product's: slower at 128 x 128; dy's rows then
+// come in 64-byte pieces, and the L2's requests, not its bytes, bound such tiles.)
+// Bound by the LDS (96 KB a stage and 128 x 128 tile, 768 cycles) beside the MFMAs (512):
+// 8192^3 in two pieces 1.20 PFLOP/s, 16380 x 2816 -> 2048 in 32 groups 270 us, 0.70.
 //
 // dy's 128 bytes of a row: chunk c (16 bytes) at c ^ ((row >> 1) & 7).  The weight's rows
 // lie as they come, 2 BK bytes each, for the transposing read ds_read_b64_tr_b16: in
@@ -94,11 +110,11 @@ __global__ __launch_bounds__(256, BM * BK > 128 * 128 ? 1 : 2) void mx4_dx_kerne
     const uint16_t* __restrict__ dy, int64_t ldy, int pieces, int width, Weight w,
     const int* __restrict__ offsets, int E, Out out, int type, int tiles_m, int tiles_k) {
     constexpr int TM = BM / 32, TK = BK / 32;             // MFMA blocks of a wave
-    constexpr int DY = BM * 128, WROW = 2 * BK, WT = 64 * WROW, STAGE = DY + WT;
+    constexpr int DY = BM * 128, WROW = 2 * BK, WT = 64 * WROW, W0 = 3 * DY;
     constexpr int PX = BM / 32;                           // dy loads a wave a stage
     constexpr int NB = BK / 128;                          // weight blocks a thread a stage
     constexpr int ACC = 4 * TM * TK;                      // block (a, b) is number a * TM + b
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[3 * DY + 2 * WT];
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const int wm = wave >> 1, wk = wave & 1;
@@ -125,31 +141,32 @@ __global__ __launch_bounds__(256, BM * BK > 128 * 128 ? 1 : 2) void mx4_dx_kerne
     // (one piece may end inside a stage: chunks past it come from zeros)
     const uint8_t* const zeros = scalar(g_zero_line);
     const int past = pieces == 1 ? width - c8 : 0x7FFFFFFF;
-    auto issue_dy = [&](int slot, int s, int i) {
+    const int end = min(past, 64 * stages);
+    auto issue_dy = [&](uint32_t slot, int s, int i) {
         const uint8_t* p = scalar(dybase + int64_t(s) * 128) + ady[i];
-        if (s * 64 >= past) p = zeros;
-        dma16(p, smem + slot * STAGE + (wave + 4 * i) * 1024);
+        if (s * 64 >= end) p = zeros;
+        dma16(p, smem + slot + (wave + 4 * i) * 1024);
     };
     // this thread's part of the weight's rows: NB blocks of row nr
     const int nr = threadIdx.x >> 2, part = (threadIdx.x & 3) * NB;
-    uint4 codes[NB];
-    uint32_t scale[NB];
+    struct Part {
+        uint4 codes[NB];
+        uint32_t scale;                                   // (the scale bytes of four blocks)
+        bool in;
+    };
     int un = 0;                                           // the piece's stage that is loaded next
     const uint8_t* const wbase = w.codes + int64_t(t.e) * w.N * (w.K / 2);
     const uint8_t* const wsbase = w.scales + int64_t(t.e) * w.N * w.SW;
-    auto load_w = [&]() {
+    auto load_w = [&](Part& d) __attribute__((always_inline)) {
         const int n = un * 64 + nr;
         const int64_t row = min(n, w.N - 1);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int kb = min(k0 / 32 + part + i, w.K / 32 - 1);     // (columns past K are not stored)
-            codes[i] = *reinterpret_cast<const uint4*>(wbase + row * (w.K / 2) + kb * 16);
-            scale[i] = wsbase[row * w.SW + kb];
-            if (n >= w.N) {
-                codes[i] = make_uint4(0, 0, 0, 0);
-                scale[i] = 0;
-            }
+            d.codes[i] = *reinterpret_cast<const uint4*>(wbase + row * (w.K / 2) + kb * 16);
         }
+        d.scale = *reinterpret_cast<const uint32_t*>(wsbase + row * w.SW + k0 / 32 + (part & ~3));
+        d.in = n < w.N;
         if (++un == per_piece) un = 0;
     };
     const int fn = (nr & 3) | (((nr >> 3) & 1) << 2);
@@ -160,26 +177,27 @@ __global__ __launch_bounds__(256, BM * BK > 128 * 128 ? 1 : 2) void mx4_dx_kerne
     for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            wput[i][h] = sbase + DY + nr * WROW + ((2 * (part + i) + h) ^ fn) * 32;
-    auto put_w = [&](uint32_t slot, int q) {
+            wput[i][h] = sbase + W0 + nr * WROW + ((2 * (part + i) + h) ^ fn) * 32;
+    auto put_w = [&](const Part& d, uint32_t slot, int q) __attribute__((always_inline)) {
         const int i = q >> 2, h = (q >> 1) & 1;
-        const float sc = __uint_as_float(scale[i] << 23);
-        const uint32_t c = (q & 3) == 0 ? codes[i].x : (q & 3) == 1 ? codes[i].y : (q & 3) == 2 ? codes[i].z : codes[i].w;
+        const float sc = __uint_as_float(d.in ? (d.scale >> (8 * ((part + i) & 3)) & 0xFF) << 23 : 0u);
+        const uint32_t cq = (q & 3) == 0 ? d.codes[i].x : (q & 3) == 1 ? d.codes[i].y : (q & 3) == 2 ? d.codes[i].z : d.codes[i].w;
+        const uint32_t c = d.in ? cq : 0u;
         const v4i v = {__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 0)),
                        __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1)),
                        __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 2)),
                        __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 3))};
         asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(wput[i][h] + slot), "v"(v), "n"(16 * (q & 1)) : "memory");
     };
-    auto put_all = [&](uint32_t slot) {
+    auto put_all = [&](const Part& d, uint32_t slot) __attribute__((always_inline)) {
 #pragma unroll
-        for (int q = 0; q < 4 * NB; ++q) put_w(slot, q);
+        for (int q = 0; q < 4 * NB; ++q) put_w(d, slot, q);
     };
     // fragments of half H of a stage: 32 contraction rows
     const uint32_t pos = (g ^ ((r >> 1) & 7)) * 16;       // chunk 4 H + g is at pos ^ (64 H)
     const uint32_t yat = sbase + (wm * 16 + r) * 128 + pos;
     const int fr = (r >> 2) | ((g & 1) << 2);             // of the rows that a lane addresses
-    const uint32_t wrow = sbase + DY + (8 * g + (r >> 2)) * WROW + (r & 3) * 8;
+    const uint32_t wrow = sbase + W0 + (8 * g + (r >> 2)) * WROW + (r & 3) * 8;
     v4i yf[2][TM];
     v2i wl[2][TK], wh[2][TK];
     auto read_y = [&](uint32_t slot, auto H, auto I) {
@@ -205,71 +223,83 @@ __global__ __launch_bounds__(256, BM * BK > 128 * 128 ? 1 : 2) void mx4_dx_kerne
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    load_w();
+    // dy is requested three stages ahead and the weight's codes four, two before they are
+    // written; past the last stage zeros come instead of dy, and codes that go unused
+    Part p0, p1;
+    auto here_now = [&](Part& d) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < PX; ++i) issue_dy(0, 0, i);
+        for (int i = 0; i < NB; ++i)
+            asm volatile("" : "+v"(d.codes[i].x), "+v"(d.codes[i].y), "+v"(d.codes[i].z), "+v"(d.codes[i].w));
+        asm volatile("" : "+v"(d.scale));
+    };
+    constexpr int LATE = PX + NB + 1;                     // the loads of one stage
+    load_w(p0);
+    load_w(p1);
+#pragma unroll
+    for (int i = 0; i < 3 * PX; ++i) issue_dy(i / PX * DY, i / PX, i % PX);
     each<TM * TK>([&](auto I) { acc_set<ACC, decltype(I)::value>(v4f{0.f, 0.f, 0.f, 0.f}); });
-    put_all(0);
-    if (stages > 1) {
-        load_w();
-#pragma unroll
-        for (int i = 0; i < PX; ++i) issue_dy(1, 1, i);
-        put_all(STAGE);
-        load_w();
-    }
+    put_all(p0, 0);
+    load_w(p0);
+    put_all(p1, WT);
+    load_w(p1);
     wait_vm<0>();
+    here_now(p0);
+    here_now(p1);
     lds_done();
     block_barrier();
     each<TM>([&](auto I) { read_y(0, H0{}, I); });
     each<TK>([&](auto I) { read_w(0, H0{}, I); });
     lds_done();
     landed(yf[0]); landed(wl[0]); landed(wh[0]);
-#pragma clang loop unroll(disable)
-    for (int s = 0; s < stages; ++s) {
-        const uint32_t here = (s & 1) * STAGE, next = STAGE - here;
+    uint32_t ynow = 0;
+    auto stage = [&](int s, Part& part, uint32_t here, uint32_t next) __attribute__((always_inline)) {
+        const uint32_t ynext = ynow == 2 * DY ? 0 : ynow + DY;
         {
             v4i wf[TK];
 #pragma unroll
             for (int a = 0; a < TK; ++a) wf[a] = v4i{wl[0][a][0], wl[0][a][1], wh[0][a][0], wh[0][a][1]};
             each<TM>([&](auto B) {
                 constexpr int b = decltype(B)::value;
-                read_y(here, H1{}, B);
+                read_y(ynow, H1{}, B);
                 each<TK / TM>([&](auto I) {
                     read_w(here, H1{}, std::integral_constant<int, b * (TK / TM) + decltype(I)::value>{});
                 });
                 column(H0{}, B, wf);
             });
         }
-        // the second half's fragments, and the next stage: dy's loads and the weight's
-        // writes of every wave
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        // the second half's fragments, and the next stage: dy's loads (all but the latest
+        // stage's) and the weight's writes of every wave
+        __builtin_amdgcn_s_waitcnt(0x0F70 | (LATE & 15) | (LATE >> 4 << 14));   // vmcnt(LATE)
+        lds_done();
         landed(yf[1]); landed(wl[1]); landed(wh[1]);
         block_barrier();
         {
             v4i wf[TK];
 #pragma unroll
             for (int a = 0; a < TK; ++a) wf[a] = v4i{wl[1][a][0], wl[1][a][1], wh[1][a][0], wh[1][a][1]};
-            const bool more = s + 2 < stages;
-            if (more) {
-                put_all(here);
-                load_w();
-            }
+            put_all(part, here);
+            load_w(part);
             // (past the last stage the reads find what the slot held, and go unused)
             each<TM>([&](auto B) {
                 constexpr int b = decltype(B)::value;
-                read_y(next, H0{}, B);
+                read_y(ynext, H0{}, B);
                 each<TK / TM>([&](auto I) {
                     read_w(next, H0{}, std::integral_constant<int, b * (TK / TM) + decltype(I)::value>{});
                 });
-                if (more) {
 #pragma unroll
-                    for (int i = b * PX / TM; i < (b + 1) * PX / TM; ++i) issue_dy(s & 1, s + 2, i);
-                }
+                for (int i = b * PX / TM; i < (b + 1) * PX / TM; ++i) issue_dy(ynow, s + 3, i);
                 column(H1{}, B, wf);
             });
         }
         lds_done();
         landed(yf[0]); landed(wl[0]); landed(wh[0]);
+        ynow = ynext;
+    };
+#pragma clang loop unroll(disable)
+    for (int s = 0; s < stages; s += 2) {
+        stage(s, p0, 0, WT);
+        if (s + 1 == stages) break;
+        stage(s + 1, p1, WT, 0);
     }
     wait_vm<0>();                                         // (the last load_w may be on its way)
     block_barrier();                                      // every wave has read its last stage
@@ -285,21 +315,30 @@ int mx4_split_pieces(int type) { return type == kBf16 ? 1 : type == kF16 ? 2 : 3
 hipError_t mx4_split(hipStream_t st, const void* dy, int type, int64_t ldy, void* out, int64_t R,
                      int N) {
     const int width = int(mx4_split_width(N));
+    const int size = type == kF32 ? 4 : 2;
+    const bool vec = reinterpret_cast<uintptr_t>(dy) % 16 == 0 && (ldy * size) % 16 == 0;
     by_type(type, [&](auto T) {
         constexpr int t = decltype(T)::value;
         constexpr int P = t == kBf16 ? 1 : t == kF16 ? 2 : 3;
-        hipLaunchKernelGGL((mx4_split_kernel<t, P>), dim3(unsigned((R * width + 255) / 256)),
-                           dim3(256), 0, st, static_cast<const char*>(dy), ldy,
-                           static_cast<uint16_t*>(out), R, N, width);
+        auto go = [&](auto V) {
+            hipLaunchKernelGGL((mx4_split_kernel<t, decltype(V)::value, P>),
+                               dim3(unsigned((R * (width / 8) + 255) / 256)), dim3(256), 0, st,
+                               static_cast<const char*>(dy), ldy, static_cast<uint16_t*>(out), R, N,
+                               width);
+        };
+        if (vec) go(std::true_type{});
+        else go(std::false_type{});
     });
     return hipGetLastError();
 }
 
 namespace {
 
-// Whether 256 x 256 tiles (one block a CU) are faster than 128 x 128 (two), by the
-// times that a round of either takes: 8192^3 1004 against 1140 us, 4096^3 131 against
-// 149; 4096 x 1280 -> 5120 94 against 74, 16380 x 2816 -> 2048 in 32 groups the same.
+// Whether 256 x 256 tiles (one block a CU) are faster than 128 x 128 (two), by the times
+// that a round of either takes.  fp16 dy, two pieces, with the split: 8192^3 1840 against
+// 2280 us, 4096^3 240 / 299, 4096 x 1280 -> 5120 160 / 139, 1000 x 4096 -> 4096 209 / 95;
+// bf16, 16384 rows 2816 -> 2048 in 8 groups 238 / 220, in 128 groups 532 / 405, 65520
+// rows in 64 groups 798 / 889.
 bool large_dx_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
     const double stages = double((N + 63) / 64);
     auto tiles = [&](int64_t b) {                          // (a group's last tile half full)
@@ -308,10 +347,10 @@ bool large_dx_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
     };
     const int64_t cus = device_cus();
     const int64_t t128 = tiles(128), t256 = tiles(256);
-    const double large = double((t256 + cus - 1) / cus) * (8.0 + 1.95 * stages);
-    const double small = double(t128 / (2 * cus)) * (4.0 + 1.1 * stages) +
-                         (t128 % (2 * cus) > cus ? 4.0 + 1.1 * stages
-                          : t128 % (2 * cus) > 0 ? 4.0 + 0.65 * stages : 0.0);
+    const double large = double((t256 + cus - 1) / cus) * (8.0 + 1.67 * stages);
+    const double small = double(t128 / (2 * cus)) * (4.0 + 1.06 * stages) +
+                         (t128 % (2 * cus) > cus ? 4.0 + 1.06 * stages
+                          : t128 % (2 * cus) > 0 ? 4.0 + 0.68 * stages : 0.0);
     return large < small;
 }
 
