@@ -264,25 +264,27 @@ __global__ __launch_bounds__(NW * 64) void mx4_few_kernel(Rows x, Weight w,
 
 // -------------------------------------------------------------------- tiles
 // BM x BN tiles of y by a block of 4 waves in 2 x 2 (a wave every other 16 rows, one half
-// of the columns), x already quantized.  K in
-// steps of 128 values, 64 bytes of codes a row and one MFMA of each block, through
-// a ring of four LDS slots that direct global->LDS loads fill four steps ahead.
-// During step t a wave runs its MFMAs on one set of fragments, reads step t + 1's into
-// the other and issues its loads of step t + 4 into the slot of step t, whose last
-// reads the barrier before has seen; the wait and barrier after it see step t + 2
-// land.  So a load has two steps and more to arrive, and a step costs one barrier.
+// of the columns), x already quantized.  K in steps of 128 values, one MFMA of each
+// block, loaded in pairs, 128 bytes of codes a row, through two LDS slots that direct
+// global->LDS loads fill.  During a step a wave runs its MFMAs on one set of fragments and
+// reads the next step's into the other.  After a pair's first step one wait and barrier
+// mean that every wave has read all of the pair, and that the next one is in; during its
+// second step the loads of the pair after that go into its slot.  (64-byte pieces through
+// a ring of four single steps, a barrier a step, had a longer lead and were slower: 4096 x
+// 1280 -> 10240 60 against 56 us with the quantizer, 16380 x 2048 -> 2816 in 32 groups 106 /
+// 101; 8192^3 360 either way.)
 //
-// Chunk c (16 bytes, one block) of a step's row sits at c ^ ((row >> 1) & 3): a
-// 16-byte LDS read serves the lanes 0-3, 12-15, 20-23 and 24-27 together (and so on),
-// which then cover all 64 banks once.  Lane group g holds chunk g, whose scale in
+// Chunk c (16 bytes, one block) of a pair's row sits at c ^ ((row >> 1) & 7): a 16-byte
+// LDS read serves the lanes 0-3, 12-15, 20-23 and 24-27 together (and so on), which
+// then cover all 64 banks once.  Lane group g holds chunk g of a step, whose scale in
 // the row's 16 scale bytes of 512 values (four steps) is byte 4t + g.  The MFMA takes
 // its scale from a byte of a register that the instruction names, the same for all
 // lanes, so each 16 bytes are transposed (4 x 4) where they lie in LDS: lane group g
-// then reads one dword, whose byte t is step t's, and shifts it step by step.  That pass also clears the bytes of
-// blocks past K: 2^-127 in both operands, whose products vanish in fp32 (every code is
-// a number, so what the codes there are does not matter: loads past a row's end
-// repeat its last block).  Scales arrive two groups of four steps ahead, and are
-// transposed one ahead.
+// then reads one dword, whose byte t is step t's, and shifts it step by step.  That pass
+// also clears the bytes of blocks past K: 2^-127 in both operands, whose products vanish
+// in fp32 (every code is a number, so what the codes there are does not matter: loads
+// past a row's end repeat its last block).  Scales arrive two groups of four steps ahead,
+// and are transposed one ahead.
 //
 // The fragment reads are inline assembly (with the builtins the compiler waits for
 // every direct load before each LDS read); nothing is in flight over a loop edge:
@@ -313,14 +315,14 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
     int tiles_n) {
     constexpr int TM = BM / 32, TN = BN / 32;             // MFMA blocks of a wave
     constexpr int ROWS = BM + BN;                         // x rows first
-    constexpr int STEP = ROWS * 64, SCALES = ROWS * 16;
-    constexpr int PX = BM / 64, PW = BN / 64;             // code loads a wave a step
+    constexpr int PAIR = ROWS * 128, SCALES = ROWS * 16;
+    constexpr int PX = BM / 32, PW = BN / 32;             // code loads a wave a pair of steps
     constexpr int PL = PX + PW;
     constexpr int PSX = BM / 64, PS = ROWS / 64;          // scale loads of x, of both, a block
     constexpr int PER_S = (PS + 3) / 4;
     constexpr int PER_T = (ROWS + 255) / 256;             // scale rows a thread transposes
     constexpr int ACC = 4 * TM * TN;                      // block (a, b) is number a * TM + b
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * STEP + 2 * SCALES];
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * PAIR + 2 * SCALES];
     __shared__ float bias_of[BN];
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
@@ -336,9 +338,10 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
     }
     const int K = w.K, KB = K / 2;
     const int steps = (K + 127) / 128, groups = (K + 511) / 512;
-    // Sources: a wave-uniform base and a lane's 32-bit offset from the tile's first
-    // row (a tile spans less than 4 GiB), or, for rows that a list names, the lane's
-    // own address.  Load i of a wave brings 16 rows.
+    // Sources: a wave-uniform base and a lane's 32-bit offset from the tile's first row (a
+    // tile spans less than 4 GiB), load i 32 rows after the first and the last row for
+    // those past it; or, for rows that a list names, the row.  A load of a wave brings 8
+    // rows, its first row is wave * 8 + 32 i.
     const int64_t w0 = int64_t(t.e) * w.N + n0;
     const uint8_t* const wbase = w.codes + w0 * KB;
     const uint8_t* const wsbase = w.scales + w0 * w.SW;
@@ -349,19 +352,16 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
         return GATHER ? min(max(rows[i], 0), tokens - 1) : i - t.row;
     };
     auto w_row = [&](int j) { return min(n0 + j, w.N - 1) - n0; };
-    const int lr = lane >> 2;
-    const uint32_t c16 = uint32_t((lane & 3) ^ ((lr >> 1) & 3)) * 16;
-    std::conditional_t<GATHER, const uint8_t*, uint32_t> ax[PX];
-    uint32_t aw[PW];
+    const int lr = wave * 8 + (lane >> 3);
+    const uint32_t c16 = uint32_t((lane & 7) ^ ((lr >> 1) & 7)) * 16;
+    const uint32_t first = uint32_t(lr) * uint32_t(KB) + c16;
+    const uint32_t xlast = uint32_t(min(t.end - t.row, BM) - 1) * uint32_t(KB) + c16;
+    const uint32_t wlast = uint32_t(min(w.N - n0, BN) - 1) * uint32_t(KB) + c16;
+    int listed[GATHER ? PX : 1];
+    if constexpr (GATHER) {
 #pragma unroll
-    for (int i = 0; i < PX; ++i) {
-        const int j = (wave + 4 * i) * 16 + lr;
-        if constexpr (GATHER) ax[i] = xbase + int64_t(x_row(j)) * KB + c16;
-        else ax[i] = uint32_t(x_row(j)) * uint32_t(KB) + c16;
+        for (int i = 0; i < PX; ++i) listed[i] = x_row(lr + 32 * i);
     }
-#pragma unroll
-    for (int i = 0; i < PW; ++i)
-        aw[i] = uint32_t(w_row((wave + 4 * i) * 16 + lr)) * uint32_t(KB) + c16;
     uint32_t as[PER_S];                                   // 16-byte units: 64 GiB of scales
     const uint8_t* sbs[PER_S];
 #pragma unroll
@@ -371,22 +371,21 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
         as[i] = uint32_t(b < PSX ? x_row(b * 64 + lane) : w_row((b - PSX) * 64 + lane)) *
                 uint32_t(w.SW / 16);
     }
-    // load i of this wave's PX + PW (x first) into the slot, from byte k of the rows
-    // less back (for the last step's chunks past the row's end: its last chunk)
-    auto issue_codes = [&](int slot, int64_t k, uint32_t back, int i) {
+    // load i of this wave's PX + PW (x first) of pair p into its slot, less back (for a last
+    // pair's chunks past the row's end: its last chunk)
+    auto issue_codes = [&](int p, uint32_t back, int i) {
         const bool isx = i < PX;
-        const int b = (wave + 4 * (isx ? i : i - PX)) * 16 + (isx ? 0 : BM);
-        const uint8_t* p;
-        if (isx) {
-            if constexpr (GATHER) p = ax[i] + k - back;
-            else p = scalar(xbase + k) + uint64_t(ax[i] - back);
-        } else {
-            p = scalar(wbase + k) + uint64_t(aw[i - PX] - back);
-        }
-        dma16(p, smem + slot * STEP + b * 64);
+        const int j = isx ? i : i - PX;
+        const uint32_t at = first + uint32_t(32 * j) * uint32_t(KB);
+        const int64_t k = int64_t(p) * 128;
+        const uint8_t* from;
+        if (!isx) from = scalar(wbase + k) + uint64_t(min(at, wlast) - back);
+        else if constexpr (GATHER) from = scalar(xbase + k) + (uint64_t(uint32_t(listed[j])) * uint32_t(KB) + (c16 - back));
+        else from = scalar(xbase + k) + uint64_t(min(at, xlast) - back);
+        dma16(from, smem + (p & 1) * PAIR + (wave * 8 + 32 * j + (isx ? 0 : BM)) * 128);
     };
-    auto past_end = [&](int s) {                          // back, of step s
-        const int over = s * 64 + int(c16) + 16 - KB;
+    auto past_end = [&](int p) {                          // back, of pair p
+        const int over = p * 128 + int(c16) + 16 - KB;
         return over > 0 ? uint32_t(over) : 0u;
     };
     auto issue_scales = [&](int q) {
@@ -395,15 +394,15 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
             const int b = wave + 4 * i;
             if (PS % 4 == 0 || b < PS)
                 dma16(sbs[i] + (uint64_t(as[i] + uint32_t(q)) << 4),
-                      smem + 4 * STEP + (q & 1) * SCALES + b * 1024);
+                      smem + 2 * PAIR + (q & 1) * SCALES + b * 1024);
         }
     };
 
     const int xrow = wm * 16 + r, wrow = BM + wn * (BN / 2) + r;
     const uint32_t sbase = lds_addr(smem);
-    const uint32_t pos = (g ^ ((r >> 1) & 3)) * 16;
-    const uint32_t xat[2] = {sbase + xrow * 64 + pos, sbase + 2 * STEP + xrow * 64 + pos};
-    const uint32_t wat[2] = {sbase + wrow * 64 + pos, sbase + 2 * STEP + wrow * 64 + pos};
+    // (the second step's chunks of a pair are at ^ 64)
+    const uint32_t pos = (g ^ ((r >> 1) & 7)) * 16;
+    const uint32_t xat = sbase + xrow * 128 + pos, wat = sbase + wrow * 128 + pos;
     // fragments of even and odd steps; x's first half is read again as soon as it is used
     v4i xf[2][TM], wf[2][TN];
     constexpr int TH = TM / 2;
@@ -412,11 +411,11 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
     v4i tr[PER_T];                                        // scale rows on their way through
     auto read_x = [&](auto S, auto Fr, auto I) {
         constexpr int slot = decltype(S)::value, f = decltype(Fr)::value, i = decltype(I)::value;
-        xf[i < TH ? 0 : f][i] = read16(xat[slot >> 1], (slot & 1) * STEP + i * 2048);
+        xf[i < TH ? 0 : f][i] = read16((xat ^ (64 * (slot & 1))) + (slot >> 1) * PAIR, i * 4096);
     };
     auto read_w = [&](auto S, auto Fr, auto I) {
         constexpr int slot = decltype(S)::value, f = decltype(Fr)::value, i = decltype(I)::value;
-        wf[f][i] = read16(wat[slot >> 1], (slot & 1) * STEP + i * 1024);
+        wf[f][i] = read16((wat ^ (64 * (slot & 1))) + (slot >> 1) * PAIR, i * 2048);
     };
     auto read_scale = [&](uint32_t at, int i) {           // of block i, x's first
         sr[i] = i < TM ? read4(at + xrow * 16, i * 512) : read4(at + wrow * 16, (i - TM) * 256);
@@ -424,7 +423,7 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
     // the 4 x 4 byte transposition of each row's scales of group q, in place: the
     // reads, and after they have landed the writes
     auto scale_row = [&](int q, int i) {
-        return sbase + 4 * STEP + (q & 1) * SCALES + (threadIdx.x + 256 * i) * 16;
+        return sbase + 2 * PAIR + (q & 1) * SCALES + (threadIdx.x + 256 * i) * 16;
     };
     const bool tlast = ROWS % 256 == 0 || int(threadIdx.x) + 256 * (PER_T - 1) < ROWS;
     auto transpose_read = [&](int q) {
@@ -468,24 +467,14 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
     // in order) and used after them
     static_assert(BN <= 256, "a column a thread");
     const float bias_here = bias_at(out, n0 + min(int(threadIdx.x), BN - 1));
-    if (groups > 1) {
-        issue_scales(0);
-        issue_scales(1);
+    issue_scales(0);
+    if (groups > 1) issue_scales(1);
+    for (int p = 0; p < min((steps + 1) / 2, 2); ++p) {
+        const uint32_t back = past_end(p);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-#pragma unroll
-            for (int i = 0; i < PL; ++i) issue_codes(s, s * 64, 0, i);
-        }
-        if (threadIdx.x < BN) bias_of[threadIdx.x] = bias_here;
-    } else {
-        issue_scales(0);
-        for (int s = 0; s < min(steps, 4); ++s) {
-            const uint32_t back = past_end(s);
-#pragma unroll
-            for (int i = 0; i < PL; ++i) issue_codes(s, s * 64, back, i);
-        }
-        if (threadIdx.x < BN) bias_of[threadIdx.x] = bias_here;
+        for (int i = 0; i < PL; ++i) issue_codes(p, back, i);
     }
+    if (threadIdx.x < BN) bias_of[threadIdx.x] = bias_here;
     lds_done();
     // meanwhile the accumulators start from the bias
     block_barrier();
@@ -495,8 +484,8 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
         asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(b4)::"memory");
         each<TM>([&](auto B) { acc_set<ACC, a * TM + decltype(B)::value>(__builtin_bit_cast(v4f, b4)); });
     });
-    // (the scales went out first, then the codes step by step: step 0's are in too)
-    if (groups > 1) wait_vm<3 * PL>();
+    // (the scales went out first, then the codes pair by pair: pair 0's are in too)
+    if (steps > 2) wait_vm<PL>();
     else wait_vm<0>();
     block_barrier();
     transpose_read(0);
@@ -505,7 +494,7 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
     transpose_write(0);
     lds_done();
     block_barrier();
-    each<TM + TN>([&](auto I) { read_scale(sbase + 4 * STEP + 4 * g, decltype(I)::value); });
+    each<TM + TN>([&](auto I) { read_scale(sbase + 2 * PAIR + 4 * g, decltype(I)::value); });
     each<TM>([&](auto I) { read_x(C0{}, C0{}, I); });
     each<TN>([&](auto I) { read_w(C0{}, C0{}, I); });
     lds_done();
@@ -514,21 +503,19 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
     for (int b = 0; b < TM; ++b) sx[b] = sr[b];
 #pragma unroll
     for (int a = 0; a < TN; ++a) sw[a] = sr[TM + a];
-    if (groups > 1) wait_vm<2 * PL>();                    // step 1 in
-    block_barrier();                                            // step 0's slot is read
 
-    // step s = 4q + J; FULL: step s + 4 exists and is whole
+    // step s = 4q + J; FULL: pair s / 2 + 2 exists and is whole
     auto step = [&](auto Jc, auto Full, int q) {
         constexpr int J = decltype(Jc)::value, F = J & 1;
         constexpr bool FULL = decltype(Full)::value;
         using Next = std::integral_constant<int, (J + 1) & 3>;
         using NF = std::integral_constant<int, 1 - F>;
         const int s = 4 * q + J;
-        const bool more = FULL || s + 4 < steps;
-        const int64_t k = int64_t(s + 4) * 64;
-        const uint32_t back = FULL ? 0u : past_end(s + 4);
-        const uint32_t sat = sbase + 4 * STEP + 4 * g + ((q + 1) & 1) * SCALES;
-        if (J == 0 && q + 2 < groups) issue_scales(q + 2);
+        const int ahead = s / 2 + 2;
+        const bool more = (J & 1) && (FULL || 2 * ahead < steps);
+        const uint32_t back = FULL ? 0u : past_end(ahead);
+        const uint32_t sat = sbase + 2 * PAIR + 4 * g + ((q + 1) & 1) * SCALES;
+        if (J == 1 && q + 2 < groups) issue_scales(q + 2);
         // (past the last group or step the reads find what was there, and go unused)
         if constexpr (J == 1) transpose_read(q + 1);
         if constexpr (J == 2) transpose_write(q + 1);
@@ -545,7 +532,7 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
             }
             if (more) {
 #pragma unroll
-                for (int i = b * PL / TM; i < (b + 1) * PL / TM; ++i) issue_codes(J, k, back, i);
+                for (int i = b * PL / TM; i < (b + 1) * PL / TM; ++i) issue_codes(ahead, back, i);
             }
             each<TN / 4>([&](auto A) {
                 constexpr int a = 4 * decltype(A)::value;
@@ -565,12 +552,11 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
         for (int b = 0; b < TM; ++b) sx[b] = J == 3 ? sr[b] : int(uint32_t(sx[b]) >> 8);
 #pragma unroll
         for (int a = 0; a < TN; ++a) sw[a] = J == 3 ? sr[TM + a] : int(uint32_t(sw[a]) >> 8);
-        // step s + 2 in: of what was issued later, steps s + 3 and s + 4 may be on the way
-        // (a group's scales go out before its first step's codes)
-        if (more) wait_vm<2 * PL>();
-        else if (s + 3 < steps) wait_vm<PL>();
-        else wait_vm<0>();
-        block_barrier();
+        // every wave has read its pair's last fragments; the next pair is in
+        if constexpr (F == 0) {
+            wait_vm<0>();
+            block_barrier();
+        }
     };
     const int whole = K / 128;
     using Yes = std::true_type;
