@@ -463,10 +463,7 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
     using C2 = std::integral_constant<int, 2>;
     using C3 = std::integral_constant<int, 3>;
 
-    // the bias of the tile's columns is read ahead of the direct loads (loads complete
-    // in order) and used after them
     static_assert(BN <= 256, "a column a thread");
-    const float bias_here = bias_at(out, n0 + min(int(threadIdx.x), BN - 1));
     issue_scales(0);
     if (groups > 1) issue_scales(1);
     for (int p = 0; p < min((steps + 1) / 2, 2); ++p) {
@@ -474,16 +471,20 @@ __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void mx4_tile_ker
 #pragma unroll
         for (int i = 0; i < PL; ++i) issue_codes(p, back, i);
     }
-    if (threadIdx.x < BN) bias_of[threadIdx.x] = bias_here;
-    lds_done();
     // meanwhile the accumulators start from the bias
-    block_barrier();
-    each<TN>([&](auto A) {
-        constexpr int a = decltype(A)::value;
-        v4i b4 = read16(lds_addr(bias_of) + (wn * (BN / 2) + 4 * g) * 4, a * 64);
-        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(b4)::"memory");
-        each<TM>([&](auto B) { acc_set<ACC, a * TM + decltype(B)::value>(__builtin_bit_cast(v4f, b4)); });
-    });
+    if (out.bias) {
+        if (threadIdx.x < BN) bias_of[threadIdx.x] = bias_at(out, n0 + int(threadIdx.x));
+        lds_done();
+        block_barrier();
+        each<TN>([&](auto A) {
+            constexpr int a = decltype(A)::value;
+            v4i b4 = read16(lds_addr(bias_of) + (wn * (BN / 2) + 4 * g) * 4, a * 64);
+            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(b4)::"memory");
+            each<TM>([&](auto B) { acc_set<ACC, a * TM + decltype(B)::value>(__builtin_bit_cast(v4f, b4)); });
+        });
+    } else {
+        each<TM * TN>([&](auto B) { acc_set<ACC, decltype(B)::value>(v4f{0.f, 0.f, 0.f, 0.f}); });
+    }
     // (the scales went out first, then the codes pair by pair: pair 0's are in too)
     if (steps > 2) wait_vm<PL>();
     else wait_vm<0>();
