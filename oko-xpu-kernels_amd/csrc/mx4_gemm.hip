@@ -659,9 +659,10 @@ namespace {
 
 // Whether 256 x 256 tiles (one block a CU, half the operand bytes a product) are
 // faster than 128 x 128 (two blocks a CU, so that one's start and end overlap the
-// other's steps, and finer rounds), by the times that a round of either takes, fitted
-// to both over seven shapes: 8192^3 330 against 430 us, 4096^3 49 against 58; 4096 x 10240
-// x 1280 66 against 51, 32 experts' 16380 x 2816 x 2048 133 against 104.
+// other's steps, and finer rounds), by the times that a round of either takes, fitted to
+// both over 13 shapes.  With the quantizer, 256 against 128: 8192^3 342 / 405 us, 2048 x
+// 8192 x 8192 83 / 98, 4096^3 54 / 60; 4096 x 1280 -> 5120 44 / 34, 4096 x 2560 -> 10240 88 / 84,
+// 1000 x 4096 x 4096 39 / 22, 16380 x 2048 -> 2816 in 32 groups 128 / 111.
 bool large_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
     const double steps = double((K + 127) / 128);
     auto tiles = [&](int64_t b) {                          // (a group's last tile half full)
@@ -670,10 +671,10 @@ bool large_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
     };
     const int64_t cus = device_cus();
     const int64_t t128 = tiles(128), t256 = tiles(256);
-    const double large = double((t256 + cus - 1) / cus) * (10.0 + 1.13 * steps);
-    const double small = double(t128 / (2 * cus)) * (2.6 + 0.8 * steps) +
-                         (t128 % (2 * cus) > cus ? 2.6 + 0.8 * steps
-                          : t128 % (2 * cus) > 0 ? 2.6 + 0.45 * steps : 0.0);
+    const double large = double((t256 + cus - 1) / cus) * (10.0 + 1.07 * steps);
+    const double small = double(t128 / (2 * cus)) * (2.6 + 0.68 * steps) +
+                         (t128 % (2 * cus) > cus ? 2.6 + 0.68 * steps
+                          : t128 % (2 * cus) > 0 ? 2.6 + 0.46 * steps : 0.0);
     return large < small;
 }
 
