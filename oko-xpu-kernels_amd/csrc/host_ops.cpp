@@ -65,8 +65,11 @@ struct Library {
     decltype(&xpuint8_moe_sort_stream) moe_sort;
     decltype(&xpuint8_moe_dispatch_stream) moe_dispatch;
     decltype(&xpuint8_moe_combine_stream) moe_combine;
+    decltype(&xpuint8_mxfp4_dx_workspace_size) mx_dx_size;
+    decltype(&xpuint8_mxfp4_dx_stream) mx_dx;
+    decltype(&xpuint8_moe_combine_grad_stream) moe_combine_grad;
 };
-constexpr int kEntries = 28;
+constexpr int kEntries = 31;
 static_assert(sizeof(Library) == kEntries * sizeof(void*), "one address per entry");
 
 Library g_lib;
@@ -678,26 +681,98 @@ PyObject* host_moe_dispatch(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
-// moe_combine(z, routing, weights): moe.combine without a gradient, fp32 weights
+// an index into kTypes
+bool type_arg(PyObject* o, int32_t& type) {
+    const long t = PyLong_AsLong(o);
+    if (t == -1 && PyErr_Occurred()) throw python_error();
+    type = int32_t(t);
+    return t >= 0 && t <= 2;
+}
+
+// moe_combine(z, routing, weights, type): moe.combine without a gradient, fp32 weights or
+// none, the result in the type
 PyObject* host_moe_combine(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    return guarded(n_args, 3, [&]() -> PyObject* {
+    return guarded(n_args, 4, [&]() -> PyObject* {
         const Tensor* z = floating(a[0]);
         Routing r;
-        if (!z || z->dim() != 2 || !routing_arg(a[1], *z, r)) Py_RETURN_NONE;
-        const Tensor* w = on(plain(a[2], at::kFloat), *z);
+        int32_t type;
+        if (!z || z->dim() != 2 || !routing_arg(a[1], *z, r) || !type_arg(a[3], type)) Py_RETURN_NONE;
         const int64_t t = r.position->size(0), top = r.position->size(1), d = z->size(1);
-        if (!w || w->dim() != 2 || w->size(0) != t || w->size(1) != top || z->size(0) != t * top)
-            Py_RETURN_NONE;
+        if (z->size(0) != t * top) Py_RETURN_NONE;
+        const Tensor* w = nullptr;
+        if (a[2] != Py_None) {
+            w = on(plain(a[2], at::kFloat), *z);
+            if (!w || w->dim() != 2 || w->size(0) != t || w->size(1) != top) Py_RETURN_NONE;
+        }
         const void* st = current_stream(*z);
         Tensor out;
         call("moe.combine", [&] {
-            out = empty({t, d}, z->scalar_type(), *z);
+            out = empty({t, d}, kTypes[type], *z);
             return g_lib.moe_combine(st, z->data_ptr(), type_of(*z), d, ints(r.position),
-                                     ints(r.offsets), static_cast<const float*>(w->data_ptr()),
-                                     out.data_ptr(), type_of(*z), t, top,
-                                     r.offsets->numel() - 1, d);
+                                     ints(r.offsets),
+                                     w ? static_cast<const float*>(w->data_ptr()) : nullptr,
+                                     out.data_ptr(), type, t, top, r.offsets->numel() - 1, d);
         });
         return THPVariable_Wrap(out);
+    });
+}
+
+// moe_combine_grad(dy, z, weights, routing): the gradients of moe.combine
+PyObject* host_moe_combine_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 4, [&]() -> PyObject* {
+        const Tensor* z = floating(a[1]);
+        const Tensor* dy = z ? on(plain(a[0], z->scalar_type()), *z) : nullptr;
+        const Tensor* w = z ? on(plain(a[2], at::kFloat), *z) : nullptr;
+        Routing r;
+        if (!dy || !w || z->dim() != 2 || dy->dim() != 2 || !routing_arg(a[3], *z, r)) Py_RETURN_NONE;
+        const int64_t t = r.position->size(0), top = r.position->size(1), d = z->size(1);
+        if (z->size(0) != t * top || dy->size(0) != t || dy->size(1) != d || w->numel() != t * top)
+            Py_RETURN_NONE;
+        const void* st = current_stream(*z);
+        Tensor dz, dw;
+        call("moe.combine (gradient)", [&] {
+            dz = empty({t * top, d}, z->scalar_type(), *z);
+            dw = empty({t, top}, at::kFloat, *z);
+            return g_lib.moe_combine_grad(st, dy->data_ptr(), type_of(*z), d, z->data_ptr(), d,
+                                          ints(r.position), ints(r.offsets),
+                                          static_cast<const float*>(w->data_ptr()), dz.data_ptr(),
+                                          static_cast<float*>(dw.data_ptr()), t, top,
+                                          r.offsets->numel() - 1, d);
+        });
+        return pair(dz, dw);
+    });
+}
+
+// mx_dx(dy, codes, scales, offsets, type): dy [.., N] times the (experts') weight, the rows
+// of dy flat, in the type
+PyObject* host_mx_dx(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 5, [&]() -> PyObject* {
+        const Tensor* dy = floating(a[0]);
+        const Tensor *c, *s, *o = nullptr;
+        int32_t type;
+        if (!dy || dy->dim() < 1 || !mx_pair(a[1], a[2], c, s) || !on(c, *dy) || !type_arg(a[4], type))
+            Py_RETURN_NONE;
+        if (a[3] != Py_None) {
+            o = on(plain(a[3], at::kInt), *dy);
+            if (!o || c->dim() != 3 || o->numel() != c->size(0) + 1) Py_RETURN_NONE;
+        } else if (c->dim() != 2) {
+            Py_RETURN_NONE;
+        }
+        const int64_t e = o ? c->size(0) : 0, n = c->size(-2), k = c->size(-1) * 2;
+        const int64_t r = dy->numel() / dy->size(-1);
+        if (dy->size(-1) != n) Py_RETURN_NONE;
+        const int64_t need = g_lib.mx_dx_size(type_of(*dy), type, r, e, n, k);
+        if (need < 0) fail("mxfp4 dx");
+        const void* st = current_stream(*dy);
+        Tensor work, dx;
+        call("mxfp4 dx", [&] {
+            if (need > 0) work = workspace(need, *dy);
+            dx = empty({r, k}, kTypes[type], *dy);
+            return g_lib.mx_dx(st, dy->data_ptr(), type_of(*dy), n, bytes(c), bytes(s),
+                               o ? ints(o) : nullptr, e, dx.data_ptr(), type, r, n, k,
+                               need > 0 ? work.data_ptr() : nullptr, need);
+        });
+        return THPVariable_Wrap(dx);
     });
 }
 
@@ -741,6 +816,8 @@ PyMethodDef kMethods[] = {XPU_HOST("bind", host_bind),
                           XPU_HOST("moe_sort", host_moe_sort),
                           XPU_HOST("moe_dispatch", host_moe_dispatch),
                           XPU_HOST("moe_combine", host_moe_combine),
+                          XPU_HOST("moe_combine_grad", host_moe_combine_grad),
+                          XPU_HOST("mx_dx", host_mx_dx),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host",
                        "The int8 API's hot calls in native code (see host_ops.cpp).", -1, kMethods};

@@ -48,7 +48,9 @@ _HOST_ENTRIES = (
     "xpuint8_mxfp4_linear_workspace_size", "xpuint8_mxfp4_linear_stream",
     "xpuint8_mxfp4_grouped_linear_workspace_size", "xpuint8_mxfp4_grouped_linear_stream",
     "xpuint8_moe_sort_workspace_size", "xpuint8_moe_sort_stream",
-    "xpuint8_moe_dispatch_stream", "xpuint8_moe_combine_stream")
+    "xpuint8_moe_dispatch_stream", "xpuint8_moe_combine_stream",
+    "xpuint8_mxfp4_dx_workspace_size", "xpuint8_mxfp4_dx_stream",
+    "xpuint8_moe_combine_grad_stream")
 
 
 def _candidate_paths():

@@ -67,6 +67,11 @@ def _wants_grad(*tensors):
                                            for t in tensors)
 
 
+def _native(name, *args):
+    """The native host path's call, or None where it leaves the work to ctypes."""
+    return None if L.HOST is None else getattr(L.HOST, name)(*args)
+
+
 def _check_pair(codes, scales, lead=None):
     """The K behind codes and scales, both on the GPU and of matching shapes."""
     for t, name in ((codes, "codes"), (scales, "scales")):
@@ -180,7 +185,10 @@ def _linear(x, codes, scales, bias):
 
 
 def _dx(dy, codes, scales, offsets, out_dtype):
-    """dy [R, N] times the (experts') weight, [R, K]."""
+    """dy [.., N] times the (experts') weight, [R, K]."""
+    r = _native("mx_dx", dy, codes, scales, offsets, TYPES[out_dtype])
+    if r is not None:
+        return r
     n, k = codes.shape[-2], codes.shape[-1] * 2
     dy2, ld = _rows(dy)
     r = dy2.shape[0]
@@ -207,7 +215,8 @@ class _LinearFn(torch.autograd.Function):
     def forward(ctx, x, codes, scales, bias):
         ctx.save_for_backward(codes, scales)
         ctx.bias_dtype = None if bias is None else bias.dtype
-        return _linear(x, codes, scales, bias)
+        y = _native("mx_linear", x, codes, scales, bias)
+        return _linear(x, codes, scales, bias) if y is None else y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -268,7 +277,8 @@ class _GroupedFn(torch.autograd.Function):
     def forward(ctx, x, codes, scales, routing, gather):
         ctx.save_for_backward(codes, scales, *routing)
         ctx.gather = gather
-        return _grouped(x, codes, scales, routing, gather)
+        y = _native("mx_grouped", x, codes, scales, routing, gather)
+        return _grouped(x, codes, scales, routing, gather) if y is None else y
 
     @staticmethod
     @torch.autograd.function.once_differentiable

@@ -100,3 +100,43 @@ def test_experts(dev, monkeypatch, t):
         both(monkeypatch, lambda: moe.dispatch(z[:t], r), name)
         both(monkeypatch, lambda: moe.combine(z, r), name)
         both(monkeypatch, lambda: mxfp4.grouped_linear(z, codes, scales, r), name)
+
+
+def dys(dev, m, n, dtype=torch.bfloat16):
+    base = randn(m + 2, n + 16, seed=8, dtype=dtype).to(dev)
+    return {"plain": base[:m, :n].contiguous(), "columns": base[:m, :n], "misaligned": base[1:m + 1, 3:n + 3],
+            "expanded": base[:1, :n].expand(m, n), "one value": base[:1, :1].expand(m, n)}
+
+
+@pytest.mark.parametrize("m", [3, 150])
+def test_gradients(dev, monkeypatch, m):
+    k, n, top, experts = 288, 48, 3, 6
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        codes, scales = mxfp4.quantize(randn(n, k, seed=5).to(dev))
+        x = randn(m, k, seed=1, dtype=dtype).to(dev).requires_grad_()
+        b = randn(n, seed=6).to(dev).requires_grad_()
+        for name, dy in dys(dev, m, n, dtype).items():
+            assert both(monkeypatch, lambda: torch.autograd.grad(mxfp4.linear(x, codes, scales, b), (x, b), dy), name)
+            assert both(monkeypatch, lambda: torch.autograd.grad(
+                mxfp4.linear(x[None], codes, scales), x, dy[None]), name)
+        codes, scales = mxfp4.quantize(randn(experts, n, k, seed=5).to(dev))
+        routing = moe.sort(router(m, top, experts, seed=m, dropped=0.1).to(dev), experts)
+        w = torch.rand(m, top, device=dev).requires_grad_()
+        z = randn(m * top, k, seed=2, dtype=dtype).to(dev).requires_grad_()
+        for gather, xs in ((True, x), (False, z)):
+            for name, dy in dys(dev, m * top, n, dtype).items():
+                assert both(monkeypatch, lambda: torch.autograd.grad(
+                    mxfp4.grouped_linear(xs, codes, scales, routing, gather=gather), xs, dy), name)
+        for name, dy in dys(dev, m * top, k, dtype).items():
+            assert both(monkeypatch, lambda: torch.autograd.grad(moe.dispatch(x, routing), x, dy), name)
+        for name, dy in dys(dev, m, k, dtype).items():
+            assert both(monkeypatch, lambda: torch.autograd.grad(moe.combine(z, routing, w), (z, w), dy), name)
+
+
+def test_second_derivatives_are_refused(dev):
+    codes, scales = mxfp4.quantize(randn(48, 288, seed=5).to(dev))
+    x = randn(9, 288, seed=1, dtype=torch.bfloat16).to(dev).requires_grad_()
+    dy = randn(9, 48, seed=2, dtype=torch.bfloat16).to(dev).requires_grad_()
+    dx, = torch.autograd.grad(mxfp4.linear(x, codes, scales), x, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
