@@ -1,8 +1,7 @@
 // The host path of the Python API's hot calls (xpu_kernels.int8 linear, ffn, the
-// backward's products and the quantizer; xpu_kernels.mxfp4 and moe without gradients) as
-// a CPython extension: argument
-// checks, the packed weight's lookup, allocations and the library call in
-// native code.  In Python these cost more than the small calls' kernels: linear
+// backward's products and the quantizer; xpu_kernels.mxfp4 and moe with their gradients)
+// as a CPython extension: argument checks, the packed weight's lookup, allocations and
+// the library call in native code.  In Python these cost more than the small calls' kernels: linear
 // at 16 x 4096 x 4096 took 17.6 us of host time for 8.5 us of GPU work, 6.9 of
 // them the library's two launches.
 //
@@ -19,12 +18,17 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/Storage.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
 #include <cstdio>
 #include <cstring>
 #include <exception>
+#include <optional>
+#include <stdexcept>
+#include <string>
 #include <vector>
 
 #include "xpuint8.h"
@@ -561,35 +565,254 @@ PyObject* host_mx_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
-// mx_linear(x, codes, scales, bias): mxfp4.linear without a gradient
+// ---------------------------------------------------- forward, on checked tensors
+Tensor run_linear(const Tensor& x, const Tensor& c, const Tensor& s, const Tensor* b) {
+    const int64_t n = c.size(0), k = c.size(1) * 2, m = x.numel() / k;
+    const int64_t need = g_lib.mx_linear_size(m, n, k);
+    if (need < 0) fail("mxfp4.linear");
+    const void* st = current_stream(x);
+    Tensor work, y;
+    call("mxfp4.linear", [&] {
+        if (need > 0) work = workspace(need, x);
+        y = empty(with_last(x, n), x.scalar_type(), x);
+        return g_lib.mx_linear(st, x.data_ptr(), type_of(x), k, bytes(&c), bytes(&s),
+                               b ? b->data_ptr() : nullptr, b ? type_of(*b) : 0, y.data_ptr(), m,
+                               n, k, need > 0 ? work.data_ptr() : nullptr, need);
+    });
+    return y;
+}
+// `rows`: the tokens that the sorted rows are read from, null for x sorted already
+Tensor run_grouped(const Tensor& x, const Tensor& c, const Tensor& s, const Tensor* rows,
+                   const Tensor& offsets, int64_t r) {
+    const int64_t e = c.size(0), n = c.size(1), k = c.size(2) * 2, t = x.size(0);
+    const int64_t need = g_lib.mx_grouped_size(r, t, e, n, k);
+    if (need < 0) fail("mxfp4.grouped_linear");
+    const void* st = current_stream(x);
+    Tensor work, y;
+    call("mxfp4.grouped_linear", [&] {
+        if (need > 0) work = workspace(need, x);
+        y = empty({r, n}, x.scalar_type(), x);
+        return g_lib.mx_grouped(st, x.data_ptr(), type_of(x), k, rows ? ints(rows) : nullptr, t,
+                                bytes(&c), bytes(&s), ints(&offsets), e, y.data_ptr(), r, n, k,
+                                need > 0 ? work.data_ptr() : nullptr, need);
+    });
+    return y;
+}
+Tensor run_dispatch(const Tensor& x, const Tensor& position, const Tensor& offsets) {
+    const int64_t t = x.size(0), d = x.size(1), top = position.size(1);
+    const void* st = current_stream(x);
+    Tensor out;
+    call("moe.dispatch", [&] {
+        out = empty({t * top, d}, x.scalar_type(), x);
+        return g_lib.moe_dispatch(st, x.data_ptr(), type_of(x), d, ints(&position), ints(&offsets),
+                                  out.data_ptr(), t, top, offsets.numel() - 1, d);
+    });
+    return out;
+}
+Tensor run_combine(const Tensor& z, const Tensor* w, const Tensor& position,
+                   const Tensor& offsets, int32_t type) {
+    const int64_t t = position.size(0), top = position.size(1), d = z.size(1);
+    const void* st = current_stream(z);
+    Tensor out;
+    call("moe.combine", [&] {
+        out = empty({t, d}, kTypes[type], z);
+        return g_lib.moe_combine(st, z.data_ptr(), type_of(z), d, ints(&position), ints(&offsets),
+                                 w ? static_cast<const float*>(w->data_ptr()) : nullptr,
+                                 out.data_ptr(), type, t, top, offsets.numel() - 1, d);
+    });
+    return out;
+}
+
+// ------------------------------------------------------------------- gradients
+// The backward passes as autograd nodes of C++: they run in the engine's thread without the
+// GIL, which the current stream's accessor alone takes.  What they compute is what the
+// Python functions' backward computes, by the same library calls.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+const void* stream_of(const Tensor& t) {
+    struct Gil {
+        PyGILState_STATE s = PyGILState_Ensure();
+        ~Gil() { PyGILState_Release(s); }
+    } gil;
+    try {
+        return current_stream(t);
+    } catch (python_error& e) {
+        e.persist();
+        throw;
+    }
+}
+void check(int rc, const char* what) {
+    if (rc != 0) throw std::runtime_error(std::string(what) + ": " + g_lib.last_error());
+}
+// x [.., n] as rows with a stride
+struct Rows {
+    Tensor t;
+    int64_t ld;
+};
+Rows rows_of(const Tensor& x) {
+    Tensor t = x.reshape({-1, x.size(-1)});
+    const bool many = t.size(0) > 1;
+    if (t.stride(1) != 1 || (many && t.stride(0) < t.size(1))) t = t.contiguous();
+    return {t, t.size(0) > 1 ? t.stride(0) : t.size(1)};
+}
+// the gradients that f() gives, which have no derivative themselves: an error where one is
+// asked for
+template <class F>
+variable_list once(const variable_list& in, const F& f) {
+    variable_list grads;
+    {
+        at::NoGradGuard no_grad;
+        grads = f();
+    }
+    bool wanted = false;
+    for (const Tensor& g : in) wanted |= g.defined() && g.requires_grad();
+    if (!wanted || !at::GradMode::is_enabled()) return grads;
+    for (Tensor& g : grads)
+        if (g.defined()) g = g.detach().requires_grad_(true);
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that was marked with @once_differentiable",
+        int64_t(grads.size()));
+    return (*error)(std::move(grads));
+}
+Tensor grad_dx(const Tensor& dy, const Tensor& c, const Tensor& s, const Tensor* offsets,
+               int32_t type) {
+    const Rows d = rows_of(dy);
+    const int64_t n = c.size(-2), k = c.size(-1) * 2, e = offsets ? c.size(0) : 0, r = d.t.size(0);
+    const int64_t need = g_lib.mx_dx_size(type_of(dy), type, r, e, n, k);
+    if (need < 0) check(1, "mxfp4 dx");
+    Tensor work, dx = empty({r, k}, kTypes[type], dy);
+    if (need > 0) work = workspace(need, dy);
+    check(g_lib.mx_dx(stream_of(dy), d.t.data_ptr(), type_of(dy), d.ld, bytes(&c), bytes(&s),
+                      offsets ? ints(offsets) : nullptr, e, dx.data_ptr(), type, r, n, k,
+                      need > 0 ? work.data_ptr() : nullptr, need), "mxfp4 dx");
+    return dx;
+}
+Tensor grad_sum(const Tensor& dxs, const Tensor& position, const Tensor& offsets, int32_t type) {
+    const Rows z = rows_of(dxs);
+    const int64_t t = position.size(0), top = position.size(1), d = z.t.size(1);
+    Tensor out = empty({t, d}, kTypes[type], dxs);
+    check(g_lib.moe_combine(stream_of(dxs), z.t.data_ptr(), type_of(dxs), z.ld, ints(&position),
+                            ints(&offsets), nullptr, out.data_ptr(), type, t, top,
+                            offsets.numel() - 1, d), "moe.combine");
+    return out;
+}
+// int8.column_sum
+Tensor column_sum(const Tensor& dy) {
+    if (dy.scalar_type() != at::kBFloat16 || dy.size(1) % 16 != 0) return dy.sum(0);
+    Tensor d = dy.contiguous();
+    if (reinterpret_cast<uintptr_t>(d.data_ptr()) % 16 != 0) d = d.clone();
+    const int64_t m = d.size(0), n = d.size(1), need = g_lib.colsum_size(m, n);
+    if (need < 0) check(1, "column_sum");
+    Tensor work = workspace(std::max<int64_t>(need, 16), d), out = empty({n}, at::kBFloat16, d);
+    check(g_lib.colsum(stream_of(d), d.data_ptr(), out.data_ptr(), m, n, work.data_ptr(), need),
+          "column_sum");
+    return out;
+}
+
+struct LinearFn : torch::autograd::Function<LinearFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& c, const Tensor& s,
+                          const std::optional<Tensor>& b) {
+        ctx->save_for_backward({c, s});
+        ctx->saved_data["bias"] = int64_t(b ? b->scalar_type() : at::ScalarType::Undefined);
+        return run_linear(x, c, s, b ? &*b : nullptr);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list in) {
+        return once(in, [&]() -> variable_list {
+            const variable_list saved = ctx->get_saved_variables();
+            const Tensor &dy = in[0], &c = saved[0];
+            const auto type = at::ScalarType(ctx->saved_data["bias"].toInt());
+            Tensor dx, db;
+            if (ctx->needs_input_grad(0))
+                dx = grad_dx(dy, c, saved[1], nullptr, type_of(dy)).reshape(with_last(dy, c.size(1) * 2));
+            if (type != at::ScalarType::Undefined && ctx->needs_input_grad(3))
+                db = column_sum(dy.reshape({-1, dy.size(-1)})).to(type);
+            return {dx, Tensor(), Tensor(), db};
+        });
+    }
+};
+
+struct GroupedFn : torch::autograd::Function<GroupedFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& c, const Tensor& s,
+                          const Tensor& position, const Tensor& rows, const Tensor& offsets,
+                          bool gather) {
+        ctx->save_for_backward({c, s, position, offsets});
+        ctx->saved_data["gather"] = gather;
+        return run_grouped(x, c, s, gather ? &rows : nullptr, offsets, rows.numel());
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list in) {
+        return once(in, [&]() -> variable_list {
+            const variable_list saved = ctx->get_saved_variables();
+            const Tensor &dy = in[0], &offsets = saved[3];
+            const bool gather = ctx->saved_data["gather"].toBool();
+            // a token's rows are summed in fp32 and rounded once
+            Tensor dx = grad_dx(dy, saved[0], saved[1], &offsets, gather ? 2 : type_of(dy));
+            if (gather) dx = grad_sum(dx, saved[2], offsets, type_of(dy));
+            return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        });
+    }
+};
+
+struct DispatchFn : torch::autograd::Function<DispatchFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& position,
+                          const Tensor& offsets) {
+        ctx->save_for_backward({position, offsets});
+        return run_dispatch(x, position, offsets);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list in) {
+        return once(in, [&]() -> variable_list {
+            const variable_list saved = ctx->get_saved_variables();
+            return {grad_sum(in[0], saved[0], saved[1], type_of(in[0])), Tensor(), Tensor()};
+        });
+    }
+};
+
+struct CombineFn : torch::autograd::Function<CombineFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& z, const Tensor& w,
+                          const Tensor& position, const Tensor& offsets) {
+        ctx->save_for_backward({z, w, position, offsets});
+        return run_combine(z, &w, position, offsets, type_of(z));
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list in) {
+        return once(in, [&]() -> variable_list {
+            const variable_list saved = ctx->get_saved_variables();
+            const Tensor &z = saved[0], &w = saved[1], &position = saved[2], &offsets = saved[3];
+            const Rows dy = rows_of(in[0]);
+            const int64_t t = position.size(0), top = position.size(1), d = z.size(1);
+            Tensor dz = empty({t * top, d}, z.scalar_type(), z), dw = empty({t, top}, at::kFloat, z);
+            check(g_lib.moe_combine_grad(stream_of(z), dy.t.data_ptr(), type_of(z), dy.ld, z.data_ptr(),
+                                         d, ints(&position), ints(&offsets),
+                                         static_cast<const float*>(w.data_ptr()), dz.data_ptr(),
+                                         static_cast<float*>(dw.data_ptr()), t, top,
+                                         offsets.numel() - 1, d), "moe.combine (gradient)");
+            return {dz, dw, Tensor(), Tensor()};
+        });
+    }
+};
+
+bool wants_grad(const Tensor& a, const Tensor* b = nullptr) {
+    return at::GradMode::is_enabled() && (a.requires_grad() || (b && b->requires_grad()));
+}
+
+// -------------------------------------------------- functions of xpu_kernels.mxfp4, moe
+// mx_linear(x, codes, scales, bias): mxfp4.linear
 PyObject* host_mx_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded(n_args, 4, [&]() -> PyObject* {
         const Tensor* x = floating(a[0]);
         const Tensor *c, *s, *b = nullptr;
-        if (!x || x->dim() < 1 || !mx_pair(a[1], a[2], c, s) || c->dim() != 2 || !on(c, *x))
+        if (!x || x->dim() < 1 || !mx_pair(a[1], a[2], c, s) || c->dim() != 2 || !on(c, *x) ||
+            x->size(-1) != c->size(1) * 2)
             Py_RETURN_NONE;
-        const int64_t n = c->size(0), k = c->size(1) * 2, m = x->numel() / x->size(-1);
-        if (x->size(-1) != k) Py_RETURN_NONE;
         if (a[3] != Py_None) {
             b = on(floating(a[3]), *x);
-            if (!b || b->dim() != 1 || b->numel() != n) Py_RETURN_NONE;
+            if (!b || b->dim() != 1 || b->numel() != c->size(0)) Py_RETURN_NONE;
         }
-        const int64_t need = g_lib.mx_linear_size(m, n, k);
-        if (need < 0) fail("mxfp4.linear");
-        const void* st = current_stream(*x);
-        Tensor work, y;
-        call("mxfp4.linear", [&] {
-            if (need > 0) work = workspace(need, *x);
-            y = empty(with_last(*x, n), x->scalar_type(), *x);
-            return g_lib.mx_linear(st, x->data_ptr(), type_of(*x), k, bytes(c), bytes(s),
-                                   b ? b->data_ptr() : nullptr, b ? type_of(*b) : 0, y.data_ptr(),
-                                   m, n, k, need > 0 ? work.data_ptr() : nullptr, need);
-        });
-        return THPVariable_Wrap(y);
+        if (!wants_grad(*x, b)) return THPVariable_Wrap(run_linear(*x, *c, *s, b));
+        return THPVariable_Wrap(LinearFn::apply(*x, *c, *s, b ? std::optional<Tensor>(*b) : std::nullopt));
     });
 }
 
-// mx_grouped(x, codes, scales, routing, gather): mxfp4.grouped_linear without a gradient
+// mx_grouped(x, codes, scales, routing, gather): mxfp4.grouped_linear
 PyObject* host_mx_grouped(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded(n_args, 5, [&]() -> PyObject* {
         const Tensor* x = floating(a[0]);
@@ -600,24 +823,13 @@ PyObject* host_mx_grouped(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             Py_RETURN_NONE;
         const int gather = PyObject_IsTrue(a[4]);
         if (gather < 0) throw python_error();
-        const int64_t e = c->size(0), n = c->size(1), k = c->size(2) * 2, t = x->size(0);
         const int64_t rows = r.order->numel();
-        if (x->size(1) != k || r.offsets->numel() != e + 1 ||
-            t != (gather ? r.position->size(0) : rows))
+        if (x->size(1) != c->size(2) * 2 || r.offsets->numel() != c->size(0) + 1 ||
+            x->size(0) != (gather ? r.position->size(0) : rows))
             Py_RETURN_NONE;
-        const int64_t need = g_lib.mx_grouped_size(rows, t, e, n, k);
-        if (need < 0) fail("mxfp4.grouped_linear");
-        const void* st = current_stream(*x);
-        Tensor work, y;
-        call("mxfp4.grouped_linear", [&] {
-            if (need > 0) work = workspace(need, *x);
-            y = empty({rows, n}, x->scalar_type(), *x);
-            return g_lib.mx_grouped(st, x->data_ptr(), type_of(*x), k,
-                                    gather ? ints(r.rows) : nullptr, t, bytes(c), bytes(s),
-                                    ints(r.offsets), e, y.data_ptr(), rows, n, k,
-                                    need > 0 ? work.data_ptr() : nullptr, need);
-        });
-        return THPVariable_Wrap(y);
+        if (!wants_grad(*x))
+            return THPVariable_Wrap(run_grouped(*x, *c, *s, gather ? r.rows : nullptr, *r.offsets, rows));
+        return THPVariable_Wrap(GroupedFn::apply(*x, *c, *s, *r.position, *r.rows, *r.offsets, gather != 0));
     });
 }
 
@@ -661,118 +873,31 @@ PyObject* host_moe_sort(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
-// moe_dispatch(x, routing): moe.dispatch without a gradient
+// moe_dispatch(x, routing): moe.dispatch
 PyObject* host_moe_dispatch(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded(n_args, 2, [&]() -> PyObject* {
         const Tensor* x = floating(a[0]);
         Routing r;
         if (!x || x->dim() != 2 || !routing_arg(a[1], *x, r) || x->size(0) != r.position->size(0))
             Py_RETURN_NONE;
-        const int64_t t = x->size(0), d = x->size(1), top = r.position->size(1);
-        const void* st = current_stream(*x);
-        Tensor out;
-        call("moe.dispatch", [&] {
-            out = empty({t * top, d}, x->scalar_type(), *x);
-            return g_lib.moe_dispatch(st, x->data_ptr(), type_of(*x), d, ints(r.position),
-                                      ints(r.offsets), out.data_ptr(), t, top,
-                                      r.offsets->numel() - 1, d);
-        });
-        return THPVariable_Wrap(out);
+        if (!wants_grad(*x)) return THPVariable_Wrap(run_dispatch(*x, *r.position, *r.offsets));
+        return THPVariable_Wrap(DispatchFn::apply(*x, *r.position, *r.offsets));
     });
 }
 
-// an index into kTypes
-bool type_arg(PyObject* o, int32_t& type) {
-    const long t = PyLong_AsLong(o);
-    if (t == -1 && PyErr_Occurred()) throw python_error();
-    type = int32_t(t);
-    return t >= 0 && t <= 2;
-}
-
-// moe_combine(z, routing, weights, type): moe.combine without a gradient, fp32 weights or
-// none, the result in the type
+// moe_combine(z, routing, weights): moe.combine, fp32 weights
 PyObject* host_moe_combine(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    return guarded(n_args, 4, [&]() -> PyObject* {
+    return guarded(n_args, 3, [&]() -> PyObject* {
         const Tensor* z = floating(a[0]);
         Routing r;
-        int32_t type;
-        if (!z || z->dim() != 2 || !routing_arg(a[1], *z, r) || !type_arg(a[3], type)) Py_RETURN_NONE;
-        const int64_t t = r.position->size(0), top = r.position->size(1), d = z->size(1);
-        if (z->size(0) != t * top) Py_RETURN_NONE;
-        const Tensor* w = nullptr;
-        if (a[2] != Py_None) {
-            w = on(plain(a[2], at::kFloat), *z);
-            if (!w || w->dim() != 2 || w->size(0) != t || w->size(1) != top) Py_RETURN_NONE;
-        }
-        const void* st = current_stream(*z);
-        Tensor out;
-        call("moe.combine", [&] {
-            out = empty({t, d}, kTypes[type], *z);
-            return g_lib.moe_combine(st, z->data_ptr(), type_of(*z), d, ints(r.position),
-                                     ints(r.offsets),
-                                     w ? static_cast<const float*>(w->data_ptr()) : nullptr,
-                                     out.data_ptr(), type, t, top, r.offsets->numel() - 1, d);
-        });
-        return THPVariable_Wrap(out);
-    });
-}
-
-// moe_combine_grad(dy, z, weights, routing): the gradients of moe.combine
-PyObject* host_moe_combine_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    return guarded(n_args, 4, [&]() -> PyObject* {
-        const Tensor* z = floating(a[1]);
-        const Tensor* dy = z ? on(plain(a[0], z->scalar_type()), *z) : nullptr;
-        const Tensor* w = z ? on(plain(a[2], at::kFloat), *z) : nullptr;
-        Routing r;
-        if (!dy || !w || z->dim() != 2 || dy->dim() != 2 || !routing_arg(a[3], *z, r)) Py_RETURN_NONE;
-        const int64_t t = r.position->size(0), top = r.position->size(1), d = z->size(1);
-        if (z->size(0) != t * top || dy->size(0) != t || dy->size(1) != d || w->numel() != t * top)
+        if (!z || z->dim() != 2 || !routing_arg(a[1], *z, r)) Py_RETURN_NONE;
+        const Tensor* w = on(plain(a[2], at::kFloat), *z);
+        const int64_t t = r.position->size(0), top = r.position->size(1);
+        if (!w || w->dim() != 2 || w->size(0) != t || w->size(1) != top || z->size(0) != t * top)
             Py_RETURN_NONE;
-        const void* st = current_stream(*z);
-        Tensor dz, dw;
-        call("moe.combine (gradient)", [&] {
-            dz = empty({t * top, d}, z->scalar_type(), *z);
-            dw = empty({t, top}, at::kFloat, *z);
-            return g_lib.moe_combine_grad(st, dy->data_ptr(), type_of(*z), d, z->data_ptr(), d,
-                                          ints(r.position), ints(r.offsets),
-                                          static_cast<const float*>(w->data_ptr()), dz.data_ptr(),
-                                          static_cast<float*>(dw.data_ptr()), t, top,
-                                          r.offsets->numel() - 1, d);
-        });
-        return pair(dz, dw);
-    });
-}
-
-// mx_dx(dy, codes, scales, offsets, type): dy [.., N] times the (experts') weight, the rows
-// of dy flat, in the type
-PyObject* host_mx_dx(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    return guarded(n_args, 5, [&]() -> PyObject* {
-        const Tensor* dy = floating(a[0]);
-        const Tensor *c, *s, *o = nullptr;
-        int32_t type;
-        if (!dy || dy->dim() < 1 || !mx_pair(a[1], a[2], c, s) || !on(c, *dy) || !type_arg(a[4], type))
-            Py_RETURN_NONE;
-        if (a[3] != Py_None) {
-            o = on(plain(a[3], at::kInt), *dy);
-            if (!o || c->dim() != 3 || o->numel() != c->size(0) + 1) Py_RETURN_NONE;
-        } else if (c->dim() != 2) {
-            Py_RETURN_NONE;
-        }
-        const int64_t e = o ? c->size(0) : 0, n = c->size(-2), k = c->size(-1) * 2;
-        const int64_t r = dy->numel() / dy->size(-1);
-        if (dy->size(-1) != n) Py_RETURN_NONE;
-        const int64_t need = g_lib.mx_dx_size(type_of(*dy), type, r, e, n, k);
-        if (need < 0) fail("mxfp4 dx");
-        const void* st = current_stream(*dy);
-        Tensor work, dx;
-        call("mxfp4 dx", [&] {
-            if (need > 0) work = workspace(need, *dy);
-            dx = empty({r, k}, kTypes[type], *dy);
-            return g_lib.mx_dx(st, dy->data_ptr(), type_of(*dy), n, bytes(c), bytes(s),
-                               o ? ints(o) : nullptr, e, dx.data_ptr(), type, r, n, k,
-                               need > 0 ? work.data_ptr() : nullptr, need);
-        });
-        return THPVariable_Wrap(dx);
+        if (!wants_grad(*z, w))
+            return THPVariable_Wrap(run_combine(*z, w, *r.position, *r.offsets, type_of(*z)));
+        return THPVariable_Wrap(CombineFn::apply(*z, *w, *r.position, *r.offsets));
     });
 }
 
@@ -816,8 +941,6 @@ PyMethodDef kMethods[] = {XPU_HOST("bind", host_bind),
                           XPU_HOST("moe_sort", host_moe_sort),
                           XPU_HOST("moe_dispatch", host_moe_dispatch),
                           XPU_HOST("moe_combine", host_moe_combine),
-                          XPU_HOST("moe_combine_grad", host_moe_combine_grad),
-                          XPU_HOST("mx_dx", host_mx_dx),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host",
                        "The int8 API's hot calls in native code (see host_ops.cpp).", -1, kMethods};

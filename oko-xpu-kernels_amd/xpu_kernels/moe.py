@@ -22,7 +22,7 @@ import torch
 
 from . import mxfp4
 from .int8 import _lib as L
-from .mxfp4 import TYPES, _check_float, _native, _opt, _rows, _wants_grad, _work
+from .mxfp4 import TYPES, _check_float, _opt, _rows, _wants_grad, _work
 
 __all__ = ["Routing", "combine", "dispatch", "ffn", "sort"]
 
@@ -104,9 +104,6 @@ def _dispatch(x, routing):
 
 
 def _combine(z, routing, weights, out_dtype):
-    r = _native("moe_combine", z, routing, weights, TYPES[out_dtype])
-    if r is not None:
-        return r
     t, top = routing.position.shape
     d = z.shape[1]
     out = torch.empty((t, d), dtype=out_dtype, device=z.device)
@@ -126,8 +123,7 @@ class _DispatchFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, routing):
         ctx.save_for_backward(*routing)
-        xs = _native("moe_dispatch", x, routing)
-        return _dispatch(x, routing) if xs is None else xs
+        return _dispatch(x, routing)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -146,9 +142,6 @@ class _CombineFn(torch.autograd.Function):
     def backward(ctx, dy):
         z, weights, *routing = ctx.saved_tensors
         routing = Routing(*routing)
-        r = _native("moe_combine_grad", dy, z, weights, routing)
-        if r is not None:
-            return *r, None
         t, top = routing.position.shape
         d = z.shape[1]
         dz = torch.empty((t * top, d), dtype=z.dtype, device=z.device)
@@ -170,7 +163,7 @@ def dispatch(x, routing):
     """x [T, D] -> [T*top, D]: each token's row at each of its slots' places, in
     the experts' order; zeros in the rows of no expert.  The gradient sums a
     token's rows in fp32."""
-    if L.HOST is not None and type(routing) is Routing and not _wants_grad(x):
+    if L.HOST is not None and type(routing) is Routing:
         r = L.HOST.moe_dispatch(x, routing)
         if r is not None:
             return r
@@ -187,8 +180,8 @@ def combine(z, routing, weights):
     """z [T*top, D] in the experts' order -> [T, D]: each token's rows times
     ``weights`` [T, top] (used in fp32), summed in fp32 in slot order.  Gradients
     reach z and weights."""
-    if L.HOST is not None and type(routing) is Routing and not _wants_grad(z, weights):
-        r = L.HOST.moe_combine(z, routing, weights, TYPES.get(getattr(z, "dtype", None), -1))
+    if L.HOST is not None and type(routing) is Routing:
+        r = L.HOST.moe_combine(z, routing, weights)
         if r is not None:
             return r
     _check_float(z, "z")

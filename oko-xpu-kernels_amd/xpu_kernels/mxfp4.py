@@ -67,11 +67,6 @@ def _wants_grad(*tensors):
                                            for t in tensors)
 
 
-def _native(name, *args):
-    """The native host path's call, or None where it leaves the work to ctypes."""
-    return None if L.HOST is None else getattr(L.HOST, name)(*args)
-
-
 def _check_pair(codes, scales, lead=None):
     """The K behind codes and scales, both on the GPU and of matching shapes."""
     for t, name in ((codes, "codes"), (scales, "scales")):
@@ -186,9 +181,6 @@ def _linear(x, codes, scales, bias):
 
 def _dx(dy, codes, scales, offsets, out_dtype):
     """dy [.., N] times the (experts') weight, [R, K]."""
-    r = _native("mx_dx", dy, codes, scales, offsets, TYPES[out_dtype])
-    if r is not None:
-        return r
     n, k = codes.shape[-2], codes.shape[-1] * 2
     dy2, ld = _rows(dy)
     r = dy2.shape[0]
@@ -215,8 +207,7 @@ class _LinearFn(torch.autograd.Function):
     def forward(ctx, x, codes, scales, bias):
         ctx.save_for_backward(codes, scales)
         ctx.bias_dtype = None if bias is None else bias.dtype
-        y = _native("mx_linear", x, codes, scales, bias)
-        return _linear(x, codes, scales, bias) if y is None else y
+        return _linear(x, codes, scales, bias)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -235,7 +226,7 @@ def linear(x, codes, scales, bias=None):
     codes [N, K/2] and scales [N, scale_width(K)]; fp32 sums rounded once to x's
     type.  ``bias`` [N] is bf16, fp16 or fp32.  Gradients: dx = dy @ wq, straight
     through x's quantization, and the bias's column sum; the weight has none."""
-    if L.HOST is not None and not _wants_grad(x, bias):
+    if L.HOST is not None:
         r = L.HOST.mx_linear(x, codes, scales, bias)
         if r is not None:
             return r
@@ -277,8 +268,7 @@ class _GroupedFn(torch.autograd.Function):
     def forward(ctx, x, codes, scales, routing, gather):
         ctx.save_for_backward(codes, scales, *routing)
         ctx.gather = gather
-        y = _native("mx_grouped", x, codes, scales, routing, gather)
-        return _grouped(x, codes, scales, routing, gather) if y is None else y
+        return _grouped(x, codes, scales, routing, gather)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -302,7 +292,7 @@ def grouped_linear(x, codes, scales, routing, gather=False):
     [T, K], each quantized once and read by every row that is its.  Returns
     [T*top, N] in x's type; the gradient reaches x."""
     from . import moe
-    if L.HOST is not None and type(routing) is moe.Routing and not _wants_grad(x):
+    if L.HOST is not None and type(routing) is moe.Routing:
         r = L.HOST.mx_grouped(x, codes, scales, routing, gather)
         if r is not None:
             return r
