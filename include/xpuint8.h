@@ -578,9 +578,9 @@ int xpuint8_mxfp4_grouped_linear_stream(const void *stream, const void *x, int32
 /* dx [R, K] = dy [R, N] wq, of one weight (offsets NULL) or of the experts' over
  * their rows, the gradient straight through x's quantization; fp32 sums, one
  * rounding to dx_type.  work (E: 0 for one weight) holds the weight as bf16 for the
- * shapes that go through it (one weight, bf16 dy and dx, N % 16 == 0, R >= 128), or dy's
+ * shapes that go through it (some of one weight, bf16 dy and dx, N % 16 == 0), or dy's
  * exact bf16 pieces where it is not bf16 in whole 16-byte aligned chunks (N % 8, the
- * row stride % 8); NULL will do for a dy that is, of fewer rows or several experts. */
+ * row stride % 8); NULL will do for several experts and a dy that is. */
 int64_t xpuint8_mxfp4_dx_workspace_size(int32_t type, int32_t dx_type, int64_t R, int64_t E,
                                         int64_t N, int64_t K);
 int xpuint8_mxfp4_dx_stream(const void *stream, const void *dy, int32_t type, int64_t ldy,

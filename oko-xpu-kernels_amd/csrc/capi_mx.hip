@@ -101,11 +101,10 @@ bool dy_direct(const void* dy, int32_t type, int64_t ldy, int64_t N) {
 }
 
 // Whether dx of one weight goes through the weight as bf16 in the workspace and the
-// bf16 product (gemm_bf16_nn), whose tiles fit more shapes: bf16 of whole 16s, from 128
-// rows on (with the weight's conversion 64 against 96 us at 4096 x 5120 -> 1280, 33 against 39
-// at 256 x 4096 -> 4096; below, the conversion is most of it).
+// framework's bf16 product (gemm_bf16_nn): bf16 of whole 16s, where that is the faster.
 bool dx_by_bf16(int32_t type, int32_t dx_type, bool grouped, int64_t R, int64_t N, int64_t K) {
-    return type == kBf16 && dx_type == kBf16 && !grouped && N % 16 == 0 && K % 16 == 0 && R >= 128;
+    return type == kBf16 && dx_type == kBf16 && !grouped && N % 16 == 0 && K % 16 == 0 &&
+           mx4_dx_bf16_faster(R, N, K);
 }
 
 }  // namespace

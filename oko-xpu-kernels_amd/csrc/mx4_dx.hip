@@ -339,7 +339,10 @@ namespace {
 // 2280 us, 4096^3 240 / 299, 4096 x 1280 -> 5120 160 / 139, 1000 x 4096 -> 4096 209 / 95;
 // bf16, 16384 rows 2816 -> 2048 in 8 groups 238 / 220, in 128 groups 532 / 405, 65520
 // rows in 64 groups 798 / 889.
-bool large_dx_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
+struct TileTimes {
+    double small, large;
+};
+TileTimes tile_times(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
     const double stages = double((N + 63) / 64);
     auto tiles = [&](int64_t b) {                          // (a group's last tile half full)
         const int64_t tm = grouped ? R / b + std::min<int64_t>(E, R) / 2 + 1 : (R + b - 1) / b;
@@ -350,11 +353,28 @@ bool large_dx_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
     const double large = double((t256 + cus - 1) / cus) * (8.0 + 1.67 * stages);
     const double small = double(t128 / (2 * cus)) * (4.0 + 1.06 * stages) +
                          (t128 % (2 * cus) > cus ? 4.0 + 1.06 * stages
-                          : t128 % (2 * cus) > 0 ? 4.0 + 0.68 * stages : 0.0);
-    return large < small;
+                          : t128 % (2 * cus) > 0 ? 4.0 + 0.6 * stages : 0.0);
+    return {small, large};
+}
+bool large_dx_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
+    const TileTimes t = tile_times(grouped, R, E, N, K);
+    return t.large < t.small;
 }
 
 }  // namespace
+
+// The weight's conversion (42 MB at 4096 x 4096), two launches and a reduction of fp32
+// slices against one launch of tiles with 64 rows of the weight a stage, of which short
+// contractions and many rows fill the CUs.  Both measured, us, bf16 product against tiles:
+// N 4096, K 4096: 29 / 37 at 1 row, 30 / 37 at 127, 121 / 113 at 4096; N 8192, K 2048 34 / 69 at
+// 16 rows; N 2048, K 8192 27 / 21 at 64; N 1024, K 1024 19 / 12 at 16; 4096 rows, N 5120, K 1280
+// 64 / 96.
+bool mx4_dx_bf16_faster(int64_t R, int64_t N, int64_t K) {
+    const TileTimes t = tile_times(false, R, 1, N, K);
+    const double flop = 2.0 * double(R) * double(N) * double(K);
+    const double bf16 = 15.0 + 0.0014 * double(N) + double(N) * double(K) * 2.5 / 5.0e6 + flop / 1.2e9;
+    return bf16 < std::min(t.small, t.large);
+}
 
 hipError_t mx4_dx(hipStream_t st, const void* dy, int64_t ldy, int pieces, const uint8_t* wc,
                   const uint8_t* ws, const int* offsets, int E, void* dx, int type, int64_t R,

@@ -34,6 +34,8 @@ int64_t mx4_split_width(int64_t N);
 int mx4_split_pieces(int type);
 hipError_t mx4_split(hipStream_t st, const void* dy, int type, int64_t ldy, void* out, int64_t R,
                      int N);
+// whether the weight read back and a bf16 product are faster than mx4_dx (one weight, bf16)
+bool mx4_dx_bf16_faster(int64_t R, int64_t N, int64_t K);
 hipError_t mx4_dx(hipStream_t st, const void* dy, int64_t ldy, int pieces, const uint8_t* wc,
                   const uint8_t* ws, const int* offsets, int E, void* dx, int type, int64_t R,
                   int N, int K);

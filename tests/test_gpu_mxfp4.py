@@ -292,6 +292,20 @@ def test_linear_gradients(dev, dtype, m, k, n):
 @pytest.mark.parametrize("m,k,n", [(127, 96, 64), (128, 96, 64), (129, 1056, 272), (128, 96, 72),
                                    (700, 2080, 1040)])
 def test_linear_gradient_of_many_rows(dev, m, k, n):
+    """Gradients of a bf16 product of more rows than a tile, contiguous and strided."""
+    (codes, scales), wq = weight(n, k, 3, dev)
+    x = randn(m, k, seed=m, dtype=torch.bfloat16).to(dev).requires_grad_()
+    y = mxfp4.linear(x, codes, scales)
+    base = randn(m, n + 24, seed=4, dtype=torch.bfloat16).to(dev)
+    for dy in (base[:, :n].contiguous(), base[:, :n], base[:, 3:n + 3], base[:, :1].expand(m, n)):
+        dx, = torch.autograd.grad(y, x, dy, retain_graph=True)
+        d = dy.cpu().double()
+        assert_close(dx, d @ wq, d.abs() @ wq.abs(), 3 * n)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 512, 1536), (1, 512, 1472), (5, 96, 4096), (16, 512, 2560),
+                                   (300, 512, 4096), (65, 2080, 4112), (129, 544, 4104)])
+def test_linear_gradient_of_long_contractions(dev, m, k, n):
     """Both sides of the sizes at which dx of a bf16 product is taken from the weight read
     back, contiguous and strided."""
     (codes, scales), wq = weight(n, k, 3, dev)
