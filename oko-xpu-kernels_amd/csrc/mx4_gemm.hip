@@ -46,7 +46,7 @@ __device__ __forceinline__ v4f mfma4(const v4i& w, int sw, const v4i& x, int sx,
 // waves do not hold at once, which is walked in chunks with x read again for each.
 //
 // MI355X, kernel alone: 1 x 4096 x 4096 5.9 us; 48 x 4096 x 14336 12.9 us (2.4 TB/s of
-// weight); 16 rows of 13 experts of 2048 x 2816 11.2 us (3.6 TB/s).
+// weight); 16 rows of some 13 experts, 2048 -> 2816, 10 to 11 us (3.6 TB/s).
 template <int T, bool VEC>
 struct Block {                                            // 32 values as they are stored
     uint4 v[T == kF32 ? 8 : 4];
@@ -594,19 +594,40 @@ namespace {
 
 constexpr int64_t kFusedK = 8 * 2 * 512;              // values of a row that the waves hold
 
+// How the kernel of few rows divides a product with MB blocks of rows a block, and about
+// how long it takes.  A wave has 512 values of K (1024 of one block of rows beyond 4096).
+// A block takes nt blocks of weight rows, so that there are as many blocks as the device
+// holds at once (four waves a SIMD by registers, two with four blocks of rows), since each
+// reads all its rows of x again.  Of many groups some are empty, or end inside a block.
+struct FewPlan {
+    int waves, nt;
+    double us;
+};
+FewPlan few_plan(int MB, bool grouped, int64_t R, int E, int64_t N, int64_t K) {
+    FewPlan p;
+    p.waves = K <= 4 * 512 ? 4 : K <= 8 * 512 || MB == 1 ? 8 : 16;
+    const int64_t tiles = (N + 15) / 16, full = (R + 16 * MB - 1) / (16 * MB);
+    const int64_t busy = grouped ? std::max(std::min<int64_t>(R, E), full + E / 2) : full;
+    const int64_t cols = std::max<int64_t>(1, int64_t(device_cus()) * (MB == 4 ? 8 : 16) / p.waves / busy);
+    p.nt = int(std::clamp<int64_t>((tiles + cols - 1) / cols, 1, kFewTiles));
+    // (fitted to 17 to 512 rows of 25 weights)
+    const double rounds = double(tiles * busy) / double(cols * busy * p.nt);
+    const double turns = double(p.nt) * std::max(1.0, rounds);
+    p.us = K <= 2048   ? 5.3 + 1.25 * turns
+           : K <= 4096 ? 6.9 + 1.2 * turns
+           : K <= 8192 ? 6.9 + 2.4 * turns
+                       : 6.5 + 6.0 * turns * double((K + 8191) / 8192);
+    return p;
+}
+
 // rows of x in their own type or quantized (codes), on the kernel of few rows
 template <int T, bool VEC, bool FUSED, int MB>
 hipError_t few(hipStream_t st, const Rows& x, const Weight& w, const int* offsets, int E,
                const Out& o) {
     const int tiles = (o.N + 15) / 16;
     const int64_t tm = most_tiles(offsets != nullptr, o.R, E, 16 * MB);
-    // Weight blocks a block: as many blocks as the device holds at once (four waves a SIMD
-    // by registers, two with four blocks of rows), since each reads all its rows of x
-    // again.  Of many groups most are empty, or hold one row.
-    const int64_t busy = offsets ? std::min<int64_t>(o.R, E) : tm;
-    const int nw = w.K <= 4 * 512 ? 4 : 8;
-    const int64_t want = int64_t(device_cus()) * (MB == 4 ? 8 : 16) / nw;
-    const int nt = int(std::clamp<int64_t>((tiles * busy + want - 1) / want, 1, kFewTiles));
+    const FewPlan plan = few_plan(MB, offsets != nullptr, o.R, E, o.N, w.K);
+    const int nw = plan.waves, nt = plan.nt;
     auto go = [&](auto W, auto S, auto D, auto C) {
         constexpr int nw = decltype(W)::value, ss = decltype(S)::value, d = decltype(D)::value;
         hipLaunchKernelGGL((mx4_few_kernel<T, VEC, FUSED, MB, nw, ss, d, decltype(C)::value>),
@@ -618,23 +639,36 @@ hipError_t few(hipStream_t st, const Rows& x, const Weight& w, const int* offset
     using Two = std::integral_constant<int, 2>;
     using Four = std::integral_constant<int, 4>;
     using Eight = std::integral_constant<int, 8>;
-    using Groups = std::integral_constant<int, MB == 1 ? 2 : 1>;
+    using Sixteen = std::integral_constant<int, 16>;
     auto whole = [&](auto W, auto S) {                   // (one step: nothing to request ahead)
         if (nt == 1) return go(W, S, One{}, std::false_type{});
         return go(W, S, Two{}, std::false_type{});
     };
     if (nw == 4) return whole(Four{}, One{});
     if (w.K <= 8 * 512) return whole(Eight{}, One{});
-    if constexpr (FUSED) return whole(Eight{}, Groups{});
-    else return go(Eight{}, Groups{}, Two{}, std::true_type{});
+    if constexpr (FUSED) return whole(Eight{}, Two{});
+    else if constexpr (MB == 1) return go(Eight{}, Two{}, Two{}, std::true_type{});
+    else if constexpr (MB == 2) {
+        if (w.K <= 16 * 512) return whole(Sixteen{}, One{});
+        return go(Sixteen{}, One{}, Two{}, std::true_type{});
+    }
+    return hipErrorInvalidValue;                          // (more rows: up to 4096 values)
 }
 
 }  // namespace
 
-// Up to 16 rows a group on average the weight's bytes are the product's time and the
-// quantizer's launch (2 to 3 us) would be a third of the rest.
+namespace {
+// Up to 16 rows, or 8 a group on average, one block of rows is enough (of 16 on average
+// nearly half of the groups would have two): blocks of 16 against 32, us, 8 groups of 8 rows
+// 2048 -> 1024 6.2 / 8.6; 32 groups 2048 -> 2816 of 8 rows 22 / 22, of 11 25 / 22, of 16 30 / 22;
+// 64 groups of 11 4096 -> 1024 38 / 29.
+bool one_block(bool grouped, int64_t R, int E) { return R <= (grouped ? 8 * int64_t(E) : 16); }
+}  // namespace
+
+// With one block of rows the weight's bytes are the product's time and the quantizer's
+// launch (2 to 3 us) would be a third of the rest.
 bool mx4_fused(int64_t R, bool grouped, int E, int64_t K) {
-    return R <= 16 * int64_t(grouped ? E : 1) && K <= kFusedK;
+    return one_block(grouped, R, E) && K <= kFusedK;
 }
 
 hipError_t mx4_product_fused(hipStream_t st, const void* x, int type, int64_t ldx,
@@ -657,13 +691,16 @@ hipError_t mx4_product_fused(hipStream_t st, const void* x, int type, int64_t ld
 
 namespace {
 
-// Whether 256 x 256 tiles (one block a CU, half the operand bytes a product) are
-// faster than 128 x 128 (two blocks a CU, so that one's start and end overlap the
-// other's steps, and finer rounds), by the times that a round of either takes, fitted to
-// both over 13 shapes.  With the quantizer, 256 against 128: 8192^3 342 / 405 us, 2048 x
-// 8192 x 8192 83 / 98, 4096^3 54 / 60; 4096 x 1280 -> 5120 44 / 34, 4096 x 2560 -> 10240 88 / 84,
-// 1000 x 4096 x 4096 39 / 22, 16380 x 2048 -> 2816 in 32 groups 128 / 111.
-bool large_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
+// The times, us, of 128 x 128 tiles (two blocks a CU, so that one's start and end overlap the
+// other's steps, and finer rounds) and of 256 x 256 tiles (one block a CU, half the operand
+// bytes a product), by what a round of either takes, fitted to both over 13 shapes.  With
+// the quantizer, 256 against 128: 8192^3 342 / 405 us, 2048 x 8192 x 8192 83 / 98, 4096^3
+// 54 / 60; 4096 x 1280 -> 5120 44 / 34, 4096 x 2560 -> 10240 88 / 84, 1000 x 4096 x 4096 39 / 22,
+// 16380 x 2048 -> 2816 in 32 groups 128 / 111.
+struct TileTimes {
+    double small, large;
+};
+TileTimes tile_times(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
     const double steps = double((K + 127) / 128);
     auto tiles = [&](int64_t b) {                          // (a group's last tile half full)
         const int64_t tm = grouped ? R / b + std::min<int64_t>(E, R) / 2 + 1 : (R + b - 1) / b;
@@ -674,8 +711,9 @@ bool large_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
     const double large = double((t256 + cus - 1) / cus) * (10.0 + 1.07 * steps);
     const double small = double(t128 / (2 * cus)) * (2.6 + 0.68 * steps) +
                          (t128 % (2 * cus) > cus ? 2.6 + 0.68 * steps
-                          : t128 % (2 * cus) > 0 ? 2.6 + 0.46 * steps : 0.0);
-    return large < small;
+                          : t128 % (2 * cus) > cus / 2 ? 2.6 + 0.46 * steps
+                          : t128 % (2 * cus) > 0 ? 2.3 + 0.34 * steps : 0.0);
+    return {small, large};
 }
 
 }  // namespace
@@ -686,18 +724,26 @@ hipError_t mx4_product(hipStream_t st, const uint8_t* xc, const uint8_t* xs, con
                        int K) {
     const Weight w{wc, ws, N, K, int(mx_scale_width(K))};
     const Out o = make_out(y, type, bias, bias_type, R, N);
-    // Up to 64 rows the kernel of few rows: 64 x 4096 x 4096 12.5 us with the quantizer against
-    // 17.5 in tiles, 64 x 4096 x 14336 16.1 / 18.2, 48 x 14336 x 4096 27 / 38; 96 rows would
-    // take its block twice, and tiles need 17.5.
+    const TileTimes tiles = tile_times(offsets != nullptr, R, E, N, K);
+    // The kernel of few rows, with one block of rows always, with more (up to where a
+    // block's rows of x would be read many times over) where its weight blocks take less time
+    // than tiles.  With the quantizer, us, few rows against tiles: 64 x 4096 x 4096 10.6 / 15.7,
+    // 256 rows 15.0 / 17.3, 512 rows 20.8 / 18.7; 64 x 8192 x 4096 14.5 / 25.1, 128 rows 19.2 /
+    // 26.9; 32 x 14336 x 4096 21 / 40, 64 rows 33 / 42, 128 rows 58 / 46; 128 x 2048 x 14336 14.1 / 11.5.
+    // Groups, up to 64 rows on average: 32 groups of 40 rows 2048 -> 2816 25 / 30, of 64 33 / 39, of
+    // 100 44 / 44; 64 groups of 40 rows 4096 -> 1024 40 / 46, of 64 56 / 51, of 200 110 / 80.
     const int64_t per_group = offsets ? (R + E - 1) / E : R;
-    if (per_group <= 64) {
+    const int mb = one_block(offsets != nullptr, R, E) ? 1 : per_group <= 32 || K > 8 * 512 ? 2 : 4;
+    const bool blocks = offsets ? per_group <= 64
+                                : R <= 512 && few_plan(mb, false, R, E, N, K).us < std::min(tiles.small, tiles.large);
+    if (mb == 1 || blocks) {
         const Rows in{nullptr, 0, xc, xs, rows, int(tokens)};
         hipError_t e = hipSuccess;
         by_type(type, [&](auto T) {
             constexpr int t = decltype(T)::value;
-            e = per_group <= 16   ? few<t, true, false, 1>(st, in, w, offsets, E, o)
-                : per_group <= 32 ? few<t, true, false, 2>(st, in, w, offsets, E, o)
-                                  : few<t, true, false, 4>(st, in, w, offsets, E, o);
+            e = mb == 1   ? few<t, true, false, 1>(st, in, w, offsets, E, o)
+                : mb == 2 ? few<t, true, false, 2>(st, in, w, offsets, E, o)
+                          : few<t, true, false, 4>(st, in, w, offsets, E, o);
         });
         return e;
     }
@@ -715,7 +761,7 @@ hipError_t mx4_product(hipStream_t st, const uint8_t* xc, const uint8_t* xs, con
     };
     using I128 = std::integral_constant<int, 128>;
     using I256 = std::integral_constant<int, 256>;
-    if (large_tiles(offsets != nullptr, R, E, N, K)) go(I256{}, I256{});
+    if (tiles.large < tiles.small) go(I256{}, I256{});
     else go(I128{}, I128{});
     return hipGetLastError();
 }

@@ -152,6 +152,17 @@ def test_linear_few_rows(dev, dtype, m, k, n):
     check_linear(dev, x, n, bias=randn(n, seed=2, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype,m,k,n", [
+    (torch.bfloat16, 130, 4096, 520), (torch.float16, 300, 3104, 1040), (torch.float32, 500, 2048, 264),
+    (torch.bfloat16, 97, 8192, 1000), (torch.bfloat16, 33, 16416, 40), (torch.float16, 64, 8224, 4120),
+    (torch.bfloat16, 511, 4128, 72)])
+def test_linear_several_blocks_of_few_rows(dev, dtype, m, k, n):
+    """More rows than a block of the kernel of few rows takes, K on both sides of what its
+    waves hold."""
+    x = randn(m, k, seed=m, dtype=dtype)
+    check_linear(dev, x, n, bias=randn(n, seed=2, dtype=dtype))
+
+
 @pytest.mark.parametrize("t,top,experts,k,n,dropped", [
     (3, 3, 40, 2080, 2056, 0.0), (60, 4, 10, 544, 300, 0.1), (60, 4, 10, 4160, 136, 0.1),
     (100, 5, 9, 288, 520, 0.05), (70, 6, 8, 4128, 72, 0.0), (31, 2, 4, 8224, 40, 0.2)])
