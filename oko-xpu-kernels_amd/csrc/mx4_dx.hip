@@ -57,8 +57,8 @@ __global__ __launch_bounds__(256) void mx4_split_kernel(const char* __restrict__
 }
 
 // ------------------------------------------------------------------- tiles
-// BM x BK tiles of dx by a block of 4 waves in 2 x 2 (a wave every other 16 rows, one
-// half of the columns), 64 contraction rows a stage (two MFMAs of each block); dy in
+// BM x BK tiles of dx by a block of 4 waves in WM x 4 / WM (of two by rows, each has every
+// other 16 of them), 64 contraction rows a stage (two MFMAs of each block); dy in
 // three LDS slots, the weight in two.  While a stage's first half runs, a wave reads the
 // second half's fragments; one wait and barrier then mean that every wave has read the
 // stage, and that the next one is in; while the second half runs, it reads the next
@@ -104,20 +104,29 @@ __device__ __forceinline__ void acc_bf16_4(const v4i& w0, const v4i& w1, const v
     if constexpr (COUNT == 64) XPU_BF16_4(XPU_A64);
     else XPU_BF16_4(XPU_A256);
 }
+template <int B0, int B1>
+__device__ __forceinline__ void acc_bf16_2(const v4i& w0, const v4i& w1, const v4i& x) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 a[%3:%4], %0, %2, a[%3:%4]\n\t"
+                 "v_mfma_f32_16x16x32_bf16 a[%5:%6], %1, %2, a[%5:%6]\n\t"
+                 ::"v"(w0), "v"(w1), "v"(x), "n"(4 * B0), "n"(4 * B0 + 3), "n"(4 * B1), "n"(4 * B1 + 3)
+                 : XPU_A64);
+}
 
-template <int BM, int BK>
-__global__ __launch_bounds__(256, BM * BK > 128 * 128 ? 1 : 2) void mx4_dx_kernel(
+template <int BM, int BK, int WM>
+__global__ __launch_bounds__(256, BM * BK > 128 * 128 ? 1 : BM < 128 ? 3 : 2) void mx4_dx_kernel(
     const uint16_t* __restrict__ dy, int64_t ldy, int pieces, int width, Weight w,
     const int* __restrict__ offsets, int E, Out out, int type, int tiles_m, int tiles_k) {
-    constexpr int TM = BM / 32, TK = BK / 32;             // MFMA blocks of a wave
+    constexpr int WK = 4 / WM;                            // waves by rows, by columns
+    constexpr int TM = BM / 16 / WM, TK = BK / 16 / WK;   // MFMA blocks of a wave
     constexpr int DY = BM * 128, WROW = 2 * BK, WT = 64 * WROW, W0 = 3 * DY;
     constexpr int PX = BM / 32;                           // dy loads a wave a stage
     constexpr int NB = BK / 128;                          // weight blocks a thread a stage
-    constexpr int ACC = 4 * TM * TK;                      // block (a, b) is number a * TM + b
+    constexpr int ACC = TM * TK > 16 ? 256 : 64;          // block (a, b) is number a * TM + b
+    static_assert(4 * TM * TK <= ACC && TK % 2 == 0, "registers, and blocks a column takes together");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[3 * DY + 2 * WT];
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-    const int wm = wave >> 1, wk = wave & 1;
+    const int wm = wave / WK, wk = wave % WK;
     int tm, tk;
     if (!tile_of(blockIdx.x, tiles_m, tiles_k, tm, tk)) return;
     RowTile t;
@@ -202,7 +211,7 @@ __global__ __launch_bounds__(256, BM * BK > 128 * 128 ? 1 : 2) void mx4_dx_kerne
     v2i wl[2][TK], wh[2][TK];
     auto read_y = [&](uint32_t slot, auto H, auto I) {
         constexpr int h = decltype(H)::value, i = decltype(I)::value;
-        yf[h][i] = read16((yat ^ (64 * h)) + slot, i * 32 * 128);
+        yf[h][i] = read16((yat ^ (64 * h)) + slot, i * 16 * WM * 128);
     };
     auto read_w = [&](uint32_t slot, auto H, auto I) {
         constexpr int h = decltype(H)::value, i = decltype(I)::value;
@@ -215,11 +224,15 @@ __global__ __launch_bounds__(256, BM * BK > 128 * 128 ? 1 : 2) void mx4_dx_kerne
     // column b of half h
     auto column = [&](auto H, auto B, const v4i (&wf)[TK]) {
         constexpr int h = decltype(H)::value, b = decltype(B)::value;
-        each<TK / 4>([&](auto A) {
-            constexpr int a = 4 * decltype(A)::value;
-            acc_bf16_4<ACC, a * TM + b, (a + 1) * TM + b, (a + 2) * TM + b, (a + 3) * TM + b>(
-                wf[a], wf[a + 1], wf[a + 2], wf[a + 3], yf[h][b]);
-        });
+        if constexpr (TK == 2) {
+            acc_bf16_2<b, TM + b>(wf[0], wf[1], yf[h][b]);
+        } else {
+            each<TK / 4>([&](auto A) {
+                constexpr int a = 4 * decltype(A)::value;
+                acc_bf16_4<ACC, a * TM + b, (a + 1) * TM + b, (a + 2) * TM + b, (a + 3) * TM + b>(
+                    wf[a], wf[a + 1], wf[a + 2], wf[a + 3], yf[h][b]);
+            });
+        }
         __builtin_amdgcn_sched_barrier(0);
     };
 
@@ -303,8 +316,8 @@ __global__ __launch_bounds__(256, BM * BK > 128 * 128 ? 1 : 2) void mx4_dx_kerne
     }
     wait_vm<0>();                                         // (the last load_w may be on its way)
     block_barrier();                                      // every wave has read its last stage
-    store_tile<TM, TK>(out, type, t.row + 16 * wm, t.end, k0 + wk * (BK / 2),
-                       reinterpret_cast<float*>(smem) + wave * 16 * (BK / 2));
+    store_tile<TM, TK, 16 * WM>(out, type, t.row + 16 * wm, t.end, k0 + wk * (BK / WK),
+                                reinterpret_cast<float*>(smem) + wave * 16 * (BK / WK));
 }
 
 }  // namespace
@@ -360,20 +373,29 @@ bool large_dx_tiles(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
     const TileTimes t = tile_times(grouped, R, E, N, K);
     return t.large < t.small;
 }
+// Whether tiles of 32 rows (three blocks a CU, a wave 32 columns) are faster than 128: up to 64
+// rows a group on average, where most of a large tile would be empty, or while they are few
+// enough to run all at once.  us, 32 against 128 rows: 32 groups 2816 -> 2048 of 8 rows 41 / 75, of
+// 32 62 / 75, of 64 83 / 93, of 100 105 / 97; 64 groups 1024 -> 4096 of 16 69 / 102, of 200 314 / 260;
+// 256 rows of one weight, fp16, 4096 x 4096 62 / 80.
+bool few_dx_rows(bool grouped, int64_t R, int E, int64_t K) {
+    const int64_t rows = grouped ? R / 32 + std::min<int64_t>(E, R) / 2 + 1 : (R + 31) / 32;
+    return R <= 64 * int64_t(grouped ? E : 1) || rows * ((K + 127) / 128) <= 2 * device_cus();
+}
 
 }  // namespace
 
 // The weight's conversion (42 MB at 4096 x 4096), two launches and a reduction of fp32
 // slices against one launch of tiles with 64 rows of the weight a stage, of which short
 // contractions and many rows fill the CUs.  Both measured, us, bf16 product against tiles:
-// N 4096, K 4096: 29 / 37 at 1 row, 30 / 37 at 127, 121 / 113 at 4096; N 8192, K 2048 34 / 69 at
-// 16 rows; N 2048, K 8192 27 / 21 at 64; N 1024, K 1024 19 / 12 at 16; 4096 rows, N 5120, K 1280
-// 64 / 96.
+// N 4096, K 4096: 29 / 24 at 1 row, 121 / 113 at 4096; N 8192, K 2048 34 / 54 at 16 rows; N 2048,
+// K 8192 27 / 15 at 64; 4096 rows, N 5120, K 1280 64 / 96.
 bool mx4_dx_bf16_faster(int64_t R, int64_t N, int64_t K) {
     const TileTimes t = tile_times(false, R, 1, N, K);
     const double flop = 2.0 * double(R) * double(N) * double(K);
     const double bf16 = 15.0 + 0.0014 * double(N) + double(N) * double(K) * 2.5 / 5.0e6 + flop / 1.2e9;
-    return bf16 < std::min(t.small, t.large);
+    const double few = few_dx_rows(false, R, 1, K) ? 3.5 + 0.4 * double((N + 63) / 64) : t.small;
+    return bf16 < std::min({few, t.small, t.large});
 }
 
 hipError_t mx4_dx(hipStream_t st, const void* dy, int64_t ldy, int pieces, const uint8_t* wc,
@@ -383,17 +405,23 @@ hipError_t mx4_dx(hipStream_t st, const void* dy, int64_t ldy, int pieces, const
     const Out o = make_out(dx, type, nullptr, 0, R, K);
     // pieces lie side by side, mx4_split_width(N) columns each; one piece may end early
     const int width = pieces == 1 ? N : int(mx4_split_width(N));
-    auto go = [&](auto B) {
-        constexpr int b = decltype(B)::value;
-        const int tiles_k = (K + b - 1) / b;
-        const int tiles_m = int(most_tiles(offsets != nullptr, R, E, b));
-        hipLaunchKernelGGL((mx4_dx_kernel<b, b>),
+    auto go = [&](auto M, auto C, auto W) {
+        constexpr int bm = decltype(M)::value, bk = decltype(C)::value, wm = decltype(W)::value;
+        const int tiles_k = (K + bk - 1) / bk;
+        const int tiles_m = int(most_tiles(offsets != nullptr, R, E, bm));
+        hipLaunchKernelGGL((mx4_dx_kernel<bm, bk, wm>),
                            dim3(unsigned((int64_t(tiles_m) * tiles_k + 7) / 8 * 8)), dim3(256), 0,
                            st, static_cast<const uint16_t*>(dy), ldy, pieces, width, w, offsets, E,
                            o, type, tiles_m, tiles_k);
     };
-    if (large_dx_tiles(offsets != nullptr, R, E, N, K)) go(std::integral_constant<int, 256>{});
-    else go(std::integral_constant<int, 128>{});
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I32 = std::integral_constant<int, 32>;
+    using I128 = std::integral_constant<int, 128>;
+    using I256 = std::integral_constant<int, 256>;
+    if (few_dx_rows(offsets != nullptr, R, E, K)) go(I32{}, I128{}, I1{});
+    else if (large_dx_tiles(offsets != nullptr, R, E, N, K)) go(I256{}, I256{}, I2{});
+    else go(I128{}, I128{}, I2{});
     return hipGetLastError();
 }
 

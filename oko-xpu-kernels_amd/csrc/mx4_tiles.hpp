@@ -135,9 +135,9 @@ __device__ __forceinline__ bool tile_of(int b, int tiles_m, int tiles_n, int& tm
 }
 
 // The results of a wave's TM x TN blocks (block (a, b) in registers 4 (a TM + b) up, b's
-// rows row0 + 32 b up) to the rows below end and the columns n up.  `mine`: 16 x 16 TN fp32 of idle LDS
+// rows row0 + STEP b up) to the rows below end and the columns n up.  `mine`: 16 x 16 TN fp32 of idle LDS
 // of the wave's own, through which types and edges go that 16-byte stores do not serve.
-template <int TM, int TN>
+template <int TM, int TN, int STEP = 32>
 __device__ __forceinline__ void store_tile(const Out& out, int type, int row0, int end, int n,
                                            float* mine) {
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
@@ -146,7 +146,7 @@ __device__ __forceinline__ void store_tile(const Out& out, int type, int row0, i
     auto store = [&](auto T) {
         each<TM>([&](auto B) {
             constexpr int b = decltype(B)::value;
-            const int row = row0 + 32 * b + r;
+            const int row = row0 + STEP * b + r;
             store_row<decltype(T)::value, TN>(out, row, row < end, n, [&](auto A) {
                 return acc_get<decltype(A)::value * TM + b>();
             });
@@ -166,7 +166,7 @@ __device__ __forceinline__ void store_tile(const Out& out, int type, int row0, i
 #pragma clang loop unroll(disable)
         for (int i = lane; i < 16 * (4 * TN); i += 64) {
             const int rr = i / (4 * TN), c = 4 * (i % (4 * TN));
-            const int row = row0 + 32 * b + rr;
+            const int row = row0 + STEP * b + rr;
             const v4f v = *reinterpret_cast<const v4f*>(mine + rr * (16 * TN) + c);
             if (row >= end) continue;
             if (type == kBf16) store4<kBf16>(out, row, n + c, v);

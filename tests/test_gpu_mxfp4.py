@@ -329,6 +329,37 @@ def test_linear_gradient_of_long_contractions(dev, m, k, n):
         assert_close(dx, d @ wq, d.abs() @ wq.abs(), 3 * n)
 
 
+@pytest.mark.parametrize("dtype,m,k,n", [
+    (torch.float16, 64, 4224, 136), (torch.float16, 65, 33056, 72), (torch.float32, 31, 160, 200),
+    (torch.float32, 33, 1056, 1000), (torch.bfloat16, 64, 96, 1032), (torch.float16, 260, 16416, 40)])
+def test_linear_gradient_in_tiles_of_few_rows(dev, dtype, m, k, n):
+    """Row and column ends of the small tiles, one piece of dy and several, and shapes
+    that go to the larger ones."""
+    (codes, scales), wq = weight(n, k, 3, dev)
+    x = randn(m, k, seed=m, dtype=dtype).to(dev).requires_grad_()
+    dy = randn(m, n, seed=4, dtype=dtype)
+    dx, = torch.autograd.grad(mxfp4.linear(x, codes, scales), x, dy.to(dev))
+    d = dy.double()
+    assert_close(dx, d @ wq, d.abs() @ wq.abs(), 3 * n)
+
+
+@pytest.mark.parametrize("t,top,experts,k,n,dropped", [
+    (50, 2, 3, 1056, 264, 0.1), (97, 2, 3, 160, 520, 0.0), (700, 1, 11, 288, 72, 0.1), (33, 1, 1, 96, 1000, 0.0)])
+def test_grouped_gradient_of_few_rows(dev, t, top, experts, k, n, dropped):
+    """Groups on both sides of 32 and 64 rows."""
+    ids = router(t, top, experts, seed=t, dropped=dropped)
+    routing = moe.sort(ids.to(dev), experts)
+    _, opos, orows, ooff = O.sort(ids, experts)
+    codes, scales = mxfp4.quantize(randn(experts, n, k, seed=7, scale=0.05).to(dev))
+    wt = O.dequantize(codes.cpu(), scales.cpu()).transpose(1, 2)
+    r = t * top
+    x = randn(r, k, seed=8, dtype=torch.bfloat16).to(dev).requires_grad_()
+    dy = randn(r, n, seed=9, dtype=torch.bfloat16)
+    dx, = torch.autograd.grad(mxfp4.grouped_linear(x, codes, scales, routing), x, dy.to(dev))
+    d, same = dy.double(), torch.arange(r, dtype=torch.int32)
+    assert_close(dx, O.grouped(d, wt, same, ooff), O.grouped(d.abs(), wt.abs(), same, ooff), n)
+
+
 def test_linear_gradient_of_strided_dy(dev):
     x = randn(50, 96, seed=1, dtype=torch.bfloat16).to(dev).requires_grad_()
     (codes, scales), wq = weight(64, 96, 3, dev)
