@@ -303,9 +303,8 @@ __global__ __launch_bounds__(NW * 64) void mx4_few_kernel(Rows x, Weight w,
     "], %" #S ", %9 op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t"
 template <int COUNT, int B0, int B1, int B2, int B3>
 __device__ __forceinline__ void acc_mfma4(const v4i* w, const int* sw, const v4i& x, int sx) {
-    static_assert(COUNT == 64 || COUNT == 128 || COUNT == 256, "a list of registers");
+    static_assert(COUNT == 64 || COUNT == 256, "a list of registers");
     if constexpr (COUNT == 64) XPU_MFMA4(XPU_A64);
-    else if constexpr (COUNT == 128) XPU_MFMA4(XPU_A128);
     else XPU_MFMA4(XPU_A256);
 }
 template <int BM, int BN, bool GATHER>
@@ -644,15 +643,18 @@ hipError_t few(hipStream_t st, const Rows& x, const Weight& w, const int* offset
         if (nt == 1) return go(W, S, One{}, std::false_type{});
         return go(W, S, Two{}, std::false_type{});
     };
-    if (nw == 4) return whole(Four{}, One{});
-    if (w.K <= 8 * 512) return whole(Eight{}, One{});
-    if constexpr (FUSED) return whole(Eight{}, Two{});
-    else if constexpr (MB == 1) return go(Eight{}, Two{}, Two{}, std::true_type{});
-    else if constexpr (MB == 2) {
-        if (w.K <= 16 * 512) return whole(Sixteen{}, One{});
-        return go(Sixteen{}, One{}, Two{}, std::true_type{});
+    if constexpr (MB == 1 && !FUSED) {                    // (a K that cannot be quantized in place)
+        return go(Eight{}, Two{}, Two{}, std::true_type{});
+    } else {
+        if (nw == 4) return whole(Four{}, One{});
+        if (w.K <= 8 * 512) return whole(Eight{}, One{});
+        if constexpr (FUSED) return whole(Eight{}, Two{});
+        if constexpr (MB == 2) {
+            if (w.K <= 16 * 512) return whole(Sixteen{}, One{});
+            return go(Sixteen{}, One{}, Two{}, std::true_type{});
+        }
+        return hipErrorInvalidValue;                      // (four blocks: up to 4096 values)
     }
-    return hipErrorInvalidValue;                          // (more rows: up to 4096 values)
 }
 
 }  // namespace

@@ -123,10 +123,6 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p));
 }
 
-// every direct load of this wave has landed (before the barrier that lets others
-// read it)
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // the most row tiles of BM rows that R rows in E groups can make, the rows of no
 // group included
 int64_t most_tiles(bool grouped, int64_t R, int E, int BM) {

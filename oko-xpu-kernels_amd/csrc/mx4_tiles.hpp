@@ -62,7 +62,6 @@ __device__ __forceinline__ void block_barrier() {
 #define XPU_A60 XPU_A10(), XPU_A10(1), XPU_A10(2), XPU_A10(3), XPU_A10(4), XPU_A10(5)
 #define XPU_A64 XPU_A60, "a60", "a61", "a62", "a63"
 #define XPU_A120 XPU_A60, XPU_A10(6), XPU_A10(7), XPU_A10(8), XPU_A10(9), XPU_A10(10), XPU_A10(11)
-#define XPU_A128 XPU_A120, "a120", "a121", "a122", "a123", "a124", "a125", "a126", "a127"
 #define XPU_A256 XPU_A120, XPU_A10(12), XPU_A10(13), XPU_A10(14), XPU_A10(15), XPU_A10(16),     \
                  XPU_A10(17), XPU_A10(18), XPU_A10(19), XPU_A10(20), XPU_A10(21), XPU_A10(22),  \
                  XPU_A10(23), XPU_A10(24), "a250", "a251", "a252", "a253", "a254", "a255"
@@ -76,7 +75,6 @@ __device__ __forceinline__ void block_barrier() {
 template <int COUNT, int BLOCK>
 __device__ __forceinline__ void acc_set(const v4f& v) {
     if constexpr (COUNT == 64) XPU_ACC_SET(XPU_A64);
-    else if constexpr (COUNT == 128) XPU_ACC_SET(XPU_A128);
     else XPU_ACC_SET(XPU_A256);
 }
 template <int BLOCK>
