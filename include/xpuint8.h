@@ -555,7 +555,8 @@ int xpuint8_mxfp4_dequantize_stream(const void *stream, const uint8_t *codes,
                                     int64_t K);
 
 /* y [M, N] = xq wq^T (+ bias [N]): x [M, K] quantized in the call, the weight codes
- * [N, K/2] and scales [N, W]; fp32 sums, one rounding to y's type, which is x's. */
+ * [N, K/2] and scales [N, W]; fp32 sums, one rounding to y's type, which is x's.
+ * K <= 2^24 here and in the products below. */
 int64_t xpuint8_mxfp4_linear_workspace_size(int64_t M, int64_t N, int64_t K);
 int xpuint8_mxfp4_linear_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
                                 const uint8_t *codes, const uint8_t *scales, const void *bias,

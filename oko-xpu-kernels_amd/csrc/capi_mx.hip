@@ -36,8 +36,9 @@ int check_product(int64_t R, int64_t tokens, int64_t N, int64_t K, bool grouped,
     if (R <= 0 || tokens <= 0 || N <= 0) return fail(2, "rows, tokens and N must be positive");
     if (K <= 0) return fail(2, "K must be positive");
     if (K % 32 != 0) return fail(3, "K must be a multiple of the MXFP4 block (32)");
-    if (R > kMaxDim || tokens > kMaxDim || N > kMaxDim || K > kMaxDim)
-        return fail(4, "rows, tokens, N and K must be < 2^31");
+    if (R > kMaxDim || tokens > kMaxDim || N > kMaxDim)
+        return fail(4, "rows, tokens and N must be < 2^31");
+    if (K > int64_t(1) << 24) return fail(4, "K must be at most 2^24");    // (256 rows of a tile: 2 GiB)
     if (grouped && (E < 1 || E > kMaxExperts)) return fail(2, "experts must be 1..1024");
     if (tokens * (K / 32) >= kMaxUnits || N * (K / 32) >= kMaxUnits || tokens * N >= kMaxUnits * 16)
         return fail(4, "an operand of more than 2^32 blocks is not supported");

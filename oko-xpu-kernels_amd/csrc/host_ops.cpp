@@ -1,9 +1,9 @@
 // The host path of the Python API's hot calls (xpu_kernels.int8 linear, ffn, the
 // backward's products and the quantizer; xpu_kernels.mxfp4 and moe with their gradients)
 // as a CPython extension: argument checks, the packed weight's lookup, allocations and
-// the library call in native code.  In Python these cost more than the small calls' kernels: linear
-// at 16 x 4096 x 4096 took 17.6 us of host time for 8.5 us of GPU work, 6.9 of
-// them the library's two launches.
+// the library call in native code.  In Python these cost more than the small calls'
+// kernels: linear at 16 x 4096 x 4096 took 17.6 us of host time for 8.5 us of GPU work,
+// 6.9 of them the library's two launches.
 //
 // Every function takes the plain case only -- dense CUDA tensors of exactly the
 // dtype, shape, alignment and device the kernels read, no subclass, no

@@ -121,6 +121,10 @@ def test_library_refusals(lib, fn, args, code, substr):
 def test_library_sizes(lib):
     assert lib.xpuint8_mxfp4_scale_width(1280) == 48 and lib.xpuint8_mxfp4_scale_width(48) == -1
     assert lib.xpuint8_mxfp4_linear_workspace_size(4, 8, 48) == -1
+    assert lib.xpuint8_mxfp4_linear_workspace_size(100, 8, 1 << 24) > 0
+    assert lib.xpuint8_mxfp4_linear_workspace_size(100, 8, (1 << 24) + 32) == -1
+    assert b"2^24" in lib.xpuint8_last_error()
+    assert lib.xpuint8_mxfp4_dx_workspace_size(0, 0, 100, 0, 8, (1 << 24) + 32) == -1
     assert lib.xpuint8_mxfp4_linear_workspace_size(1000, 8, 64) >= 1000 * (32 + 16)
     assert lib.xpuint8_mxfp4_grouped_linear_workspace_size(8, 4, 0, 8, 64) == -1
     assert lib.xpuint8_mxfp4_dx_workspace_size(2, 2, 10, 0, 100, 64) >= 10 * 128 * 3 * 2
