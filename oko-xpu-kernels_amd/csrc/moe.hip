@@ -23,9 +23,10 @@ namespace {
 // With the counters of every wave before it, and those of every block before, a wave
 // knows where its first slot of each key goes, and a second pass over the same
 // registers hands out the places.  Up to 8192 slots are one launch of one block; more
-// take a launch of the counts first, in blocks of 2048 slots (8192 from 128 K on, so
-// that no block reads more than a few dozen others' counts).  Bound by latency: the
-// loads of the keys, some 200 cycles for each 64 of a wave, a store a slot.
+// take a launch of the counts first, in blocks of 2048 slots (8192 from 128 K on: each
+// block reads the counts of all).  Bound by latency: the loads of the keys, some 200 cycles
+// for each 64 of a wave, a store a slot.  32 slots 3.5 us, 64 K slots 4.6 + 9.7 us (27 with the
+// keys read again from memory in the second pass).
 constexpr int kSortWaves = 16;
 constexpr int kSortThreads = kSortWaves * 64;
 constexpr int kMaxExperts = 1024;
@@ -200,21 +201,23 @@ hipError_t sort_launch(hipStream_t st, const I* ids, int* counts, int* order, in
 // They go by tokens, not by rows: a token's own row is read (or its sum kept in
 // registers) once for all its slots, and the row of slot j is at position[t, j];
 // positions are every row exactly once, so every row is written, zeros where no
-// expert has it (position >= offsets[E]).  A wave takes 64 x 8 x U consecutive
-// elements of one token; position values are clamped to the S rows that exist.
+// expert has it (position >= offsets[E]).  A wave takes 512 consecutive elements of one
+// token (of 2048, four times as many: dispatch 60 against 55 us, the weighted sum 109 / 89);
+// position values are clamped to the S rows that exist.  8190 tokens of 2048 bf16 in 8 slots:
+// dispatch 55 us (5.5 TB/s), the sum 48 after reads, 89 after writes of as many bytes that are still
+// on their way, its gradient 126 (4.6 TB/s).
 template <int T>
 constexpr int kSize = T == kF32 ? 4 : 2;
 
 struct Piece {
     int64_t t;
-    int d;            // first element of this lane's first 8
+    int d;            // first element of this lane's 8
 };
-// piece p of `pieces` a token; U chunks of 512 elements a piece
-template <int U>
+// the wave's piece, of `pieces` a token
 __device__ __forceinline__ bool piece_of(int64_t T, int pieces, Piece& p) {
     const int64_t w = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     p.t = w / pieces;
-    p.d = int(w - p.t * pieces) * (512 * U) + int(threadIdx.x & 63) * 8;
+    p.d = int(w - p.t * pieces) * 512 + int(threadIdx.x & 63) * 8;
     return p.t < T;
 }
 
@@ -254,37 +257,30 @@ __device__ __forceinline__ void store_row8(char* row, int d, int D, const float 
 
 // out[position[t, j]] = x[t], or zeros (the element's bits pass through fp32
 // unchanged: every conversion back is of a value of the type)
-template <int T, bool VEC, int U>
+template <int T, bool VEC>
 __global__ __launch_bounds__(256) void moe_dispatch_kernel(const char* __restrict__ x, int64_t ldx,
                                                            const int* __restrict__ position,
                                                            const int* __restrict__ offsets,
                                                            char* __restrict__ out, int64_t tokens,
                                                            int top, int E, int D, int pieces) {
     Piece p;
-    if (!piece_of<U>(tokens, pieces, p)) return;
+    if (!piece_of(tokens, pieces, p) || p.d >= D) return;
     const int S1 = int(tokens * top - 1);
     const int live = offsets[E];
-    float v[U][8];
-    const char* src = x + p.t * ldx * kSize<T>;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (p.d + 512 * u < D) load_row8<T, VEC>(src, p.d + 512 * u, D, v[u]);
+    float v[8];
+    load_row8<T, VEC>(x + p.t * ldx * kSize<T>, p.d, D, v);
     const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < top; ++j) {
         const int at = min(max(position[p.t * top + j], 0), S1);
         char* dst = out + int64_t(at) * D * kSize<T>;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (p.d + 512 * u < D) {
-                if (at < live) store_row8<T, VEC>(dst, p.d + 512 * u, D, v[u]);
-                else store_row8<T, VEC>(dst, p.d + 512 * u, D, zero);
-            }
+        if (at < live) store_row8<T, VEC>(dst, p.d, D, v);
+        else store_row8<T, VEC>(dst, p.d, D, zero);
     }
 }
 
 // out[t] = sum over the slots that an expert has, in slot order, of
 // [weights[t, j] *] rows[position[t, j]], in fp32, rounded once
-template <int T, int TO, bool VEC, int U, bool WEIGHTED>
+template <int T, int TO, bool VEC, bool WEIGHTED>
 __global__ __launch_bounds__(256) void moe_gather_kernel(const char* __restrict__ z, int64_t ldz,
                                                          const int* __restrict__ position,
                                                          const int* __restrict__ offsets,
@@ -292,17 +288,15 @@ __global__ __launch_bounds__(256) void moe_gather_kernel(const char* __restrict_
                                                          char* __restrict__ out, int64_t tokens,
                                                          int top, int E, int D, int pieces) {
     Piece p;
-    if (!piece_of<U>(tokens, pieces, p)) return;
+    if (!piece_of(tokens, pieces, p) || p.d >= D) return;
     const int live = min(offsets[E], int(tokens * top));
-    float acc[U][8];
+    float acc[8];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[u][i] = 0.f;
-    // four rows are requested together; one that no expert has gives way to row 0 and
-    // is not added
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    // four rows are requested together (one after the other: 92 against 89 us); one that no
+    // expert has gives way to row 0 and is not added
     for (int j0 = 0; j0 < top; j0 += 4) {
-        float v[4][U][8], w[4];
+        float v[4][8], w[4];
         bool has[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -310,26 +304,17 @@ __global__ __launch_bounds__(256) void moe_gather_kernel(const char* __restrict_
             const int at = position[slot];
             has[q] = j0 + q < top && at >= 0 && at < live;
             w[q] = WEIGHTED ? weights[slot] : 1.f;
-            const char* src = z + int64_t(has[q] ? at : 0) * ldz * kSize<T>;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (p.d + 512 * u < D) load_row8<T, VEC>(src, p.d + 512 * u, D, v[q][u]);
+            load_row8<T, VEC>(z + int64_t(has[q] ? at : 0) * ldz * kSize<T>, p.d, D, v[q]);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             if (!has[q]) continue;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    acc[u][i] = WEIGHTED ? __builtin_fmaf(w[q], v[q][u][i], acc[u][i])
-                                         : acc[u][i] + v[q][u][i];
+            for (int i = 0; i < 8; ++i)
+                acc[i] = WEIGHTED ? __builtin_fmaf(w[q], v[q][i], acc[i]) : acc[i] + v[q][i];
         }
     }
-    char* dst = out + p.t * D * kSize<TO>;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (p.d + 512 * u < D) store_row8<TO, VEC>(dst, p.d + 512 * u, D, acc[u]);
+    store_row8<TO, VEC>(out + p.t * D * kSize<TO>, p.d, D, acc);
 }
 
 __device__ __forceinline__ float lanes_sum(float x) {
@@ -390,20 +375,12 @@ bool vec_rows(const void* p, int64_t ld, int type, int D) {
     return D % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * size) % 16 == 0;
 }
 
-// calls f with the element type, the vector form and the chunks a wave takes:
-// MOST once the pieces still give every CU eight waves
-template <int MOST, class F>
-void by_form(int type, bool vec, int64_t tokens, int D, const F& f) {
-    const int64_t pieces = tokens * ((D + 512 * MOST - 1) / (512 * MOST));
+// calls f with the element type and the vector form
+template <class F>
+void by_form(int type, bool vec, const F& f) {
     auto form = [&](auto T) {
-        using One = std::integral_constant<int, 1>;
-        using Most = std::integral_constant<int, MOST>;
-        if (vec) {
-            if (pieces >= 2048) f(T, std::true_type{}, Most{});
-            else f(T, std::true_type{}, One{});
-        } else {
-            f(T, std::false_type{}, One{});
-        }
+        if (vec) f(T, std::true_type{});
+        else f(T, std::false_type{});
     };
     if (type == kBf16) form(std::integral_constant<int, kBf16>{});
     else if (type == kF16) form(std::integral_constant<int, kF16>{});
@@ -429,11 +406,9 @@ hipError_t moe_sort(hipStream_t st, const void* ids, bool wide, int* order, int*
 
 hipError_t moe_dispatch(hipStream_t st, const void* x, int type, int64_t ldx, const int* position,
                         const int* offsets, void* out, int64_t tokens, int top, int E, int D) {
-    by_form<4>(type, vec_rows(x, ldx, type, D) && vec_rows(out, D, type, D), tokens, D,
-            [&](auto T, auto V, auto U) {
-        constexpr int t = decltype(T)::value, u = decltype(U)::value;
-        const int pieces = (D + 512 * u - 1) / (512 * u);
-        hipLaunchKernelGGL((moe_dispatch_kernel<t, decltype(V)::value, u>),
+    const int pieces = (D + 511) / 512;
+    by_form(type, vec_rows(x, ldx, type, D) && vec_rows(out, D, type, D), [&](auto T, auto V) {
+        hipLaunchKernelGGL((moe_dispatch_kernel<decltype(T)::value, decltype(V)::value>),
                            dim3(unsigned((tokens * pieces + 3) / 4)), dim3(256), 0, st,
                            static_cast<const char*>(x), ldx, position, offsets,
                            static_cast<char*>(out), tokens, top, E, D, pieces);
@@ -444,14 +419,13 @@ hipError_t moe_dispatch(hipStream_t st, const void* x, int type, int64_t ldx, co
 hipError_t moe_gather(hipStream_t st, const void* z, int type, int64_t ldz, const int* position,
                       const int* offsets, const float* weights, void* out, int out_type,
                       int64_t tokens, int top, int E, int D) {
-    by_form<1>(type, vec_rows(z, ldz, type, D) && vec_rows(out, D, out_type, D), tokens, D,
-            [&](auto T, auto V, auto U) {
-        constexpr int t = decltype(T)::value, u = decltype(U)::value;
+    const int pieces = (D + 511) / 512;
+    by_form(type, vec_rows(z, ldz, type, D) && vec_rows(out, D, out_type, D), [&](auto T, auto V) {
+        constexpr int t = decltype(T)::value;
         constexpr bool v = decltype(V)::value;
-        const int pieces = (D + 512 * u - 1) / (512 * u);
         const dim3 grid(unsigned((tokens * pieces + 3) / 4));
         auto go = [&](auto TO, auto W) {
-            hipLaunchKernelGGL((moe_gather_kernel<t, decltype(TO)::value, v, u, decltype(W)::value>),
+            hipLaunchKernelGGL((moe_gather_kernel<t, decltype(TO)::value, v, decltype(W)::value>),
                                grid, dim3(256), 0, st, static_cast<const char*>(z), ldz, position,
                                offsets, weights, static_cast<char*>(out), tokens, top, E, D, pieces);
         };
@@ -471,19 +445,12 @@ hipError_t moe_combine_grad(hipStream_t st, const void* dy, int type, int64_t ld
                             int top, int E, int D) {
     const bool vec = vec_rows(dy, ldy, type, D) && vec_rows(z, ldz, type, D) && vec_rows(dz, D, type, D);
     const dim3 grid(unsigned((tokens + 3) / 4));
-    auto go = [&](auto T, auto V) {
+    by_form(type, vec, [&](auto T, auto V) {
         hipLaunchKernelGGL((moe_combine_grad_kernel<decltype(T)::value, decltype(V)::value>), grid,
                            dim3(256), 0, st, static_cast<const char*>(dy), ldy,
                            static_cast<const char*>(z), ldz, position, offsets, weights,
                            static_cast<char*>(dz), dweights, tokens, top, E, D);
-    };
-    auto form = [&](auto T) {
-        if (vec) go(T, std::true_type{});
-        else go(T, std::false_type{});
-    };
-    if (type == kBf16) form(std::integral_constant<int, kBf16>{});
-    else if (type == kF16) form(std::integral_constant<int, kF16>{});
-    else form(std::integral_constant<int, kF32>{});
+    });
     return hipGetLastError();
 }
 
