@@ -91,8 +91,8 @@ __device__ __forceinline__ v2i read_tr(uint32_t addr, int off) {
 #define XPU_ONE_BF16(W, LO, HI)                                                                 \
     "v_mfma_f32_16x16x32_bf16 a[%" #LO ":%" #HI "], %" #W ", %4, a[%" #LO ":%" #HI "]\n\t"
 #define XPU_BF16_4(CLOBBERS)                                                                    \
-    asm volatile(XPU_ONE_BF16(0, 5, 6) XPU_ONE_BF16(1, 7, 8) XPU_ONE_BF16(2, 9, 10)             \
-                 XPU_ONE_BF16(3, 11, 12)                                                        \
+    asm volatile(XPU_MFMA_WAIT XPU_ONE_BF16(0, 5, 6) XPU_ONE_BF16(1, 7, 8)                      \
+                 XPU_ONE_BF16(2, 9, 10) XPU_ONE_BF16(3, 11, 12)                                 \
                  ::"v"(w0), "v"(w1), "v"(w2), "v"(w3), "v"(x), "n"(4 * B0), "n"(4 * B0 + 3),    \
                  "n"(4 * B1), "n"(4 * B1 + 3), "n"(4 * B2), "n"(4 * B2 + 3), "n"(4 * B3),       \
                  "n"(4 * B3 + 3)                                                                \
@@ -106,7 +106,8 @@ __device__ __forceinline__ void acc_bf16_4(const v4i& w0, const v4i& w1, const v
 }
 template <int B0, int B1>
 __device__ __forceinline__ void acc_bf16_2(const v4i& w0, const v4i& w1, const v4i& x) {
-    asm volatile("v_mfma_f32_16x16x32_bf16 a[%3:%4], %0, %2, a[%3:%4]\n\t"
+    asm volatile(XPU_MFMA_WAIT
+                 "v_mfma_f32_16x16x32_bf16 a[%3:%4], %0, %2, a[%3:%4]\n\t"
                  "v_mfma_f32_16x16x32_bf16 a[%5:%6], %1, %2, a[%5:%6]\n\t"
                  ::"v"(w0), "v"(w1), "v"(x), "n"(4 * B0), "n"(4 * B0 + 3), "n"(4 * B1), "n"(4 * B1 + 3)
                  : XPU_A64);

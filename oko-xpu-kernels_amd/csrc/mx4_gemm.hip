@@ -291,7 +291,7 @@ __global__ __launch_bounds__(NW * 64) void mx4_few_kernel(Rows x, Weight w,
 // each step ends with a wait that redefines what it read.
 // blocks B0 .. B3 += W blocks (codes w, scale byte 0 of sw) * one X block
 #define XPU_MFMA4(CLOBBERS)                                                                     \
-    asm volatile(XPU_ONE_MFMA(0, 4, 10, 11) XPU_ONE_MFMA(1, 5, 12, 13)                          \
+    asm volatile(XPU_MFMA_WAIT XPU_ONE_MFMA(0, 4, 10, 11) XPU_ONE_MFMA(1, 5, 12, 13)            \
                  XPU_ONE_MFMA(2, 6, 14, 15) XPU_ONE_MFMA(3, 7, 16, 17)                          \
                  ::"v"(w[0]), "v"(w[1]), "v"(w[2]), "v"(w[3]), "v"(sw[0]), "v"(sw[1]),          \
                  "v"(sw[2]), "v"(sw[3]), "v"(x), "v"(sx), "n"(4 * B0), "n"(4 * B0 + 3),         \

@@ -55,8 +55,11 @@ __device__ __forceinline__ void block_barrier() {
 // at every turn of the loop or spilled (compilers move an MFMA builtin over barriers,
 // and its accumulator with it).  Every such instruction clobbers all of them, so
 // nothing else is kept there.  The compiler neither sees these MFMAs nor places the
-// waits that they need: two wait states between a VALU write and an MFMA that reads it,
-// eighteen between an MFMA and a read of its result by anything but an MFMA on it.
+// waits that they need: two wait states between a VALU write and an MFMA that reads it
+// (each statement of MFMAs begins with them, XPU_MFMA_WAIT: what the compiler put right
+// before it is not known), eighteen between an MFMA and a read of its result by anything
+// but an MFMA on it (store_tile).
+#define XPU_MFMA_WAIT "s_nop 1\n\t"
 #define XPU_A10(p) "a" #p "0", "a" #p "1", "a" #p "2", "a" #p "3", "a" #p "4", "a" #p "5", \
                    "a" #p "6", "a" #p "7", "a" #p "8", "a" #p "9"
 #define XPU_A60 XPU_A10(), XPU_A10(1), XPU_A10(2), XPU_A10(3), XPU_A10(4), XPU_A10(5)
