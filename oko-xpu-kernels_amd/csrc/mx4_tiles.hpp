@@ -53,8 +53,8 @@ __device__ __forceinline__ void block_barrier() {
 // The accumulators of a tile live in the accumulation registers a0 up, named in the
 // instructions: 4 registers an MFMA block, COUNT in all.  As values they were copied
 // at every turn of the loop or spilled (compilers move an MFMA builtin over barriers,
-// and its accumulator with it).  Every such instruction clobbers all of them, so
-// nothing else is kept there.  The compiler neither sees these MFMAs nor places the
+// and its accumulator with it).  Every statement on them clobbers all of them, the reads at
+// the end too, so that nothing else is kept there until the last one is read.  The compiler neither sees these MFMAs nor places the
 // waits that they need: two wait states between a VALU write and an MFMA that reads it
 // (each statement of MFMAs begins with them, XPU_MFMA_WAIT: what the compiler put right
 // before it is not known), eighteen between an MFMA and a read of its result by anything
@@ -80,13 +80,17 @@ __device__ __forceinline__ void acc_set(const v4f& v) {
     if constexpr (COUNT == 64) XPU_ACC_SET(XPU_A64);
     else XPU_ACC_SET(XPU_A256);
 }
-template <int BLOCK>
+#define XPU_ACC_GET(CLOBBERS)                                                                   \
+    asm volatile("v_accvgpr_read_b32 %0, a[%4]\n\tv_accvgpr_read_b32 %1, a[%5]\n\t"             \
+                 "v_accvgpr_read_b32 %2, a[%6]\n\tv_accvgpr_read_b32 %3, a[%7]"                 \
+                 : "=v"(a), "=v"(b), "=v"(c), "=v"(d)                                           \
+                 : "n"(4 * BLOCK), "n"(4 * BLOCK + 1), "n"(4 * BLOCK + 2), "n"(4 * BLOCK + 3)   \
+                 : CLOBBERS)
+template <int COUNT, int BLOCK>
 __device__ __forceinline__ v4f acc_get() {
     float a, b, c, d;
-    asm volatile("v_accvgpr_read_b32 %0, a[%4]\n\tv_accvgpr_read_b32 %1, a[%5]\n\t"
-                 "v_accvgpr_read_b32 %2, a[%6]\n\tv_accvgpr_read_b32 %3, a[%7]"
-                 : "=v"(a), "=v"(b), "=v"(c), "=v"(d)
-                 : "n"(4 * BLOCK), "n"(4 * BLOCK + 1), "n"(4 * BLOCK + 2), "n"(4 * BLOCK + 3));
+    if constexpr (COUNT == 64) XPU_ACC_GET(XPU_A64);
+    else XPU_ACC_GET(XPU_A256);
     return v4f{a, b, c, d};
 }
 // zeros in the rows of a tile
@@ -142,14 +146,15 @@ template <int TM, int TN, int STEP = 32>
 __device__ __forceinline__ void store_tile(const Out& out, int type, int row0, int end, int n,
                                            float* mine) {
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-    // the last MFMAs' results before the compiler, which does not see them, reads them
+    constexpr int ACC = TM * TN > 16 ? 256 : 64;
+    // the last MFMAs' results before they are read
     asm volatile("s_nop 15\n\ts_nop 15");
     auto store = [&](auto T) {
         each<TM>([&](auto B) {
             constexpr int b = decltype(B)::value;
             const int row = row0 + STEP * b + r;
             store_row<decltype(T)::value, TN>(out, row, row < end, n, [&](auto A) {
-                return acc_get<decltype(A)::value * TM + b>();
+                return acc_get<ACC, decltype(A)::value * TM + b>();
             });
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -161,7 +166,7 @@ __device__ __forceinline__ void store_tile(const Out& out, int type, int row0, i
         constexpr int b = decltype(B)::value;
         each<TN>([&](auto A) {
             constexpr int a = decltype(A)::value;
-            *reinterpret_cast<v4f*>(mine + r * (16 * TN) + 16 * a + 4 * g) = acc_get<a * TM + b>();
+            *reinterpret_cast<v4f*>(mine + r * (16 * TN) + 16 * a + 4 * g) = acc_get<ACC, a * TM + b>();
         });
         lds_done();
 #pragma clang loop unroll(disable)

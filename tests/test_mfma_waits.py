@@ -40,3 +40,31 @@ def test_mfma_operands_two_wait_states_after_their_writes(code):
                 last[r] = now + 1
             now += 1 + (int(args[0], 0) if op == "s_nop" else 0)
         assert count >= 16, name
+
+
+def accumulators(op, args):
+    """The AGPRs that an instruction names, as (written, read)."""
+    named = [registers(a.split()[0], "a") for a in args if a]
+    if op.startswith(("ds_write", "global_store", "buffer_store", "scratch_store", "flat_store")):
+        return set(), set().union(*named)
+    return (named[0] if named else set()), set().union(*named[1:])
+
+
+def test_accumulators_are_the_matrix_instructions_until_they_are_read(code):
+    """From the first MFMA to the last read, in the order of the code, nothing but an MFMA
+    writes an accumulator; the first read is eighteen wait states after the last MFMA."""
+    for name, body in code.items():
+        mfma = [i for i, (op, _) in enumerate(body) if op.startswith("v_mfma")]
+        mine = set().union(*(accumulators(*body[i])[0] for i in mfma))
+        assert mine == set(range(len(mine))), name         # a0 up
+        reads = [i for i, b in enumerate(body) if b[0] == "v_accvgpr_read_b32" and accumulators(*b)[1] & mine]
+        # each is read: by every one of the three ways out (bf16, fp16, and through LDS)
+        assert len(reads) == 3 * len(mine), name
+        assert reads[0] > mfma[-1], name
+        states = sum(1 + (int(args[0], 0) if op == "s_nop" else 0) for op, args in body[mfma[-1] + 1:reads[0]])
+        assert states >= 18, f"{name}: read {states} states after the last MFMA"
+        for i in range(mfma[0] + 1, len(body)):
+            op, args = body[i]
+            if not op.startswith("v_mfma") and (i < reads[-1]):
+                written = accumulators(op, args)[0] & mine
+                assert not written, f"{name}: {op} {', '.join(args)} writes an accumulator"
