@@ -589,6 +589,13 @@ int xpuint8_mxfp4_dx_stream(const void *stream, const void *dy, int32_t type, in
                             int64_t E, void *dx, int32_t dx_type, int64_t R, int64_t N, int64_t K,
                             void *work, int64_t work_bytes);
 
+/* dbias [N] = dy's column sums, dy [M, N] of row stride ldy (elements): fp32 sums in a
+ * fixed order, one rounding to dbias_type, whatever dy's type.  N < 2^28. */
+int64_t xpuint8_mxfp4_dbias_workspace_size(int64_t M, int64_t N);
+int xpuint8_mxfp4_dbias_stream(const void *stream, const void *dy, int32_t type, int64_t ldy,
+                               void *dbias, int32_t dbias_type, int64_t M, int64_t N, void *work,
+                               int64_t work_bytes);
+
 /* ---- mixture of experts -------------------------------------------------
  * T tokens of `top` slots each; slot s = t * top + j holds an expert's index in
  * [0, E) or anything else for a slot that no expert takes.  E <= 1024.

@@ -47,6 +47,12 @@ int check_product(int64_t R, int64_t tokens, int64_t N, int64_t K, bool grouped,
     return 0;
 }
 
+int check_dbias(int64_t M, int64_t N) {
+    if (M <= 0 || N <= 0) return fail(2, "rows and N must be positive");
+    if (M > kMaxDim || N >= int64_t(1) << 28) return fail(4, "rows must be < 2^31 and N < 2^28");
+    return 0;
+}
+
 int check_moe(int64_t T, int64_t top, int64_t E) {
     if (T <= 0 || top <= 0) return fail(2, "tokens and slots must be positive");
     if (E < 1 || E > kMaxExperts) return fail(2, "experts must be 1..1024");
@@ -234,6 +240,27 @@ int xpuint8_mxfp4_dx_stream(const void* stream, const void* dy, int32_t type, in
     }
     return launched(mx4_dx(st, dy, ldy, pieces, codes, scales, offsets, grouped ? int(E) : 1, dx,
                            dx_type, R, int(N), int(K)), "mxfp4_dx");
+}
+
+int64_t xpuint8_mxfp4_dbias_workspace_size(int64_t M, int64_t N) {
+    if (check_dbias(M, N) != 0) return -1;
+    return mx4_dbias_work_bytes(M, N);
+}
+
+int xpuint8_mxfp4_dbias_stream(const void* stream, const void* dy, int32_t type, int64_t ldy,
+                               void* dbias, int32_t dbias_type, int64_t M, int64_t N, void* work,
+                               int64_t work_bytes) {
+    XPU_TRY(check_dbias(M, N));
+    XPU_TRY(check_type(type, "type"));
+    XPU_TRY(check_type(dbias_type, "dbias_type"));
+    if (ldy < N) return fail(2, "the row stride must be >= N");
+    if (!dy) return fail(6, "dy must not be null");
+    XPU_NONNULL(dbias); XPU_NONNULL(work);
+    if (work_bytes < mx4_dbias_work_bytes(M, N))
+        return fail(2, "work must hold xpuint8_mxfp4_dbias_workspace_size bytes");
+    XPU_TRY(ensure_device());
+    return launched(mx4_dbias(as_stream(stream), dy, type, ldy, dbias, dbias_type, M, int(N),
+                              static_cast<float*>(work)), "mxfp4_dbias");
 }
 
 // ------------------------------------------------------------------ experts

@@ -72,8 +72,10 @@ struct Library {
     decltype(&xpuint8_mxfp4_dx_workspace_size) mx_dx_size;
     decltype(&xpuint8_mxfp4_dx_stream) mx_dx;
     decltype(&xpuint8_moe_combine_grad_stream) moe_combine_grad;
+    decltype(&xpuint8_mxfp4_dbias_workspace_size) mx_dbias_size;
+    decltype(&xpuint8_mxfp4_dbias_stream) mx_dbias;
 };
-constexpr int kEntries = 31;
+constexpr int kEntries = 33;
 static_assert(sizeof(Library) == kEntries * sizeof(void*), "one address per entry");
 
 Library g_lib;
@@ -675,15 +677,15 @@ variable_list once(const variable_list& in, const F& f) {
         int64_t(grads.size()));
     return (*error)(std::move(grads));
 }
-Tensor grad_dx(const Tensor& dy, const Tensor& c, const Tensor& s, const Tensor* offsets,
+Tensor grad_dx(const Rows& d, const Tensor& c, const Tensor& s, const Tensor* offsets,
                int32_t type) {
-    const Rows d = rows_of(dy);
-    const int64_t n = c.size(-2), k = c.size(-1) * 2, e = offsets ? c.size(0) : 0, r = d.t.size(0);
+    const Tensor& dy = d.t;
+    const int64_t n = c.size(-2), k = c.size(-1) * 2, e = offsets ? c.size(0) : 0, r = dy.size(0);
     const int64_t need = g_lib.mx_dx_size(type_of(dy), type, r, e, n, k);
     if (need < 0) check(1, "mxfp4 dx");
     Tensor work, dx = empty({r, k}, kTypes[type], dy);
     if (need > 0) work = workspace(need, dy);
-    check(g_lib.mx_dx(stream_of(dy), d.t.data_ptr(), type_of(dy), d.ld, bytes(&c), bytes(&s),
+    check(g_lib.mx_dx(stream_of(dy), dy.data_ptr(), type_of(dy), d.ld, bytes(&c), bytes(&s),
                       offsets ? ints(offsets) : nullptr, e, dx.data_ptr(), type, r, n, k,
                       need > 0 ? work.data_ptr() : nullptr, need), "mxfp4 dx");
     return dx;
@@ -697,16 +699,13 @@ Tensor grad_sum(const Tensor& dxs, const Tensor& position, const Tensor& offsets
                             offsets.numel() - 1, d), "moe.combine");
     return out;
 }
-// int8.column_sum
-Tensor column_sum(const Tensor& dy) {
-    if (dy.scalar_type() != at::kBFloat16 || dy.size(1) % 16 != 0) return dy.sum(0);
-    Tensor d = dy.contiguous();
-    if (reinterpret_cast<uintptr_t>(d.data_ptr()) % 16 != 0) d = d.clone();
-    const int64_t m = d.size(0), n = d.size(1), need = g_lib.colsum_size(m, n);
-    if (need < 0) check(1, "column_sum");
-    Tensor work = workspace(std::max<int64_t>(need, 16), d), out = empty({n}, at::kBFloat16, d);
-    check(g_lib.colsum(stream_of(d), d.data_ptr(), out.data_ptr(), m, n, work.data_ptr(), need),
-          "column_sum");
+// dy's column sums in the bias's type
+Tensor grad_bias(const Rows& dy, int32_t type) {
+    const int64_t m = dy.t.size(0), n = dy.t.size(1), need = g_lib.mx_dbias_size(m, n);
+    if (need < 0) check(1, "mxfp4 bias gradient");
+    Tensor work = workspace(need, dy.t), out = empty({n}, kTypes[type], dy.t);
+    check(g_lib.mx_dbias(stream_of(dy.t), dy.t.data_ptr(), type_of(dy.t), dy.ld, out.data_ptr(), type,
+                         m, n, work.data_ptr(), need), "mxfp4 bias gradient");
     return out;
 }
 
@@ -714,19 +713,19 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& c, const Tensor& s,
                           const std::optional<Tensor>& b) {
         ctx->save_for_backward({c, s});
-        ctx->saved_data["bias"] = int64_t(b ? b->scalar_type() : at::ScalarType::Undefined);
+        ctx->saved_data["bias"] = int64_t(b ? type_of(*b) : -1);
         return run_linear(x, c, s, b ? &*b : nullptr);
     }
     static variable_list backward(AutogradContext* ctx, variable_list in) {
         return once(in, [&]() -> variable_list {
             const variable_list saved = ctx->get_saved_variables();
             const Tensor &dy = in[0], &c = saved[0];
-            const auto type = at::ScalarType(ctx->saved_data["bias"].toInt());
+            const auto bias = int32_t(ctx->saved_data["bias"].toInt());
+            const Rows rows = rows_of(dy);
             Tensor dx, db;
             if (ctx->needs_input_grad(0))
-                dx = grad_dx(dy, c, saved[1], nullptr, type_of(dy)).reshape(with_last(dy, c.size(1) * 2));
-            if (type != at::ScalarType::Undefined && ctx->needs_input_grad(3))
-                db = column_sum(dy.reshape({-1, dy.size(-1)})).to(type);
+                dx = grad_dx(rows, c, saved[1], nullptr, type_of(dy)).reshape(with_last(dy, c.size(1) * 2));
+            if (bias >= 0 && ctx->needs_input_grad(3)) db = grad_bias(rows, bias);
             return {dx, Tensor(), Tensor(), db};
         });
     }
@@ -746,7 +745,7 @@ struct GroupedFn : torch::autograd::Function<GroupedFn> {
             const Tensor &dy = in[0], &offsets = saved[3];
             const bool gather = ctx->saved_data["gather"].toBool();
             // a token's rows are summed in fp32 and rounded once
-            Tensor dx = grad_dx(dy, saved[0], saved[1], &offsets, gather ? 2 : type_of(dy));
+            Tensor dx = grad_dx(rows_of(dy), saved[0], saved[1], &offsets, gather ? 2 : type_of(dy));
             if (gather) dx = grad_sum(dx, saved[2], offsets, type_of(dy));
             return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
         });

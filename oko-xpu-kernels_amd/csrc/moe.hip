@@ -221,24 +221,7 @@ __device__ __forceinline__ bool piece_of(int64_t T, int pieces, Piece& p) {
     return p.t < T;
 }
 
-// A row's 8 elements at d, of which those past D are left alone (the vector form is
-// taken for rows of whole, aligned 8s only)
-template <int T, bool VEC>
-__device__ __forceinline__ void load_row8(const char* row, int d, int D, float (&v)[8]) {
-    if constexpr (VEC) {
-        load8<T, true>(row + int64_t(d) * kSize<T>, v);
-    } else if (d + 8 <= D) {
-        load8<T, false>(row + int64_t(d) * kSize<T>, v);
-    } else {
-        for (int i = 0; i < 8; ++i) {
-            v[i] = 0.f;
-            if (d + i >= D) continue;
-            if constexpr (T == kF32) v[i] = reinterpret_cast<const float*>(row)[d + i];
-            else if constexpr (T == kBf16) v[i] = bf16_to_f32(reinterpret_cast<const uint16_t*>(row)[d + i]);
-            else v[i] = float(reinterpret_cast<const _Float16*>(row)[d + i]);
-        }
-    }
-}
+// a row's 8 elements at d, of which those past D are left alone
 template <int T, bool VEC>
 __device__ __forceinline__ void store_row8(char* row, int d, int D, const float (&v)[8]) {
     if constexpr (VEC) {

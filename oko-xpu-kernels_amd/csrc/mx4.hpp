@@ -58,6 +58,26 @@ __device__ __forceinline__ void load8(const void* p, float (&v)[8]) {
     }
 }
 
+// Eight values at d of a row of D, zeros for those past it (the vector form is taken for
+// rows of whole, aligned 8s only).
+template <int T, bool VEC>
+__device__ __forceinline__ void load_row8(const char* row, int64_t d, int64_t D, float (&v)[8]) {
+    constexpr int size = T == kF32 ? 4 : 2;
+    if constexpr (VEC) {
+        load8<T, true>(row + d * size, v);
+    } else if (d + 8 <= D) {
+        load8<T, false>(row + d * size, v);
+    } else {
+        for (int i = 0; i < 8; ++i) {
+            v[i] = 0.f;
+            if (d + i >= D) continue;
+            if constexpr (T == kF32) v[i] = reinterpret_cast<const float*>(row)[d + i];
+            else if constexpr (T == kBf16) v[i] = bf16_to_f32(reinterpret_cast<const uint16_t*>(row)[d + i]);
+            else v[i] = float(reinterpret_cast<const _Float16*>(row)[d + i]);
+        }
+    }
+}
+
 // two fp32 values rounded to a 16-bit type, packed
 template <int T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {

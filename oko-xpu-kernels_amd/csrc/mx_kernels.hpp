@@ -40,6 +40,12 @@ hipError_t mx4_dx(hipStream_t st, const void* dy, int64_t ldy, int pieces, const
                   const uint8_t* ws, const int* offsets, int E, void* dx, int type, int64_t R,
                   int N, int K);
 
+// mx4_bias.hip: out [N] = dy's column sums, dy [M, N] of row stride ldy, through part
+// (mx4_dbias_work_bytes)
+int64_t mx4_dbias_work_bytes(int64_t M, int64_t N);
+hipError_t mx4_dbias(hipStream_t st, const void* dy, int type, int64_t ldy, void* out, int out_type,
+                     int64_t M, int N, float* part);
+
 // moe.hip: slots sorted by expert, rows out to them and back, gradients
 int64_t moe_sort_work_bytes(int64_t S, int E);
 hipError_t moe_sort(hipStream_t st, const void* ids, bool wide, int* order, int* position,

@@ -26,7 +26,6 @@ from __future__ import annotations
 import torch
 
 from .int8 import _lib as L
-from .int8 import ops as _int8_ops
 
 __all__ = ["dequantize", "grouped_linear", "linear", "pad_scales", "quantize", "scale_width"]
 
@@ -202,6 +201,22 @@ def _dx(dy, codes, scales, offsets, out_dtype):
     return dx
 
 
+def _dbias(dy, dtype):
+    """The column sums of dy [.., N] in fp32, rounded once to ``dtype``."""
+    dy2, ld = _rows(dy)
+    m, n = dy2.shape
+    out = torch.empty((n,), dtype=dtype, device=dy.device)
+    if not m:
+        return out.zero_()
+    lib = L._lib()
+    need = lib.xpuint8_mxfp4_dbias_workspace_size(m, n)
+    work = _work(need, dy2)
+    if lib.xpuint8_mxfp4_dbias_stream(L._stream(dy.device), dy2.data_ptr(), TYPES[dy2.dtype], ld,
+                                      out.data_ptr(), TYPES[dtype], m, n, _opt(work), need) != 0:
+        L._err(lib, "mxfp4 bias gradient")
+    return out
+
+
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, codes, scales, bias):
@@ -217,7 +232,7 @@ class _LinearFn(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dx = _dx(dy, codes, scales, None, dy.dtype).reshape(*dy.shape[:-1], codes.shape[-1] * 2)
         if ctx.needs_input_grad[3]:
-            dbias = _int8_ops.column_sum(dy.reshape(-1, dy.shape[-1])).to(ctx.bias_dtype)
+            dbias = _dbias(dy, ctx.bias_dtype)
         return dx, None, None, dbias
 
 
@@ -225,7 +240,8 @@ def linear(x, codes, scales, bias=None):
     """``xq @ wq.T + bias``: x [.., K] quantized to MXFP4 in the call, the weight
     codes [N, K/2] and scales [N, scale_width(K)]; fp32 sums rounded once to x's
     type.  ``bias`` [N] is bf16, fp16 or fp32.  Gradients: dx = dy @ wq, straight
-    through x's quantization, and the bias's column sum; the weight has none."""
+    through x's quantization, and for the bias dy's column sums in fp32, rounded once to
+    the bias's type; the weight has none."""
     if L.HOST is not None:
         r = L.HOST.mx_linear(x, codes, scales, bias)
         if r is not None:

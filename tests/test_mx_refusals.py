@@ -1,0 +1,43 @@
+"""Refusals and sizes of the MXFP4 and mixture-of-experts entries beyond those of
+test_mx_contract, without a device."""
+
+import ctypes
+
+import pytest
+
+from xpu_kernels.int8 import _lib as L
+
+P, Z, ODD = ctypes.c_void_p(0x1000), ctypes.c_void_p(0), ctypes.c_void_p(0x1008)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    path = L.library_path()
+    assert path is not None, "libxpuint8.so is not built (run __graft_entry__.build())"
+    return L.open_library(path)
+
+
+@pytest.mark.parametrize("fn,args,code,substr", [
+    # stream, dy, type, ldy, dbias, dbias_type, M, N, work, work_bytes
+    ("mxfp4_dbias_stream", (Z, P, 0, 8, P, 0, 0, 8, P, 32), 2, "positive"),
+    ("mxfp4_dbias_stream", (Z, P, 0, 8, P, 0, 1 << 31, 8, P, 32), 4, "2^31"),
+    ("mxfp4_dbias_stream", (Z, P, 0, 1 << 28, P, 0, 1, 1 << 28, P, 32), 4, "2^28"),
+    ("mxfp4_dbias_stream", (Z, P, 3, 8, P, 0, 4, 8, P, 32), 6, "type"),
+    ("mxfp4_dbias_stream", (Z, P, 0, 8, P, 3, 4, 8, P, 32), 6, "dbias_type"),
+    ("mxfp4_dbias_stream", (Z, P, 0, 7, P, 0, 4, 8, P, 32), 2, "stride"),
+    ("mxfp4_dbias_stream", (Z, Z, 0, 8, P, 0, 4, 8, P, 32), 6, "null"),
+    ("mxfp4_dbias_stream", (Z, P, 0, 8, ODD, 0, 4, 8, P, 32), 6, "aligned"),
+    ("mxfp4_dbias_stream", (Z, P, 0, 8, P, 0, 4, 8, Z, 32), 6, "work"),
+    ("mxfp4_dbias_stream", (Z, P, 0, 8, P, 0, 33, 8, P, 63), 2, "workspace_size"),
+])
+def test_library_refusals(lib, fn, args, code, substr):
+    rc = getattr(lib, "xpuint8_" + fn)(*args)
+    msg = lib.xpuint8_last_error().decode()
+    assert rc == code and substr in msg, (rc, msg)
+
+
+def test_bias_gradient_workspace(lib):
+    """One fp32 sum a column (whole 8s of them) and 32 rows."""
+    size = lib.xpuint8_mxfp4_dbias_workspace_size
+    assert size(1, 1) == size(32, 8) == 32 and size(33, 9) == 2 * 64
+    assert size(0, 8) == size(8, 0) == size(1, 1 << 28) == -1
