@@ -789,6 +789,10 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
     }
 };
 
+// a forward-mode tangent, which the Python path refuses
+bool has_tangent(const Tensor& a, const Tensor* b = nullptr) {
+    return a._fw_grad(0).defined() || (b && b->_fw_grad(0).defined());
+}
 bool wants_grad(const Tensor& a, const Tensor* b = nullptr) {
     return at::GradMode::is_enabled() && (a.requires_grad() || (b && b->requires_grad()));
 }
@@ -806,6 +810,7 @@ PyObject* host_mx_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             b = on(floating(a[3]), *x);
             if (!b || b->dim() != 1 || b->numel() != c->size(0)) Py_RETURN_NONE;
         }
+        if (has_tangent(*x, b)) Py_RETURN_NONE;
         if (!wants_grad(*x, b)) return THPVariable_Wrap(run_linear(*x, *c, *s, b));
         return THPVariable_Wrap(LinearFn::apply(*x, *c, *s, b ? std::optional<Tensor>(*b) : std::nullopt));
     });
@@ -824,7 +829,7 @@ PyObject* host_mx_grouped(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (gather < 0) throw python_error();
         const int64_t rows = r.order->numel();
         if (x->size(1) != c->size(2) * 2 || r.offsets->numel() != c->size(0) + 1 ||
-            x->size(0) != (gather ? r.position->size(0) : rows))
+            x->size(0) != (gather ? r.position->size(0) : rows) || has_tangent(*x))
             Py_RETURN_NONE;
         if (!wants_grad(*x))
             return THPVariable_Wrap(run_grouped(*x, *c, *s, gather ? r.rows : nullptr, *r.offsets, rows));
@@ -877,7 +882,8 @@ PyObject* host_moe_dispatch(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded(n_args, 2, [&]() -> PyObject* {
         const Tensor* x = floating(a[0]);
         Routing r;
-        if (!x || x->dim() != 2 || !routing_arg(a[1], *x, r) || x->size(0) != r.position->size(0))
+        if (!x || x->dim() != 2 || !routing_arg(a[1], *x, r) || x->size(0) != r.position->size(0) ||
+            has_tangent(*x))
             Py_RETURN_NONE;
         if (!wants_grad(*x)) return THPVariable_Wrap(run_dispatch(*x, *r.position, *r.offsets));
         return THPVariable_Wrap(DispatchFn::apply(*x, *r.position, *r.offsets));
@@ -892,7 +898,8 @@ PyObject* host_moe_combine(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (!z || z->dim() != 2 || !routing_arg(a[1], *z, r)) Py_RETURN_NONE;
         const Tensor* w = on(plain(a[2], at::kFloat), *z);
         const int64_t t = r.position->size(0), top = r.position->size(1);
-        if (!w || w->dim() != 2 || w->size(0) != t || w->size(1) != top || z->size(0) != t * top)
+        if (!w || w->dim() != 2 || w->size(0) != t || w->size(1) != top || z->size(0) != t * top ||
+            has_tangent(*z, w))
             Py_RETURN_NONE;
         if (!wants_grad(*z, w))
             return THPVariable_Wrap(run_combine(*z, w, *r.position, *r.offsets, type_of(*z)));

@@ -17,13 +17,14 @@ infinity or NaN reads back as NaNs.
     y = mxfp4.linear(x, codes, scales, bias)          # [.., K] -> [.., N], x's type
 
 The weight is frozen; gradients reach ``x`` (straight through its quantization)
-and ``bias``.  Everything runs in ``libxpuint8.so`` on torch's current stream,
+and ``bias``; forward-mode derivatives are refused.  Everything runs in ``libxpuint8.so`` on torch's current stream,
 without synchronising; there is no counterpart in the reference.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .int8 import _lib as L
 
@@ -62,8 +63,13 @@ def _check_float(t, name):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                           for t in tensors)
+    """Whether any of the tensors (or Nones) needs a gradient; a forward-mode tangent,
+    which no operator here carries on, is refused."""
+    tensors = [t for t in tensors if t is not None]
+    if any(unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("the MXFP4 and mixture-of-experts operators have no "
+                                  "forward-mode derivative")
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 def _check_pair(codes, scales, lead=None):
