@@ -581,9 +581,13 @@ int xpuint8_mxfp4_grouped_linear_stream(const void *stream, const void *x, int32
  * rounding to dx_type.  work (E: 0 for one weight) holds the weight as bf16 for the
  * shapes that go through it (some of one weight, bf16 dy and dx, N % 16 == 0), or dy's
  * exact bf16 pieces where it is not bf16 in whole 16-byte aligned chunks (N % 8, the
- * row stride % 8); NULL will do for several experts and a dy that is. */
+ * row stride % 8).  _size serves any dy of the type; _size_of is what this dy takes, 0
+ * (and work NULL) for one that the kernels read where it lies. */
 int64_t xpuint8_mxfp4_dx_workspace_size(int32_t type, int32_t dx_type, int64_t R, int64_t E,
                                         int64_t N, int64_t K);
+int64_t xpuint8_mxfp4_dx_workspace_size_of(const void *dy, int32_t type, int64_t ldy,
+                                           int32_t dx_type, int64_t R, int64_t E, int64_t N,
+                                           int64_t K);
 int xpuint8_mxfp4_dx_stream(const void *stream, const void *dy, int32_t type, int64_t ldy,
                             const uint8_t *codes, const uint8_t *scales, const int32_t *offsets,
                             int64_t E, void *dx, int32_t dx_type, int64_t R, int64_t N, int64_t K,

@@ -114,6 +114,14 @@ bool dx_by_bf16(int32_t type, int32_t dx_type, bool grouped, int64_t R, int64_t 
            mx4_dx_bf16_faster(R, N, K);
 }
 
+// dx's workspaces: the weight as bf16 and its product's slices, or dy's pieces
+int64_t bf16_dx_bytes(int64_t R, int64_t N, int64_t K) {
+    return up(2 * N * K) + up(bf16_dx_work_bytes(int(R), int(N), int(K)));
+}
+int64_t split_bytes(int32_t type, int64_t R, int64_t N) {
+    return up(R * mx4_split_width(N) * mx4_split_pieces(type) * 2);
+}
+
 }  // namespace
 }  // namespace xpuint8
 
@@ -194,9 +202,15 @@ int64_t xpuint8_mxfp4_dx_workspace_size(int32_t type, int32_t dx_type, int64_t R
                                         int64_t N, int64_t K) {
     if (check_product(R, R, N, K, E > 0, E) != 0 || check_type(type, "type") != 0) return -1;
     if (dx_by_bf16(type, dx_type, E > 0, R, N, K))
-        return std::max(up(2 * N * K) + up(bf16_dx_work_bytes(int(R), int(N), int(K))),
-                        up(R * mx4_split_width(N) * 2));
-    return up(R * mx4_split_width(N) * mx4_split_pieces(type) * 2);
+        return std::max(bf16_dx_bytes(R, N, K), split_bytes(type, R, N));
+    return split_bytes(type, R, N);
+}
+
+int64_t xpuint8_mxfp4_dx_workspace_size_of(const void* dy, int32_t type, int64_t ldy, int32_t dx_type,
+                                           int64_t R, int64_t E, int64_t N, int64_t K) {
+    if (xpuint8_mxfp4_dx_workspace_size(type, dx_type, R, E, N, K) < 0) return -1;
+    if (!dy_direct(dy, type, ldy, N)) return split_bytes(type, R, N);
+    return ldy == N && dx_by_bf16(type, dx_type, E > 0, R, N, K) ? bf16_dx_bytes(R, N, K) : 0;
 }
 
 int xpuint8_mxfp4_dx_stream(const void* stream, const void* dy, int32_t type, int64_t ldy,
@@ -211,7 +225,6 @@ int xpuint8_mxfp4_dx_stream(const void* stream, const void* dy, int32_t type, in
     XPU_NONNULL(codes); XPU_NONNULL(scales); XPU_NONNULL(dx);
     const bool grouped = offsets != nullptr;
     const bool direct = dy_direct(dy, type, ldy, N);
-    const int64_t need = xpuint8_mxfp4_dx_workspace_size(type, dx_type, R, grouped ? E : 0, N, K);
     if (dx_by_bf16(type, dx_type, grouped, R, N, K) && direct && ldy == N) {
         XPU_NONNULL(work);
         if (work_bytes < up(2 * N * K))
@@ -226,7 +239,7 @@ int xpuint8_mxfp4_dx_stream(const void* stream, const void* dy, int32_t type, in
     }
     if (!direct) {
         XPU_NONNULL(work);
-        if (work_bytes < need)
+        if (work_bytes < split_bytes(type, R, N))
             return fail(2, "work must hold xpuint8_mxfp4_dx_workspace_size bytes");
         if (R * mx4_split_width(N) > kMaxDim * 256) return fail(4, "dy is too large for one launch");
     }

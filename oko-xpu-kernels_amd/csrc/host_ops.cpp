@@ -69,7 +69,7 @@ struct Library {
     decltype(&xpuint8_moe_sort_stream) moe_sort;
     decltype(&xpuint8_moe_dispatch_stream) moe_dispatch;
     decltype(&xpuint8_moe_combine_stream) moe_combine;
-    decltype(&xpuint8_mxfp4_dx_workspace_size) mx_dx_size;
+    decltype(&xpuint8_mxfp4_dx_workspace_size_of) mx_dx_size;
     decltype(&xpuint8_mxfp4_dx_stream) mx_dx;
     decltype(&xpuint8_moe_combine_grad_stream) moe_combine_grad;
     decltype(&xpuint8_mxfp4_dbias_workspace_size) mx_dbias_size;
@@ -681,7 +681,7 @@ Tensor grad_dx(const Rows& d, const Tensor& c, const Tensor& s, const Tensor* of
                int32_t type) {
     const Tensor& dy = d.t;
     const int64_t n = c.size(-2), k = c.size(-1) * 2, e = offsets ? c.size(0) : 0, r = dy.size(0);
-    const int64_t need = g_lib.mx_dx_size(type_of(dy), type, r, e, n, k);
+    const int64_t need = g_lib.mx_dx_size(dy.data_ptr(), type_of(dy), d.ld, type, r, e, n, k);
     if (need < 0) check(1, "mxfp4 dx");
     Tensor work, dx = empty({r, k}, kTypes[type], dy);
     if (need > 0) work = workspace(need, dy);

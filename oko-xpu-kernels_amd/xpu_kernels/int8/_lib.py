@@ -49,7 +49,7 @@ _HOST_ENTRIES = (
     "xpuint8_mxfp4_grouped_linear_workspace_size", "xpuint8_mxfp4_grouped_linear_stream",
     "xpuint8_moe_sort_workspace_size", "xpuint8_moe_sort_stream",
     "xpuint8_moe_dispatch_stream", "xpuint8_moe_combine_stream",
-    "xpuint8_mxfp4_dx_workspace_size", "xpuint8_mxfp4_dx_stream",
+    "xpuint8_mxfp4_dx_workspace_size_of", "xpuint8_mxfp4_dx_stream",
     "xpuint8_moe_combine_grad_stream",
     "xpuint8_mxfp4_dbias_workspace_size", "xpuint8_mxfp4_dbias_stream")
 
@@ -149,6 +149,7 @@ def _signatures():
         "xpuint8_mxfp4_grouped_linear_stream": ([vp, vp, i32, i64, vp, i64, vp, vp, vp, i64, vp]
                                                 + [i64] * 3 + [vp, i64], c_int),
         "xpuint8_mxfp4_dx_workspace_size": ([i32] * 2 + [i64] * 4, i64),
+        "xpuint8_mxfp4_dx_workspace_size_of": ([vp, i32, i64, i32] + [i64] * 4, i64),
         "xpuint8_mxfp4_dx_stream": ([vp, vp, i32, i64, vp, vp, vp, i64, vp, i32] + [i64] * 3
                                     + [vp, i64], c_int),
         "xpuint8_mxfp4_dbias_workspace_size": ([i64] * 2, i64),

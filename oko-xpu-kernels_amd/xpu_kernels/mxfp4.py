@@ -195,14 +195,13 @@ def _dx(dy, codes, scales, offsets, out_dtype):
     if r:
         lib = L._lib()
         e = 0 if offsets is None else offsets.numel() - 1
-        work = None
-        if e == 0 or dy2.dtype != torch.bfloat16 or n % 8 or ld % 8 or dy2.data_ptr() % 16:
-            work = _work(lib.xpuint8_mxfp4_dx_workspace_size(TYPES[dy2.dtype], TYPES[out_dtype],
-                                                             r, e, n, k), dy2)
+        need = lib.xpuint8_mxfp4_dx_workspace_size_of(dy2.data_ptr(), TYPES[dy2.dtype], ld,
+                                                      TYPES[out_dtype], r, e, n, k)
+        work = _work(need, dy2)
         if lib.xpuint8_mxfp4_dx_stream(L._stream(dy.device), dy2.data_ptr(), TYPES[dy2.dtype], ld,
                                        codes.data_ptr(), scales.data_ptr(), _opt(offsets), e,
                                        dx.data_ptr(), TYPES[out_dtype], r, n, k, _opt(work),
-                                       0 if work is None else work.numel()) != 0:
+                                       need) != 0:
             L._err(lib, "mxfp4 dx")
     return dx
 

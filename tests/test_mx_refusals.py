@@ -41,3 +41,36 @@ def test_bias_gradient_workspace(lib):
     size = lib.xpuint8_mxfp4_dbias_workspace_size
     assert size(1, 1) == size(32, 8) == 32 and size(33, 9) == 2 * 64
     assert size(0, 8) == size(8, 0) == size(1, 1 << 28) == -1
+
+
+def test_dx_workspace_of_a_dy(lib):
+    """What dx takes beside its result: nothing where dy is read where it lies, its bf16
+    pieces where it is not, the weight as bf16 where dx goes through it."""
+    of, any_dy = lib.xpuint8_mxfp4_dx_workspace_size_of, lib.xpuint8_mxfp4_dx_workspace_size
+    # experts: dy, type, ldy, dx_type, R, E, N, K
+    assert of(P, 0, 4096, 2, 1000, 8, 4096, 256) == 0
+    assert of(P, 0, 8192, 0, 1000, 8, 4096, 256) == 0
+    pieces = 1000 * 4096 * 2
+    assert of(ODD, 0, 4096, 0, 1000, 8, 4096, 256) == any_dy(0, 0, 1000, 8, 4096, 256) == pieces
+    assert of(P, 0, 4100, 0, 1000, 8, 4096, 256) == pieces
+    assert of(P, 1, 4096, 1, 1000, 8, 4096, 256) == 2 * pieces
+    assert of(P, 2, 4096, 2, 1000, 8, 4096, 256) == 3 * pieces
+    # one weight, by tiles and through its bf16 values
+    assert of(P, 0, 2048, 0, 64, 0, 2048, 8192) == 0
+    through = of(P, 0, 5120, 0, 4096, 0, 5120, 1280)
+    assert through >= 2 * 5120 * 1280
+    assert any_dy(0, 0, 4096, 0, 5120, 1280) >= max(through, 4096 * 5120 * 2)
+    assert of(P, 0, 5128, 0, 4096, 0, 5120, 1280) == 0
+    assert of(P, 0, 64, 0, 4, 0, 64, 48) == of(P, 3, 64, 0, 4, 0, 64, 64) == -1
+
+
+@pytest.mark.parametrize("args,code,substr", [
+    # stream, dy, type, ldy, codes, scales, offsets, E, dx, dx_type, R, N, K, work, work_bytes
+    ((Z, P, 0, 5120, P, P, Z, 0, P, 0, 4096, 5120, 1280, Z, 0), 6, "work"),
+    ((Z, P, 0, 5120, P, P, Z, 0, P, 0, 4096, 5120, 1280, P, 64), 2, "workspace_size"),
+    ((Z, ODD, 0, 4096, P, P, P, 8, P, 0, 1000, 4096, 256, P, 1000 * 4096 * 2 - 1), 2, "workspace_size"),
+])
+def test_dx_refuses_too_little_work(lib, args, code, substr):
+    rc = lib.xpuint8_mxfp4_dx_stream(*args)
+    msg = lib.xpuint8_last_error().decode()
+    assert rc == code and substr in msg, (rc, msg)
