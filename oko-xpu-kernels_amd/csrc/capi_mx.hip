@@ -47,6 +47,21 @@ int check_product(int64_t R, int64_t tokens, int64_t N, int64_t K, bool grouped,
     return 0;
 }
 
+// the tiles of a product and of its gradient
+int check_blocks(int64_t blocks) {
+    if (!mx4_blocks_fit(blocks)) return fail(4, "rows x N or rows x K is too large for one launch");
+    return 0;
+}
+int check_linear(int64_t R, int64_t tokens, int64_t N, int64_t K, bool grouped, int64_t E) {
+    XPU_TRY(check_product(R, tokens, N, K, grouped, E));
+    if (mx4_fused(R, grouped, int(E), K)) return 0;
+    return check_blocks(mx4_product_blocks(grouped, R, grouped ? int(E) : 1, N, K));
+}
+int check_gradient(int64_t R, int64_t N, int64_t K, bool grouped, int64_t E) {
+    XPU_TRY(check_product(R, R, N, K, grouped, E));
+    return check_blocks(mx4_dx_blocks(grouped, R, grouped ? int(E) : 1, N, K));
+}
+
 int check_dbias(int64_t M, int64_t N) {
     if (M <= 0 || N <= 0) return fail(2, "rows and N must be positive");
     if (M > kMaxDim || N >= int64_t(1) << 28) return fail(4, "rows must be < 2^31 and N < 2^28");
@@ -62,7 +77,7 @@ int check_moe(int64_t T, int64_t top, int64_t E) {
 }
 
 int check_rows_of(int64_t T, int64_t top, int64_t E, int64_t D) {
-    if (check_moe(T, top, E) != 0) return 2;
+    XPU_TRY(check_moe(T, top, E));
     if (D <= 0) return fail(2, "D must be positive");
     if (D > kMaxDim / 2 || T * ((D + 511) / 512) > kMaxDim * 4)
         return fail(4, "tokens x D is too large for one launch");
@@ -158,7 +173,7 @@ int xpuint8_mxfp4_dequantize_stream(const void* stream, const uint8_t* codes,
 }
 
 int64_t xpuint8_mxfp4_linear_workspace_size(int64_t M, int64_t N, int64_t K) {
-    if (check_product(M, M, N, K, false, 0) != 0) return -1;
+    if (check_linear(M, M, N, K, false, 0) != 0) return -1;
     return mx4_fused(M, false, 0, K) ? 0 : quantized_bytes(M, K);
 }
 
@@ -166,7 +181,7 @@ int xpuint8_mxfp4_linear_stream(const void* stream, const void* x, int32_t type,
                                 const uint8_t* codes, const uint8_t* scales, const void* bias,
                                 int32_t bias_type, void* y, int64_t M, int64_t N, int64_t K,
                                 void* work, int64_t work_bytes) {
-    XPU_TRY(check_product(M, M, N, K, false, 0));
+    XPU_TRY(check_linear(M, M, N, K, false, 0));
     XPU_TRY(check_type(type, "type"));
     if (bias) XPU_TRY(check_type(bias_type, "bias_type"));
     if (ldx < K) return fail(2, "the row stride must be >= K");
@@ -178,7 +193,7 @@ int xpuint8_mxfp4_linear_stream(const void* stream, const void* x, int32_t type,
 
 int64_t xpuint8_mxfp4_grouped_linear_workspace_size(int64_t R, int64_t tokens, int64_t E,
                                                     int64_t N, int64_t K) {
-    if (check_product(R, tokens, N, K, true, E) != 0) return -1;
+    if (check_linear(R, tokens, N, K, true, E) != 0) return -1;
     return mx4_fused(R, true, int(E), K) ? 0 : quantized_bytes(tokens, K);
 }
 
@@ -187,7 +202,7 @@ int xpuint8_mxfp4_grouped_linear_stream(const void* stream, const void* x, int32
                                         const uint8_t* codes, const uint8_t* scales,
                                         const int32_t* offsets, int64_t E, void* y, int64_t R,
                                         int64_t N, int64_t K, void* work, int64_t work_bytes) {
-    XPU_TRY(check_product(R, tokens, N, K, true, E));
+    XPU_TRY(check_linear(R, tokens, N, K, true, E));
     XPU_TRY(check_type(type, "type"));
     if (!rows && tokens != R) return fail(2, "without rows, x must have R rows");
     if (ldx < K) return fail(2, "the row stride must be >= K");
@@ -200,7 +215,7 @@ int xpuint8_mxfp4_grouped_linear_stream(const void* stream, const void* x, int32
 
 int64_t xpuint8_mxfp4_dx_workspace_size(int32_t type, int32_t dx_type, int64_t R, int64_t E,
                                         int64_t N, int64_t K) {
-    if (check_product(R, R, N, K, E > 0, E) != 0 || check_type(type, "type") != 0) return -1;
+    if (check_gradient(R, N, K, E > 0, E) != 0 || check_type(type, "type") != 0) return -1;
     if (dx_by_bf16(type, dx_type, E > 0, R, N, K))
         return std::max(bf16_dx_bytes(R, N, K), split_bytes(type, R, N));
     return split_bytes(type, R, N);
@@ -217,7 +232,7 @@ int xpuint8_mxfp4_dx_stream(const void* stream, const void* dy, int32_t type, in
                             const uint8_t* codes, const uint8_t* scales, const int32_t* offsets,
                             int64_t E, void* dx, int32_t dx_type, int64_t R, int64_t N, int64_t K,
                             void* work, int64_t work_bytes) {
-    XPU_TRY(check_product(R, R, N, K, offsets != nullptr, offsets ? E : 0));
+    XPU_TRY(check_gradient(R, N, K, offsets != nullptr, offsets ? E : 0));
     XPU_TRY(check_type(type, "type"));
     XPU_TRY(check_type(dx_type, "dx_type"));
     if (ldy < N) return fail(2, "the row stride must be >= N");
@@ -241,7 +256,6 @@ int xpuint8_mxfp4_dx_stream(const void* stream, const void* dy, int32_t type, in
         XPU_NONNULL(work);
         if (work_bytes < split_bytes(type, R, N))
             return fail(2, "work must hold xpuint8_mxfp4_dx_workspace_size bytes");
-        if (R * mx4_split_width(N) > kMaxDim * 256) return fail(4, "dy is too large for one launch");
     }
     XPU_TRY(ensure_device());
     hipStream_t st = as_stream(stream);

@@ -213,11 +213,12 @@ struct Piece {
     int64_t t;
     int d;            // first element of this lane's 8
 };
-// the wave's piece, of `pieces` a token
-__device__ __forceinline__ bool piece_of(int64_t T, int pieces, Piece& p) {
+// the wave's piece, of `pieces` a token; the launch starts at token t0
+__device__ __forceinline__ bool piece_of(int64_t t0, int64_t T, int pieces, Piece& p) {
     const int64_t w = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-    p.t = w / pieces;
-    p.d = int(w - p.t * pieces) * 512 + int(threadIdx.x & 63) * 8;
+    const int64_t t = w / pieces;
+    p.t = t0 + t;
+    p.d = int(w - t * pieces) * 512 + int(threadIdx.x & 63) * 8;
     return p.t < T;
 }
 
@@ -244,10 +245,11 @@ template <int T, bool VEC>
 __global__ __launch_bounds__(256) void moe_dispatch_kernel(const char* __restrict__ x, int64_t ldx,
                                                            const int* __restrict__ position,
                                                            const int* __restrict__ offsets,
-                                                           char* __restrict__ out, int64_t tokens,
-                                                           int top, int E, int D, int pieces) {
+                                                           char* __restrict__ out, int64_t t0,
+                                                           int64_t tokens, int top, int E, int D,
+                                                           int pieces) {
     Piece p;
-    if (!piece_of(tokens, pieces, p) || p.d >= D) return;
+    if (!piece_of(t0, tokens, pieces, p) || p.d >= D) return;
     const int S1 = int(tokens * top - 1);
     const int live = offsets[E];
     float v[8];
@@ -268,10 +270,11 @@ __global__ __launch_bounds__(256) void moe_gather_kernel(const char* __restrict_
                                                          const int* __restrict__ position,
                                                          const int* __restrict__ offsets,
                                                          const float* __restrict__ weights,
-                                                         char* __restrict__ out, int64_t tokens,
-                                                         int top, int E, int D, int pieces) {
+                                                         char* __restrict__ out, int64_t t0,
+                                                         int64_t tokens, int top, int E, int D,
+                                                         int pieces) {
     Piece p;
-    if (!piece_of(tokens, pieces, p) || p.d >= D) return;
+    if (!piece_of(t0, tokens, pieces, p) || p.d >= D) return;
     const int live = min(offsets[E], int(tokens * top));
     float acc[8];
 #pragma unroll
@@ -319,8 +322,8 @@ __global__ __launch_bounds__(256) void moe_combine_grad_kernel(
     const char* __restrict__ dy, int64_t ldy, const char* __restrict__ z, int64_t ldz,
     const int* __restrict__ position, const int* __restrict__ offsets,
     const float* __restrict__ weights, char* __restrict__ dz, float* __restrict__ dweights,
-    int64_t tokens, int top, int E, int D) {
-    const int64_t t = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+    int64_t t0, int64_t tokens, int top, int E, int D) {
+    const int64_t t = t0 + int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     if (t >= tokens) return;
     const int lane = threadIdx.x & 63;
     const int S = int(tokens * top);
@@ -391,10 +394,12 @@ hipError_t moe_dispatch(hipStream_t st, const void* x, int type, int64_t ldx, co
                         const int* offsets, void* out, int64_t tokens, int top, int E, int D) {
     const int pieces = (D + 511) / 512;
     by_form(type, vec_rows(x, ldx, type, D) && vec_rows(out, D, type, D), [&](auto T, auto V) {
-        hipLaunchKernelGGL((moe_dispatch_kernel<decltype(T)::value, decltype(V)::value>),
-                           dim3(unsigned((tokens * pieces + 3) / 4)), dim3(256), 0, st,
-                           static_cast<const char*>(x), ldx, position, offsets,
-                           static_cast<char*>(out), tokens, top, E, D, pieces);
+        in_launches(tokens, 4 * kMaxBlocks / pieces, [&](int64_t t0, int64_t n) {
+            hipLaunchKernelGGL((moe_dispatch_kernel<decltype(T)::value, decltype(V)::value>),
+                               dim3(unsigned((n * pieces + 3) / 4)), dim3(256), 0, st,
+                               static_cast<const char*>(x), ldx, position, offsets,
+                               static_cast<char*>(out), t0, tokens, top, E, D, pieces);
+        });
     });
     return hipGetLastError();
 }
@@ -406,11 +411,13 @@ hipError_t moe_gather(hipStream_t st, const void* z, int type, int64_t ldz, cons
     by_form(type, vec_rows(z, ldz, type, D) && vec_rows(out, D, out_type, D), [&](auto T, auto V) {
         constexpr int t = decltype(T)::value;
         constexpr bool v = decltype(V)::value;
-        const dim3 grid(unsigned((tokens * pieces + 3) / 4));
         auto go = [&](auto TO, auto W) {
-            hipLaunchKernelGGL((moe_gather_kernel<t, decltype(TO)::value, v, decltype(W)::value>),
-                               grid, dim3(256), 0, st, static_cast<const char*>(z), ldz, position,
-                               offsets, weights, static_cast<char*>(out), tokens, top, E, D, pieces);
+            in_launches(tokens, 4 * kMaxBlocks / pieces, [&](int64_t t0, int64_t n) {
+                hipLaunchKernelGGL((moe_gather_kernel<t, decltype(TO)::value, v, decltype(W)::value>),
+                                   dim3(unsigned((n * pieces + 3) / 4)), dim3(256), 0, st,
+                                   static_cast<const char*>(z), ldz, position, offsets, weights,
+                                   static_cast<char*>(out), t0, tokens, top, E, D, pieces);
+            });
         };
         if (weights) go(T, std::true_type{});
         else if (type == out_type) go(T, std::false_type{});
@@ -427,12 +434,14 @@ hipError_t moe_combine_grad(hipStream_t st, const void* dy, int type, int64_t ld
                             const float* weights, void* dz, float* dweights, int64_t tokens,
                             int top, int E, int D) {
     const bool vec = vec_rows(dy, ldy, type, D) && vec_rows(z, ldz, type, D) && vec_rows(dz, D, type, D);
-    const dim3 grid(unsigned((tokens + 3) / 4));
     by_form(type, vec, [&](auto T, auto V) {
-        hipLaunchKernelGGL((moe_combine_grad_kernel<decltype(T)::value, decltype(V)::value>), grid,
-                           dim3(256), 0, st, static_cast<const char*>(dy), ldy,
-                           static_cast<const char*>(z), ldz, position, offsets, weights,
-                           static_cast<char*>(dz), dweights, tokens, top, E, D);
+        in_launches(tokens, 4 * kMaxBlocks, [&](int64_t t0, int64_t n) {
+            hipLaunchKernelGGL((moe_combine_grad_kernel<decltype(T)::value, decltype(V)::value>),
+                               dim3(unsigned((n + 3) / 4)), dim3(256), 0, st,
+                               static_cast<const char*>(dy), ldy, static_cast<const char*>(z), ldz,
+                               position, offsets, weights, static_cast<char*>(dz), dweights, t0,
+                               tokens, top, E, D);
+        });
     });
     return hipGetLastError();
 }

@@ -335,10 +335,12 @@ hipError_t mx4_split(hipStream_t st, const void* dy, int type, int64_t ldy, void
         constexpr int t = decltype(T)::value;
         constexpr int P = t == kBf16 ? 1 : t == kF16 ? 2 : 3;
         auto go = [&](auto V) {
-            hipLaunchKernelGGL((mx4_split_kernel<t, decltype(V)::value, P>),
-                               dim3(unsigned((R * (width / 8) + 255) / 256)), dim3(256), 0, st,
-                               static_cast<const char*>(dy), ldy, static_cast<uint16_t*>(out), R, N,
-                               width);
+            in_launches(R, 256 * kMaxBlocks / (width / 8), [&](int64_t at, int64_t rows) {
+                hipLaunchKernelGGL((mx4_split_kernel<t, decltype(V)::value, P>),
+                                   dim3(unsigned((rows * (width / 8) + 255) / 256)), dim3(256), 0, st,
+                                   static_cast<const char*>(dy) + at * ldy * size, ldy,
+                                   static_cast<uint16_t*>(out) + at * width * P, rows, N, width);
+            });
         };
         if (vec) go(std::true_type{});
         else go(std::false_type{});
@@ -399,6 +401,23 @@ bool mx4_dx_bf16_faster(int64_t R, int64_t N, int64_t K) {
     return bf16 < std::min({few, t.small, t.large});
 }
 
+namespace {
+// rows and columns of the tiles: 32 x 128, 128 x 128 or 256 x 256
+struct TileSize {
+    int rows, cols;
+};
+TileSize dx_tile(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
+    if (few_dx_rows(grouped, R, E, K)) return {32, 128};
+    if (large_dx_tiles(grouped, R, E, N, K)) return {256, 256};
+    return {128, 128};
+}
+}  // namespace
+
+int64_t mx4_dx_blocks(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
+    const TileSize t = dx_tile(grouped, R, E, N, K);
+    return (most_tiles(grouped, R, E, t.rows) * ((K + t.cols - 1) / t.cols) + 7) / 8 * 8;
+}
+
 hipError_t mx4_dx(hipStream_t st, const void* dy, int64_t ldy, int pieces, const uint8_t* wc,
                   const uint8_t* ws, const int* offsets, int E, void* dx, int type, int64_t R,
                   int N, int K) {
@@ -420,8 +439,9 @@ hipError_t mx4_dx(hipStream_t st, const void* dy, int64_t ldy, int pieces, const
     using I32 = std::integral_constant<int, 32>;
     using I128 = std::integral_constant<int, 128>;
     using I256 = std::integral_constant<int, 256>;
-    if (few_dx_rows(offsets != nullptr, R, E, K)) go(I32{}, I128{}, I1{});
-    else if (large_dx_tiles(offsets != nullptr, R, E, N, K)) go(I256{}, I256{}, I2{});
+    const int tile_rows = dx_tile(offsets != nullptr, R, E, N, K).rows;
+    if (tile_rows == 32) go(I32{}, I128{}, I1{});
+    else if (tile_rows == 256) go(I256{}, I256{}, I2{});
     else go(I128{}, I128{}, I2{});
     return hipGetLastError();
 }

@@ -720,13 +720,14 @@ TileTimes tile_times(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
 
 }  // namespace
 
-hipError_t mx4_product(hipStream_t st, const uint8_t* xc, const uint8_t* xs, const int* rows,
-                       int64_t tokens, const uint8_t* wc, const uint8_t* ws, const int* offsets,
-                       int E, void* y, int type, const void* bias, int bias_type, int64_t R, int N,
-                       int K) {
-    const Weight w{wc, ws, N, K, int(mx_scale_width(K))};
-    const Out o = make_out(y, type, bias, bias_type, R, N);
-    const TileTimes tiles = tile_times(offsets != nullptr, R, E, N, K);
+namespace {
+// How a product of quantized x goes: on the kernel of few rows with `blocks` blocks of 16 of
+// them, or (0) in tiles of tile x tile.
+struct ProductPlan {
+    int blocks, tile;
+};
+ProductPlan product_plan(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
+    const TileTimes tiles = tile_times(grouped, R, E, N, K);
     // The kernel of few rows, with one block of rows always, with more (up to where a
     // block's rows of x would be read many times over) where its weight blocks take less time
     // than tiles.  With the quantizer, us, few rows against tiles: 64 x 4096 x 4096 10.6 / 15.7,
@@ -734,11 +735,31 @@ hipError_t mx4_product(hipStream_t st, const uint8_t* xc, const uint8_t* xs, con
     // 26.9; 32 x 14336 x 4096 21 / 40, 64 rows 33 / 42, 128 rows 58 / 46; 128 x 2048 x 14336 14.1 / 11.5.
     // Groups, up to 64 rows on average: 32 groups of 40 rows 2048 -> 2816 25 / 30, of 64 33 / 39, of
     // 100 44 / 44; 64 groups of 40 rows 4096 -> 1024 40 / 46, of 64 56 / 51, of 200 110 / 80.
-    const int64_t per_group = offsets ? (R + E - 1) / E : R;
-    const int mb = one_block(offsets != nullptr, R, E) ? 1 : per_group <= 32 || K > 8 * 512 ? 2 : 4;
-    const bool blocks = offsets ? per_group <= 64
+    const int64_t per_group = grouped ? (R + E - 1) / E : R;
+    const int mb = one_block(grouped, R, E) ? 1 : per_group <= 32 || K > 8 * 512 ? 2 : 4;
+    const bool blocks = grouped ? per_group <= 64
                                 : R <= 512 && few_plan(mb, false, R, E, N, K).us < std::min(tiles.small, tiles.large);
-    if (mb == 1 || blocks) {
+    return {mb == 1 || blocks ? mb : 0, tiles.large < tiles.small ? 256 : 128};
+}
+int64_t tile_blocks(bool grouped, int64_t R, int E, int64_t N, int tile) {
+    return (most_tiles(grouped, R, E, tile) * ((N + tile - 1) / tile) + 7) / 8 * 8;
+}
+}  // namespace
+
+// (the kernel of few rows has at most 2^31 threads, a block of it up to 64 x 16 columns)
+int64_t mx4_product_blocks(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
+    const ProductPlan p = product_plan(grouped, R, E, N, K);
+    return p.blocks ? 0 : tile_blocks(grouped, R, E, N, p.tile);
+}
+
+hipError_t mx4_product(hipStream_t st, const uint8_t* xc, const uint8_t* xs, const int* rows,
+                       int64_t tokens, const uint8_t* wc, const uint8_t* ws, const int* offsets,
+                       int E, void* y, int type, const void* bias, int bias_type, int64_t R, int N,
+                       int K) {
+    const Weight w{wc, ws, N, K, int(mx_scale_width(K))};
+    const Out o = make_out(y, type, bias, bias_type, R, N);
+    const ProductPlan plan = product_plan(offsets != nullptr, R, E, N, K);
+    if (const int mb = plan.blocks) {
         const Rows in{nullptr, 0, xc, xs, rows, int(tokens)};
         hipError_t e = hipSuccess;
         by_type(type, [&](auto T) {
@@ -753,7 +774,7 @@ hipError_t mx4_product(hipStream_t st, const uint8_t* xc, const uint8_t* xs, con
         constexpr int BM = decltype(M)::value, BN = decltype(N_)::value;
         const int tiles_n = (N + BN - 1) / BN;
         const int tiles_m = int(most_tiles(offsets != nullptr, R, E, BM));
-        const dim3 grid(unsigned((int64_t(tiles_m) * tiles_n + 7) / 8 * 8));
+        const dim3 grid(unsigned(tile_blocks(offsets != nullptr, R, E, N, BM)));
         if (rows)
             hipLaunchKernelGGL((mx4_tile_kernel<BM, BN, true>), grid, dim3(256), 0, st, xc, xs,
                                rows, int(tokens), w, offsets, E, o, type, tiles_m, tiles_n);
@@ -763,7 +784,7 @@ hipError_t mx4_product(hipStream_t st, const uint8_t* xc, const uint8_t* xs, con
     };
     using I128 = std::integral_constant<int, 128>;
     using I256 = std::integral_constant<int, 256>;
-    if (tiles.large < tiles.small) go(I256{}, I256{});
+    if (plan.tile == 256) go(I256{}, I256{});
     else go(I128{}, I128{});
     return hipGetLastError();
 }

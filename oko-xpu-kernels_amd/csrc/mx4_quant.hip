@@ -78,9 +78,8 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* __re
 }
 
 template <int T, bool VEC>
-void launch_quantize(hipStream_t st, const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales,
+void launch_quantize(hipStream_t st, const char* p, int64_t ldx, uint8_t* codes, uint8_t* scales,
                      int64_t groups, int G, int K) {
-    const char* p = static_cast<const char*>(x);
     // four groups a wave once that still leaves each CU several waves: 35 against 36 us at
     // 16381 x 5120 in a row, 8.3 / 8.7 at 4096 x 4096 (reading back gains nothing by it)
     if (groups >= 16384)
@@ -92,9 +91,8 @@ void launch_quantize(hipStream_t st, const void* x, int64_t ldx, uint8_t* codes,
 }
 
 template <int T>
-void launch_dequantize(hipStream_t st, const uint8_t* codes, const uint8_t* scales, void* out,
+void launch_dequantize(hipStream_t st, const uint8_t* codes, const uint8_t* scales, char* p,
                        int64_t groups, int G, int K) {
-    char* p = static_cast<char*>(out);
     hipLaunchKernelGGL((mx4_dequantize_kernel<T>), dim3(unsigned((groups + 3) / 4)), dim3(256), 0,
                        st, codes, scales, p, groups, G, K);
 }
@@ -106,23 +104,34 @@ hipError_t mx4_quantize(hipStream_t st, const void* x, int type, int64_t ldx, ui
     const int G = (K + 511) / 512;
     const int size = type == kF32 ? 4 : 2;
     const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * size) % 16 == 0;
-    auto go = [&](auto T) {
-        constexpr int t = decltype(T)::value;
-        if (vec) launch_quantize<t, true>(st, x, ldx, codes, scales, M * G, G, K);
-        else launch_quantize<t, false>(st, x, ldx, codes, scales, M * G, G, K);
-    };
-    if (type == kBf16) go(std::integral_constant<int, kBf16>{});
-    else if (type == kF16) go(std::integral_constant<int, kF16>{});
-    else go(std::integral_constant<int, kF32>{});
+    in_launches(M, 16 * kMaxBlocks / G, [&](int64_t at, int64_t rows) {
+        auto go = [&](auto T) {
+            constexpr int t = decltype(T)::value;
+            const char* p = static_cast<const char*>(x) + at * ldx * size;
+            uint8_t* c = codes + at * (K / 2);
+            uint8_t* s = scales + at * (G * 16);
+            if (vec) launch_quantize<t, true>(st, p, ldx, c, s, rows * G, G, K);
+            else launch_quantize<t, false>(st, p, ldx, c, s, rows * G, G, K);
+        };
+        if (type == kBf16) go(std::integral_constant<int, kBf16>{});
+        else if (type == kF16) go(std::integral_constant<int, kF16>{});
+        else go(std::integral_constant<int, kF32>{});
+    });
     return hipGetLastError();
 }
 
 hipError_t mx4_dequantize(hipStream_t st, const uint8_t* codes, const uint8_t* scales, void* out,
                           int type, int64_t M, int K) {
     const int G = (K + 511) / 512;
-    if (type == kBf16) launch_dequantize<kBf16>(st, codes, scales, out, M * G, G, K);
-    else if (type == kF16) launch_dequantize<kF16>(st, codes, scales, out, M * G, G, K);
-    else launch_dequantize<kF32>(st, codes, scales, out, M * G, G, K);
+    const int size = type == kF32 ? 4 : 2;
+    in_launches(M, 4 * kMaxBlocks / G, [&](int64_t at, int64_t rows) {
+        const uint8_t* c = codes + at * (K / 2);
+        const uint8_t* s = scales + at * (G * 16);
+        char* o = static_cast<char*>(out) + at * K * size;
+        if (type == kBf16) launch_dequantize<kBf16>(st, c, s, o, rows * G, G, K);
+        else if (type == kF16) launch_dequantize<kF16>(st, c, s, o, rows * G, G, K);
+        else launch_dequantize<kF32>(st, c, s, o, rows * G, G, K);
+    });
     return hipGetLastError();
 }
 

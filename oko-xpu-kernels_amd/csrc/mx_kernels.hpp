@@ -8,6 +8,14 @@
 
 namespace xpuint8 {
 
+// the blocks of 256 threads that one dimension of a launch can have (fewer than 2^32 threads)
+constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
+// f(first, count) for n items in as few launches as there must be, `most` of them in one
+template <class F>
+void in_launches(int64_t n, int64_t most, const F& f) {
+    for (int64_t at = 0; at < n; at += most) f(at, n - at < most ? n - at : most);
+}
+
 // mx4_quant.hip: x [M, K] (row stride ldx) to codes and scales, and back
 hipError_t mx4_quantize(hipStream_t st, const void* x, int type, int64_t ldx, uint8_t* codes,
                         uint8_t* scales, int64_t M, int K);
@@ -22,6 +30,9 @@ hipError_t mx4_product_fused(hipStream_t st, const void* x, int type, int64_t ld
                              const int* rows, int64_t tokens, const uint8_t* wc,
                              const uint8_t* ws, const int* offsets, int E, void* y,
                              const void* bias, int bias_type, int64_t R, int N, int K);
+// (the blocks of mx4_product's launch, which mx4_blocks_fit must hold of)
+int64_t mx4_product_blocks(bool grouped, int64_t R, int E, int64_t N, int64_t K);
+inline bool mx4_blocks_fit(int64_t blocks) { return blocks <= kMaxBlocks; }
 hipError_t mx4_product(hipStream_t st, const uint8_t* xc, const uint8_t* xs, const int* rows,
                        int64_t tokens, const uint8_t* wc, const uint8_t* ws, const int* offsets,
                        int E, void* y, int type, const void* bias, int bias_type, int64_t R, int N,
@@ -36,6 +47,7 @@ hipError_t mx4_split(hipStream_t st, const void* dy, int type, int64_t ldy, void
                      int N);
 // whether the weight read back and a bf16 product are faster than mx4_dx (one weight, bf16)
 bool mx4_dx_bf16_faster(int64_t R, int64_t N, int64_t K);
+int64_t mx4_dx_blocks(bool grouped, int64_t R, int E, int64_t N, int64_t K);
 hipError_t mx4_dx(hipStream_t st, const void* dy, int64_t ldy, int pieces, const uint8_t* wc,
                   const uint8_t* ws, const int* offsets, int E, void* dx, int type, int64_t R,
                   int N, int K);

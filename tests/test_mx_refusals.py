@@ -74,3 +74,30 @@ def test_dx_refuses_too_little_work(lib, args, code, substr):
     rc = lib.xpuint8_mxfp4_dx_stream(*args)
     msg = lib.xpuint8_last_error().decode()
     assert rc == code and substr in msg, (rc, msg)
+
+
+def test_products_of_more_blocks_than_a_launch_has(lib):
+    """Refused by the sizes already, before anything is allocated."""
+    tile, few = (1024 * 65, 1024, 1024, 1 << 22, 32), (1024, 1024, 1024, 1 << 22, 32)
+    assert lib.xpuint8_mxfp4_grouped_linear_workspace_size(*tile) == -1
+    assert b"one launch" in lib.xpuint8_last_error()
+    assert lib.xpuint8_mxfp4_grouped_linear_workspace_size(*few) == 0
+    assert lib.xpuint8_mxfp4_dx_workspace_size(0, 0, 1024, 1024, 8, 1 << 24) == -1
+    assert b"one launch" in lib.xpuint8_last_error()
+    assert lib.xpuint8_mxfp4_dx_workspace_size(0, 0, 1024, 1, 8, 1 << 24) > 0
+    # 48 GiB of bf16 results are not too many
+    assert lib.xpuint8_mxfp4_linear_workspace_size(1 << 20, 24576, 4096) > 0
+    assert lib.xpuint8_mxfp4_dx_workspace_size(0, 0, 1 << 20, 0, 4096, 24576) > 0
+
+
+@pytest.mark.parametrize("fn,args,code,substr", [
+    ("mxfp4_grouped_linear_stream", (Z, P, 0, 32, P, 1024, P, P, P, 1024, P, 66560, 1 << 22, 32, P, 1 << 40),
+     4, "one launch"),
+    ("mxfp4_dx_stream", (Z, P, 0, 8, P, P, P, 1024, P, 0, 1024, 8, 1 << 24, Z, 0), 4, "one launch"),
+    ("moe_dispatch_stream", (Z, P, 0, 8, P, P, P, 1 << 31, 1, 4, 8), 4, "2^31"),
+    ("moe_combine_stream", (Z, P, 0, 8, P, P, P, P, 0, 4, 2, 1025, 8), 2, "1024"),
+])
+def test_refusals_of_sizes(lib, fn, args, code, substr):
+    rc = getattr(lib, "xpuint8_" + fn)(*args)
+    msg = lib.xpuint8_last_error().decode()
+    assert rc == code and substr in msg, (rc, msg)
