@@ -315,8 +315,9 @@ __device__ __forceinline__ float lanes_sum(float x) {
 
 // the gradients of the weighted sum: dz[position[t, j]] = weights[t, j] * dy[t]
 // (zeros where no expert has the row), dweights[t, j] = <dy[t], z[position[t, j]]>
-// (0 there), one wave a token: dy's row is read from HBM once and from the cache
-// for the slots after the first
+// (0 there), one wave a token, slot by slot.  dy's row is read again for each slot, mostly
+// past the L2, through which z and dz stream meanwhile: 8190 tokens of 2048 bf16 in 8
+// slots read 474 MB, where z's live rows and dy are 289
 template <int T, bool VEC>
 __global__ __launch_bounds__(256) void moe_combine_grad_kernel(
     const char* __restrict__ dy, int64_t ldy, const char* __restrict__ z, int64_t ldz,

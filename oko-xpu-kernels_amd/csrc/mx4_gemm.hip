@@ -289,6 +289,10 @@ __global__ __launch_bounds__(NW * 64) void mx4_few_kernel(Rows x, Weight w,
 // The fragment reads are inline assembly (with the builtins the compiler waits for
 // every direct load before each LDS read); nothing is in flight over a loop edge:
 // each step ends with a wait that redefines what it read.
+//
+// The 256 x 256 forms hold 256 accumulators and 256 other registers a lane and spill 32 of
+// the latter (41 with GATHER): stored before the main loop and read after it, with GATHER
+// one pair in the loop too.  The 128 x 128 forms spill none.
 // blocks B0 .. B3 += W blocks (codes w, scale byte 0 of sw) * one X block
 #define XPU_MFMA4(CLOBBERS)                                                                     \
     asm volatile(XPU_MFMA_WAIT XPU_ONE_MFMA(0, 4, 10, 11) XPU_ONE_MFMA(1, 5, 12, 13)            \
@@ -735,6 +739,9 @@ ProductPlan product_plan(bool grouped, int64_t R, int E, int64_t N, int64_t K) {
     // 26.9; 32 x 14336 x 4096 21 / 40, 64 rows 33 / 42, 128 rows 58 / 46; 128 x 2048 x 14336 14.1 / 11.5.
     // Groups, up to 64 rows on average: 32 groups of 40 rows 2048 -> 2816 25 / 30, of 64 33 / 39, of
     // 100 44 / 44; 64 groups of 40 rows 4096 -> 1024 40 / 46, of 64 56 / 51, of 200 110 / 80.
+    // The mean is all that the host knows; a batch of one expert's rows alone takes no longer:
+    // 1024 rows, 32 experts 2048 -> 2816, even 30, all to one 26; 2048 rows 33 / 34; 4096 rows, 64
+    // experts 4096 -> 1024 58 / 56 (the one weight, read for every 64 rows, stays in the caches).
     const int64_t per_group = grouped ? (R + E - 1) / E : R;
     const int mb = one_block(grouped, R, E) ? 1 : per_group <= 32 || K > 8 * 512 ? 2 : 4;
     const bool blocks = grouped ? per_group <= 64
