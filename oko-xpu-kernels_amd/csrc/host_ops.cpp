@@ -647,13 +647,13 @@ const void* stream_of(const Tensor& t) {
 void check(int rc, const char* what) {
     if (rc != 0) throw std::runtime_error(std::string(what) + ": " + g_lib.last_error());
 }
-// x [.., n] as rows with a stride
+// x [.., n] as rows with a stride, a sign that is a flag of the view applied
 struct Rows {
     Tensor t;
     int64_t ld;
 };
 Rows rows_of(const Tensor& x) {
-    Tensor t = x.reshape({-1, x.size(-1)});
+    Tensor t = x.resolve_neg().reshape({-1, x.size(-1)});
     const bool many = t.size(0) > 1;
     if (t.stride(1) != 1 || (many && t.stride(0) < t.size(1))) t = t.contiguous();
     return {t, t.size(0) > 1 ? t.stride(0) : t.size(1)};

@@ -194,7 +194,7 @@ def combine(z, routing, weights):
         raise ValueError(f"weights must be [{t}, {top}], got {tuple(weights.shape)}")
     if weights.device != z.device:
         raise TypeError(f"weights is on {weights.device} but z is on {z.device}")
-    weights = weights.float().contiguous()
+    weights = weights.float().resolve_neg().contiguous()
     if _wants_grad(z, weights):
         return _CombineFn.apply(z, weights, routing)
     return _combine(z, routing, weights, z.dtype)

@@ -95,8 +95,9 @@ def _check_pair(codes, scales, lead=None):
 
 
 def _rows(x):
-    """``x`` [.., K] as rows with a stride: (tensor [M, K] or a view, row stride)."""
-    x2 = x.reshape(-1, x.shape[-1])
+    """``x`` [.., K] as rows with a stride: (tensor [M, K] or a view, row stride); a
+    sign that is a flag of the view is applied."""
+    x2 = x.resolve_neg().reshape(-1, x.shape[-1])
     if x2.stride(-1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
         x2 = x2.contiguous()
     ld = x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
@@ -259,7 +260,7 @@ def linear(x, codes, scales, bias=None):
             raise ValueError(f"bias must have shape ({codes.shape[0]},), got {tuple(bias.shape)}")
         if bias.device != x.device:
             raise TypeError(f"bias is on {bias.device} but x is on {x.device}")
-        bias = bias.contiguous()
+        bias = bias.resolve_neg().contiguous()
     if _wants_grad(x, bias):
         return _LinearFn.apply(x, codes, scales, bias)
     return _linear(x, codes, scales, bias)
