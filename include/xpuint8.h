@@ -580,8 +580,8 @@ int xpuint8_mxfp4_grouped_linear_stream(const void *stream, const void *x, int32
  * their rows, the gradient straight through x's quantization; fp32 sums, one
  * rounding to dx_type.  work (E: 0 for one weight) holds the weight as bf16 for the
  * shapes that go through it (some of one weight, bf16 dy and dx, N % 16 == 0), or dy's
- * exact bf16 pieces where it is not bf16 in whole 16-byte aligned chunks (N % 8, the
- * row stride % 8).  _size serves any dy of the type; _size_of is what this dy takes, 0
+ * bf16 pieces where it is not bf16 in whole 16-byte aligned chunks (N % 8, the row
+ * stride % 8); their sum is dy, but for an fp32's bits below 2^-133, which are dropped.  _size serves any dy of the type; _size_of is what this dy takes, 0
  * (and work NULL) for one that the kernels read where it lies. */
 int64_t xpuint8_mxfp4_dx_workspace_size(int32_t type, int32_t dx_type, int64_t R, int64_t E,
                                         int64_t N, int64_t K);

@@ -5,9 +5,11 @@
 // The contraction runs across the weight's blocks, so their scales cannot go to
 // the scaled MFMA: the weight's values, exact in bf16, go to the bf16 one
 // (v_mfma_f32_16x16x32_bf16), fp32 accumulation, one rounding at the store.  dy is
-// bf16, or 2 (fp16) or 3 (fp32) bf16 pieces whose sum is dy exactly (an fp16 value
-// has 11 significant bits, an fp32 one 24, a bf16 one 8; mx4_split): the pieces lie
-// side by side and the contraction runs over the weight's rows once for each.
+// bf16, or 2 (fp16) or 3 (fp32) bf16 pieces whose sum is dy (an fp16 value has 11
+// significant bits, an fp32 one 24, a bf16 one 8; mx4_split): exactly, but for an fp32's
+// bits below bf16's least subnormal, 2^-133, which values under 2^-109 can have and which
+// are dropped.  The pieces lie side by side and the contraction runs over the weight's
+// rows once for each.
 #include "mx4_tiles.hpp"
 
 namespace xpuint8 {
