@@ -13,9 +13,14 @@ from xpu_kernels.int8 import _lib as L
 LLVM = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin")
 
 
+class Op(tuple):
+    """(mnemonic, [operand]) with the instruction's address, and where it may branch to."""
+    at, target = 0, None
+
+
 def kernels(directory, wanted):
-    """{symbol: [(mnemonic, [operand])]} of the kernels whose symbol contains one of
-    ``wanted``; ``directory`` takes the library's code objects."""
+    """{symbol: [Op]} of the kernels whose symbol contains one of ``wanted``;
+    ``directory`` takes the library's code objects."""
     objdump = os.path.join(LLVM, "llvm-objdump")
     if not os.path.exists(objdump):
         pytest.skip("no llvm-objdump in " + LLVM)
@@ -41,9 +46,15 @@ def kernels(directory, wanted):
             head = re.match(r"[0-9a-f]+ <(.+)>:$", line)
             if head:
                 body = out.setdefault(head[1], [])
-            elif line.startswith("\t") and body is not None:
-                parts = line.split("//")[0].split(None, 1)
-                body.append((parts[0], [o.strip() for o in parts[1].split(",")] if len(parts) > 1 else []))
+            elif line.startswith("\t") and "//" in line and body is not None:
+                code_line, note = line.split("//", 1)
+                parts = code_line.split(None, 1)
+                op = Op((parts[0], [o.strip() for o in parts[1].split(",")] if len(parts) > 1 else []))
+                op.at = int(note.split(":")[0], 16)
+                if op[0].startswith(("s_cbranch", "s_branch")):
+                    offset = int(op[1][0])                # dwords from the next instruction, 16 bits
+                    op.target = op.at + 4 + 4 * (offset - 65536 if offset >= 32768 else offset)
+                body.append(op)
     return out
 
 

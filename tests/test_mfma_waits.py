@@ -1,5 +1,8 @@
-"""Matrix instructions written in assembly, of which the compiler knows neither what they
-read nor when: checked in the machine code that was built.  No device is needed."""
+"""Matrix instructions and LDS reads written in assembly, of which the compiler knows
+neither what they read nor when it is there: checked in the machine code that was built.
+No device is needed."""
+
+import re
 
 import pytest
 
@@ -68,3 +71,40 @@ def test_accumulators_are_the_matrix_instructions_until_they_are_read(code):
             if not op.startswith("v_mfma") and (i < reads[-1]):
                 written = accumulators(op, args)[0] & mine
                 assert not written, f"{name}: {op} {', '.join(args)} writes an accumulator"
+
+
+def after_wait(state, args):
+    """The LDS operations still in flight after an s_waitcnt."""
+    text = " ".join(args)
+    left = re.search(r"lgkmcnt\((\d+)\)", text)
+    if left:
+        return state[max(0, len(state) - int(left[1])):]
+    return state if re.search("vmcnt|expcnt", text) else ()
+
+
+def test_nothing_touches_a_register_that_an_lds_read_has_still_to_write(code):
+    """Along every path: an instruction that names the target of an LDS read comes after
+    a wait for that read."""
+    for name, body in code.items():
+        index = {op.at: i for i, op in enumerate(body)}
+        seen, open_ = set(), [(0, ())]
+        while open_:
+            i, state = open_.pop()
+            while i < len(body) and (i, state) not in seen:
+                seen.add((i, state))
+                assert len(seen) < 40 * len(body), f"{name}: too many paths"
+                op, args = body[i]
+                named = set().union(*(registers(w, "v") for a in args for w in a.split()))
+                for target in state:
+                    assert not named & target, f"{name}: {op} {', '.join(args)} before its LDS read's wait"
+                if op == "s_waitcnt":
+                    state = after_wait(state, args)
+                elif op.startswith("ds_read"):
+                    state += (frozenset(registers(args[0], "v")),)
+                elif op.startswith(("ds_", "s_load")):
+                    state += (frozenset(),)
+                if body[i].target is not None and op != "s_branch":
+                    open_.append((index[body[i].target], state))
+                if op == "s_endpgm":
+                    break
+                i = index[body[i].target] if op == "s_branch" else i + 1
