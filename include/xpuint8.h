@@ -634,6 +634,76 @@ int xpuint8_moe_combine_grad_stream(const void *stream, const void *dy, int32_t 
                                     float *dweights, int64_t T, int64_t top, int64_t E,
                                     int64_t D);
 
+/* the choice of experts: of logits [T, E] (row stride ld) the `top` experts of each token,
+ * ids [T, top], and their weights [T, top] in fp32.  Scores s are softmax(logits) or, with
+ * sigmoid = 1, sigmoid(logits); keys are s + bias (fp32 [E], NULL: none).  E / groups
+ * consecutive experts are a group, its value the sum of its two highest keys; of the
+ * experts in the top_groups groups of highest value the `top` highest keys are chosen, ties
+ * to the lower index, in the order of their keys.  weights = scale * s, with renormalize = 1
+ * divided by the sum of the chosen s.  An expert whose logit or key is -inf is never chosen;
+ * slots left over have id -1 and weight 0.  A row with a NaN logit, for softmax also with
+ * one of +inf, has NaN weights.  top <= 64, groups <= 64.  No counterpart in the reference. */
+int xpuint8_moe_route_stream(const void *stream, const void *logits, int32_t type, int64_t ld,
+                             const float *bias, int32_t sigmoid, int64_t groups,
+                             int64_t top_groups, int32_t renormalize, float scale, int32_t *ids,
+                             float *weights, int64_t T, int64_t E, int64_t top);
+
+/* dlogits [T, E] (contiguous, the logits' type) of the weights' gradient dweights [T, top];
+ * slots without an expert have none */
+int xpuint8_moe_route_grad_stream(const void *stream, const void *logits, int32_t type, int64_t ld,
+                                  const int32_t *ids, const float *dweights, int32_t sigmoid,
+                                  int32_t renormalize, float scale, void *dlogits, int64_t T,
+                                  int64_t E, int64_t top);
+
+/* ---- RMS norm -----------------------------------------------------------
+ * Rows of K values, [M, K] with row strides in elements; element types 0 bf16, 1 fp16,
+ * 2 fp32.  Inputs may have the alignment of their elements; outputs and work are contiguous
+ * and 16-byte aligned.  Statistics are fp32.  K <= 2^24.  No counterpart in the reference.
+ *
+ * h = x + residual rounded to the type (residual and h NULL: h is x);
+ * y = h / sqrt(mean(h^2) + eps) * weight (fp32 until y's rounding; weight [K] of its own
+ * type, NULL: ones) */
+int xpuint8_rms_norm_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
+                            const void *residual, int64_t ldr, const void *weight,
+                            int32_t weight_type, float eps, void *h, void *y, int64_t M,
+                            int64_t K);
+
+/* the same in int8 with a scale a row, for the int8 linears: v = h * weight in fp32, with
+ * rotate = 1 (K % 256 == 0) rotated as xpuint8_convrot_quantize_stream rotates;
+ * m = max(|v|, 1e-30), q = rint(v * (127 / m)), scale = m / 127 / sqrt(mean(h^2) + eps) */
+int xpuint8_rms_norm_int8_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
+                                 const void *residual, int64_t ldr, const void *weight,
+                                 int32_t weight_type, float eps, void *h, int8_t *q, float *scale,
+                                 int32_t rotate, int64_t M, int64_t K);
+
+/* dx [M, K], the gradient of x and of the residual, from y's gradient dy and (NULL: none)
+ * h's, dh; h is what was normalised.  dweight [K] of weight_type (NULL: not wanted, work
+ * then too) sums fp32 in a fixed order. */
+int64_t xpuint8_rms_norm_grad_workspace_size(int64_t M, int64_t K);
+int xpuint8_rms_norm_grad_stream(const void *stream, const void *dy, int32_t type, int64_t ldy,
+                                 const void *h, int64_t ldh, const void *weight,
+                                 int32_t weight_type, const void *dh, int64_t lddh, float eps,
+                                 void *dx, void *dweight, int64_t M, int64_t K, void *work,
+                                 int64_t work_bytes);
+
+/* ---- rotary positions on several axes -----------------------------------
+ * q [B, S, q_heads, D] and k [B, S, k_heads, D] (NULL: q alone) to q_out and k_out: pair j <
+ * pairs of each head turned by positions[axis[j], b, s] * inv_freq[j] radians (inverse = 1:
+ * by the opposite angle, the gradient); pairs are elements j and j + pairs (split_half = 1)
+ * or 2j and 2j + 1; elements past 2 * pairs are copied.  Angles are reduced in fp64, products
+ * are fp32.  q_strides = {b, s, head} of q, then of q_out, in elements, the last dimensions
+ * contiguous; position_strides = {axis, b, s}; positions int32, int64 or fp32 (position_type
+ * 0, 1, 2); an axis outside [0, axes) does not turn.  Buffers have the alignment of their
+ * elements.  pairs <= 512, D <= 4096.  Strides are read on the host.  No counterpart in the
+ * reference. */
+int xpuint8_rope_axes_stream(const void *stream, const void *q, void *q_out,
+                             const int64_t *q_strides, int64_t q_heads, const void *k, void *k_out,
+                             const int64_t *k_strides, int64_t k_heads, int32_t type,
+                             const void *positions, int32_t position_type,
+                             const int64_t *position_strides, int64_t axes,
+                             const double *inv_freq, const int32_t *axis, int64_t pairs,
+                             int32_t inverse, int32_t split_half, int64_t B, int64_t S, int64_t D);
+
 #ifdef __cplusplus
 }
 #endif

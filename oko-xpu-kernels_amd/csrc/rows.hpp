@@ -1,0 +1,138 @@
+// Pieces of rows on the device: 8 consecutive values of a row of any alignment, and
+// sums and maxima over the lanes of a wave, for the row operators (norm.hip, rotary.hip,
+// route.hip).
+//
+// gfx950 takes 16-byte global accesses at any address of the element's alignment, so a
+// row that starts anywhere (an odd row length, a column slice) is read and written in
+// the same instructions as an aligned one; only a row's last piece, if it is cut, goes
+// element by element.
+#pragma once
+
+#include "mx4.hpp"
+
+namespace xpuint8 {
+
+template <int T>
+constexpr int kElem = T == kF32 ? 4 : 2;
+
+// 8 values as they lie in memory
+template <int T>
+struct Piece8 {
+    uint32_t w[T == kF32 ? 8 : 4];
+};
+template <int T>
+struct __attribute__((packed, aligned(T == kF32 ? 4 : 2))) Loose8 {
+    uint32_t w[T == kF32 ? 8 : 4];
+};
+
+// the piece at d < n of a row of n; EVEN: n is a multiple of 8, no piece is cut
+template <int T, bool EVEN>
+__device__ __forceinline__ Piece8<T> piece_load(const void* row, int64_t d, int64_t n) {
+    Piece8<T> p;
+    if (EVEN || d + 8 <= n) {
+        const auto* q = reinterpret_cast<const Loose8<T>*>(static_cast<const char*>(row) + d * kElem<T>);
+#pragma unroll
+        for (int i = 0; i < int(sizeof(p.w) / 4); ++i) p.w[i] = q->w[i];
+        return p;
+    }
+#pragma unroll
+    for (int i = 0; i < int(sizeof(p.w) / 4); ++i) p.w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (d + i >= n) continue;
+        if constexpr (T == kF32) p.w[i] = static_cast<const uint32_t*>(row)[d + i];
+        else p.w[i / 2] |= uint32_t(static_cast<const uint16_t*>(row)[d + i]) << (16 * (i & 1));
+    }
+    return p;
+}
+
+template <int T, bool EVEN>
+__device__ __forceinline__ void piece_store(void* row, int64_t d, int64_t n, const Piece8<T>& p) {
+    if (EVEN || d + 8 <= n) {
+        auto* q = reinterpret_cast<Loose8<T>*>(static_cast<char*>(row) + d * kElem<T>);
+#pragma unroll
+        for (int i = 0; i < int(sizeof(p.w) / 4); ++i) q->w[i] = p.w[i];
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (d + i >= n) continue;
+        if constexpr (T == kF32) static_cast<uint32_t*>(row)[d + i] = p.w[i];
+        else static_cast<uint16_t*>(row)[d + i] = uint16_t(p.w[i / 2] >> (16 * (i & 1)));
+    }
+}
+
+template <int T>
+__device__ __forceinline__ void piece_expand(const Piece8<T>& p, float (&v)[8]) {
+    if constexpr (T == kF32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(p.w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (T == kBf16) {
+                v[2 * i] = bf16lo(p.w[i]);
+                v[2 * i + 1] = bf16hi(p.w[i]);
+            } else {
+                const xpu_v2h h = __builtin_bit_cast(xpu_v2h, p.w[i]);
+                v[2 * i] = float(h[0]);
+                v[2 * i + 1] = float(h[1]);
+            }
+        }
+    }
+}
+template <int T>
+__device__ __forceinline__ Piece8<T> piece_round(const float (&v)[8]) {
+    Piece8<T> p;
+    if constexpr (T == kF32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p.w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p.w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    }
+    return p;
+}
+
+// 8 values of a vector of n whose type is known at run time only; ones for none, zeros
+// past its end
+template <bool EVEN>
+__device__ __forceinline__ void vector_load(const void* w, int type, int64_t d, int64_t n,
+                                            float (&v)[8]) {
+    if (!w) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 1.f;
+    } else if (type == kBf16) {
+        piece_expand(piece_load<kBf16, EVEN>(w, d, n), v);
+    } else if (type == kF16) {
+        piece_expand(piece_load<kF16, EVEN>(w, d, n), v);
+    } else {
+        piece_expand(piece_load<kF32, EVEN>(w, d, n), v);
+    }
+}
+
+// The sum over N (8, 16, 32 or 64) consecutive lanes, in every one of them: DPP inside
+// a row of 16 lanes, whose steps each add two disjoint groups of equal partial sums,
+// then across rows.  The order is fixed.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float x) {
+    x += dpp<kDppXor1>(x);
+    x += dpp<kDppXor2>(x);
+    x += dpp<kDppXor7>(x);
+    if constexpr (N >= 16) x += dpp<kDppXor15>(x);
+    if constexpr (N >= 32) x += swz_xor<16>(x);
+    if constexpr (N >= 64) x += __shfl_xor(x, 32);
+    return x;
+}
+template <int N>
+__device__ __forceinline__ float lanes_max(float x) {
+    x = fmaxf(x, dpp<kDppXor1>(x));
+    x = fmaxf(x, dpp<kDppXor2>(x));
+    x = fmaxf(x, dpp<kDppXor7>(x));
+    if constexpr (N >= 16) x = fmaxf(x, dpp<kDppXor15>(x));
+    if constexpr (N >= 32) x = fmaxf(x, swz_xor<16>(x));
+    if constexpr (N >= 64) x = fmaxf(x, __shfl_xor(x, 32));
+    return x;
+}
+
+}  // namespace xpuint8

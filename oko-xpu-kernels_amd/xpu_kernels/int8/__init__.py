@@ -39,6 +39,7 @@ from .ops import (
     linear_dw,
     linear_dx,
     linear_dx_int8,
+    linear_quantized,
     pack_weight,
     prepare_weight,
     prepare_weight_fused,
@@ -55,7 +56,8 @@ __all__ = [
     "ACTIVATIONS", "Int8Linear", "PAIRED_ACTIVATIONS", "TrainableInt8Linear", "available",
     "dequant", "dequant_act_quantize", "dequant_slice", "dequant_weight",
     "dequant_weight_torch", "device_name", "expand_scale", "ffn", "ffn_situ", "int8_linear",
-    "int_mm", "linear", "linear_acc", "linear_dw", "linear_dx", "linear_dx_int8", "load",
+    "int_mm", "linear", "linear_acc", "linear_dw", "linear_dx", "linear_dx_int8",
+    "linear_quantized", "load",
     "pack_weight", "prepare_weight", "prepare_weight_fused", "quantize", "quantize_act", "quantize_row",
     "quantize_row_torch", "rotate", "selftest", "unsupported_reason",
 ]

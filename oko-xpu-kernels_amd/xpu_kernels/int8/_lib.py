@@ -10,6 +10,7 @@ stream behind ``torch.cuda.current_stream(device)``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import sys
@@ -72,7 +73,7 @@ def _candidate_paths():
 #: every exported symbol: name -> (argtypes, restype).  Mirrors include/xpuint8.h.
 def _signatures():
     vp, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
-    c_int, c_str = ctypes.c_int, ctypes.c_char_p
+    c_int, c_str, f32 = ctypes.c_int, ctypes.c_char_p, ctypes.c_float
     return {
         "xpuint8_init": ([], c_int),
         "xpuint8_device_name": ([], c_str),
@@ -160,6 +161,20 @@ def _signatures():
         "xpuint8_moe_combine_stream": ([vp, vp, i32, i64] + [vp] * 4 + [i32] + [i64] * 4, c_int),
         "xpuint8_moe_combine_grad_stream": ([vp, vp, i32, i64, vp, i64] + [vp] * 5 + [i64] * 4,
                                             c_int),
+        "xpuint8_moe_route_stream": ([vp, vp, i32, i64, vp, i32, i64, i64, i32, f32, vp, vp]
+                                     + [i64] * 3, c_int),
+        "xpuint8_moe_route_grad_stream": ([vp, vp, i32, i64, vp, vp, i32, i32, f32, vp]
+                                          + [i64] * 3, c_int),
+        "xpuint8_rms_norm_stream": ([vp, vp, i32, i64, vp, i64, vp, i32, f32, vp, vp, i64, i64],
+                                    c_int),
+        "xpuint8_rms_norm_int8_stream": ([vp, vp, i32, i64, vp, i64, vp, i32, f32, vp, vp, vp, i32,
+                                          i64, i64], c_int),
+        "xpuint8_rms_norm_grad_workspace_size": ([i64] * 2, i64),
+        "xpuint8_rms_norm_grad_stream": ([vp, vp, i32, i64, vp, i64, vp, i32, vp, i64, f32, vp, vp,
+                                          i64, i64, vp, i64], c_int),
+        "xpuint8_rope_axes_stream": ([vp] * 4 + [i64] + [vp] * 3 + [i64, i32, vp, i32, vp, i64, vp,
+                                                                    vp, i64, i32, i32] + [i64] * 3,
+                                     c_int),
     }
 
 
@@ -264,6 +279,15 @@ def _stream(device):
         index = device.index if device.index is not None else torch.cuda.current_device()
         return _RAW_STREAM(index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_STAY = contextlib.nullcontext()
+
+
+def _on(device):
+    """The device current for a call on its tensors: the library launches on the current
+    one, which need not be theirs."""
+    return _STAY if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _ptr(t):

@@ -911,6 +911,55 @@ def _linear_bf16(lib, x2, w8c, ws, b, b16, m, n, k, packed=None):
     return out
 
 
+def linear_quantized(q, scale, w8, w_scale, bias=None):
+    """:func:`linear` of an activation that is quantized already, by :func:`quantize` or
+    ``norm.rms_norm_int8`` (or, against a weight that is not rotated, row by row without
+    the rotation): int8 q [.., K] and its scales [..] -> bf16 [.., N],
+    ``float(q @ w8.T) * (w_scale * scale) + bias``.  K and N multiples of 16.  No
+    counterpart in the reference, whose linear quantizes its input itself."""
+    if not isinstance(q, torch.Tensor) or q.dtype != torch.int8 or q.dim() < 1:
+        raise TypeError(f"q must be an int8 [.., K] tensor, got "
+                        f"{getattr(q, 'dtype', type(q).__name__)}")
+    if not isinstance(w8, torch.Tensor) or w8.dtype != torch.int8 or w8.dim() != 2:
+        raise TypeError("w8 must be an int8 [N, K] tensor")
+    n, k = w8.shape
+    if q.shape[-1] != k:
+        raise ValueError(f"K mismatch: activation {q.shape[-1]} vs weight {k}")
+    if k % 16 or n % 16 or not k or not n:
+        raise ValueError(f"K={k} and N={n} must be positive multiples of 16")
+    m = q.numel() // k
+    if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32:
+        raise TypeError(f"scale must be a float32 tensor, got "
+                        f"{getattr(scale, 'dtype', type(scale).__name__)}")
+    if scale.numel() != m:
+        raise ValueError(f"scale has {scale.numel()} values but q has {m} rows")
+    if isinstance(w_scale, torch.Tensor) and w_scale.numel() not in (1, n):
+        raise ValueError(f"weight scale has {w_scale.numel()} values; expected 1 or N={n}")
+    if isinstance(bias, torch.Tensor) and bias.numel() not in (1, n):
+        raise ValueError(f"bias has {bias.numel()} values; expected 1 or N={n}")
+    if q.device.type != "cuda":
+        raise TypeError(f"expected a GPU (ROCm) tensor, got {q.device}")
+    for t, name in ((scale, "scale"), (w8, "w8"), (w_scale, "w_scale"), (bias, "bias")):
+        if isinstance(t, torch.Tensor) and t.device != q.device:
+            raise TypeError(f"{name} is on {t.device} but q is on {q.device}")
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
+                                       for t in (scale, w_scale, bias)):
+        raise RuntimeError("linear_quantized has no gradient; call it under torch.no_grad(), or "
+                           "int8_linear for one")
+    out = torch.empty((*q.shape[:-1], n), device=q.device, dtype=torch.bfloat16)
+    if not m:
+        return out
+    lib = _lib()
+    qc, wc = _c(q), _c(w8)
+    xs, ws = expand_scale(scale, m, q.device), expand_scale(w_scale, n, q.device)
+    b, b16 = _bias_arg(bias, n, q.device)
+    with _L._on(q.device):
+        if lib.xpuint8_linear_gemm_stream(_stream(q.device), _ptr(qc), _ptr(xs), _ptr(wc), _ptr(ws),
+                                          _opt(b), b16, _ptr(out), m, n, k) != 0:
+            _err(lib, "linear_quantized")
+    return out
+
+
 def _residual_tail(out, residual, residual_scale, input_dtype, shape, m, n):
     """ops.py:639-646 after the GEMM: a residual the store did not fuse (an
     fp32 model, a per-row or full-size scale, an fp32 scale whose addcmul

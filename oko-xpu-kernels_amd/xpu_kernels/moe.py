@@ -1,6 +1,7 @@
-"""Mixture-of-experts routing on gfx950: tokens sorted by expert and back, with
-the weights applied, their gradients, and an FFN of MXFP4 experts.
+"""Mixture-of-experts routing on gfx950: the choice of experts, tokens sorted by expert
+and back, with the weights applied, their gradients, and an FFN of MXFP4 experts.
 
+    expert_ids, weights = moe.route(logits, top)  # [T, E] -> [T, top] each
     routing = moe.sort(expert_ids, n_experts)     # expert_ids [T, top], integers
     xs = moe.dispatch(x, routing)                 # [T, D] -> [T*top, D], by expert
     ...                                           # the experts, on their rows
@@ -24,9 +25,12 @@ from . import mxfp4
 from .int8 import _lib as L
 from .mxfp4 import TYPES, _check_float, _opt, _rows, _wants_grad, _work
 
-__all__ = ["Routing", "combine", "dispatch", "ffn", "sort"]
+__all__ = ["Routing", "combine", "dispatch", "ffn", "route", "sort"]
 
 MAX_EXPERTS = 1024
+MAX_TOP = 64
+MAX_GROUPS = 64
+SCORES = ("softmax", "sigmoid")
 
 
 class Routing(NamedTuple):
@@ -49,6 +53,108 @@ def _check_routing(routing, device):
     if (routing.position.dim() != 2 or routing.position.numel() != n or routing.rows.numel() != n
             or routing.offsets.numel() < 2):
         raise ValueError("routing's tensors do not belong together")
+
+
+def _route(logits, bias, how, top):
+    sigmoid, groups, top_groups, renormalize, scale = how
+    t, e = logits.shape
+    ids = torch.empty((t, top), dtype=torch.int32, device=logits.device)
+    weights = torch.empty((t, top), dtype=torch.float32, device=logits.device)
+    if t:
+        l2, ld = _rows(logits)
+        lib = L._lib()
+        with L._on(logits.device):
+            if lib.xpuint8_moe_route_stream(L._stream(logits.device), l2.data_ptr(),
+                                            TYPES[logits.dtype], ld, _opt(bias), sigmoid, groups,
+                                            top_groups, renormalize, scale, ids.data_ptr(),
+                                            weights.data_ptr(), t, e, top) != 0:
+                L._err(lib, "moe.route")
+    return ids, weights
+
+
+def _route_grad(logits, ids, dweights, how):
+    sigmoid, _, _, renormalize, scale = how
+    t, e = logits.shape
+    out = torch.empty((t, e), dtype=logits.dtype, device=logits.device)
+    if t:
+        l2, ld = _rows(logits)
+        dw = dweights.resolve_neg().contiguous()
+        lib = L._lib()
+        with L._on(logits.device):
+            if lib.xpuint8_moe_route_grad_stream(L._stream(logits.device), l2.data_ptr(),
+                                                 TYPES[logits.dtype], ld, ids.data_ptr(),
+                                                 dw.data_ptr(), sigmoid, renormalize, scale,
+                                                 out.data_ptr(), t, e, ids.shape[1]) != 0:
+                L._err(lib, "moe.route (gradient)")
+    return out
+
+
+class _RouteFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, how, top):
+        ids, weights = _route(logits, bias, how, top)
+        ctx.save_for_backward(logits, ids)
+        ctx.how = how
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        return ids, weights
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _, dweights):
+        logits, ids = ctx.saved_tensors
+        if dweights is None:
+            return None, None, None, None
+        return _route_grad(logits, ids, dweights, ctx.how), None, None, None
+
+
+def route(logits, top, *, scores="softmax", bias=None, groups=1, top_groups=1, renormalize=True,
+          scale=1.0):
+    """The experts of each token: ``logits`` [T, E] -> (ids int32 [T, top], weights fp32
+    [T, top]), in the order of choice.
+
+    Scores are the softmax over the experts, or the sigmoid, of the logits.  Experts are
+    chosen by key = score + ``bias`` (fp32 [E], for balance: it changes the choice alone,
+    and gets no gradient): with ``groups``, E / groups consecutive experts each, first the
+    ``top_groups`` groups with the largest sum of their two highest keys, then in them the
+    ``top`` highest keys, equal ones by index.  The choice is exact (made in 64 bits).
+    Weights are the chosen scores times ``scale``, with ``renormalize`` divided by their sum.
+
+    An expert whose logit or key is -inf is never chosen (a mask); slots that are left over
+    have id -1, which :func:`sort` gives to no expert, and weight 0.  A NaN logit, for the
+    softmax +inf too, makes the token's weights NaN.  The gradient of the weights reaches
+    the logits."""
+    _check_float(logits, "logits")
+    if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_EXPERTS:
+        raise ValueError(f"logits must be [T, E] with 1..{MAX_EXPERTS} experts, got "
+                         f"{tuple(logits.shape)}")
+    e = logits.shape[1]
+    if scores not in SCORES:
+        raise ValueError(f"scores must be one of {SCORES}, got {scores!r}")
+    for name, v, most in (("top", top, min(MAX_TOP, e)), ("groups", groups, MAX_GROUPS),
+                          ("top_groups", top_groups, groups)):
+        if not isinstance(v, int) or isinstance(v, bool) or not 1 <= v <= most:
+            raise ValueError(f"{name} must be a whole number in 1..{most}, got {v!r}")
+    if e % groups:
+        raise ValueError(f"{groups} groups do not divide {e} experts")
+    if top > top_groups * (e // groups):
+        raise ValueError(f"top={top} is more than the {top_groups * (e // groups)} experts of "
+                         f"{top_groups} groups")
+    if not isinstance(scale, (int, float)):
+        raise TypeError(f"scale must be a number, got {type(scale).__name__}")
+    if bias is not None:
+        _check_float(bias, "bias")
+        if bias.shape != (e,):
+            raise ValueError(f"bias must have shape ({e},), got {tuple(bias.shape)}")
+        if bias.device != logits.device:
+            raise TypeError(f"bias is on {bias.device} but the logits are on {logits.device}")
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise ValueError("bias gets no gradient: it changes the choice of experts alone")
+        bias = bias.detach().float().resolve_neg().contiguous()
+    how = (int(scores == "sigmoid"), groups, top_groups, int(bool(renormalize)), float(scale))
+    if _wants_grad(logits, bias):
+        return _RouteFn.apply(logits, bias, how, top)
+    return _route(logits, bias, how, top)
 
 
 def sort(expert_ids, n_experts):

@@ -67,7 +67,7 @@ def _wants_grad(*tensors):
     which no operator here carries on, is refused."""
     tensors = [t for t in tensors if t is not None]
     if any(unpack_dual(t).tangent is not None for t in tensors):
-        raise NotImplementedError("the MXFP4 and mixture-of-experts operators have no "
+        raise NotImplementedError("the operators of norm, mxfp4, moe and rope have no "
                                   "forward-mode derivative")
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
