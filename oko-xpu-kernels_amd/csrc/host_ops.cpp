@@ -1,5 +1,5 @@
 // The host path of the Python API's hot calls (xpu_kernels.int8 linear, ffn, the
-// backward's products and the quantizer; xpu_kernels.mxfp4 and moe with their gradients)
+// backward's products and the quantizer; xpu_kernels.mxfp4, moe, norm and rope with their gradients)
 // as a CPython extension: argument checks, the packed weight's lookup, allocations and
 // the library call in native code.  In Python these cost more than the small calls'
 // kernels: linear at 16 x 4096 x 4096 took 17.6 us of host time for 8.5 us of GPU work,
@@ -15,6 +15,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/Storage.h>
@@ -74,8 +75,15 @@ struct Library {
     decltype(&xpuint8_moe_combine_grad_stream) moe_combine_grad;
     decltype(&xpuint8_mxfp4_dbias_workspace_size) mx_dbias_size;
     decltype(&xpuint8_mxfp4_dbias_stream) mx_dbias;
+    decltype(&xpuint8_rms_norm_stream) rms_norm;
+    decltype(&xpuint8_rms_norm_int8_stream) rms_norm_int8;
+    decltype(&xpuint8_rms_norm_grad_workspace_size) rms_norm_grad_size;
+    decltype(&xpuint8_rms_norm_grad_stream) rms_norm_grad;
+    decltype(&xpuint8_rope_axes_stream) rope_axes;
+    decltype(&xpuint8_moe_route_stream) moe_route;
+    decltype(&xpuint8_moe_route_grad_stream) moe_route_grad;
 };
-constexpr int kEntries = 33;
+constexpr int kEntries = 40;
 static_assert(sizeof(Library) == kEntries * sizeof(void*), "one address per entry");
 
 Library g_lib;
@@ -907,6 +915,378 @@ PyObject* host_moe_combine(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
+// ------------------------------------------------ xpu_kernels.norm, moe.route, rope
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+PyObject* wrapped(const variable_list& v) {
+    PyObject* out = PyTuple_New(Py_ssize_t(v.size()));
+    if (!out) throw python_error();
+    for (size_t i = 0; i < v.size(); ++i) {
+        PyObject* o = v[i].defined() ? THPVariable_Wrap(v[i]) : Py_NewRef(Py_None);
+        if (!o) {
+            Py_DECREF(out);
+            throw python_error();
+        }
+        PyTuple_SET_ITEM(out, Py_ssize_t(i), o);
+    }
+    return out;
+}
+// an int or float object's value
+bool number(PyObject* o, double& v) {
+    if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
+    v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    return true;
+}
+bool whole(PyObject* o, int64_t lo, int64_t hi, int64_t& v) {
+    if (!PyLong_CheckExact(o)) return false;
+    int over = 0;
+    v = PyLong_AsLongLongAndOverflow(o, &over);
+    if (over) return false;
+    return v >= lo && v <= hi;
+}
+const std::optional<Tensor> maybe(const Tensor* t) { return t ? std::optional<Tensor>(*t) : std::nullopt; }
+
+// x, weight or None, eps, residual or None of a norm
+struct NormCall {
+    const Tensor *x = nullptr, *w = nullptr, *r = nullptr;
+    double eps = 0;
+};
+bool norm_call(PyObject* const* a, NormCall& c) {
+    c.x = floating(a[0]);
+    if (!c.x || c.x->dim() < 1 || c.x->size(-1) > int64_t(1) << 24 || !number(a[2], c.eps) || !(c.eps >= 0))
+        return false;
+    if (a[1] != Py_None) {
+        c.w = on(floating(a[1]), *c.x);
+        if (!c.w || c.w->dim() != 1 || c.w->numel() != c.x->size(-1)) return false;
+    }
+    if (a[3] != Py_None) {
+        c.r = on(plain(a[3], c.x->scalar_type()), *c.x);
+        if (!c.r || c.r->sizes() != c.x->sizes()) return false;
+    }
+    return !has_tangent(*c.x, c.w) && !(c.r && has_tangent(*c.r));
+}
+
+// (y, h or undefined)
+std::array<Tensor, 2> run_norm(const Tensor& x, const Tensor* w, double eps, const Tensor* r) {
+    const int64_t k = x.size(-1), m = x.numel() / k;
+    const void* st = current_stream(x);
+    Tensor y, h;
+    call("norm.rms_norm", [&] {
+        const c10::DeviceGuard on_x(x.device());
+        y = empty(x.sizes(), x.scalar_type(), x);
+        if (r) h = empty(x.sizes(), x.scalar_type(), x);
+        return g_lib.rms_norm(st, x.data_ptr(), type_of(x), k, r ? r->data_ptr() : nullptr, k,
+                              w ? w->data_ptr() : nullptr, w ? type_of(*w) : 0, float(eps), ptr(h),
+                              y.data_ptr(), m, k);
+    });
+    return {y, h};
+}
+
+struct NormFn : torch::autograd::Function<NormFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& w,
+                                 double eps, const std::optional<Tensor>& r) {
+        ctx->set_materialize_grads(false);
+        auto [y, h] = run_norm(x, w ? &*w : nullptr, eps, r ? &*r : nullptr);
+        ctx->save_for_backward({r ? h : x, w ? *w : Tensor()});
+        ctx->saved_data["eps"] = eps;
+        if (r) return {y, h};
+        return {y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list in) {
+        return once(in, [&]() -> variable_list {
+            const variable_list saved = ctx->get_saved_variables();
+            const Tensor &h = saved[0], &w = saved[1], &dy = in[0];
+            const Tensor dh = in.size() > 1 ? in[1] : Tensor();
+            const double eps = ctx->saved_data["eps"].toDouble();
+            const bool want = w.defined() && ctx->needs_input_grad(1);
+            Tensor dx, dw;
+            if (!dy.defined()) {
+                dx = dh;
+                if (want) dw = at::zeros_like(w);
+            } else {
+                const c10::DeviceGuard on_h(h.device());
+                const int64_t k = h.size(-1), m = h.numel() / k;
+                const Rows g = rows_of(dy);
+                Rows b{Tensor(), 0};
+                if (dh.defined()) b = rows_of(dh);
+                const int64_t need = want ? g_lib.rms_norm_grad_size(m, k) : 0;
+                if (need < 0) check(1, "norm.rms_norm (gradient)");
+                Tensor work;
+                if (want) {
+                    work = workspace(need, h);
+                    dw = empty({k}, w.scalar_type(), h);
+                }
+                dx = empty(h.sizes(), h.scalar_type(), h);
+                check(g_lib.rms_norm_grad(stream_of(h), g.t.data_ptr(), type_of(h), g.ld, h.data_ptr(), k,
+                                          ptr(w), w.defined() ? type_of(w) : 0, ptr(b.t), b.ld, float(eps),
+                                          dx.data_ptr(), ptr(dw), m, k, ptr(work), need),
+                      "norm.rms_norm (gradient)");
+            }
+            // x, weight, eps, residual (needs_input_grad counts the tensors that are there)
+            const bool to_r = in.size() > 1 && ctx->needs_input_grad(w.defined() ? 2 : 1);
+            return {ctx->needs_input_grad(0) ? dx : Tensor(), dw, Tensor(), to_r ? dx : Tensor()};
+        });
+    }
+};
+
+// rms_norm(x, weight, eps, residual): norm.rms_norm
+PyObject* host_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 4, [&]() -> PyObject* {
+        NormCall c;
+        if (!norm_call(a, c)) Py_RETURN_NONE;
+        if (wants_grad(*c.x, c.w) || (c.r && wants_grad(*c.r))) {
+            const variable_list out = NormFn::apply(*c.x, maybe(c.w), c.eps, maybe(c.r));
+            return c.r ? wrapped(out) : THPVariable_Wrap(out[0]);
+        }
+        auto [y, h] = run_norm(*c.x, c.w, c.eps, c.r);
+        return c.r ? pair(y, h) : THPVariable_Wrap(y);
+    });
+}
+
+// rms_norm_int8(x, weight, eps, residual, rotate): norm.rms_norm_int8 of inputs without gradients
+PyObject* host_rms_norm_int8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 5, [&]() -> PyObject* {
+        NormCall c;
+        if (!norm_call(a, c) || wants_grad(*c.x, c.w) || (c.r && wants_grad(*c.r))) Py_RETURN_NONE;
+        const int rotate = PyObject_IsTrue(a[4]);
+        if (rotate < 0) throw python_error();
+        const Tensor& x = *c.x;
+        const int64_t k = x.size(-1), m = x.numel() / k;
+        if (rotate && k % 256 != 0) Py_RETURN_NONE;
+        const void* st = current_stream(x);
+        Tensor q, s, h;
+        call("norm.rms_norm_int8", [&] {
+            const c10::DeviceGuard on_x(x.device());
+            q = empty(x.sizes(), at::kChar, x);
+            s = empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+            if (c.r) h = empty(x.sizes(), x.scalar_type(), x);
+            return g_lib.rms_norm_int8(st, x.data_ptr(), type_of(x), k, c.r ? c.r->data_ptr() : nullptr, k,
+                                       c.w ? c.w->data_ptr() : nullptr, c.w ? type_of(*c.w) : 0,
+                                       float(c.eps), ptr(h), static_cast<int8_t*>(q.data_ptr()),
+                                       static_cast<float*>(s.data_ptr()), rotate, m, k);
+        });
+        return c.r ? wrapped({q, s, h}) : pair(q, s);
+    });
+}
+
+struct RouteHow {
+    int32_t sigmoid, renormalize;
+    int64_t groups, top_groups;
+    double scale;
+};
+std::array<Tensor, 2> run_route(const Tensor& l, const Tensor* b, const RouteHow& how, int64_t top) {
+    const int64_t t = l.size(0), e = l.size(1);
+    const void* st = current_stream(l);
+    Tensor ids, w;
+    call("moe.route", [&] {
+        const c10::DeviceGuard on_l(l.device());
+        ids = empty({t, top}, at::kInt, l);
+        w = empty({t, top}, at::kFloat, l);
+        return g_lib.moe_route(st, l.data_ptr(), type_of(l), e,
+                               b ? static_cast<const float*>(b->data_ptr()) : nullptr, how.sigmoid,
+                               how.groups, how.top_groups, how.renormalize, float(how.scale),
+                               ints(ids), static_cast<float*>(w.data_ptr()), t, e, top);
+    });
+    return {ids, w};
+}
+
+struct RouteFn : torch::autograd::Function<RouteFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& l, const std::optional<Tensor>& b,
+                                 int64_t sigmoid, int64_t renormalize, int64_t groups,
+                                 int64_t top_groups, double scale, int64_t top) {
+        ctx->set_materialize_grads(false);
+        const RouteHow how{int32_t(sigmoid), int32_t(renormalize), groups, top_groups, scale};
+        auto [ids, w] = run_route(l, b ? &*b : nullptr, how, top);
+        ctx->save_for_backward({l, ids});
+        ctx->saved_data["sigmoid"] = sigmoid;
+        ctx->saved_data["renormalize"] = renormalize;
+        ctx->saved_data["scale"] = scale;
+        ctx->mark_non_differentiable({ids});
+        return {ids, w};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list in) {
+        return once(in, [&]() -> variable_list {
+            variable_list out(8);
+            if (!in[1].defined()) return out;
+            const variable_list saved = ctx->get_saved_variables();
+            const Tensor &l = saved[0], &ids = saved[1];
+            const c10::DeviceGuard on_l(l.device());
+            const Tensor dw = in[1].resolve_neg().contiguous();
+            const int64_t t = l.size(0), e = l.size(1);
+            out[0] = empty({t, e}, l.scalar_type(), l);
+            check(g_lib.moe_route_grad(stream_of(l), l.data_ptr(), type_of(l), e, ints(&ids),
+                                       static_cast<const float*>(dw.data_ptr()),
+                                       int32_t(ctx->saved_data["sigmoid"].toInt()),
+                                       int32_t(ctx->saved_data["renormalize"].toInt()),
+                                       float(ctx->saved_data["scale"].toDouble()), out[0].data_ptr(),
+                                       t, e, ids.size(1)), "moe.route (gradient)");
+            return out;
+        });
+    }
+};
+
+// moe_route(logits, top, scores, bias, groups, top_groups, renormalize, scale): moe.route
+PyObject* host_moe_route(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 8, [&]() -> PyObject* {
+        const Tensor* l = floating(a[0]);
+        const Tensor* b = nullptr;
+        if (!l || l->dim() != 2 || l->size(1) > 1024 || has_tangent(*l) || !PyUnicode_CheckExact(a[2]))
+            Py_RETURN_NONE;
+        RouteHow how;
+        const int64_t e = l->size(1);
+        int64_t top;
+        how.sigmoid = PyUnicode_CompareWithASCIIString(a[2], "sigmoid") == 0;
+        if (!how.sigmoid && PyUnicode_CompareWithASCIIString(a[2], "softmax") != 0) Py_RETURN_NONE;
+        if (a[3] != Py_None) {
+            b = on(plain(a[3], at::kFloat), *l);
+            if (!b || b->dim() != 1 || b->numel() != e || has_tangent(*b) || wants_grad(*b)) Py_RETURN_NONE;
+        }
+        if (!whole(a[1], 1, e < 64 ? e : 64, top) || !whole(a[4], 1, 64, how.groups) ||
+            !whole(a[5], 1, how.groups, how.top_groups) || e % how.groups != 0 ||
+            top > how.top_groups * (e / how.groups) || !number(a[7], how.scale))
+            Py_RETURN_NONE;
+        const int renormalize = PyObject_IsTrue(a[6]);
+        if (renormalize < 0) throw python_error();
+        how.renormalize = renormalize;
+        if (wants_grad(*l)) {
+            return wrapped(RouteFn::apply(*l, maybe(b), int64_t(how.sigmoid), int64_t(how.renormalize),
+                                          how.groups, how.top_groups, how.scale, top));
+        }
+        auto [ids, w] = run_route(*l, b, how, top);
+        return pair(ids, w);
+    });
+}
+
+// A tensor of heads [B, S, H, D] of any strides but a contiguous head dimension; otherwise
+// as plain, aligned to its elements
+const Tensor* heads_arg(PyObject* o) {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const Tensor& t = THPVariable_Unpack(o);
+    if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || type_of(t) < 0 ||
+        t.key_set().has_any(kWrapped) || !t.has_storage() || t.dim() != 4 || t.numel() == 0 ||
+        t.stride(3) != 1 || t.size(3) > 4096 ||
+        reinterpret_cast<uintptr_t>(t.data_ptr()) % t.element_size() != 0)
+        return nullptr;
+    return &t;
+}
+const Tensor* positions_arg(PyObject* o, const Tensor& q) {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const Tensor& t = THPVariable_Unpack(o);
+    if (!t.defined() || t.layout() != at::kStrided || t.device() != q.device() ||
+        t.key_set().has_any(kWrapped) || !t.has_storage() || t.numel() == 0 || wants_grad(t))
+        return nullptr;
+    const auto type = t.scalar_type();
+    if (type != at::kInt && type != at::kLong && type != at::kFloat) return nullptr;
+    const bool fits = t.dim() == 3 ? t.size(1) == q.size(0) && t.size(2) == q.size(1)
+                                   : t.dim() == 2 && t.size(1) == q.size(1);
+    return fits && t.size(0) >= 1 && t.size(0) <= 16 ? &t : nullptr;
+}
+// an empty result in x's layout where that is dense (rope._like)
+Tensor like_heads(const Tensor& x) {
+    Tensor out = at::empty_like(x);
+    return out.stride(3) == 1 ? out : empty(x.sizes(), x.scalar_type(), x);
+}
+struct Strides {
+    int64_t s[6];
+    Strides(const Tensor& x, const Tensor& out)
+        : s{x.stride(0), x.stride(1), x.stride(2), out.stride(0), out.stride(1), out.stride(2)} {}
+};
+// q and, where it is defined, k (of contiguous heads) into oq and ok
+int turn(const void* st, const Tensor& q, const Tensor& k, const Tensor& positions,
+         const Tensor& inv_freq, const Tensor& axis, bool inverse, bool split, Tensor& oq, Tensor& ok) {
+    const c10::DeviceGuard on_q(q.device());
+    oq = like_heads(q);
+    if (k.defined()) ok = like_heads(k);
+    const Strides qs(q, oq), ks(k.defined() ? k : q, k.defined() ? ok : oq);
+    const int d = int(positions.dim());
+    const int64_t ps[3] = {positions.stride(0), d == 2 ? 0 : positions.stride(1), positions.stride(d - 1)};
+    const auto type = positions.scalar_type();
+    return g_lib.rope_axes(st, q.data_ptr(), oq.data_ptr(), qs.s, q.size(2), ptr(k), ptr(ok),
+                           k.defined() ? ks.s : nullptr, k.defined() ? k.size(2) : 0, type_of(q),
+                           positions.data_ptr(), type == at::kInt ? 0 : type == at::kLong ? 1 : 2, ps,
+                           positions.size(0), static_cast<const double*>(inv_freq.data_ptr()),
+                           ints(&axis), axis.numel(), inverse, split, q.size(0), q.size(1), q.size(3));
+}
+
+struct TurnFn : torch::autograd::Function<TurnFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k,
+                                 const Tensor& positions, const Tensor& inv_freq, const Tensor& axis,
+                                 bool split) {
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({positions, inv_freq, axis});
+        ctx->saved_data["split"] = split;
+        const void* st = current_stream(q);
+        Tensor oq, ok;
+        call("rope.rotate_axes", [&] {
+            return turn(st, q, k ? *k : Tensor(), positions, inv_freq, axis, false, split, oq, ok);
+        });
+        if (k) return {oq, ok};
+        return {oq};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list in) {
+        return once(in, [&]() -> variable_list {
+            const variable_list saved = ctx->get_saved_variables();
+            const bool split = ctx->saved_data["split"].toBool();
+            // gradients of any strides, a sign that is a flag of the view applied
+            auto heads = [](const Tensor& t) {
+                const Tensor r = t.resolve_neg();
+                return r.stride(3) == 1 || r.size(3) == 1 ? r : r.contiguous();
+            };
+            Tensor dq, dk, oq, ok;
+            if (in[0].defined() && ctx->needs_input_grad(0)) dq = heads(in[0]);
+            if (in.size() > 1 && in[1].defined() && ctx->needs_input_grad(1)) dk = heads(in[1]);
+            if (dq.defined()) {
+                check(turn(stream_of(dq), dq, dk, saved[0], saved[1], saved[2], true, split, oq, ok),
+                      "rope.rotate_axes");
+            } else if (dk.defined()) {
+                check(turn(stream_of(dk), dk, Tensor(), saved[0], saved[1], saved[2], true, split, ok, oq),
+                      "rope.rotate_axes");
+            }
+            return {oq, ok, Tensor(), Tensor(), Tensor(), Tensor()};
+        });
+    }
+};
+
+// rotate_axes(q, k, positions, frequencies, split_half): rope.rotate_axes (the caller has
+// seen that frequencies is an AxisFrequencies)
+PyObject* host_rotate_axes(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, 5, [&]() -> PyObject* {
+        const Tensor *q = heads_arg(a[0]), *k = nullptr;
+        if (!q || !PyTuple_Check(a[3]) || PyTuple_GET_SIZE(a[3]) != 2) Py_RETURN_NONE;
+        if (a[1] != Py_None) {
+            k = on(heads_arg(a[1]), *q);
+            if (!k || k->scalar_type() != q->scalar_type() || k->size(0) != q->size(0) ||
+                k->size(1) != q->size(1) || k->size(3) != q->size(3))
+                Py_RETURN_NONE;
+        }
+        const Tensor* positions = positions_arg(a[2], *q);
+        const Tensor* inv_freq = on(plain(PyTuple_GET_ITEM(a[3], 0), at::kDouble), *q);
+        const Tensor* axis = on(plain(PyTuple_GET_ITEM(a[3], 1), at::kInt), *q);
+        if (!positions || !inv_freq || !axis || inv_freq->dim() != 1 || axis->dim() != 1 ||
+            axis->numel() != inv_freq->numel() || axis->numel() > 512 || 2 * axis->numel() > q->size(3) ||
+            q->size(2) + (k ? k->size(2) : 0) > 65536 || has_tangent(*q, k) || has_tangent(*positions))
+            Py_RETURN_NONE;
+        const int split = PyObject_IsTrue(a[4]);
+        if (split < 0) throw python_error();
+        variable_list out(2);
+        if (wants_grad(*q, k)) {
+            const variable_list r = TurnFn::apply(*q, maybe(k), *positions, *inv_freq, *axis, split != 0);
+            out[0] = r[0];
+            if (k) out[1] = r[1];
+        } else {
+            const void* st = current_stream(*q);
+            call("rope.rotate_axes", [&] {
+                return turn(st, *q, k ? *k : Tensor(), *positions, *inv_freq, *axis, false, split != 0,
+                            out[0], out[1]);
+            });
+        }
+        return wrapped(out);
+    });
+}
+
 // bind(addresses, raw_stream, packed): the library's entry points in Library's
 // order, the current-stream accessor and the packed-weight registry
 PyObject* host_bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
@@ -947,6 +1327,10 @@ PyMethodDef kMethods[] = {XPU_HOST("bind", host_bind),
                           XPU_HOST("moe_sort", host_moe_sort),
                           XPU_HOST("moe_dispatch", host_moe_dispatch),
                           XPU_HOST("moe_combine", host_moe_combine),
+                          XPU_HOST("rms_norm", host_rms_norm),
+                          XPU_HOST("rms_norm_int8", host_rms_norm_int8),
+                          XPU_HOST("moe_route", host_moe_route),
+                          XPU_HOST("rotate_axes", host_rotate_axes),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host",
                        "The int8 API's hot calls in native code (see host_ops.cpp).", -1, kMethods};

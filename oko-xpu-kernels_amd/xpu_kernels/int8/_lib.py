@@ -52,7 +52,10 @@ _HOST_ENTRIES = (
     "xpuint8_moe_dispatch_stream", "xpuint8_moe_combine_stream",
     "xpuint8_mxfp4_dx_workspace_size_of", "xpuint8_mxfp4_dx_stream",
     "xpuint8_moe_combine_grad_stream",
-    "xpuint8_mxfp4_dbias_workspace_size", "xpuint8_mxfp4_dbias_stream")
+    "xpuint8_mxfp4_dbias_workspace_size", "xpuint8_mxfp4_dbias_stream",
+    "xpuint8_rms_norm_stream", "xpuint8_rms_norm_int8_stream",
+    "xpuint8_rms_norm_grad_workspace_size", "xpuint8_rms_norm_grad_stream",
+    "xpuint8_rope_axes_stream", "xpuint8_moe_route_stream", "xpuint8_moe_route_grad_stream")
 
 
 def _candidate_paths():

@@ -124,6 +124,10 @@ def route(logits, top, *, scores="softmax", bias=None, groups=1, top_groups=1, r
     have id -1, which :func:`sort` gives to no expert, and weight 0.  A NaN logit, for the
     softmax +inf too, makes the token's weights NaN.  The gradient of the weights reaches
     the logits."""
+    if L.HOST is not None:
+        r = L.HOST.moe_route(logits, top, scores, bias, groups, top_groups, renormalize, scale)
+        if r is not None:
+            return r
     _check_float(logits, "logits")
     if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_EXPERTS:
         raise ValueError(f"logits must be [T, E] with 1..{MAX_EXPERTS} experts, got "

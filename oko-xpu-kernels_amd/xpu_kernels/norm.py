@@ -122,6 +122,10 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None):
     type) of ``h = x + residual``, rounded to the type, and then ``(y, h)``.  Gradients
     reach x, weight and residual, through y and h; the weight's is summed in fp32 in a
     fixed order and rounded once."""
+    if L.HOST is not None:
+        r = L.HOST.rms_norm(x, weight, eps, residual)
+        if r is not None:
+            return r
     _check(x, weight, eps, residual)
     eps = float(eps)
     if _wants_grad(x, weight, residual):
@@ -142,6 +146,10 @@ def rms_norm_int8(x, weight=None, eps=1e-6, residual=None, rotate=True):
     is not rounded between, and a row with an infinity or NaN has a NaN scale.
     Whole numbers have no gradient: inputs that need one are refused outside of
     ``torch.no_grad()``."""
+    if L.HOST is not None:
+        r = L.HOST.rms_norm_int8(x, weight, eps, residual, rotate)
+        if r is not None:
+            return r
     _check(x, weight, eps, residual)
     k = x.shape[-1]
     if rotate and k % GROUP:

@@ -201,6 +201,10 @@ def rotate_axes(q, k, positions, frequencies, *, split_half=True):
     Pairs are the elements j and j + P with ``split_half``, else 2j and 2j + 1; those past
     2 P stay as they are.  Strides are free but for a contiguous head dimension (others are
     copied): a [B, H, S, D] tensor goes in as ``x.transpose(1, 2)``."""
+    if L.HOST is not None and type(frequencies) is AxisFrequencies:
+        r = L.HOST.rotate_axes(q, k, positions, frequencies, split_half)
+        if r is not None:
+            return r
     _check_float(q, "q")
     if q.dim() != 4 or 0 in q.shape[2:]:
         raise ValueError(f"q must be [B, S, H, D], got {tuple(q.shape)}")
