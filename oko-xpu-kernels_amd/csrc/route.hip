@@ -9,8 +9,8 @@
 // weight 0.  A row with a NaN logit (for softmax +inf too) has NaN weights; its experts are
 // chosen by the logits, NaNs last.
 //
-// Which experts are chosen hangs on keys that may be next to each other, so keys are 64
-// bits: a wave a token, lane l holding the experts l, l + 64, ..
+// Which experts are chosen hangs on keys that may be next to each other, so the ones that
+// matter are compared in 64 bits.
 #include "block_kernels.hpp"
 #include "mx_kernels.hpp"
 #include "rows.hpp"
@@ -68,113 +68,516 @@ __device__ __forceinline__ void wave_best(double& key, int& e) {
 constexpr double kNone = -__builtin_huge_val();      // not to be chosen
 constexpr double kLowest = -1.7976931348623157e308;
 
+// A token by a whole wave, lane l holding the experts l, l + 64, ..; keys are 64 bits.
 template <int T, int V>
-__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
+__device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t) {
     const int lane = threadIdx.x & 63;
-    for (int64_t t = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); t < a.T; t += int64_t(gridDim.x) * 4) {
-        float l[V], most = -INFINITY;
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int e = 64 * i + lane;
-            l[i] = e < a.E ? logit_at<T>(a.logits, t, a.ld, e) : -INFINITY;
-            bad |= __builtin_isnan(l[i]) || (!a.how.sigmoid && l[i] == INFINITY);
-            most = fmaxf(most, l[i]);
-        }
-        const bool spoilt = __builtin_amdgcn_ballot_w64(bad) != 0;
-        most = wave_most(most);
-        double key[V], sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const bool out = l[i] == -INFINITY;
-            key[i] = out ? 0.0 : a.how.sigmoid ? 1.0 / (1.0 + exp(-double(l[i])))
-                                               : exp(double(l[i]) - double(most));
-            sum += key[i];
-        }
-        if (!a.how.sigmoid) sum = wave_total(sum);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int e = 64 * i + lane;
-            if (!a.how.sigmoid) key[i] /= sum;
-            if (a.bias && e < a.E) key[i] += double(a.bias[e]);
-            if (!a.bias && a.how.groups == 1) key[i] = l[i];       // scores rise with logits
-            if (spoilt) key[i] = l[i];
-            if (__builtin_isnan(key[i])) key[i] = kLowest;
-            if (l[i] == -INFINITY) key[i] = kNone;
-        }
-        if (a.how.groups > 1) {
-            const int n = a.E / a.how.groups;
-            double value = kNone;                     // lane g: of group g
-            for (int g = 0; g < a.how.groups; ++g) {
-                double two = 0.0;
-                int first = -1;
-                for (int k = 0; k < 2; ++k) {
-                    double best = kNone;
-                    int at = a.E;
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const int e = 64 * i + lane;
-                        if (e >= g * n && e < (g + 1) * n && e != first && key[i] > best) {
-                            best = key[i];
-                            at = e;
-                        }
-                    }
-                    wave_best(best, at);
-                    first = at;
-                    if (k == 0) two = best;
-                    else if (best != kNone) two += best;
-                }
-                if (lane == g) value = two;
-            }
-            int rank = 0;
-            for (int g = 0; g < a.how.groups; ++g) {
-                const double other = __shfl(value, g);
-                rank += other > value || (other == value && g < lane);
-            }
-            const uint64_t kept =
-                __builtin_amdgcn_ballot_w64(lane < a.how.groups && rank < a.how.top_groups);
+            float l[V], most = -INFINITY;
+            bool bad = false;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int e = 64 * i + lane;
-                if (e < a.E && !((kept >> (e / n)) & 1)) key[i] = kNone;
+                l[i] = e < a.E ? logit_at<T>(a.logits, t, a.ld, e) : -INFINITY;
+                bad |= __builtin_isnan(l[i]) || (!a.how.sigmoid && l[i] == INFINITY);
+                most = fmaxf(most, l[i]);
+            }
+            const bool spoilt = __builtin_amdgcn_ballot_w64(bad) != 0;
+            most = wave_most(most);
+            double key[V], sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const bool out = l[i] == -INFINITY;
+                key[i] = out ? 0.0 : a.how.sigmoid ? 1.0 / (1.0 + exp(-double(l[i])))
+                                                   : exp(double(l[i]) - double(most));
+                sum += key[i];
+            }
+            if (!a.how.sigmoid) sum = wave_total(sum);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int e = 64 * i + lane;
+                if (!a.how.sigmoid) key[i] /= sum;
+                if (a.bias && e < a.E) key[i] += double(a.bias[e]);
+                if (!a.bias && a.how.groups == 1) key[i] = l[i];       // scores rise with logits
+                if (spoilt) key[i] = l[i];
+                if (__builtin_isnan(key[i])) key[i] = kLowest;
+                if (l[i] == -INFINITY) key[i] = kNone;
+            }
+            if (a.how.groups > 1) {
+                const int n = a.E / a.how.groups;
+                double value = kNone;                     // lane g: of group g
+                for (int g = 0; g < a.how.groups; ++g) {
+                    double two = 0.0;
+                    int first = -1;
+                    for (int k = 0; k < 2; ++k) {
+                        double best = kNone;
+                        int at = a.E;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            const int e = 64 * i + lane;
+                            if (e >= g * n && e < (g + 1) * n && e != first && key[i] > best) {
+                                best = key[i];
+                                at = e;
+                            }
+                        }
+                        wave_best(best, at);
+                        first = at;
+                        if (k == 0) two = best;
+                        else if (best != kNone) two += best;
+                    }
+                    if (lane == g) value = two;
+                }
+                int rank = 0;
+                for (int g = 0; g < a.how.groups; ++g) {
+                    const double other = __shfl(value, g);
+                    rank += other > value || (other == value && g < lane);
+                }
+                const uint64_t kept =
+                    __builtin_amdgcn_ballot_w64(lane < a.how.groups && rank < a.how.top_groups);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const int e = 64 * i + lane;
+                    if (e < a.E && !((kept >> (e / n)) & 1)) key[i] = kNone;
+                }
+            }
+            int id = -1;                                  // lane j: of slot j
+            for (int j = 0; j < a.top; ++j) {
+                double best = kNone;
+                int at = a.E;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (key[i] > best) {
+                        best = key[i];
+                        at = 64 * i + lane;
+                    }
+                wave_best(best, at);
+                if (best == kNone) break;
+                if (lane == j) id = at;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (64 * i + lane == at) key[i] = kNone;
+            }
+            const float mine = id >= 0 ? logit_at<T>(a.logits, t, a.ld, id) : -INFINITY;
+            // divided by the sum, the scores may carry any common factor: the one that brings
+            // the largest near 1
+            double s = 0.0;
+            if (a.how.sigmoid) {
+                const double shift = a.how.renormalize ? fmin(0.0, double(wave_most(mine))) : 0.0;
+                if (id >= 0) s = mine >= 0.f ? 1.0 / (1.0 + exp(-double(mine)))
+                                             : exp(double(mine) - shift) / (1.0 + exp(double(mine)));
+            } else {
+                const double ref = a.how.renormalize ? double(wave_most(mine)) : double(most);
+                if (id >= 0) s = exp(double(mine) - ref) / (a.how.renormalize ? 1.0 : sum);
+            }
+            const double total = a.how.renormalize ? wave_total(s) : 1.0;
+            float w = id >= 0 ? float(double(a.how.scale) * s / total) : 0.f;
+            if (spoilt) w = NAN;
+            if (lane < a.top) {
+                a.ids[t * a.top + lane] = id;
+                a.weights[t * a.top + lane] = w;
+            }
+}
+
+template <int T, int V>
+__global__ __launch_bounds__(256) void route_exact_kernel(RouteArgs a) {
+    for (int64_t t = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); t < a.T; t += int64_t(gridDim.x) * 4)
+        route_token<T, V>(a, t);
+}
+
+// ------------------------------------------------------------ several tokens a wave
+// A token has L lanes of V experts, 64 / L tokens a wave.  Keys are made in fp32 first, to
+// a known error; of each the 32 bits that order like it, with the expert's place in the low
+// ones, are sorted in every lane and merged across the lanes down to the token's highest 16,
+// all in integer minima and maxima.  These 16 candidates, one a lane, then get their keys in
+// 64 bits, and each counts the ones above its own: its slot.  The choice is sure when the
+// last chosen key is above anything that the 17th could be; a token for which that does not
+// hold (more keys than 16 within 2^-13 to 2^-15 of the last one chosen, a NaN, scores that
+// underflow) goes through route_token.  Groups whose fp32 values are too near, and softmax
+// keys nearer than the sum's error, are looked at again in 64 bits.
+constexpr int kCandidates = 16;
+constexpr uint32_t kNothing = 0x00800000u;           // ordered(-inf) and the bits of a place are below
+
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = dppu<CTRL>(uint32_t(b)), hi = dppu<CTRL>(uint32_t(b >> 32));
+    return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+// x of a lane on the other side of D, where the lanes of each side hold the same: lane ^ 1,
+// ^ 2, ^ 7, ^ 15 by DPP, then ^ 16 and ^ 32
+template <int D>
+__device__ __forceinline__ uint32_t other_side(uint32_t x) {
+    if constexpr (D == 1) return dppu<kDppXor1>(x);
+    else if constexpr (D == 2) return dppu<kDppXor2>(x);
+    else if constexpr (D == 4) return dppu<kDppXor7>(x);
+    else if constexpr (D == 8) return dppu<kDppXor15>(x);
+    else return uint32_t(__shfl_xor(int(x), D));
+}
+
+// a falls along i: compare and exchange
+__device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b) {
+    const uint32_t hi = max(a, b), lo = min(a, b);
+    a = hi;
+    b = lo;
+}
+// a bitonic sequence sorted
+template <int N, int AT, int M>
+__device__ __forceinline__ void sort_bitonic(uint32_t (&a)[M]) {
+    if constexpr (N > 1) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) exchange(a[AT + i], a[AT + i + N / 2]);
+        sort_bitonic<N / 2, AT>(a);
+        sort_bitonic<N / 2, AT + N / 2>(a);
+    }
+}
+// the odd-even merge of two sorted halves, elements STEP apart, and the sort by it
+template <int N, int AT, int STEP, int M>
+__device__ __forceinline__ void merge_odd_even(uint32_t (&a)[M]) {
+    if constexpr (N == 2) {
+        exchange(a[AT], a[AT + STEP]);
+    } else {
+        merge_odd_even<N / 2, AT, 2 * STEP>(a);
+        merge_odd_even<N / 2, AT + STEP, 2 * STEP>(a);
+#pragma unroll
+        for (int i = 1; i + 1 < N; i += 2) exchange(a[AT + i * STEP], a[AT + (i + 1) * STEP]);
+    }
+}
+template <int N, int AT, int M>
+__device__ __forceinline__ void sort_odd_even(uint32_t (&a)[M]) {
+    if constexpr (N > 1) {
+        sort_odd_even<N / 2, AT>(a);
+        sort_odd_even<N / 2, AT + N / 2>(a);
+        merge_odd_even<N, AT, 1>(a);
+    }
+}
+// The sorted N values of this side of D and of the other, of which the 16 highest: in both.
+template <int N, int D>
+__device__ __forceinline__ void merge_lanes(uint32_t (&a)[kCandidates]) {
+    uint32_t b[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) b[i] = other_side<D>(a[i]);
+    if constexpr (N < kCandidates) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t u = a[i], v = b[N - 1 - i];
+            a[i] = max(u, v);
+            a[N + i] = min(u, v);
+        }
+        sort_bitonic<N, 0>(a);
+        sort_bitonic<N, N>(a);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) a[i] = max(a[i], b[N - 1 - i]);
+        sort_bitonic<N, 0>(a);
+    }
+}
+template <int L, int N, int D = 1>
+__device__ __forceinline__ void merge_token(uint32_t (&a)[kCandidates]) {
+    if constexpr (D < L) {
+        merge_lanes<N, D>(a);
+        merge_token<L, (2 * N < kCandidates ? 2 * N : kCandidates), 2 * D>(a);
+    }
+}
+
+// the maximum, and the sum, over the L lanes of a token, in each
+template <int L>
+__device__ __forceinline__ float token_max(float x) { return lanes_max<L>(x); }
+template <int L>
+__device__ __forceinline__ float token_sum(float x) { return lanes_sum<L>(x); }
+
+// bits that order like the float (no NaN), and back
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// the other groups of 2^bits lanes in a row of 16 whose range of values is above this one's,
+// and those that are not below it (groups that are not there are -inf)
+template <int K>
+__device__ __forceinline__ void count_groups(int bits, float low, float high, int& above, int& maybe) {
+    if constexpr (K < 16) {
+        if ((K & ((1 << bits) - 1)) == 0) {
+            const float ol = dpp<0x120 + K>(low), oh = dpp<0x120 + K>(high);
+            above += ol > high;
+            maybe += !(oh < low);
+        }
+        count_groups<K + 1>(bits, low, high, above, maybe);
+    }
+}
+// Whether a key of a row of 16 is above the next one by more than tol, or the same at a lower
+// expert (`place` falls along the experts); what is not to be chosen comes last in any order.
+__device__ __forceinline__ bool in_order(double key, uint32_t place, int r, double tol) {
+    const double next = dpp64<0x101>(key);            // row_shl: lane r gets r + 1's
+    const uint32_t next_place = dppu<0x101>(place);
+    return r == 15 || next == kNone || key > next + tol || (key == next && place > next_place);
+}
+template <int K>
+__device__ __forceinline__ void count_above(double key, uint32_t place, int& rank) {
+    if constexpr (K < 16) {
+        const double other = dpp64<0x120 + K>(key);   // row_ror, as far as all have been seen
+        rank += other > key || (other == key && dppu<0x120 + K>(place) > place);
+        count_above<K + 1>(key, place, rank);
+    }
+}
+__device__ __forceinline__ double row_sum(double x) {
+    x += dpp64<kDppXor1>(x);
+    x += dpp64<kDppXor2>(x);
+    x += dpp64<kDppXor7>(x);
+    x += dpp64<kDppXor15>(x);
+    return x;
+}
+template <int L>
+__device__ __forceinline__ double token_total(double x) {
+    x = row_sum(x);
+#pragma unroll
+    for (int d = 16; d < L; d *= 2) x += __shfl_xor(x, d);
+    return x;
+}
+template <int L>
+__device__ __forceinline__ bool token_any(bool x) {
+    const uint64_t m = __builtin_amdgcn_ballot_w64(x);
+    if constexpr (L == 64) return m != 0;
+    else return (m >> (threadIdx.x & (64 - L)) & ((uint64_t(1) << L) - 1)) != 0;
+}
+
+// how the experts of a token lie: group g in the 2^bits lanes from g * 2^bits on, `each` a lane
+struct Spread {
+    int bits, each;
+};
+
+// V consecutive logits from `first` on (-inf past `count`), in one load if they are whole
+template <int T, int V>
+__device__ __forceinline__ void logits_load(const void* logits, int64_t at, int count, float (&l)[V]) {
+    constexpr int W = V * kElem<T> / 4;
+    struct __attribute__((packed, aligned(kElem<T>))) Loose { uint32_t w[W]; };
+    const char* p = static_cast<const char*>(logits) + at * kElem<T>;
+    if (count == V) {
+        const Loose u = *reinterpret_cast<const Loose*>(p);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if constexpr (T == kF32) {
+                l[i] = __uint_as_float(u.w[i]);
+            } else if constexpr (T == kBf16) {
+                l[2 * i] = bf16lo(u.w[i]);
+                l[2 * i + 1] = bf16hi(u.w[i]);
+            } else {
+                const xpu_v2h h = __builtin_bit_cast(xpu_v2h, u.w[i]);
+                l[2 * i] = float(h[0]);
+                l[2 * i + 1] = float(h[1]);
             }
         }
-        int id = -1;                                  // lane j: of slot j
-        for (int j = 0; j < a.top; ++j) {
-            double best = kNone;
-            int at = a.E;
+        return;
+    }
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (key[i] > best) {
-                    best = key[i];
-                    at = 64 * i + lane;
-                }
-            wave_best(best, at);
-            if (best == kNone) break;
-            if (lane == j) id = at;
+    for (int i = 0; i < V; ++i) l[i] = i < count ? logit_at<T>(p, 0, 0, i) : -INFINITY;
+}
+
+template <int T, int L, int V, int THREADS>
+__global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, int64_t first_token) {
+    constexpr int PER = 64 / L, WAVES = THREADS / 64;
+    constexpr uint32_t kPlace = L * V - 1;            // the bits of an expert's place
+    const int lane = threadIdx.x & 63, in = lane & (L - 1), r = lane & 15;
+    const int n = a.E / a.how.groups;
+    const int group = in >> sp.bits, part = in & ((1 << sp.bits) - 1);
+    const int first = group * n + part * sp.each;     // this lane's experts
+    const int count = group < a.how.groups ? max(0, min(sp.each, n - part * sp.each)) : 0;
+    const bool plain = !a.bias && a.how.groups == 1;  // keys are the logits
+    const int64_t t0 = first_token + (int64_t(blockIdx.x) * WAVES + (threadIdx.x >> 6)) * PER;
+    if (t0 >= a.T) return;
+    const int64_t t = min(t0 + lane / L, a.T - 1);
+    float l[V], b[V];
+    logits_load<T>(a.logits, t * a.ld + first, count, l);
+    if (a.bias) logits_load<kF32>(a.bias, first, count, b);
+    float most = -INFINITY, all = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (64 * i + lane == at) key[i] = kNone;
+    for (int i = 0; i < V; ++i) {
+        all += l[i];
+        most = fmaxf(most, l[i]);
+    }
+    // a NaN or infinity anywhere (or a sum that overflows): looked for one by one
+    bool bad = false;
+    const bool odd = __builtin_amdgcn_ballot_w64(!(fabsf(all) < INFINITY)) != 0;
+    if (odd) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) bad |= __builtin_isnan(l[i]) || (!a.how.sigmoid && l[i] == INFINITY);
+    }
+    // fp32 scores.  A sigmoid s: its exponential off by 2 units (2^-24) and |l| of its
+    // argument's rounding, of which s (1 - s) < 1/4 (times |l| < 1/4) counts, the sum's and
+    // the reciprocal's 3: under 2^-21.  A softmax's: 2 and the argument's |x|, where
+    // |x| e^-|x| < 0.4, the sum's 22 additions of such terms and the reciprocal: under 2^-19
+    // of the highest score.
+    float key[V], sum = 1.f;
+    constexpr float kLog2e = 1.4426950408889634f;
+    if (!a.how.sigmoid) {
+        most = token_max<L>(most);
+        const float ref = most == -INFINITY ? 0.f : most;
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            key[i] = __builtin_amdgcn_exp2f((l[i] - ref) * kLog2e);
+            sum += key[i];
         }
-        const float mine = id >= 0 ? logit_at<T>(a.logits, t, a.ld, id) : -INFINITY;
-        // divided by the sum, the scores may carry any common factor: the one that brings
-        // the largest near 1
-        double s = 0.0;
+        sum = token_sum<L>(sum);
+    }
+    if (plain) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = l[i];
+    } else {
+        const float share = __builtin_amdgcn_rcpf(sum);
         if (a.how.sigmoid) {
-            const double shift = a.how.renormalize ? fmin(0.0, double(wave_most(mine))) : 0.0;
-            if (id >= 0) s = mine >= 0.f ? 1.0 / (1.0 + exp(-double(mine)))
-                                         : exp(double(mine) - shift) / (1.0 + exp(double(mine)));
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                key[i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-l[i] * kLog2e));
         } else {
-            const double ref = a.how.renormalize ? double(wave_most(mine)) : double(most);
-            if (id >= 0) s = exp(double(mine) - ref) / (a.how.renormalize ? 1.0 : sum);
+#pragma unroll
+            for (int i = 0; i < V; ++i) key[i] *= share;
         }
-        const double total = a.how.renormalize ? wave_total(s) : 1.0;
-        float w = id >= 0 ? float(double(a.how.scale) * s / total) : 0.f;
-        if (spoilt) w = NAN;
-        if (lane < a.top) {
-            a.ids[t * a.top + lane] = id;
-            a.weights[t * a.top + lane] = w;
+        float check = 0.f;
+        if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                key[i] += b[i];
+                check += key[i];
+            }
         }
+        if (odd || __builtin_amdgcn_ballot_w64(!(fabsf(check) < INFINITY))) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (l[i] == -INFINITY) key[i] = -INFINITY;
+                bad |= __builtin_isnan(key[i]);
+            }
+        }
+    }
+    const float off = plain ? 0.f : a.how.sigmoid ? 0x1p-21f : 0x1p-19f * __builtin_amdgcn_rcpf(sum);
+    double sum64 = sum;                           // the softmax's, exact once asked for
+    bool sum_exact = false;
+    auto exact_sum = [&] {
+        double u = 0.0;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (l[i] != -INFINITY) u += exp(double(l[i]) - double(most));
+        sum64 = token_total<L>(u);
+        sum_exact = true;
+    };
+    auto score64 = [&](float x) {
+        return a.how.sigmoid ? 1.0 / (1.0 + exp(-double(x))) : exp(double(x) - double(most)) / sum64;
+    };
+    bool dropped = false;
+    if (a.how.groups > 1) {
+        float one = -INFINITY, two = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            two = fmaxf(two, fminf(one, key[i]));
+            one = fmaxf(one, key[i]);
+        }
+        for (int d = 1; d < 1 << sp.bits; d *= 2) {
+            const float o = __shfl_xor(one, d), w = __shfl_xor(two, d);
+            two = fmaxf(fmaxf(two, w), fminf(one, o));
+            one = fmaxf(one, o);
+        }
+        const float value = two == -INFINITY ? one : one + two;
+        const float e = one == -INFINITY ? 0.f : 2.f * off + 0x1p-22f * (fabsf(one) + fabsf(value));
+        int above = 0, maybe = 0;                 // groups surely above, and perhaps
+        const float low = value - e, high = value + e;
+        if constexpr (L == 16) {
+            count_groups<1>(sp.bits, low, high, above, maybe);
+        } else {
+            for (int g = 0; g < a.how.groups; ++g) {
+                const int from = (lane & ~(L - 1)) + (g << sp.bits);
+                const float ol = __shfl(low, from), oh = __shfl(high, from);
+                if (g == group) continue;
+                above += ol > high;
+                maybe += !(oh < low);
+            }
+        }
+        // (a group with nothing to choose from is as good in as out)
+        dropped = one == -INFINITY || above >= a.how.top_groups;
+        const bool open = group < a.how.groups && !dropped && maybe >= a.how.top_groups;
+        if (__builtin_amdgcn_ballot_w64(open)) {  // values too near: in 64 bits
+            if (!a.how.sigmoid) exact_sum();
+            double first64 = kNone, second64 = kNone;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (key[i] == -INFINITY) continue;
+                const double k = score64(l[i]) + (a.bias ? double(b[i]) : 0.0);
+                second64 = fmax(second64, fmin(first64, k));
+                first64 = fmax(first64, k);
+            }
+            for (int d = 1; d < 1 << sp.bits; d *= 2) {
+                const double o = __shfl_xor(first64, d), w = __shfl_xor(second64, d);
+                second64 = fmax(fmax(second64, w), fmin(first64, o));
+                first64 = fmax(first64, o);
+            }
+            const double value64 = second64 == kNone ? first64 : first64 + second64;
+            above = 0;
+            for (int g = 0; g < a.how.groups; ++g) {
+                const double o = __shfl(value64, (lane & ~(L - 1)) + (g << sp.bits));
+                above += o > value64 || (o == value64 && g < group);
+            }
+            dropped = above >= a.how.top_groups;
+        }
+    }
+    // (-inf orders below kNothing, and so does what is dropped)
+    uint32_t c[kCandidates];
+    const uint32_t keep = dropped ? 0u : ~kPlace;
+#pragma unroll
+    for (int i = 0; i < V; ++i) c[i] = (ordered(key[i]) & keep) | (kPlace - uint32_t(in * V + i));
+    sort_odd_even<V, 0>(c);
+    merge_token<L, V>(c);
+    uint32_t mine = c[0];
+#pragma unroll
+    for (int i = 1; i < kCandidates; ++i) mine = r == i ? c[i] : mine;
+    // this lane's candidate, in 64 bits
+    const bool is = mine >= kNothing;
+    const int place = int(kPlace - (mine & kPlace)), at = place / V;
+    const int e = (at >> sp.bits) * n + (at & ((1 << sp.bits) - 1)) * sp.each + place % V;
+    const float x = is ? logit_at<T>(a.logits, t, a.ld, e) : -INFINITY;
+    double s = 0.0, k = kNone, tol = 0.0;
+    auto look = [&] {
+        if (!is) return;
+        s = plain && a.how.renormalize && !a.how.sigmoid ? exp(double(x) - double(most)) : score64(x);
+        k = plain ? double(x) : s + (a.bias ? double(a.bias[e]) : 0.0);
+        // keys nearer than the fp32 sum's error are looked at again with the exact one
+        tol = plain || a.how.sigmoid || sum_exact ? 0.0 : 0x1p-17 * s;
+    };
+    look();
+    // the candidates lie in the order of their fp32 keys' upper bits, mostly the right one:
+    // otherwise each counts those above it, with the exact sum
+    int rank = r;
+    if (__builtin_amdgcn_ballot_w64(!in_order(k, mine & kPlace, r, tol))) {
+        if (!plain && !a.how.sigmoid && !sum_exact) {
+            exact_sum();
+            look();
+        }
+        rank = 0;
+        count_above<1>(k, mine & kPlace, rank);
+    }
+    const bool chosen = is && rank < a.top;
+    if (c[kCandidates - 1] >= kNothing) {             // there may be a 17th
+        const uint32_t last = c[kCandidates - 1];
+        const float highest = unordered(last | kPlace);
+        if (plain && T != kF32) {
+            // 16-bit logits are whole in the upper bits: equal ones are in order
+        } else if (plain) {
+            bad |= chosen && !(k > double(highest));
+        } else {
+            bad |= chosen && !(k > double(highest) + 2.0 * off + 0x1p-22 * fabs(double(highest)));
+        }
+    }
+    const double total = a.how.renormalize ? row_sum(chosen ? s : 0.0) : 1.0;
+    bad |= chosen && !(total > 1e-200);
+    const bool again = token_any<L>(bad);
+    if (!again && in < 16 && rank < a.top && t0 + lane / L < a.T) {
+        a.ids[t * a.top + rank] = is ? e : -1;
+        a.weights[t * a.top + rank] = is ? float(double(a.how.scale) * s / total) : 0.f;
+    }
+    uint64_t left = __builtin_amdgcn_ballot_w64(again && in == 0 && t0 + lane / L < a.T);
+    while (left) {
+        const int who = __builtin_ctzll(left);
+        left &= left - 1;
+        route_token<T, (L * V + 63) / 64>(a, t0 + who / L);
     }
 }
 
@@ -290,10 +693,44 @@ unsigned token_blocks(int64_t T) {
 hipError_t moe_route(hipStream_t st, const void* logits, int type, int64_t ld, const float* bias,
                      const RouteHow& how, int* ids, float* weights, int64_t T, int E, int top) {
     const RouteArgs a{logits, bias, ids, weights, ld, T, E, top, how};
-    by_experts(type, E, [&](auto t, auto v) {
-        hipLaunchKernelGGL((route_kernel<decltype(t)::value, decltype(v)::value>),
-                           dim3(token_blocks(T)), dim3(256), 0, st, a);
-    });
+    int padded = 1;                                   // groups, each with as many lanes
+    while (padded < how.groups) padded *= 2;
+    const int n = E / how.groups;
+    bool done = false;
+    auto go = [&](auto t, auto lanes, auto v) {
+        constexpr int L = decltype(lanes)::value, V = decltype(v)::value, TY = decltype(t)::value;
+        if (done || padded > L || top > kCandidates) return;
+        int bits = 0;
+        while (padded << (bits + 1) <= L) ++bits;
+        const Spread sp{bits, (n + (1 << bits) - 1) >> bits};
+        if (sp.each > V) return;
+        done = true;
+        // small calls in blocks of one wave, which spread over more of the chip
+        const int64_t per = 64 / L;
+        if (T >= 2048 * per)
+            in_launches(T, kMaxBlocks * 4 * per, [&](int64_t at, int64_t m) {
+                hipLaunchKernelGGL((route_kernel<TY, L, V, 256>), dim3(unsigned((m + 4 * per - 1) / (4 * per))),
+                                   dim3(256), 0, st, a, sp, at);
+            });
+        else
+            hipLaunchKernelGGL((route_kernel<TY, L, V, 64>), dim3(unsigned((T + per - 1) / per)), dim3(64),
+                               0, st, a, sp, int64_t(0));
+    };
+    auto by = [&](auto t) {
+        go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+        go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{});
+        go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 16>{});
+        go(t, std::integral_constant<int, 32>{}, std::integral_constant<int, 16>{});
+        go(t, std::integral_constant<int, 64>{}, std::integral_constant<int, 16>{});
+    };
+    if (type == kBf16) by(std::integral_constant<int, kBf16>{});
+    else if (type == kF16) by(std::integral_constant<int, kF16>{});
+    else by(std::integral_constant<int, kF32>{});
+    if (!done)
+        by_experts(type, E, [&](auto t, auto v) {
+            hipLaunchKernelGGL((route_exact_kernel<decltype(t)::value, decltype(v)::value>),
+                               dim3(token_blocks(T)), dim3(256), 0, st, a);
+        });
     return hipGetLastError();
 }
 
