@@ -669,6 +669,137 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
     }
 }
 
+// 4 consecutive elements of a row of E from e on, whole or element by element
+template <int T>
+struct __attribute__((packed, aligned(kElem<T>))) Loose4 {
+    uint32_t w[kElem<T>];
+};
+template <int T>
+__device__ __forceinline__ void four_load(const void* row, int e, int E, float (&v)[4]) {
+    const char* p = static_cast<const char*>(row) + int64_t(e) * kElem<T>;
+    if (e + 4 <= E) {
+        const Loose4<T> u = *reinterpret_cast<const Loose4<T>*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (T == kF32) v[i] = __uint_as_float(u.w[i]);
+            else if constexpr (T == kBf16) v[i] = i & 1 ? bf16hi(u.w[i / 2]) : bf16lo(u.w[i / 2]);
+            else v[i] = float(__builtin_bit_cast(xpu_v2h, u.w[i / 2])[i & 1]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = e + i < E ? logit_at<T>(p, 0, 0, i) : -INFINITY;
+}
+template <int T>
+__device__ __forceinline__ void four_store(void* row, int e, int E, const float (&v)[4]) {
+    char* p = static_cast<char*>(row) + int64_t(e) * kElem<T>;
+    if (e + 4 <= E) {
+        Loose4<T> u;
+#pragma unroll
+        for (int i = 0; i < kElem<T>; ++i) {
+            if constexpr (T == kF32) u.w[i] = __float_as_uint(v[i]);
+            else u.w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+        }
+        *reinterpret_cast<Loose4<T>*>(p) = u;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (e + i >= E) continue;
+        if constexpr (T == kF32) reinterpret_cast<float*>(p)[i] = v[i];
+        else reinterpret_cast<uint16_t*>(p)[i] = uint16_t(pack2<T>(v[i], 0.f));
+    }
+}
+
+// The same with several tokens a wave, up to 16 slots each: slots in the 16 lanes of a row,
+// a token's experts in fours over its L lanes.  The whole row of logits is read, beside the
+// ids, not after them (its chosen few lie in as many lines); they are looked up in LDS, and
+// gradients go through it to where they are written.
+template <int T, int L, int V>
+__global__ __launch_bounds__(256) void route_grad_rows_kernel(RouteGradArgs a, int64_t first_token) {
+    constexpr int PER = 64 / L, F = V / 4;
+    __shared__ __align__(16) float lds[4][64 * V];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, in = lane & (L - 1), r = lane & 15;
+    const int64_t t0 = first_token + (int64_t(blockIdx.x) * 4 + wave) * PER;
+    if (t0 >= a.T) return;
+    const int64_t t = min(t0 + lane / L, a.T - 1);
+    const bool dense = !a.how.sigmoid && !a.how.renormalize;
+    float* row = lds[wave] + (lane & ~(L - 1)) * V;   // the token's
+    int id = r < a.top ? a.ids[t * a.top + r] : -1;
+    const float weight = r < a.top ? a.dweights[t * a.top + r] : 0.f;
+    const char* from = static_cast<const char*>(a.logits) + t * a.ld * kElem<T>;
+    float out[F][4], d;                               // d: the chosen expert's
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+        four_load<T>(from, 4 * (i * L + in), a.E, out[i]);
+        *reinterpret_cast<float4*>(row + 4 * (i * L + in)) =
+            make_float4(out[i][0], out[i][1], out[i][2], out[i][3]);
+    }
+    if (id >= a.E) id = -1;
+    const float g = id >= 0 ? weight : 0.f;
+    // (a wave's LDS accesses are in order)
+    __builtin_amdgcn_wave_barrier();
+    const float mine = id >= 0 ? row[id] : -INFINITY;
+    __builtin_amdgcn_wave_barrier();
+    if (dense) {
+        float most = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) most = fmaxf(most, out[i / 4][i % 4]);
+        most = token_max<L>(most);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float& p = out[i / 4][i % 4];
+            p = p == -INFINITY ? 0.f : expf(p - most);
+            sum += p;
+        }
+        sum = token_sum<L>(sum);
+        if (sum == 0.f) sum = 1.f;                    // (every expert masked: all zeros)
+        const float s = id >= 0 ? expf(mine - most) / sum : 0.f;
+        const float along = lanes_sum<16>(g * s);
+        d = a.how.scale * s * (g - along);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float& p = out[i / 4][i % 4];
+            p = -a.how.scale * (p / sum) * along;
+        }
+    } else {
+        const float highest = lanes_max<16>(mine);
+        float s, rest = 1.f;
+        if (a.how.sigmoid) {
+            const float shift = a.how.renormalize ? fminf(0.f, highest) : 0.f;
+            const float up = expf(mine);
+            s = id < 0 ? 0.f : mine >= 0.f ? 1.f / (1.f + expf(-mine)) : expf(mine - shift) / (1.f + up);
+            rest = 1.f / (1.f + up);                  // 1 - sigmoid
+        } else {
+            s = id >= 0 ? expf(mine - highest) : 0.f;
+        }
+        if (a.how.renormalize) {
+            const float w = s / lanes_sum<16>(s);
+            const float along = lanes_sum<16>(id >= 0 ? g * w : 0.f);
+            d = a.how.scale * w * rest * (g - along);
+        } else {
+            d = a.how.scale * s * rest * g;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i / 4][i % 4] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+        *reinterpret_cast<float4*>(row + 4 * (i * L + in)) =
+            make_float4(out[i][0], out[i][1], out[i][2], out[i][3]);
+    __builtin_amdgcn_wave_barrier();
+    if (id >= 0 && in < 16) row[id] = d;
+    __builtin_amdgcn_wave_barrier();
+    if (t0 + lane / L >= a.T) return;
+    char* to = static_cast<char*>(a.dlogits) + t * a.E * kElem<T>;
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+        const float4 v = *reinterpret_cast<const float4*>(row + 4 * (i * L + in));
+        const float u[4] = {v.x, v.y, v.z, v.w};
+        if (4 * (i * L + in) < a.E) four_store<T>(to, 4 * (i * L + in), a.E, u);
+    }
+}
+
 // f(type, logits a lane)
 template <class F>
 void by_experts(int type, int E, const F& f) {
@@ -738,10 +869,32 @@ hipError_t moe_route_grad(hipStream_t st, const void* logits, int type, int64_t 
                           const float* dweights, const RouteHow& how, void* dlogits, int64_t T,
                           int E, int top) {
     const RouteGradArgs a{logits, ids, dweights, dlogits, ld, T, E, top, how};
-    by_experts(type, E, [&](auto t, auto v) {
-        hipLaunchKernelGGL((route_grad_kernel<decltype(t)::value, decltype(v)::value>),
-                           dim3(token_blocks(T)), dim3(256), 0, st, a);
-    });
+    bool done = false;
+    auto go = [&](auto t, auto lanes, auto v) {
+        constexpr int L = decltype(lanes)::value, V = decltype(v)::value, TY = decltype(t)::value;
+        if (done || E > L * V || top > 16) return;
+        done = true;
+        constexpr int64_t per = 4 * (64 / L);
+        in_launches(T, kMaxBlocks * per, [&](int64_t at, int64_t m) {
+            hipLaunchKernelGGL((route_grad_rows_kernel<TY, L, V>), dim3(unsigned((m + per - 1) / per)),
+                               dim3(256), 0, st, a, at);
+        });
+    };
+    auto by = [&](auto t) {
+        go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+        go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{});
+        go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 16>{});
+        go(t, std::integral_constant<int, 32>{}, std::integral_constant<int, 16>{});
+        go(t, std::integral_constant<int, 64>{}, std::integral_constant<int, 16>{});
+    };
+    if (type == kBf16) by(std::integral_constant<int, kBf16>{});
+    else if (type == kF16) by(std::integral_constant<int, kF16>{});
+    else by(std::integral_constant<int, kF32>{});
+    if (!done)
+        by_experts(type, E, [&](auto t, auto v) {
+            hipLaunchKernelGGL((route_grad_kernel<decltype(t)::value, decltype(v)::value>),
+                               dim3(token_blocks(T)), dim3(256), 0, st, a);
+        });
     return hipGetLastError();
 }
 
