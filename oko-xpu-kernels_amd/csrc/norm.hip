@@ -13,7 +13,11 @@
 //
 // HBM-bound.  A row lies in registers from its one read to its write, 8 consecutive values
 // a lane and piece; the row's waves exchange one pair of numbers through LDS.
+#include <algorithm>
+#include <type_traits>
+
 #include "block_kernels.hpp"
+#include "kernels.hpp"
 #include "mx_kernels.hpp"
 #include "quantizer.hpp"
 #include "rows.hpp"
@@ -232,34 +236,69 @@ __device__ __forceinline__ void rotated_store(int8_t* row, int64_t d, float (&v)
     *reinterpret_cast<uint4*>(row + d) = make_uint4(lo.x, lo.y, hi.x, hi.y);
 }
 
-template <int T>
+// G segments meet in a slot: 4, a wave, where a row is whole waves.  A block walks over its
+// rows with the next one's reads under way.
+template <int T, int G>
 __global__ __launch_bounds__(1024) void norm_rotated_kernel(NormArgs a, int S, int R) {
-    __shared__ float2 slots[kMaxSegs];
+    constexpr bool EVEN = true;
+    __shared__ float2 slots[2][kMaxSegs / G];
     const int seg = threadIdx.x >> 4, sl = threadIdx.x & 15;
     const int r = seg / S, sg = seg - r * S;
+    const int64_t d = sg * 256 + lane_w(sl) * 16, step = int64_t(gridDim.x) * R;
     const XlaneSigns sgn = xlane_signs(sl);
-    for (int64_t row0 = int64_t(blockIdx.x) * R; row0 < a.M; row0 += int64_t(gridDim.x) * R) {
-        const int64_t row = row0 + r;
+    float w[2][8];
+    Piece8<T> x[2], res[2];
+    auto request = [&](int64_t row) {
+        if (r >= R || row >= a.M) return;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[i] = piece_load<T, EVEN>(row_of<T>(a.x, row, a.ldx), d + 8 * i, a.K);
+            if (a.residual) res[i] = piece_load<T, EVEN>(row_of<T>(a.residual, row, a.ldr), d + 8 * i, a.K);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = res[i] = Piece8<T>{};
+    request(int64_t(blockIdx.x) * R + r);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        vector_load<EVEN>(a.weight, a.weight_type, r < R ? d + 8 * i : 0, a.K, w[i]);
+    int turn = 0;
+    for (int64_t row = int64_t(blockIdx.x) * R + r; row - r < a.M; row += step, turn ^= 1) {
         const bool live = r < R && row < a.M;
         float v[1][16], sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[0][j] = 0.f;
-        if (live) rotated_input<T>(a, row, sg * 256 + lane_w(sl) * 16, v[0], sum);
-        const float dom = rotate_groups<1>(v, sgn);
-        const float most = lanes_max<16>(absmax16(v[0], 0.f) * dom);
-        sum = lanes_sum<16>(sum);
-        if (sl == 0) slots[seg] = make_float2(sum, most);
-        lds_barrier();
-        float total = 0.f, m = 1e-30f;
-        if (live) {
-            for (int i = 0; i < S; ++i) {
-                const float2 u = slots[r * S + i];
-                total += u.x;
-                m = fmaxf(m, u.y);
+        for (int i = 0; i < 2; ++i) {
+            float h[8];
+            piece_expand(x[i], h);
+            if (a.residual) {
+                float u[8];
+                piece_expand(res[i], u);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[j] += u[j];
+                const Piece8<T> p = piece_round<T>(h);
+                if (live) piece_store<T, EVEN>(row_of<T>(a.h, row, a.K), d + 8 * i, a.K, p);
+                piece_expand(p, h);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sum = __builtin_fmaf(h[j], h[j], sum);
+                v[0][8 * i + j] = h[j] * w[i][j];
             }
         }
+        request(row + step);
+        const float dom = rotate_groups<1>(v, sgn);
+        const float most = lanes_max<16 * G>(absmax16(v[0], 0.f) * dom);
+        sum = lanes_sum<16 * G>(sum);
+        // (the slots of two rows in turn: one barrier a row)
+        if ((threadIdx.x & (16 * G - 1)) == 0) slots[turn][seg / G] = make_float2(sum, most);
         lds_barrier();
         if (!live) continue;
+        float total = 0.f, m = 1e-30f;
+        for (int i = 0; i < S / G; ++i) {
+            const float2 u = slots[turn][r * (S / G) + i];
+            total += u.x;
+            m = fmaxf(m, u.y);
+        }
         if (sg == 0 && sl == 0) a.scale[row] = inverse_rms(total, a.K, a.eps) * m / 127.0f;
         rotated_store(static_cast<int8_t*>(a.y) + row * a.K, sg * 256 + lane_w_rot(sl) * 16, v[0],
                       127.0f / m * dom);
@@ -512,6 +551,7 @@ bool by_length(int64_t K, const F& f) {
     else return false;
     return true;
 }
+constexpr int64_t kRowBlocks = kMaxBlocks / 4;
 unsigned blocks_for(int64_t M, int rows, int64_t most) {
     const int64_t n = (M + rows - 1) / rows;
     return unsigned(n < most ? n : most);
@@ -525,11 +565,11 @@ hipError_t launch_norm(hipStream_t st, int type, const NormArgs& a) {
         const bool done = by_length(a.K, [&](auto s) {
             constexpr int TPR = decltype(s)::tpr, P = decltype(s)::p, N = kThreads<TPR>;
             hipLaunchKernelGGL((norm_kernel<T, TPR, P, INT8, EVEN>),
-                               dim3(blocks_for(a.M, N / TPR, kMaxBlocks / 4)), dim3(N), 0, st, a);
+                               dim3(blocks_for(a.M, N / TPR, kRowBlocks)), dim3(N), 0, st, a);
         });
         if (!done)
             hipLaunchKernelGGL((norm_long_kernel<T, INT8, EVEN>),
-                               dim3(blocks_for(a.M, 1, kMaxBlocks / 4)), dim3(1024), 0, st, a);
+                               dim3(blocks_for(a.M, 1, kRowBlocks)), dim3(1024), 0, st, a);
     }); });
     return hipGetLastError();
 }
@@ -560,10 +600,19 @@ hipError_t rms_norm_int8(hipStream_t st, const void* x, int type, int64_t ldx,
             // rows of few groups share a block of 16
             const int S = int(K / 256), R = S >= 16 ? 1 : 16 / S;
             const int threads = (S * R * 16 + 63) / 64 * 64;
-            hipLaunchKernelGGL((norm_rotated_kernel<T>), dim3(blocks_for(M, R, kMaxBlocks / 4)),
-                               dim3(threads), 0, st, a, S, R);
+            // Blocks that together request 40 KB a CU (no fewer than one, no more than its 16
+            // waves): more rows under way at once are slower.  16381 x 5120 bf16 with a
+            // residual (40 KB: 2 blocks): 118 us with 1, 111 with 2, 131 with 3, 123 with 6;
+            // 8192 x 8192 85 with 1, 91 with 2; 20000 x 4096 without one 64 with 2, 52 with 4.
+            const int bytes = threads * 16 * kElem<T> * (residual ? 2 : 1);
+            const int each = std::max(1, std::min(40960 / bytes, 1024 / threads));
+            const dim3 grid(blocks_for(M, R, int64_t(each) * device_cus()));
+            if (S % 4 == 0)
+                hipLaunchKernelGGL((norm_rotated_kernel<T, 4>), grid, dim3(threads), 0, st, a, S, R);
+            else
+                hipLaunchKernelGGL((norm_rotated_kernel<T, 1>), grid, dim3(threads), 0, st, a, S, R);
         } else {
-            hipLaunchKernelGGL((norm_rotated_long_kernel<T>), dim3(blocks_for(M, 1, kMaxBlocks / 4)),
+            hipLaunchKernelGGL((norm_rotated_long_kernel<T>), dim3(blocks_for(M, 1, kRowBlocks)),
                                dim3(1024), 0, st, a);
         }
     });

@@ -8,6 +8,9 @@
 // (once a position, for all of its heads), then walk over the heads in pieces of 16
 // values, 8 pairs.  Angles are reduced to a part of a turn in 64 bits, since in 32 a far
 // position would lose it: at position 10^6 half a unit of the product is 0.03 of a radian.
+#include <algorithm>
+#include <type_traits>
+
 #include "block_kernels.hpp"
 #include "mx_kernels.hpp"
 #include "rows.hpp"
@@ -15,16 +18,15 @@
 namespace xpuint8 {
 namespace {
 
-constexpr int kMaxPairs = 512;
-
 struct RotaryArgs {
     Heads q, k;                     // k.H = 0: q alone
     Positions pos;
     const double* inv_freq;
     const int* axis;
-    int64_t S, tokens;
+    uint32_t S, tokens, first;      // positions in all, the launch's first
     int P, D, per_head;             // pieces a head: of 8 pairs, then 16 unturned values
     int turned;                     // pieces of pairs
+    int each;                       // positions a block
     float sign;
 };
 
@@ -36,95 +38,93 @@ __device__ __forceinline__ double position_of(const Positions& p, int axis, int6
     return double(static_cast<const float*>(p.p)[at]);
 }
 
-template <int T>
-__device__ __forceinline__ float element(const char* p, int64_t i) {
-    if constexpr (T == kF32) return reinterpret_cast<const float*>(p)[i];
-    else if constexpr (T == kBf16) return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
-    else return float(reinterpret_cast<const _Float16*>(p)[i]);
-}
-template <int T>
-__device__ __forceinline__ void put(char* p, int64_t i, float v) {
-    if constexpr (T == kF32) reinterpret_cast<float*>(p)[i] = v;
-    else reinterpret_cast<uint16_t*>(p)[i] = uint16_t(pack2<T>(v, 0.f));
-}
+// A thread's piece of every head: two runs of 8 values, ends where they are cut
+struct Runs {
+    int d[2], end[2];
+    bool turn;
+};
 
-// Piece c of a head's row x to its place in out; cs: the position's cosines and sines.
-template <int T, bool SPLIT>
-__device__ __forceinline__ void turn_piece(const RotaryArgs& a, const char* x, char* out, int c,
-                                           const float2* cs) {
-    if (c >= a.turned) {               // unturned values, as they lie
-        const int64_t d = 2 * a.P + 16 * int64_t(c - a.turned);
+// A block takes a.each positions; a thread keeps to one piece of a head and goes through
+// the heads of all of them, the next one's values requested before it works on the current
+// one's (and the first before the angles are made).  EVEN: no run is cut.
+template <int T, bool SPLIT, bool EVEN>
+__global__ __launch_bounds__(512) void rotary_kernel(RotaryArgs a) {
+    extern __shared__ __align__(16) float2 cs[];      // [each][stride]
+    const int stride = 8 * a.turned;
+    const int c = threadIdx.x % a.per_head, slot = threadIdx.x / a.per_head;
+    const int slots = blockDim.x / a.per_head, H = a.q.H + a.k.H;
+    const uint32_t t0 = a.first + blockIdx.x * uint32_t(a.each);
+    const int n = int(min(a.tokens - t0, uint32_t(a.each)));
+    const int rows = slot < slots ? n * H : 0;
+    Runs w;
+    w.turn = c < a.turned;
+    if (w.turn) {
+        w.d[0] = SPLIT ? 8 * c : 16 * c;
+        w.d[1] = SPLIT ? a.P + 8 * c : 16 * c + 8;
+        w.end[0] = SPLIT ? a.P : 2 * a.P;
+        w.end[1] = 2 * a.P;
+    } else {
+        w.d[0] = 2 * a.P + 16 * (c - a.turned);
+        w.d[1] = w.d[0] + 8;
+        w.end[0] = w.end[1] = a.D;
+    }
+    auto place = [&](int row, const char*& x, char*& out) -> int {
+        const int t = int(uint32_t(row) / uint32_t(H)), h = row - t * H;
+        const uint32_t b = (t0 + t) / a.S, s = (t0 + t) - b * a.S;
+        const Heads& m = h < a.q.H ? a.q : a.k;
+        const int64_t hh = h < a.q.H ? h : h - a.q.H;
+        x = static_cast<const char*>(m.x) + (b * m.x_b + s * m.x_s + hh * m.x_h) * kElem<T>;
+        out = static_cast<char*>(m.out) + (b * m.o_b + s * m.o_s + hh * m.o_h) * kElem<T>;
+        return t;
+    };
+    Piece8<T> next[2] = {};
+    char* next_out = nullptr;
+    int next_t = 0;
+    auto request = [&](int row) {
+        if (row >= rows) return;
+        const char* x;
+        next_t = place(row, x, next_out);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (d + 8 * i < a.D)
-                piece_store<T, false>(out, d + 8 * i, a.D, piece_load<T, false>(x, d + 8 * i, a.D));
-        return;
+            if (EVEN || w.d[i] < w.end[i]) next[i] = piece_load<T, EVEN>(x, w.d[i], w.end[i]);
+    };
+    request(slot);
+    for (int i = threadIdx.x; i < n * a.P; i += blockDim.x) {
+        const int t = int(uint32_t(i) / uint32_t(a.P)), p = i - t * a.P;
+        const uint32_t b = (t0 + t) / a.S, s = (t0 + t) - b * a.S;
+        const double turns = position_of(a.pos, a.axis[p], b, s) * a.inv_freq[p] *
+                             0.15915494309189535;             // 1 / 2 pi
+        const float part = float(turns - rint(turns));
+        float sine, cosine;
+        sincospif(2.0f * part, &sine, &cosine);
+        cs[t * stride + p] = make_float2(cosine, sine * a.sign);
     }
-    const int p0 = 8 * c;
-    if (p0 + 8 <= a.P) {
-        const int64_t d0 = SPLIT ? p0 : 2 * p0, d1 = SPLIT ? a.P + p0 : 2 * p0 + 8;
-        float u[8], v[8];
-        piece_expand(piece_load<T, true>(x, d0, a.D), u);
-        piece_expand(piece_load<T, true>(x, d1, a.D), v);
-        float f[2][8];
+    __syncthreads();
+    for (int row = slot; row < rows; row += slots) {
+        const Piece8<T> x[2] = {next[0], next[1]};
+        char* out = next_out;
+        const float2* turn = cs + next_t * stride + 8 * c;
+        request(row + slots);
+        Piece8<T> y[2] = {x[0], x[1]};
+        if (w.turn) {
+            float u[2][8], f[2][8];
+            piece_expand(x[0], u[0]);
+            piece_expand(x[1], u[1]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 t = cs[p0 + i];
-            const float p = SPLIT ? u[i] : (i < 4 ? u : v)[(2 * i) & 7];
-            const float q = SPLIT ? v[i] : (i < 4 ? u : v)[(2 * i + 1) & 7];
-            const float first = p * t.x - q * t.y, second = q * t.x + p * t.y;
-            if (SPLIT) {
-                f[0][i] = first;
-                f[1][i] = second;
-            } else {
-                f[i >> 2][(2 * i) & 7] = first;
-                f[i >> 2][(2 * i + 1) & 7] = second;
+            for (int i = 0; i < 8; ++i) {
+                const float2 z = turn[i];
+                // pair i: one of each run, or neighbours in one of them
+                float& p = SPLIT ? u[0][i] : u[i >> 2][(2 * i) & 7];
+                float& q = SPLIT ? u[1][i] : u[i >> 2][(2 * i + 1) & 7];
+                (SPLIT ? f[0][i] : f[i >> 2][(2 * i) & 7]) = p * z.x - q * z.y;
+                (SPLIT ? f[1][i] : f[i >> 2][(2 * i + 1) & 7]) = q * z.x + p * z.y;
             }
+            y[0] = piece_round<T>(f[0]);
+            y[1] = piece_round<T>(f[1]);
         }
-        piece_store<T, true>(out, d0, a.D, piece_round<T>(f[0]));
-        piece_store<T, true>(out, d1, a.D, piece_round<T>(f[1]));
-        return;
-    }
-    for (int p = p0; p < a.P; ++p) {   // the last pairs, fewer than 8
-        const int64_t d0 = SPLIT ? p : 2 * p, d1 = SPLIT ? a.P + p : 2 * p + 1;
-        const float u = element<T>(x, d0), v = element<T>(x, d1);
-        const float2 t = cs[p];
-        put<T>(out, d0, u * t.x - v * t.y);
-        put<T>(out, d1, v * t.x + u * t.y);
-    }
-}
-
-template <int T, bool SPLIT, int TOKENS>
-__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
-    __shared__ float2 cs[TOKENS * kMaxPairs];
-    const int H = a.q.H + a.k.H;
-    for (int64_t t0 = int64_t(blockIdx.x) * TOKENS; t0 < a.tokens; t0 += int64_t(gridDim.x) * TOKENS) {
-        const int n = int(a.tokens - t0 < TOKENS ? a.tokens - t0 : TOKENS);
-        for (int i = threadIdx.x; i < n * a.P; i += 256) {
-            const int t = i / a.P, p = i - t * a.P;
-            const int64_t b = (t0 + t) / a.S, s = (t0 + t) - b * a.S;
-            const double turns = position_of(a.pos, a.axis[p], b, s) * a.inv_freq[p] *
-                                 0.15915494309189535;          // 1 / 2 pi
-            const float part = float(turns - rint(turns));
-            float sine, cosine;
-            sincospif(2.0f * part, &sine, &cosine);
-            cs[t * kMaxPairs + p] = make_float2(cosine, sine * a.sign);
-        }
-        __syncthreads();
-        const int units = n * H * a.per_head;
-        for (int u = threadIdx.x; u < units; u += 256) {
-            const int row = u / a.per_head, c = u - row * a.per_head;
-            const int t = row / H, h = row - t * H;
-            const int64_t b = (t0 + t) / a.S, s = (t0 + t) - b * a.S;
-            const bool is_q = h < a.q.H;
-            const Heads& w = is_q ? a.q : a.k;
-            const int64_t hh = is_q ? h : h - a.q.H;
-            const char* x = static_cast<const char*>(w.x) +
-                            (b * w.x_b + s * w.x_s + hh * w.x_h) * kElem<T>;
-            char* out = static_cast<char*>(w.out) + (b * w.o_b + s * w.o_s + hh * w.o_h) * kElem<T>;
-            turn_piece<T, SPLIT>(a, x, out, c, cs + t * kMaxPairs);
-        }
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (EVEN || w.d[i] < w.end[i]) piece_store<T, EVEN>(out, w.d[i], w.end[i], y[i]);
     }
 }
 
@@ -133,15 +133,28 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 hipError_t rope_axes(hipStream_t st, const Heads& q, const Heads& k, int type,
                      const Positions& positions, const double* inv_freq, const int* axis, int P,
                      bool inverse, bool split_half, int64_t B, int64_t S, int D) {
-    RotaryArgs a{q, k, positions, inv_freq, axis, S, B * S, P, D, 0, 0, inverse ? -1.f : 1.f};
+    RotaryArgs a{q, k, positions, inv_freq, axis, uint32_t(S), uint32_t(B * S), 0, P, D, 0, 0, 1,
+                 inverse ? -1.f : 1.f};
     a.turned = (P + 7) / 8;
     a.per_head = a.turned + (D - 2 * P + 15) / 16;
+    const int threads = a.per_head > 256 ? 512 : 256;  // (a head of 4096 has up to 257 pieces)
+    // Positions a block: enough for its threads to go round twice, once there are blocks
+    // enough for the chip (48 heads of 128, 32760 positions: 157 us with one, 156 with 2,
+    // 160 with 4; 20 of 80, 6141: 13.2, 10.3 and 9.9; by one position at 32: 4.1 for 7.1).
+    if (a.tokens >= 4096) a.each = std::max(1, std::min(16, 512 / (a.per_head * (q.H + k.H))));
     auto go = [&](auto t, auto split) {
         constexpr int T = decltype(t)::value;
         constexpr bool SPLIT = decltype(split)::value;
-        const int64_t n = (a.tokens + 3) / 4, most = kMaxBlocks;
-        hipLaunchKernelGGL((rotary_kernel<T, SPLIT, 4>), dim3(unsigned(n < most ? n : most)),
-                           dim3(256), 0, st, a);
+        auto launch = [&](auto even) {
+            in_launches(B * S, kMaxBlocks * a.each, [&](int64_t at, int64_t m) {
+                a.first = uint32_t(at);
+                hipLaunchKernelGGL((rotary_kernel<T, SPLIT, decltype(even)::value>),
+                                   dim3(unsigned((m + a.each - 1) / a.each)), dim3(threads),
+                                   a.each * a.turned * 8 * sizeof(float2), st, a);
+            });
+        };
+        if (P % 8 == 0 && (D - 2 * P) % 16 == 0) launch(std::true_type{});
+        else launch(std::false_type{});
     };
     auto by_split = [&](auto t) {
         if (split_half) go(t, std::true_type{});

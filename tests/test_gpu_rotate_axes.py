@@ -37,7 +37,9 @@ def check(got, x, positions, f, split, inverse=False):
     (2, 7, 3, 3, 50, (5, 3, 2), torch.int32), (1, 130, 2, 1, 33, (7,), torch.int64),
     (2, 3, 1, 2, 19, (1, 0, 4), torch.int32), (5, 1, 7, 7, 256, (128,), torch.int32),
     (1, 9, 2, 2, 1030, (200, 300, 12), torch.int32), (4, 6, 12, 4, 96, (10, 10, 10, 10), torch.int64),
-    (1, 2, 70, 70, 4, (1, 1), torch.int32), (1, 3, 1, 1, 4096, (512,), torch.int32)])
+    (1, 2, 70, 70, 4, (1, 1), torch.int32), (1, 3, 1, 1, 4096, (512,), torch.int32),
+    (2, 2, 2, 1, 4096, (1,), torch.int32), (1, 3, 2, 2, 4095, (3, 6), torch.int64),
+    (3, 1500, 1, 1, 24, (8, 2), torch.int32), (2, 2111, 3, 2, 10, (4,), torch.int32)])
 def test_forward_and_gradient(dev, dtype, split, b, s, hq, hk, d, sections, kind):
     q, k = randn(b, s, hq, d, seed=1, dtype=dtype), randn(b, s, hk, d, seed=2, dtype=dtype)
     dq, dk = randn(b, s, hq, d, seed=4, dtype=dtype), randn(b, s, hk, d, seed=5, dtype=dtype)
