@@ -38,7 +38,9 @@ __device__ __forceinline__ double position_of(const Positions& p, int axis, int6
     return double(static_cast<const float*>(p.p)[at]);
 }
 
-// A thread's piece of every head: two runs of 8 values, ends where they are cut
+// A thread's piece of every head: two runs of 8 values, ends where they are cut.  A head's
+// last pairs, fewer than 8, are taken with the ones before them, which two threads then
+// write alike; a run is cut only where there are not 8 at all.
 struct Runs {
     int d[2], end[2];
     bool turn;
@@ -58,14 +60,19 @@ __global__ __launch_bounds__(512) void rotary_kernel(RotaryArgs a) {
     const int rows = slot < slots ? n * H : 0;
     Runs w;
     w.turn = c < a.turned;
+    const int p0 = EVEN ? min(8 * c, a.P - 8) : 8 * c;      // (turned: its first pair)
     if (w.turn) {
-        w.d[0] = SPLIT ? 8 * c : 16 * c;
-        w.d[1] = SPLIT ? a.P + 8 * c : 16 * c + 8;
+        w.d[0] = SPLIT ? p0 : 2 * p0;
+        w.d[1] = SPLIT ? a.P + p0 : 2 * p0 + 8;
         w.end[0] = SPLIT ? a.P : 2 * a.P;
         w.end[1] = 2 * a.P;
     } else {
         w.d[0] = 2 * a.P + 16 * (c - a.turned);
         w.d[1] = w.d[0] + 8;
+        if (EVEN) {
+            w.d[0] = min(w.d[0], a.D - 8);
+            w.d[1] = min(w.d[1], a.D - 8);
+        }
         w.end[0] = w.end[1] = a.D;
     }
     auto place = [&](int row, const char*& x, char*& out) -> int {
@@ -103,7 +110,7 @@ __global__ __launch_bounds__(512) void rotary_kernel(RotaryArgs a) {
     for (int row = slot; row < rows; row += slots) {
         const Piece8<T> x[2] = {next[0], next[1]};
         char* out = next_out;
-        const float2* turn = cs + next_t * stride + 8 * c;
+        const float2* turn = cs + next_t * stride + p0;
         request(row + slots);
         Piece8<T> y[2] = {x[0], x[1]};
         if (w.turn) {
@@ -138,10 +145,12 @@ hipError_t rope_axes(hipStream_t st, const Heads& q, const Heads& k, int type,
     a.turned = (P + 7) / 8;
     a.per_head = a.turned + (D - 2 * P + 15) / 16;
     const int threads = a.per_head > 256 ? 512 : 256;  // (a head of 4096 has up to 257 pieces)
-    // Positions a block: enough for its threads to go round twice, once there are blocks
-    // enough for the chip (48 heads of 128, 32760 positions: 157 us with one, 156 with 2,
-    // 160 with 4; 20 of 80, 6141: 13.2, 10.3 and 9.9; by one position at 32: 4.1 for 7.1).
-    if (a.tokens >= 4096) a.each = std::max(1, std::min(16, 512 / (a.per_head * (q.H + k.H))));
+    // Positions a block: enough for its threads to go round twice where there are blocks
+    // enough for the chip, once where not (48 heads of 128, 32760 positions: 157 us with one,
+    // 156 with 2, 160 with 4; 20 of 80, 6141: 13.2, 10.3 and 9.9).
+    const int64_t units = int64_t(a.per_head) * (q.H + k.H);
+    a.each = int(std::max<int64_t>(1, std::min({(a.tokens >= 4096 ? 512 : 256) / units,
+                                                 int64_t(4096 / (8 * a.turned)), B * S / 512})));
     auto go = [&](auto t, auto split) {
         constexpr int T = decltype(t)::value;
         constexpr bool SPLIT = decltype(split)::value;
@@ -153,7 +162,7 @@ hipError_t rope_axes(hipStream_t st, const Heads& q, const Heads& k, int type,
                                    a.each * a.turned * 8 * sizeof(float2), st, a);
             });
         };
-        if (P % 8 == 0 && (D - 2 * P) % 16 == 0) launch(std::true_type{});
+        if (P >= 8 && (D == 2 * P || D - 2 * P >= 8)) launch(std::true_type{});
         else launch(std::false_type{});
     };
     auto by_split = [&](auto t) {
