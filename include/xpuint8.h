@@ -656,23 +656,26 @@ int xpuint8_moe_route_grad_stream(const void *stream, const void *logits, int32_
                                   int64_t E, int64_t top);
 
 /* ---- RMS norm -----------------------------------------------------------
- * Rows of K values, [M, K] with row strides in elements; element types 0 bf16, 1 fp16,
- * 2 fp32.  Inputs may have the alignment of their elements; outputs and work are contiguous
+ * M rows of K values; element types 0 bf16, 1 fp16, 2 fp32.  An input's rows lie in runs of
+ * `inner` rows (a divisor of M, 1 for evenly spaced rows; the heads of a position, say): rows
+ * ld elements apart in a run, runs outer apart (inner 1: rows are outer apart, ld is not
+ * read).  Inputs may have the alignment of their elements; outputs and work are contiguous
  * and 16-byte aligned.  Statistics are fp32.  K <= 2^24.  No counterpart in the reference.
  *
  * h = x + residual rounded to the type (residual and h NULL: h is x);
  * y = h / sqrt(mean(h^2) + eps) * weight (fp32 until y's rounding; weight [K] of its own
  * type, NULL: ones) */
 int xpuint8_rms_norm_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
-                            const void *residual, int64_t ldr, const void *weight,
-                            int32_t weight_type, float eps, void *h, void *y, int64_t M,
-                            int64_t K);
+                            int64_t outer_x, const void *residual, int64_t ldr, int64_t outer_r,
+                            int64_t inner, const void *weight, int32_t weight_type, float eps,
+                            void *h, void *y, int64_t M, int64_t K);
 
 /* the same in int8 with a scale a row, for the int8 linears: v = h * weight in fp32, with
  * rotate = 1 (K % 256 == 0) rotated as xpuint8_convrot_quantize_stream rotates;
  * m = max(|v|, 1e-30), q = rint(v * (127 / m)), scale = m / 127 / sqrt(mean(h^2) + eps) */
 int xpuint8_rms_norm_int8_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
-                                 const void *residual, int64_t ldr, const void *weight,
+                                 int64_t outer_x, const void *residual, int64_t ldr,
+                                 int64_t outer_r, int64_t inner, const void *weight,
                                  int32_t weight_type, float eps, void *h, int8_t *q, float *scale,
                                  int32_t rotate, int64_t M, int64_t K);
 
@@ -681,9 +684,9 @@ int xpuint8_rms_norm_int8_stream(const void *stream, const void *x, int32_t type
  * then too) sums fp32 in a fixed order. */
 int64_t xpuint8_rms_norm_grad_workspace_size(int64_t M, int64_t K);
 int xpuint8_rms_norm_grad_stream(const void *stream, const void *dy, int32_t type, int64_t ldy,
-                                 const void *h, int64_t ldh, const void *weight,
-                                 int32_t weight_type, const void *dh, int64_t lddh, float eps,
-                                 void *dx, void *dweight, int64_t M, int64_t K, void *work,
+                                 int64_t outer_dy, const void *h, int64_t ldh, int64_t outer_h,
+                                 const void *weight, int32_t weight_type, const void *dh,
+                                 int64_t lddh, int64_t outer_dh, int64_t inner, float eps, void *dx, void *dweight, int64_t M, int64_t K, void *work,
                                  int64_t work_bytes);
 
 /* ---- rotary positions on several axes -----------------------------------

@@ -9,23 +9,27 @@
 
 namespace xpuint8 {
 
-// norm.hip.  x [M, K] plus residual (null: none; h then too) is h, y = h / rms(h) * weight
-// (null: ones).
-hipError_t rms_norm(hipStream_t st, const void* x, int type, int64_t ldx, const void* residual,
-                    int64_t ldr, const void* weight, int weight_type, float eps, void* h, void* y,
-                    int64_t M, int64_t K);
+// norm.hip.  An input's rows lie in runs of `inner` (which divides M): ld apart in a run, runs
+// outer apart (inner 1: rows outer apart).
+struct Lines {
+    int64_t ld, outer;
+};
+// x [M, K] plus residual (null: none; h then too) is h, y = h / rms(h) * weight (null: ones)
+hipError_t rms_norm(hipStream_t st, const void* x, int type, const Lines& lx,
+                    const void* residual, const Lines& lr, int64_t inner, const void* weight,
+                    int weight_type, float eps, void* h, void* y, int64_t M, int64_t K);
 // the same with int8 codes and a scale a row for y, rotated by 256s or not
-hipError_t rms_norm_int8(hipStream_t st, const void* x, int type, int64_t ldx,
-                         const void* residual, int64_t ldr, const void* weight, int weight_type,
-                         float eps, void* h, int8_t* q, float* scale, bool rotate, int64_t M,
-                         int64_t K);
+hipError_t rms_norm_int8(hipStream_t st, const void* x, int type, const Lines& lx,
+                         const void* residual, const Lines& lr, int64_t inner,
+                         const void* weight, int weight_type, float eps, void* h, int8_t* q,
+                         float* scale, bool rotate, int64_t M, int64_t K);
 // dx [M, K] from dy and (null: none) dh, the gradients of y and h; dweight [K] of
 // weight_type (null: not wanted) through part (rms_norm_grad_work_bytes)
 int64_t rms_norm_grad_work_bytes(int64_t M, int64_t K);
-hipError_t rms_norm_grad(hipStream_t st, const void* dy, int type, int64_t ldy, const void* h,
-                         int64_t ldh, const void* weight, int weight_type, const void* dh,
-                         int64_t lddh, float eps, void* dx, void* dweight, int64_t M, int64_t K,
-                         float* part);
+hipError_t rms_norm_grad(hipStream_t st, const void* dy, int type, const Lines& ldy,
+                         const void* h, const Lines& lh, const void* weight, int weight_type,
+                         const void* dh, const Lines& ldh, int64_t inner, float eps, void* dx,
+                         void* dweight, int64_t M, int64_t K, float* part);
 
 // rotary.hip.  One tensor of heads [B, S, H, D] and its result.
 struct Heads {

@@ -34,12 +34,25 @@ int check_rows(int64_t M, int64_t K) {
     return 0;
 }
 
-int check_norm(const void* x, int32_t type, int64_t ldx, const void* residual, int64_t ldr,
-               const void* weight, int32_t weight_type, float eps, const void* h, int64_t M,
-               int64_t K) {
+// M rows in runs of `inner`; rows of a run do not overlap, runs may lie anywhere
+int check_inner(int64_t inner, int64_t M) {
+    if (inner < 1 || M % inner != 0) return fail(2, "inner must be positive and divide the rows");
+    return 0;
+}
+int check_lines(const void* p, const Lines& l, int64_t inner, int64_t M, int64_t K) {
+    if (p && (l.outer < (inner == 1 && M > 1 ? K : 0) || (inner > 1 && l.ld < K)))
+        return fail(2, "the row strides must be >= K");
+    return 0;
+}
+
+int check_norm(const void* x, int32_t type, const Lines& lx, const void* residual, const Lines& lr,
+               int64_t inner, const void* weight, int32_t weight_type, float eps, const void* h,
+               int64_t M, int64_t K) {
     XPU_TRY(check_rows(M, K));
     XPU_TRY(check_type(type, "type"));
-    if (ldx < K || (residual && ldr < K)) return fail(2, "the row strides must be >= K");
+    XPU_TRY(check_inner(inner, M));
+    XPU_TRY(check_lines(x, lx, inner, M, K));
+    XPU_TRY(check_lines(residual, lr, inner, M, K));
     if (!(eps >= 0.f)) return fail(2, "eps must not be negative");
     if (!x) return fail(6, "x must not be null");
     XPU_TRY(check_aligned(x, type, "x"));
@@ -72,27 +85,30 @@ using namespace xpuint8;
 extern "C" {
 
 int xpuint8_rms_norm_stream(const void* stream, const void* x, int32_t type, int64_t ldx,
-                            const void* residual, int64_t ldr, const void* weight,
-                            int32_t weight_type, float eps, void* h, void* y, int64_t M,
-                            int64_t K) {
-    XPU_TRY(check_norm(x, type, ldx, residual, ldr, weight, weight_type, eps, h, M, K));
+                            int64_t outer_x, const void* residual, int64_t ldr, int64_t outer_r,
+                            int64_t inner, const void* weight, int32_t weight_type, float eps,
+                            void* h, void* y, int64_t M, int64_t K) {
+    const Lines lx{ldx, outer_x}, lr{ldr, outer_r};
+    XPU_TRY(check_norm(x, type, lx, residual, lr, inner, weight, weight_type, eps, h, M, K));
     XPU_NONNULL(y);
     XPU_TRY(ensure_device());
-    return launched(rms_norm(as_stream(stream), x, type, ldx, residual, ldr, weight, weight_type,
-                             eps, h, y, M, K), "rms_norm");
+    return launched(rms_norm(as_stream(stream), x, type, lx, residual, lr, inner, weight,
+                             weight_type, eps, h, y, M, K), "rms_norm");
 }
 
 int xpuint8_rms_norm_int8_stream(const void* stream, const void* x, int32_t type, int64_t ldx,
-                                 const void* residual, int64_t ldr, const void* weight,
+                                 int64_t outer_x, const void* residual, int64_t ldr,
+                                 int64_t outer_r, int64_t inner, const void* weight,
                                  int32_t weight_type, float eps, void* h, int8_t* q, float* scale,
                                  int32_t rotate, int64_t M, int64_t K) {
-    XPU_TRY(check_norm(x, type, ldx, residual, ldr, weight, weight_type, eps, h, M, K));
+    const Lines lx{ldx, outer_x}, lr{ldr, outer_r};
+    XPU_TRY(check_norm(x, type, lx, residual, lr, inner, weight, weight_type, eps, h, M, K));
     if (rotate != 0 && rotate != 1) return fail(2, "rotate must be 0 or 1");
     if (rotate && K % 256 != 0)
         return fail(3, "K must be a multiple of the ConvRot group size (256) to be rotated");
     XPU_NONNULL(q); XPU_NONNULL(scale);
     XPU_TRY(ensure_device());
-    return launched(rms_norm_int8(as_stream(stream), x, type, ldx, residual, ldr, weight,
+    return launched(rms_norm_int8(as_stream(stream), x, type, lx, residual, lr, inner, weight,
                                   weight_type, eps, h, q, scale, rotate != 0, M, K),
                     "rms_norm_int8");
 }
@@ -103,13 +119,17 @@ int64_t xpuint8_rms_norm_grad_workspace_size(int64_t M, int64_t K) {
 }
 
 int xpuint8_rms_norm_grad_stream(const void* stream, const void* dy, int32_t type, int64_t ldy,
-                                 const void* h, int64_t ldh, const void* weight,
-                                 int32_t weight_type, const void* dh, int64_t lddh, float eps,
-                                 void* dx, void* dweight, int64_t M, int64_t K, void* work,
+                                 int64_t outer_dy, const void* h, int64_t ldh, int64_t outer_h,
+                                 const void* weight, int32_t weight_type, const void* dh,
+                                 int64_t lddh, int64_t outer_dh, int64_t inner, float eps, void* dx, void* dweight, int64_t M, int64_t K, void* work,
                                  int64_t work_bytes) {
     XPU_TRY(check_rows(M, K));
     XPU_TRY(check_type(type, "type"));
-    if (ldy < K || ldh < K || (dh && lddh < K)) return fail(2, "the row strides must be >= K");
+    const Lines dy_lines{ldy, outer_dy}, h_lines{ldh, outer_h}, dh_lines{lddh, outer_dh};
+    XPU_TRY(check_inner(inner, M));
+    XPU_TRY(check_lines(dy, dy_lines, inner, M, K));
+    XPU_TRY(check_lines(h, h_lines, inner, M, K));
+    XPU_TRY(check_lines(dh, dh_lines, inner, M, K));
     if (!(eps >= 0.f)) return fail(2, "eps must not be negative");
     if (!dy || !h) return fail(6, "dy and h must not be null");
     XPU_TRY(check_aligned(dy, type, "dy"));
@@ -127,8 +147,8 @@ int xpuint8_rms_norm_grad_stream(const void* stream, const void* dy, int32_t typ
             return fail(2, "work must hold xpuint8_rms_norm_grad_workspace_size bytes");
     }
     XPU_TRY(ensure_device());
-    return launched(rms_norm_grad(as_stream(stream), dy, type, ldy, h, ldh, weight, weight_type,
-                                  dh, lddh, eps, dx, dweight, M, K, static_cast<float*>(work)),
+    return launched(rms_norm_grad(as_stream(stream), dy, type, dy_lines, h, h_lines, weight,
+                                  weight_type, dh, dh_lines, inner, eps, dx, dweight, M, K, static_cast<float*>(work)),
                     "rms_norm_grad");
 }
 

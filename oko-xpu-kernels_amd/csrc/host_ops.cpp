@@ -16,6 +16,7 @@
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/Storage.h>
@@ -23,6 +24,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <array>
 #include <cstdio>
 #include <cstring>
@@ -949,28 +951,93 @@ bool whole(PyObject* o, int64_t lo, int64_t hi, int64_t& v) {
 }
 const std::optional<Tensor> maybe(const Tensor* t) { return t ? std::optional<Tensor>(*t) : std::nullopt; }
 
+// The rows of a tensor as norm.py's _runs and _lines see them: runs of `inner` rows, ld apart,
+// runs outer apart.
+struct Lines {
+    int64_t inner = 1, ld = 0, outer = 0;
+};
+bool runs_of(const Tensor& t, Lines& l) {
+    const int64_t k = t.size(-1);
+    if (t.stride(-1) != 1 && k > 1) return false;
+    int64_t n[2] = {0, 0}, s[2] = {k, k};
+    int levels = 0;
+    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+        if (t.size(d) == 1) continue;
+        if (levels && t.stride(d) == n[levels - 1] * s[levels - 1]) {
+            n[levels - 1] *= t.size(d);
+        } else {
+            if (levels == 2) return false;
+            n[levels] = t.size(d);
+            s[levels++] = t.stride(d);
+        }
+    }
+    if (levels && s[0] < k) return false;
+    l = levels == 2 ? Lines{n[0], s[0], s[1]} : Lines{1, s[0], s[0]};
+    return true;
+}
+// the same in runs of `inner`
+bool in_runs(Lines& l, int64_t inner) {
+    if (l.inner == inner) return true;
+    if (l.inner != 1) return false;
+    l = Lines{inner, l.outer, l.outer * inner};
+    return true;
+}
+// a plain tensor (see plain) of a floating type whose rows lie in runs, of any alignment
+const Tensor* lines_arg(PyObject* o, Lines& l) {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const Tensor& t = THPVariable_Unpack(o);
+    if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || type_of(t) < 0 ||
+        t.key_set().has_any(kWrapped) || !t.has_storage() || t.dim() < 1 || t.numel() == 0 ||
+        reinterpret_cast<uintptr_t>(t.data_ptr()) % t.element_size() != 0 || !runs_of(t, l))
+        return nullptr;
+    return &t;
+}
+
+// The gradient of a leaf ends in a node that lives as long as any graph of the leaf and
+// belongs to the stream that was current when it was made.  A backward pass that is captured
+// makes that stream wait for the capturing one, which, if it is not captured too, ends the
+// capture and with it the process; a call that would lead there is refused (in Python, which
+// knows the streams, _capture.refuse_foreign_leaf).
+void check_leaf(const Tensor* t) {
+    if (!t || !t->requires_grad() || t->grad_fn()) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node) return;
+    const auto made = node->stream();
+    if (!made || c10::impl::VirtualGuardImpl(t->device().type()).getStream(t->device()) == *made) return;
+    PyObject* module = PyImport_ImportModule("xpu_kernels._capture");
+    PyObject* r = module ? PyObject_CallMethod(module, "refuse_foreign_leaf", "LiL", (long long)made->id(),
+                                               int(made->device_index()), (long long)made->device_type())
+                         : nullptr;
+    Py_XDECREF(module);
+    if (!r) throw python_error();
+    Py_DECREF(r);
+}
+
 // x, weight or None, eps, residual or None of a norm
 struct NormCall {
     const Tensor *x = nullptr, *w = nullptr, *r = nullptr;
+    Lines lx, lr;
     double eps = 0;
 };
 bool norm_call(PyObject* const* a, NormCall& c) {
-    c.x = floating(a[0]);
-    if (!c.x || c.x->dim() < 1 || c.x->size(-1) > int64_t(1) << 24 || !number(a[2], c.eps) || !(c.eps >= 0))
-        return false;
+    c.x = lines_arg(a[0], c.lx);
+    if (!c.x || c.x->size(-1) > int64_t(1) << 24 || !number(a[2], c.eps) || !(c.eps >= 0)) return false;
     if (a[1] != Py_None) {
         c.w = on(floating(a[1]), *c.x);
         if (!c.w || c.w->dim() != 1 || c.w->numel() != c.x->size(-1)) return false;
     }
     if (a[3] != Py_None) {
-        c.r = on(plain(a[3], c.x->scalar_type()), *c.x);
-        if (!c.r || c.r->sizes() != c.x->sizes()) return false;
+        c.r = on(lines_arg(a[3], c.lr), *c.x);
+        if (!c.r || c.r->scalar_type() != c.x->scalar_type() || c.r->sizes() != c.x->sizes()) return false;
+        const int64_t inner = std::max(c.lx.inner, c.lr.inner);
+        if (!in_runs(c.lx, inner) || !in_runs(c.lr, inner)) return false;
     }
     return !has_tangent(*c.x, c.w) && !(c.r && has_tangent(*c.r));
 }
 
 // (y, h or undefined)
-std::array<Tensor, 2> run_norm(const Tensor& x, const Tensor* w, double eps, const Tensor* r) {
+std::array<Tensor, 2> run_norm(const Tensor& x, const Lines& lx, const Tensor* w, double eps,
+                               const Tensor* r, const Lines& lr) {
     const int64_t k = x.size(-1), m = x.numel() / k;
     const void* st = current_stream(x);
     Tensor y, h;
@@ -978,8 +1045,8 @@ std::array<Tensor, 2> run_norm(const Tensor& x, const Tensor* w, double eps, con
         const c10::DeviceGuard on_x(x.device());
         y = empty(x.sizes(), x.scalar_type(), x);
         if (r) h = empty(x.sizes(), x.scalar_type(), x);
-        return g_lib.rms_norm(st, x.data_ptr(), type_of(x), k, r ? r->data_ptr() : nullptr, k,
-                              w ? w->data_ptr() : nullptr, w ? type_of(*w) : 0, float(eps), ptr(h),
+        return g_lib.rms_norm(st, x.data_ptr(), type_of(x), lx.ld, lx.outer, r ? r->data_ptr() : nullptr,
+                              lr.ld, lr.outer, lx.inner, w ? w->data_ptr() : nullptr, w ? type_of(*w) : 0, float(eps), ptr(h),
                               y.data_ptr(), m, k);
     });
     return {y, h};
@@ -987,9 +1054,10 @@ std::array<Tensor, 2> run_norm(const Tensor& x, const Tensor* w, double eps, con
 
 struct NormFn : torch::autograd::Function<NormFn> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& w,
-                                 double eps, const std::optional<Tensor>& r) {
+                                 double eps, const std::optional<Tensor>& r, const Lines& lx,
+                                 const Lines& lr) {
         ctx->set_materialize_grads(false);
-        auto [y, h] = run_norm(x, w ? &*w : nullptr, eps, r ? &*r : nullptr);
+        auto [y, h] = run_norm(x, lx, w ? &*w : nullptr, eps, r ? &*r : nullptr, lr);
         ctx->save_for_backward({r ? h : x, w ? *w : Tensor()});
         ctx->saved_data["eps"] = eps;
         if (r) return {y, h};
@@ -1009,9 +1077,19 @@ struct NormFn : torch::autograd::Function<NormFn> {
             } else {
                 const c10::DeviceGuard on_h(h.device());
                 const int64_t k = h.size(-1), m = h.numel() / k;
-                const Rows g = rows_of(dy);
-                Rows b{Tensor(), 0};
-                if (dh.defined()) b = rows_of(dh);
+                // h as it was normalised, its gradients in the same runs or copied
+                Lines lh, lg, lb;
+                if (!runs_of(h, lh)) check(1, "norm.rms_norm (gradient)");
+                auto lines = [&](const Tensor& t, Lines& l) {
+                    const Tensor r = t.resolve_neg();
+                    if (runs_of(r, l) && in_runs(l, lh.inner)) return r;
+                    l = Lines{1, k, k};
+                    in_runs(l, lh.inner);
+                    return r.contiguous();
+                };
+                const Tensor g = lines(dy, lg);
+                Tensor b;
+                if (dh.defined()) b = lines(dh, lb);
                 const int64_t need = want ? g_lib.rms_norm_grad_size(m, k) : 0;
                 if (need < 0) check(1, "norm.rms_norm (gradient)");
                 Tensor work;
@@ -1020,14 +1098,16 @@ struct NormFn : torch::autograd::Function<NormFn> {
                     dw = empty({k}, w.scalar_type(), h);
                 }
                 dx = empty(h.sizes(), h.scalar_type(), h);
-                check(g_lib.rms_norm_grad(stream_of(h), g.t.data_ptr(), type_of(h), g.ld, h.data_ptr(), k,
-                                          ptr(w), w.defined() ? type_of(w) : 0, ptr(b.t), b.ld, float(eps),
-                                          dx.data_ptr(), ptr(dw), m, k, ptr(work), need),
+                check(g_lib.rms_norm_grad(stream_of(h), g.data_ptr(), type_of(h), lg.ld, lg.outer,
+                                          h.data_ptr(), lh.ld, lh.outer, ptr(w),
+                                          w.defined() ? type_of(w) : 0, ptr(b), lb.ld, lb.outer, lh.inner,
+                                          float(eps), dx.data_ptr(), ptr(dw), m, k, ptr(work), need),
                       "norm.rms_norm (gradient)");
             }
-            // x, weight, eps, residual (needs_input_grad counts the tensors that are there)
+            // x, weight, eps, residual, their rows (needs_input_grad counts the tensors that are there)
             const bool to_r = in.size() > 1 && ctx->needs_input_grad(w.defined() ? 2 : 1);
-            return {ctx->needs_input_grad(0) ? dx : Tensor(), dw, Tensor(), to_r ? dx : Tensor()};
+            return {ctx->needs_input_grad(0) ? dx : Tensor(), dw, Tensor(), to_r ? dx : Tensor(), Tensor(),
+                    Tensor()};
         });
     }
 };
@@ -1038,10 +1118,11 @@ PyObject* host_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         NormCall c;
         if (!norm_call(a, c)) Py_RETURN_NONE;
         if (wants_grad(*c.x, c.w) || (c.r && wants_grad(*c.r))) {
-            const variable_list out = NormFn::apply(*c.x, maybe(c.w), c.eps, maybe(c.r));
+            for (const Tensor* t : {c.x, c.w, c.r}) check_leaf(t);
+            const variable_list out = NormFn::apply(*c.x, maybe(c.w), c.eps, maybe(c.r), c.lx, c.lr);
             return c.r ? wrapped(out) : THPVariable_Wrap(out[0]);
         }
-        auto [y, h] = run_norm(*c.x, c.w, c.eps, c.r);
+        auto [y, h] = run_norm(*c.x, c.lx, c.w, c.eps, c.r, c.lr);
         return c.r ? pair(y, h) : THPVariable_Wrap(y);
     });
 }
@@ -1063,7 +1144,8 @@ PyObject* host_rms_norm_int8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             q = empty(x.sizes(), at::kChar, x);
             s = empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
             if (c.r) h = empty(x.sizes(), x.scalar_type(), x);
-            return g_lib.rms_norm_int8(st, x.data_ptr(), type_of(x), k, c.r ? c.r->data_ptr() : nullptr, k,
+            return g_lib.rms_norm_int8(st, x.data_ptr(), type_of(x), c.lx.ld, c.lx.outer,
+                                       c.r ? c.r->data_ptr() : nullptr, c.lr.ld, c.lr.outer, c.lx.inner,
                                        c.w ? c.w->data_ptr() : nullptr, c.w ? type_of(*c.w) : 0,
                                        float(c.eps), ptr(h), static_cast<int8_t*>(q.data_ptr()),
                                        static_cast<float*>(s.data_ptr()), rotate, m, k);
@@ -1152,6 +1234,7 @@ PyObject* host_moe_route(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (renormalize < 0) throw python_error();
         how.renormalize = renormalize;
         if (wants_grad(*l)) {
+            check_leaf(l);
             return wrapped(RouteFn::apply(*l, maybe(b), int64_t(how.sigmoid), int64_t(how.renormalize),
                                           how.groups, how.top_groups, how.scale, top));
         }
@@ -1273,6 +1356,8 @@ PyObject* host_rotate_axes(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (split < 0) throw python_error();
         variable_list out(2);
         if (wants_grad(*q, k)) {
+            check_leaf(q);
+            check_leaf(k);
             const variable_list r = TurnFn::apply(*q, maybe(k), *positions, *inv_freq, *axis, split != 0);
             out[0] = r[0];
             if (k) out[1] = r[1];
@@ -1284,6 +1369,15 @@ PyObject* host_rotate_axes(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             });
         }
         return wrapped(out);
+    });
+}
+
+// check_leaves(tensors or Nones ..): the same for calls that go through Python
+PyObject* host_check_leaves(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, n_args, [&]() -> PyObject* {
+        for (Py_ssize_t i = 0; i < n_args; ++i)
+            if (THPVariable_Check(a[i])) check_leaf(&THPVariable_Unpack(a[i]));
+        Py_RETURN_NONE;
     });
 }
 
@@ -1331,6 +1425,7 @@ PyMethodDef kMethods[] = {XPU_HOST("bind", host_bind),
                           XPU_HOST("rms_norm_int8", host_rms_norm_int8),
                           XPU_HOST("moe_route", host_moe_route),
                           XPU_HOST("rotate_axes", host_rotate_axes),
+                          XPU_HOST("check_leaves", host_check_leaves),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host",
                        "The int8 API's hot calls in native code (see host_ops.cpp).", -1, kMethods};

@@ -32,14 +32,23 @@ struct NormArgs {
     void* h;
     void* y;              // int8 codes in the int8 form
     float* scale;
-    int64_t ldx, ldr, M, K;
+    Lines lx, lr;
+    int64_t M, K;
+    uint32_t inner;
     int weight_type;
     float eps;
 };
 
+// a row of an input: of `inner` rows each, by two strides
 template <int T>
-__device__ __forceinline__ const char* row_of(const void* p, int64_t row, int64_t ld) {
-    return static_cast<const char*>(p) + row * ld * kElem<T>;
+__device__ __forceinline__ const char* line_of(const void* p, int64_t row, uint32_t inner,
+                                               const Lines& l) {
+    int64_t at = row * l.outer;
+    if (inner > 1) {
+        const uint32_t o = uint32_t(row) / inner;
+        at = o * l.outer + int64_t(uint32_t(row) - o * inner) * l.ld;
+    }
+    return static_cast<const char*>(p) + at * kElem<T>;
 }
 template <int T>
 __device__ __forceinline__ char* row_of(void* p, int64_t row, int64_t ld) {
@@ -49,11 +58,11 @@ __device__ __forceinline__ char* row_of(void* p, int64_t row, int64_t ld) {
 // h's piece at d: read, added and (where there is a residual) stored
 template <int T, bool EVEN>
 __device__ __forceinline__ Piece8<T> stream_piece(const NormArgs& a, int64_t row, int64_t d) {
-    Piece8<T> p = piece_load<T, EVEN>(row_of<T>(a.x, row, a.ldx), d, a.K);
+    Piece8<T> p = piece_load<T, EVEN>(line_of<T>(a.x, row, a.inner, a.lx), d, a.K);
     if (a.residual) {
         float u[8], v[8];
         piece_expand(p, u);
-        piece_expand(piece_load<T, EVEN>(row_of<T>(a.residual, row, a.ldr), d, a.K), v);
+        piece_expand(piece_load<T, EVEN>(line_of<T>(a.residual, row, a.inner, a.lr), d, a.K), v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[i] += v[i];
         p = piece_round<T>(u);
@@ -183,8 +192,8 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
         const float m = fmaxf(most, 1e-30f), inv = 127.0f / m;
         if (INT8 && threadIdx.x == 0) a.scale[row] = r * m / 127.0f;
         // each thread reads what it has written itself
-        const char* from = a.residual ? row_of<T>(static_cast<const void*>(a.h), row, a.K)
-                                      : row_of<T>(a.x, row, a.ldx);
+        const char* from = a.residual ? row_of<T>(a.h, row, a.K)
+                                      : line_of<T>(a.x, row, a.inner, a.lx);
         for (int64_t d = 8 * int64_t(threadIdx.x); d < a.K; d += 8 * 1024) {
             float v[8], w[8];
             piece_expand(piece_load<T, EVEN>(from, d, a.K), v);
@@ -252,8 +261,8 @@ __global__ __launch_bounds__(1024) void norm_rotated_kernel(NormArgs a, int S, i
         if (r >= R || row >= a.M) return;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            x[i] = piece_load<T, EVEN>(row_of<T>(a.x, row, a.ldx), d + 8 * i, a.K);
-            if (a.residual) res[i] = piece_load<T, EVEN>(row_of<T>(a.residual, row, a.ldr), d + 8 * i, a.K);
+            x[i] = piece_load<T, EVEN>(line_of<T>(a.x, row, a.inner, a.lx), d + 8 * i, a.K);
+            if (a.residual) res[i] = piece_load<T, EVEN>(line_of<T>(a.residual, row, a.inner, a.lr), d + 8 * i, a.K);
         }
     };
 #pragma unroll
@@ -337,7 +346,8 @@ __global__ __launch_bounds__(1024) void norm_rotated_long_kernel(NormArgs a) {
         NormArgs b = a;                // h is there now; each lane reads what it has written
         if (a.residual) {
             b.x = a.h;
-            b.ldx = a.K;
+            b.lx = Lines{a.K, a.K};
+            b.inner = 1;
             b.residual = nullptr;
         }
         for (int64_t g0 = 0; g0 < groups; g0 += kMaxSegs) {
@@ -361,7 +371,9 @@ struct GradArgs {
     const void* dh;
     void* dx;
     float* part;          // [blocks, K], null: the weight's gradient is not wanted
-    int64_t ldy, ldh, lddh, M, K;
+    Lines ldy, lh, ldh;
+    int64_t M, K;
+    uint32_t inner;
     int weight_type;
     float eps;
 };
@@ -391,9 +403,9 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_grad_kernel(GradArgs a) {
             const int64_t d = 8 * (int64_t(i) * TPR + t);
             h[i] = dy[i] = dh[i] = Piece8<T>{};
             if (live && d < a.K) {
-                h[i] = piece_load<T, EVEN>(row_of<T>(a.h, row, a.ldh), d, a.K);
-                dy[i] = piece_load<T, EVEN>(row_of<T>(a.dy, row, a.ldy), d, a.K);
-                if (a.dh) dh[i] = piece_load<T, EVEN>(row_of<T>(a.dh, row, a.lddh), d, a.K);
+                h[i] = piece_load<T, EVEN>(line_of<T>(a.h, row, a.inner, a.lh), d, a.K);
+                dy[i] = piece_load<T, EVEN>(line_of<T>(a.dy, row, a.inner, a.ldy), d, a.K);
+                if (a.dh) dh[i] = piece_load<T, EVEN>(line_of<T>(a.dh, row, a.inner, a.ldh), d, a.K);
             }
         }
         float sum = 0.f, along = 0.f;
@@ -458,7 +470,7 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(GradArgs a) {
     __shared__ float2 slots[16];
     float* part = a.part ? a.part + int64_t(blockIdx.x) * a.K : nullptr;
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-        const char *hr = row_of<T>(a.h, row, a.ldh), *dyr = row_of<T>(a.dy, row, a.ldy);
+        const char *hr = line_of<T>(a.h, row, a.inner, a.lh), *dyr = line_of<T>(a.dy, row, a.inner, a.ldy);
         float sum = 0.f, along = 0.f;
         for (int64_t d = 8 * int64_t(threadIdx.x); d < a.K; d += 8 * 1024) {
             float u[8], g[8], w[8];
@@ -479,7 +491,7 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(GradArgs a) {
             piece_expand(piece_load<T, EVEN>(hr, d, a.K), u);
             piece_expand(piece_load<T, EVEN>(dyr, d, a.K), g);
             vector_load<EVEN>(a.weight, a.weight_type, d, a.K, w);
-            if (a.dh) piece_expand(piece_load<T, EVEN>(row_of<T>(a.dh, row, a.lddh), d, a.K), o);
+            if (a.dh) piece_expand(piece_load<T, EVEN>(line_of<T>(a.dh, row, a.inner, a.ldh), d, a.K), o);
             if (part && row != int64_t(blockIdx.x)) piece_expand(piece_load<kF32, EVEN>(part, d, a.K), dw);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -581,18 +593,18 @@ int grad_rows(int64_t K) { return K <= 64 ? 32 : K <= 128 ? 16 : K <= 256 ? 8 : 
 
 }  // namespace
 
-hipError_t rms_norm(hipStream_t st, const void* x, int type, int64_t ldx, const void* residual,
-                    int64_t ldr, const void* weight, int weight_type, float eps, void* h, void* y,
-                    int64_t M, int64_t K) {
-    return launch_norm<false>(st, type, NormArgs{x, residual, weight, h, y, nullptr, ldx, ldr, M, K,
-                                                 weight_type, eps});
+hipError_t rms_norm(hipStream_t st, const void* x, int type, const Lines& lx,
+                    const void* residual, const Lines& lr, int64_t inner, const void* weight,
+                    int weight_type, float eps, void* h, void* y, int64_t M, int64_t K) {
+    return launch_norm<false>(st, type, NormArgs{x, residual, weight, h, y, nullptr, lx, lr, M, K,
+                                                 uint32_t(inner), weight_type, eps});
 }
 
-hipError_t rms_norm_int8(hipStream_t st, const void* x, int type, int64_t ldx,
-                         const void* residual, int64_t ldr, const void* weight, int weight_type,
-                         float eps, void* h, int8_t* q, float* scale, bool rotate, int64_t M,
+hipError_t rms_norm_int8(hipStream_t st, const void* x, int type, const Lines& lx,
+                         const void* residual, const Lines& lr, int64_t inner,
+                         const void* weight, int weight_type, float eps, void* h, int8_t* q, float* scale, bool rotate, int64_t M,
                          int64_t K) {
-    const NormArgs a{x, residual, weight, h, q, scale, ldx, ldr, M, K, weight_type, eps};
+    const NormArgs a{x, residual, weight, h, q, scale, lx, lr, M, K, uint32_t(inner), weight_type, eps};
     if (!rotate) return launch_norm<true>(st, type, a);
     by_type(type, [&](auto t) {
         constexpr int T = decltype(t)::value;
@@ -600,12 +612,12 @@ hipError_t rms_norm_int8(hipStream_t st, const void* x, int type, int64_t ldx,
             // rows of few groups share a block of 16
             const int S = int(K / 256), R = S >= 16 ? 1 : 16 / S;
             const int threads = (S * R * 16 + 63) / 64 * 64;
-            // Blocks that together request 40 KB a CU (no fewer than one, no more than its 16
+            // Blocks that together request 40 KB a CU, 60 without a residual (no fewer than one, no more than its 16
             // waves): more rows under way at once are slower.  16381 x 5120 bf16 with a
             // residual (40 KB: 2 blocks): 118 us with 1, 111 with 2, 131 with 3, 123 with 6;
             // 8192 x 8192 85 with 1, 91 with 2; 20000 x 4096 without one 64 with 2, 52 with 4.
             const int bytes = threads * 16 * kElem<T> * (residual ? 2 : 1);
-            const int each = std::max(1, std::min(40960 / bytes, 1024 / threads));
+            const int each = std::max(1, std::min((residual ? 40960 : 61440) / bytes, 1024 / threads));
             const dim3 grid(blocks_for(M, R, int64_t(each) * device_cus()));
             if (S % 4 == 0)
                 hipLaunchKernelGGL((norm_rotated_kernel<T, 4>), grid, dim3(threads), 0, st, a, S, R);
@@ -623,12 +635,12 @@ int64_t rms_norm_grad_work_bytes(int64_t M, int64_t K) {
     return int64_t(blocks_for(M, grad_rows(K), kGradBlocks)) * K * 4;
 }
 
-hipError_t rms_norm_grad(hipStream_t st, const void* dy, int type, int64_t ldy, const void* h,
-                         int64_t ldh, const void* weight, int weight_type, const void* dh,
-                         int64_t lddh, float eps, void* dx, void* dweight, int64_t M, int64_t K,
+hipError_t rms_norm_grad(hipStream_t st, const void* dy, int type, const Lines& ldy,
+                         const void* h, const Lines& lh, const void* weight, int weight_type,
+                         const void* dh, const Lines& ldh, int64_t inner, float eps, void* dx, void* dweight, int64_t M, int64_t K,
                          float* part) {
-    const GradArgs a{dy, h, weight, dh, dx, dweight ? part : nullptr, ldy, ldh, lddh, M, K,
-                     weight_type, eps};
+    const GradArgs a{dy, h, weight, dh, dx, dweight ? part : nullptr, ldy, lh, ldh, M, K,
+                     uint32_t(inner), weight_type, eps};
     const unsigned blocks = blocks_for(M, grad_rows(K), kGradBlocks);
     by_type(type, [&](auto t) { by_even(K, [&](auto e) {
         constexpr int T = decltype(t)::value;

@@ -168,13 +168,13 @@ def _signatures():
                                      + [i64] * 3, c_int),
         "xpuint8_moe_route_grad_stream": ([vp, vp, i32, i64, vp, vp, i32, i32, f32, vp]
                                           + [i64] * 3, c_int),
-        "xpuint8_rms_norm_stream": ([vp, vp, i32, i64, vp, i64, vp, i32, f32, vp, vp, i64, i64],
-                                    c_int),
-        "xpuint8_rms_norm_int8_stream": ([vp, vp, i32, i64, vp, i64, vp, i32, f32, vp, vp, vp, i32,
-                                          i64, i64], c_int),
+        "xpuint8_rms_norm_stream": ([vp, vp, i32, i64, i64, vp, i64, i64, i64, vp, i32, f32, vp,
+                                     vp, i64, i64], c_int),
+        "xpuint8_rms_norm_int8_stream": ([vp, vp, i32, i64, i64, vp, i64, i64, i64, vp, i32, f32,
+                                          vp, vp, vp, i32, i64, i64], c_int),
         "xpuint8_rms_norm_grad_workspace_size": ([i64] * 2, i64),
-        "xpuint8_rms_norm_grad_stream": ([vp, vp, i32, i64, vp, i64, vp, i32, vp, i64, f32, vp, vp,
-                                          i64, i64, vp, i64], c_int),
+        "xpuint8_rms_norm_grad_stream": ([vp, vp, i32, i64, i64, vp, i64, i64, vp, i32, vp, i64,
+                                          i64, i64, f32, vp, vp, i64, i64, vp, i64], c_int),
         "xpuint8_rope_axes_stream": ([vp] * 4 + [i64] + [vp] * 3 + [i64, i32, vp, i32, vp, i64, vp,
                                                                     vp, i64, i32, i32] + [i64] * 3,
                                      c_int),

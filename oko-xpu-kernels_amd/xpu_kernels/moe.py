@@ -23,7 +23,7 @@ import torch
 
 from . import mxfp4
 from .int8 import _lib as L
-from .mxfp4 import TYPES, _check_float, _opt, _rows, _wants_grad, _work
+from .mxfp4 import TYPES, _check_float, _check_leaves, _opt, _rows, _wants_grad, _work
 
 __all__ = ["Routing", "combine", "dispatch", "ffn", "route", "sort"]
 
@@ -157,6 +157,7 @@ def route(logits, top, *, scores="softmax", bias=None, groups=1, top_groups=1, r
         bias = bias.detach().float().resolve_neg().contiguous()
     how = (int(scores == "sigmoid"), groups, top_groups, int(bool(renormalize)), float(scale))
     if _wants_grad(logits, bias):
+        _check_leaves(logits)
         return _RouteFn.apply(logits, bias, how, top)
     return _route(logits, bias, how, top)
 

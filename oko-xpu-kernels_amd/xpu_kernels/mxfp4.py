@@ -72,6 +72,12 @@ def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
+def _check_leaves(*tensors):
+    """Refuse a captured call whose backward pass would break the capture."""
+    if L.HOST is not None:
+        L.HOST.check_leaves(*tensors)
+
+
 def _check_pair(codes, scales, lead=None):
     """The K behind codes and scales, both on the GPU and of matching shapes."""
     for t, name in ((codes, "codes"), (scales, "scales")):

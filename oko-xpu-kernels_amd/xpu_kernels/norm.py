@@ -11,6 +11,8 @@ values of ``h`` in its type (bf16, fp16 or fp32) to the one rounding of ``y``; a
 squares beyond fp32's range makes the row zeros, as in fp32 arithmetic.  ``weight`` [K]
 is of any of the three types, or None for ones.  All of it runs in ``libxpuint8.so`` on
 torch's current stream without synchronising; there is no counterpart in the reference.
+Rows may lie evenly apart, or in even runs as the heads in the columns of a projection do
+(``qkv[..., :H * D].unflatten(-1, (H, D))``); other layouts are copied first.
 """
 
 from __future__ import annotations
@@ -18,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from .int8 import _lib as L
-from .mxfp4 import TYPES, _check_float, _opt, _rows, _wants_grad, _work
+from .mxfp4 import TYPES, _check_float, _check_leaves, _opt, _wants_grad, _work
 
 __all__ = ["rms_norm", "rms_norm_int8"]
 
@@ -48,6 +50,48 @@ def _check(x, weight, eps, residual):
             raise TypeError(f"residual is on {residual.device} but x is on {x.device}")
 
 
+def _runs(x):
+    """(inner, ld, outer) of the rows of ``x`` [.., K]: runs of ``inner`` rows, ld apart, runs
+    outer apart; None for rows that do not lie so, or overlap."""
+    k = x.shape[-1]
+    if x.stride(-1) != 1 and k > 1:
+        return None
+    levels = []                                  # (rows, stride), the innermost first
+    for n, s in reversed(list(zip(x.shape[:-1], x.stride()[:-1]))):
+        if n == 1:
+            continue
+        if levels and s == levels[-1][0] * levels[-1][1]:
+            levels[-1] = (levels[-1][0] * n, levels[-1][1])
+        else:
+            levels.append((n, s))
+    if not levels:
+        return 1, k, k
+    if len(levels) > 2 or levels[0][1] < k:
+        return None
+    if len(levels) == 1:
+        return 1, levels[0][1], levels[0][1]
+    return levels[0][0], levels[0][1], levels[1][1]
+
+
+def _lines(*tensors):
+    """The inputs (some None) as the kernels read them: (inner, [(tensor, ld, outer)])."""
+    tensors = [None if t is None else t.resolve_neg() for t in tensors]
+    runs = [None if t is None else _runs(t) for t in tensors]
+    inner = next((r[0] for r in runs if r is not None and r[0] > 1), 1)
+    out = []
+    for t, r in zip(tensors, runs):
+        if t is None:
+            out.append((None, 0, 0))
+            continue
+        if r is None or r[0] not in (1, inner):
+            t = t.contiguous()
+            r = 1, t.shape[-1], t.shape[-1]
+        if r[0] != inner:
+            r = inner, r[2], r[2] * inner
+        out.append((t, r[1], r[2]))
+    return inner, out
+
+
 def _weight(weight):
     """(the weight dense, its type's number)"""
     if weight is None:
@@ -59,15 +103,15 @@ def _forward(x, weight, eps, residual):
     """(y, h): h is None without a residual."""
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     h = None if residual is None else torch.empty_like(y)
-    x2, ldx = _rows(x)
-    if x2.shape[0]:
-        r2, ldr = (None, 0) if residual is None else _rows(residual)
+    if x.numel():
+        inner, ((x2, ldx, ox), (r2, ldr, outer_r)) = _lines(x, residual)
         w, wt = _weight(weight)
+        k = x.shape[-1]
         lib = L._lib()
         with L._on(x.device):
             if lib.xpuint8_rms_norm_stream(L._stream(x.device), x2.data_ptr(), TYPES[x.dtype], ldx,
-                                           _opt(r2), ldr, _opt(w), wt, eps, _opt(h), y.data_ptr(),
-                                           x2.shape[0], x2.shape[1]) != 0:
+                                           ox, _opt(r2), ldr, outer_r, inner, _opt(w), wt, eps,
+                                           _opt(h), y.data_ptr(), x.numel() // k, k) != 0:
                 L._err(lib, "norm.rms_norm")
     return y, h
 
@@ -76,21 +120,20 @@ def _backward(dy, h, weight, dh, eps, want_dweight):
     """(dx in h's shape, dweight or None)"""
     dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     dweight = torch.empty_like(weight, memory_format=torch.contiguous_format) if want_dweight else None
-    h2, ldh = _rows(h)
-    m, k = h2.shape
-    if not m:
+    if not h.numel():
         return dx, dweight.zero_() if want_dweight else None
-    dy2, ldy = _rows(dy)
-    dh2, lddh = (None, 0) if dh is None else _rows(dh)
+    k = h.shape[-1]
+    m = h.numel() // k
+    inner, ((h2, ldh, oh), (dy2, ldy, oy), (dh2, lddh, odh)) = _lines(h, dy, dh)
     w, wt = _weight(weight)
     lib = L._lib()
     need = lib.xpuint8_rms_norm_grad_workspace_size(m, k) if want_dweight else 0
     work = _work(need, h2)
     with L._on(h.device):
         if lib.xpuint8_rms_norm_grad_stream(L._stream(h.device), dy2.data_ptr(), TYPES[h.dtype], ldy,
-                                            h2.data_ptr(), ldh, _opt(w), wt, _opt(dh2), lddh, eps,
-                                            dx.data_ptr(), _opt(dweight), m, k, _opt(work),
-                                            need) != 0:
+                                            oy, h2.data_ptr(), ldh, oh, _opt(w), wt, _opt(dh2),
+                                            lddh, odh, inner, eps, dx.data_ptr(), _opt(dweight), m,
+                                            k, _opt(work), need) != 0:
             L._err(lib, "norm.rms_norm (gradient)")
     return dx, dweight
 
@@ -129,6 +172,7 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None):
     _check(x, weight, eps, residual)
     eps = float(eps)
     if _wants_grad(x, weight, residual):
+        _check_leaves(x, weight, residual)
         return _NormFn.apply(x, weight, eps, residual)
     y, h = _forward(x, weight, eps, residual)
     return y if h is None else (y, h)
@@ -161,15 +205,14 @@ def rms_norm_int8(x, weight=None, eps=1e-6, residual=None, rotate=True):
     q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    x2, ldx = _rows(x)
-    if x2.shape[0]:
-        r2, ldr = (None, 0) if residual is None else _rows(residual)
+    if x.numel():
+        inner, ((x2, ldx, ox), (r2, ldr, outer_r)) = _lines(x, residual)
         w, wt = _weight(weight)
         lib = L._lib()
         with L._on(x.device):
             if lib.xpuint8_rms_norm_int8_stream(L._stream(x.device), x2.data_ptr(), TYPES[x.dtype],
-                                                ldx, _opt(r2), ldr, _opt(w), wt, float(eps),
-                                                _opt(h), q.data_ptr(), scale.data_ptr(),
-                                                1 if rotate else 0, x2.shape[0], k) != 0:
+                                                ldx, ox, _opt(r2), ldr, outer_r, inner, _opt(w), wt,
+                                                float(eps), _opt(h), q.data_ptr(), scale.data_ptr(),
+                                                1 if rotate else 0, x.numel() // k, k) != 0:
                 L._err(lib, "norm.rms_norm_int8")
     return (q, scale) if h is None else (q, scale, h)

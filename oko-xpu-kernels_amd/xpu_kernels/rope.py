@@ -19,7 +19,7 @@ from typing import NamedTuple
 import torch
 
 from .int8 import _lib as L
-from .mxfp4 import TYPES, _check_float, _opt, _wants_grad
+from .mxfp4 import TYPES, _check_float, _check_leaves, _opt, _wants_grad
 
 __all__ = ["AxisFrequencies", "axis_frequencies", "rms_rope_split_half_dequant", "rotate_axes",
            "rows_dq"]
@@ -244,6 +244,7 @@ def rotate_axes(q, k, positions, frequencies, *, split_half=True):
         raise ValueError("positions get no gradient")
     positions = positions.detach().resolve_neg()
     if _wants_grad(q, k):
+        _check_leaves(q, k)
         r = _TurnFn.apply(q, k, positions, *frequencies, bool(split_half))
         return (r, None) if k is None else r
     return _turn(q, k, positions, frequencies, False, bool(split_half))

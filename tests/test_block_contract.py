@@ -61,18 +61,18 @@ def lib():
 
 
 def norm_args(**kw):
-    a = dict(st=Z, x=P, type=0, ldx=64, r=Z, ldr=0, w=P, wt=2, eps=1e-6, h=Z, y=P, M=4, K=64)
+    a = dict(st=Z, x=P, type=0, ldx=64, ox=64, r=Z, ldr=0, outer_r=0, inner=1, w=P, wt=2, eps=1e-6, h=Z, y=P, M=4, K=64)
     return tuple({**a, **kw}.values())
 
 
 def int8_args(**kw):
-    a = dict(st=Z, x=P, type=0, ldx=256, r=Z, ldr=0, w=P, wt=2, eps=1e-6, h=Z, q=P, s=P, rot=1, M=4,
+    a = dict(st=Z, x=P, type=0, ldx=256, ox=256, r=Z, ldr=0, outer_r=0, inner=1, w=P, wt=2, eps=1e-6, h=Z, q=P, s=P, rot=1, M=4,
              K=256)
     return tuple({**a, **kw}.values())
 
 
 def grad_args(**kw):
-    a = dict(st=Z, dy=P, type=0, ldy=64, h=P, ldh=64, w=P, wt=2, dh=Z, lddh=0, eps=1e-6, dx=P, dw=P,
+    a = dict(st=Z, dy=P, type=0, ldy=64, oy=64, h=P, ldh=64, oh=64, w=P, wt=2, dh=Z, lddh=0, odh=0, inner=1, eps=1e-6, dx=P, dw=P,
              M=4, K=64, work=P, n=1 << 20)
     return tuple({**a, **kw}.values())
 
@@ -96,22 +96,25 @@ def route_grad_args(**kw):
 
 @pytest.mark.parametrize("fn,args,code,substr", [
     ("rms_norm", norm_args(M=0), 2, "positive"), ("rms_norm", norm_args(K=0), 2, "positive"),
-    ("rms_norm", norm_args(M=1 << 31), 4, "2^31"), ("rms_norm", norm_args(K=1 << 25, ldx=1 << 25), 4, "2^24"),
+    ("rms_norm", norm_args(M=1 << 31), 4, "2^31"), ("rms_norm", norm_args(K=1 << 25, ox=1 << 25), 4, "2^24"),
     ("rms_norm", norm_args(type=3), 6, "type"), ("rms_norm", norm_args(wt=3), 6, "weight_type"),
-    ("rms_norm", norm_args(ldx=63), 2, "stride"), ("rms_norm", norm_args(r=P, ldr=63, h=P), 2, "stride"),
+    ("rms_norm", norm_args(ox=63), 2, "stride"), ("rms_norm", norm_args(r=P, outer_r=63, h=P), 2, "stride"),
     ("rms_norm", norm_args(eps=-1.0), 2, "eps"), ("rms_norm", norm_args(eps=float("nan")), 2, "eps"),
     ("rms_norm", norm_args(x=Z), 6, "null"), ("rms_norm", norm_args(x=ODD), 6, "aligned"),
-    ("rms_norm", norm_args(r=P, ldr=64), 6, "together"), ("rms_norm", norm_args(h=P), 6, "together"),
-    ("rms_norm", norm_args(r=ODD, ldr=64, h=P), 6, "aligned"),
-    ("rms_norm", norm_args(r=P, ldr=64, h=B8), 6, "16-byte"), ("rms_norm", norm_args(w=ODD), 6, "weight"),
+    ("rms_norm", norm_args(r=P, outer_r=64), 6, "together"), ("rms_norm", norm_args(h=P), 6, "together"),
+    ("rms_norm", norm_args(r=ODD, outer_r=64, h=P), 6, "aligned"),
+    ("rms_norm", norm_args(r=P, outer_r=64, h=B8), 6, "16-byte"), ("rms_norm", norm_args(w=ODD), 6, "weight"),
     ("rms_norm", norm_args(y=Z), 6, "null"), ("rms_norm", norm_args(y=B8), 6, "16-byte"),
+    ("rms_norm", norm_args(inner=0), 2, "inner"), ("rms_norm", norm_args(inner=3), 2, "divide"),
+    ("rms_norm", norm_args(inner=2, ldx=63, ox=128), 2, "stride"), ("rms_norm", norm_args(inner=2, ox=-1), 2, "stride"),
+    ("rms_norm_grad", grad_args(inner=3), 2, "divide"), ("rms_norm_grad", grad_args(inner=2, ldh=63), 2, "stride"),
     ("rms_norm_int8", int8_args(K=255), 3, "256"), ("rms_norm_int8", int8_args(rot=2), 2, "rotate"),
     ("rms_norm_int8", int8_args(q=Z), 6, "null"), ("rms_norm_int8", int8_args(s=B8), 6, "16-byte"),
     ("rms_norm_int8", int8_args(M=-1), 2, "positive"),
     ("rms_norm_grad", grad_args(M=0), 2, "positive"), ("rms_norm_grad", grad_args(type=-1), 6, "type"),
-    ("rms_norm_grad", grad_args(ldy=63), 2, "stride"), ("rms_norm_grad", grad_args(ldh=63), 2, "stride"),
-    ("rms_norm_grad", grad_args(dh=P, lddh=63), 2, "stride"), ("rms_norm_grad", grad_args(dy=Z), 6, "null"),
-    ("rms_norm_grad", grad_args(dh=ODD, lddh=64), 6, "aligned"), ("rms_norm_grad", grad_args(dx=B8), 6, "16-byte"),
+    ("rms_norm_grad", grad_args(oy=63), 2, "stride"), ("rms_norm_grad", grad_args(oh=63), 2, "stride"),
+    ("rms_norm_grad", grad_args(dh=P, odh=63), 2, "stride"), ("rms_norm_grad", grad_args(dy=Z), 6, "null"),
+    ("rms_norm_grad", grad_args(dh=ODD, odh=64), 6, "aligned"), ("rms_norm_grad", grad_args(dx=B8), 6, "16-byte"),
     ("rms_norm_grad", grad_args(w=Z), 6, "needs a weight"), ("rms_norm_grad", grad_args(work=Z), 6, "work"),
     ("rms_norm_grad", grad_args(n=4 * 64 - 1), 2, "workspace_size"),
     ("rope_axes", rope_args(B=0), 2, "positive"), ("rope_axes", rope_args(S=1 << 31), 4, "2^31"),

@@ -171,6 +171,29 @@ def test_layouts(dev, dtype):
         a, = torch.autograd.grad(norm.rms_norm(xg, w[:k]), xg, dy)
         b, = torch.autograd.grad(norm.rms_norm(xs, w[:k]), xs, wide[..., 1:k + 1])
         assert torch.equal(a, b)
+    # heads in the columns of one projection, and layouts that are neither rows nor runs
+    qkv = stream(12, 3 * 4 * 72 + 5, dtype, 2).to(dev).reshape(3, 4, -1)
+    wq = (1 + 0.2 * randn(72, seed=3)).to(dev)
+    q, k = (qkv[..., i * 288 + 1:(i + 1) * 288 + 1].unflatten(-1, (4, 72)) for i in (0, 1))
+    for x, r in ((q, k), (q, k.contiguous()), (q.contiguous(), k), (q.transpose(1, 2), k.transpose(1, 2)),
+                 (q[:, ::2], k[:, 1::2]), (q[:, :, ::2], k[:, :, ::2]), (q, k.transpose(0, 1).contiguous().transpose(0, 1)),
+                 (q[:1], k[:1]), (q[:, :1], k[:, :1]), (q[:, :, :1], k[:, :, :1]),
+                 (q[:1].expand(3, 4, 4, 72), k[:, :1].expand(3, 4, 4, 72)), (q[:, :, :1].expand(3, 4, 4, 72), k)):
+        xc, rc = x.contiguous(), r.contiguous()
+        y, h = norm.rms_norm(x, wq, residual=r)
+        yc, hc = norm.rms_norm(xc, wq, residual=rc)
+        assert torch.equal(y, yc) and torch.equal(h, hc) and torch.equal(norm.rms_norm(x, wq), norm.rms_norm(xc, wq))
+        for a, b in zip(norm.rms_norm_int8(x, wq, residual=r, rotate=False),
+                        norm.rms_norm_int8(xc, wq, residual=rc, rotate=False)):
+            assert torch.equal(a, b)
+        for dy in (r, rc):
+            xs, xg = x.detach().requires_grad_(), xc.clone().requires_grad_()
+            a, = torch.autograd.grad(norm.rms_norm(xs, wq), xs, dy)
+            b, = torch.autograd.grad(norm.rms_norm(xg, wq), xg, rc)
+            assert torch.equal(a, b)
+            a = torch.autograd.grad(norm.rms_norm(xs, wq, residual=r), xs, (dy, x))
+            b = torch.autograd.grad(norm.rms_norm(xg, wq, residual=rc), xg, (rc, xc))
+            assert torch.equal(a[0], b[0])
     empty = torch.empty(0, 1280, dtype=dtype, device=dev)
     assert norm.rms_norm(empty, w[:1280]).shape == (0, 1280)
     q, s, h = norm.rms_norm_int8(empty, w[:1280], residual=empty)
