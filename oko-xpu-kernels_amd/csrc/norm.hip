@@ -107,15 +107,30 @@ __device__ __forceinline__ void codes_store(int8_t* row, int64_t d, int64_t n, c
         p->y = q.y;
         return;
     }
-    for (int i = 0; i < 8; ++i)
-        if (d + i < n) row[d + i] = int8_t((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+    struct __attribute__((packed, aligned(1))) Four { uint32_t v; };
+    struct __attribute__((packed, aligned(1))) Two { uint16_t v; };
+    const int c = int(n - d);          // 1..7: in runs of 4, 2 and 1
+    if (c & 4) reinterpret_cast<Four*>(row + d)->v = q.x;
+    const uint32_t rest = c & 4 ? q.y : q.x;
+    if (c & 2) reinterpret_cast<Two*>(row + d + (c & 4))->v = uint16_t(rest);
+    if (c & 1) row[d + c - 1] = int8_t(rest >> (c & 2 ? 16 : 0));
 }
 
 template <int TPR>
 constexpr int kThreads = TPR > 256 ? TPR : 256;
 
+// Rows that are not whole pieces.  Where a row has 8 values at least, its last piece is the
+// last 8 of them: it overlaps the piece before, the values of both are the same and are
+// written twice, and sums leave the first `skip` of them out.  Shorter rows go value by value.
+enum Cut : int { kWhole = 0, kOverlap = 1, kShort = 2 };
+constexpr bool whole(int cut) { return cut != kShort; }
+template <int CUT>
+__device__ __forceinline__ int64_t place(int64_t d, int64_t K) {
+    return CUT == kOverlap && d > K - 8 ? K - 8 : d;
+}
+
 // TPR threads a row, P pieces of 8 a thread: piece i of thread t is 8 (i TPR + t).
-template <int T, int TPR, int P, bool INT8, bool EVEN>
+template <int T, int TPR, int P, bool INT8, int CUT>
 __global__ __launch_bounds__(kThreads<TPR>) void norm_kernel(NormArgs a) {
     __shared__ float2 slots[16];
     constexpr int R = kThreads<TPR> / TPR;
@@ -129,8 +144,9 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_kernel(NormArgs a) {
         for (int i = 0; i < P; ++i) {
             const int64_t d = 8 * (int64_t(i) * TPR + t);
             if (live && d < a.K) {
-                p[i] = stream_piece<T, EVEN>(a, row, d);
-                vector_load<EVEN>(a.weight, a.weight_type, d, a.K, w[i]);
+                const int64_t at = place<CUT>(d, a.K);
+                p[i] = stream_piece<T, whole(CUT)>(a, row, at);
+                vector_load<whole(CUT)>(a.weight, a.weight_type, at, a.K, w[i]);
             } else {
                 p[i] = Piece8<T>{};
             }
@@ -140,9 +156,12 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_kernel(NormArgs a) {
         for (int i = 0; i < P; ++i) {
             float v[8];
             piece_expand(p[i], v);
-            if (!(live && 8 * (int64_t(i) * TPR + t) < a.K)) continue;
+            const int64_t d = 8 * (int64_t(i) * TPR + t);
+            if (!(live && d < a.K)) continue;
+            const int skip = int(d - place<CUT>(d, a.K));
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
+                if (CUT == kOverlap && j < skip) continue;
                 sum = __builtin_fmaf(v[j], v[j], sum);
                 if constexpr (INT8) most = fmaxf(most, fabsf(v[j] * w[i][j]));
             }
@@ -154,35 +173,39 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_kernel(NormArgs a) {
         if (INT8 && t == 0) a.scale[row] = r * m / 127.0f;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int64_t d = 8 * (int64_t(i) * TPR + t);
+            int64_t d = 8 * (int64_t(i) * TPR + t);
             if (d >= a.K) continue;
+            d = place<CUT>(d, a.K);
             float v[8];
             piece_expand(p[i], v);
             if constexpr (INT8) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = v[j] * w[i][j] * inv;
-                codes_store<EVEN>(static_cast<int8_t*>(a.y) + row * a.K, d, a.K, rint_pack8(v));
+                codes_store<whole(CUT)>(static_cast<int8_t*>(a.y) + row * a.K, d, a.K, rint_pack8(v));
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = v[j] * r * w[i][j];
-                piece_store<T, EVEN>(row_of<T>(a.y, row, a.K), d, a.K, piece_round<T>(v));
+                piece_store<T, whole(CUT)>(row_of<T>(a.y, row, a.K), d, a.K, piece_round<T>(v));
             }
         }
     }
 }
 
 // Rows of more than 32768: a block a row, which is read again (h, from cache) to be written.
-template <int T, bool INT8, bool EVEN>
+template <int T, bool INT8, int CUT>
 __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
     __shared__ float2 slots[16];
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
         float sum = 0.f, most = 0.f;
         for (int64_t d = 8 * int64_t(threadIdx.x); d < a.K; d += 8 * 1024) {
+            const int64_t at = place<CUT>(d, a.K);
+            const int skip = int(d - at);
             float v[8], w[8];
-            piece_expand(stream_piece<T, EVEN>(a, row, d), v);
-            if constexpr (INT8) vector_load<EVEN>(a.weight, a.weight_type, d, a.K, w);
+            piece_expand(stream_piece<T, whole(CUT)>(a, row, at), v);
+            if constexpr (INT8) vector_load<whole(CUT)>(a.weight, a.weight_type, at, a.K, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
+                if (CUT == kOverlap && j < skip) continue;
                 sum = __builtin_fmaf(v[j], v[j], sum);
                 if constexpr (INT8) most = fmaxf(most, fabsf(v[j] * w[j]));
             }
@@ -191,21 +214,22 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
         const float r = inverse_rms(sum, a.K, a.eps);
         const float m = fmaxf(most, 1e-30f), inv = 127.0f / m;
         if (INT8 && threadIdx.x == 0) a.scale[row] = r * m / 127.0f;
-        // each thread reads what it has written itself
+        // each thread reads what it has written itself (an overlapping piece too)
         const char* from = a.residual ? row_of<T>(a.h, row, a.K)
                                       : line_of<T>(a.x, row, a.inner, a.lx);
-        for (int64_t d = 8 * int64_t(threadIdx.x); d < a.K; d += 8 * 1024) {
+        for (int64_t at = 8 * int64_t(threadIdx.x); at < a.K; at += 8 * 1024) {
+            const int64_t d = place<CUT>(at, a.K);
             float v[8], w[8];
-            piece_expand(piece_load<T, EVEN>(from, d, a.K), v);
-            vector_load<EVEN>(a.weight, a.weight_type, d, a.K, w);
+            piece_expand(piece_load<T, whole(CUT)>(from, d, a.K), v);
+            vector_load<whole(CUT)>(a.weight, a.weight_type, d, a.K, w);
             if constexpr (INT8) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = v[j] * w[j] * inv;
-                codes_store<EVEN>(static_cast<int8_t*>(a.y) + row * a.K, d, a.K, rint_pack8(v));
+                codes_store<whole(CUT)>(static_cast<int8_t*>(a.y) + row * a.K, d, a.K, rint_pack8(v));
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = v[j] * r * w[j];
-                piece_store<T, EVEN>(row_of<T>(a.y, row, a.K), d, a.K, piece_round<T>(v));
+                piece_store<T, whole(CUT)>(row_of<T>(a.y, row, a.K), d, a.K, piece_round<T>(v));
             }
         }
     }
@@ -380,7 +404,7 @@ struct GradArgs {
 
 // A block walks over its rows and keeps the weight's gradient over them in registers; the
 // blocks' sums are added in order by a launch of their own.
-template <int T, int TPR, int P, bool EVEN>
+template <int T, int TPR, int P, int CUT>
 __global__ __launch_bounds__(kThreads<TPR>) void norm_grad_kernel(GradArgs a) {
     __shared__ float2 slots[16];
     constexpr int R = kThreads<TPR> / TPR;
@@ -392,7 +416,7 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_grad_kernel(GradArgs a) {
         const int64_t d = 8 * (int64_t(i) * TPR + t);
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[i][j] = dw[i][j] = 0.f;
-        if (d < a.K) vector_load<EVEN>(a.weight, a.weight_type, d, a.K, w[i]);
+        if (d < a.K) vector_load<whole(CUT)>(a.weight, a.weight_type, place<CUT>(d, a.K), a.K, w[i]);
     }
     for (int64_t row0 = int64_t(blockIdx.x) * R; row0 < a.M; row0 += int64_t(gridDim.x) * R) {
         const int64_t row = row0 + mine;
@@ -403,19 +427,23 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_grad_kernel(GradArgs a) {
             const int64_t d = 8 * (int64_t(i) * TPR + t);
             h[i] = dy[i] = dh[i] = Piece8<T>{};
             if (live && d < a.K) {
-                h[i] = piece_load<T, EVEN>(line_of<T>(a.h, row, a.inner, a.lh), d, a.K);
-                dy[i] = piece_load<T, EVEN>(line_of<T>(a.dy, row, a.inner, a.ldy), d, a.K);
-                if (a.dh) dh[i] = piece_load<T, EVEN>(line_of<T>(a.dh, row, a.inner, a.ldh), d, a.K);
+                const int64_t at = place<CUT>(d, a.K);
+                h[i] = piece_load<T, whole(CUT)>(line_of<T>(a.h, row, a.inner, a.lh), at, a.K);
+                dy[i] = piece_load<T, whole(CUT)>(line_of<T>(a.dy, row, a.inner, a.ldy), at, a.K);
+                if (a.dh) dh[i] = piece_load<T, whole(CUT)>(line_of<T>(a.dh, row, a.inner, a.ldh), at, a.K);
             }
         }
         float sum = 0.f, along = 0.f;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
+            const int64_t d = 8 * (int64_t(i) * TPR + t);
+            const int skip = int(d - place<CUT>(d, a.K));
             float u[8], g[8];
             piece_expand(h[i], u);
             piece_expand(dy[i], g);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
+                if (CUT == kOverlap && j < skip) continue;
                 sum = __builtin_fmaf(u[j], u[j], sum);
                 along = __builtin_fmaf(g[j] * w[i][j], u[j], along);
             }
@@ -426,26 +454,31 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_grad_kernel(GradArgs a) {
         const float back = r * r * r * (along / float(a.K));
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int64_t d = 8 * (int64_t(i) * TPR + t);
+            int64_t d = 8 * (int64_t(i) * TPR + t);
             if (d >= a.K) continue;
+            const int skip = int(d - place<CUT>(d, a.K));
+            d -= skip;
             float u[8], g[8], o[8];
             piece_expand(h[i], u);
             piece_expand(dy[i], g);
             piece_expand(dh[i], o);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                dw[i][j] = __builtin_fmaf(g[j], u[j] * r, dw[i][j]);
+                if (!(CUT == kOverlap && j < skip)) dw[i][j] = __builtin_fmaf(g[j], u[j] * r, dw[i][j]);
                 o[j] += __builtin_fmaf(g[j] * w[i][j], r, -(u[j] * back));
             }
-            piece_store<T, EVEN>(row_of<T>(a.dx, row, a.K), d, a.K, piece_round<T>(o));
+            piece_store<T, whole(CUT)>(row_of<T>(a.dx, row, a.K), d, a.K, piece_round<T>(o));
         }
     }
     if (!a.part) return;
     if constexpr (R > 1) {             // the block's rows side by side: one sum
 #pragma unroll
-        for (int i = 0; i < P; ++i)
+        for (int i = 0; i < P; ++i) {
+            const int d = 8 * (i * TPR + t), skip = d < a.K ? int(d - place<CUT>(d, a.K)) : 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) cols[mine][8 * (i * TPR + t) + j] = dw[i][j];
+            for (int j = 0; j < 8; ++j)
+                if (!(CUT == kOverlap && j < skip)) cols[mine][d - skip + j] = dw[i][j];
+        }
         __syncthreads();
         for (int c = threadIdx.x; c < a.K; c += kThreads<TPR>) {
             float s = 0.f;
@@ -457,15 +490,23 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_grad_kernel(GradArgs a) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int64_t d = 8 * (int64_t(i) * TPR + t);
-            if (d < a.K)
-                piece_store<kF32, EVEN>(a.part + int64_t(blockIdx.x) * a.K, d, a.K, piece_round<kF32>(dw[i]));
+            if (d >= a.K) continue;
+            float* to = a.part + int64_t(blockIdx.x) * a.K;
+            if (CUT == kOverlap && d > a.K - 8) {
+                const int skip = int(d - (a.K - 8));
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j >= skip) to[a.K - 8 + j] = dw[i][j];
+            } else {
+                piece_store<kF32, whole(CUT)>(to, d, a.K, piece_round<kF32>(dw[i]));
+            }
         }
     }
 }
 
 // Rows longer than a block's registers: read twice, the weight's gradient kept in `part`
 // (every thread its own columns).
-template <int T, bool EVEN>
+template <int T, int CUT>
 __global__ __launch_bounds__(1024) void norm_grad_long_kernel(GradArgs a) {
     __shared__ float2 slots[16];
     float* part = a.part ? a.part + int64_t(blockIdx.x) * a.K : nullptr;
@@ -473,12 +514,15 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(GradArgs a) {
         const char *hr = line_of<T>(a.h, row, a.inner, a.lh), *dyr = line_of<T>(a.dy, row, a.inner, a.ldy);
         float sum = 0.f, along = 0.f;
         for (int64_t d = 8 * int64_t(threadIdx.x); d < a.K; d += 8 * 1024) {
+            const int64_t at = place<CUT>(d, a.K);
+            const int skip = int(d - at);
             float u[8], g[8], w[8];
-            piece_expand(piece_load<T, EVEN>(hr, d, a.K), u);
-            piece_expand(piece_load<T, EVEN>(dyr, d, a.K), g);
-            vector_load<EVEN>(a.weight, a.weight_type, d, a.K, w);
+            piece_expand(piece_load<T, whole(CUT)>(hr, at, a.K), u);
+            piece_expand(piece_load<T, whole(CUT)>(dyr, at, a.K), g);
+            vector_load<whole(CUT)>(a.weight, a.weight_type, at, a.K, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
+                if (CUT == kOverlap && j < skip) continue;
                 sum = __builtin_fmaf(u[j], u[j], sum);
                 along = __builtin_fmaf(g[j] * w[j], u[j], along);
             }
@@ -487,19 +531,22 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(GradArgs a) {
         const float r = inverse_rms(sum, a.K, a.eps);
         const float back = r * r * r * (along / float(a.K));
         for (int64_t d = 8 * int64_t(threadIdx.x); d < a.K; d += 8 * 1024) {
-            float u[8], g[8], w[8], o[8] = {}, dw[8] = {};
-            piece_expand(piece_load<T, EVEN>(hr, d, a.K), u);
-            piece_expand(piece_load<T, EVEN>(dyr, d, a.K), g);
-            vector_load<EVEN>(a.weight, a.weight_type, d, a.K, w);
-            if (a.dh) piece_expand(piece_load<T, EVEN>(line_of<T>(a.dh, row, a.inner, a.ldh), d, a.K), o);
-            if (part && row != int64_t(blockIdx.x)) piece_expand(piece_load<kF32, EVEN>(part, d, a.K), dw);
+            const int64_t at = place<CUT>(d, a.K);
+            const int skip = int(d - at);
+            float u[8], g[8], w[8], o[8] = {};
+            piece_expand(piece_load<T, whole(CUT)>(hr, at, a.K), u);
+            piece_expand(piece_load<T, whole(CUT)>(dyr, at, a.K), g);
+            vector_load<whole(CUT)>(a.weight, a.weight_type, at, a.K, w);
+            if (a.dh)
+                piece_expand(piece_load<T, whole(CUT)>(line_of<T>(a.dh, row, a.inner, a.ldh), at, a.K), o);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                dw[j] = __builtin_fmaf(g[j], u[j] * r, dw[j]);
+                const float term = g[j] * (u[j] * r);
+                if (part && j >= skip && at + j < a.K)
+                    part[at + j] = row == int64_t(blockIdx.x) ? term : part[at + j] + term;
                 o[j] += __builtin_fmaf(g[j] * w[j], r, -(u[j] * back));
             }
-            piece_store<T, EVEN>(row_of<T>(a.dx, row, a.K), d, a.K, piece_round<T>(o));
-            if (part) piece_store<kF32, EVEN>(part, d, a.K, piece_round<kF32>(dw));
+            piece_store<T, whole(CUT)>(row_of<T>(a.dx, row, a.K), at, a.K, piece_round<T>(o));
         }
     }
 }
@@ -535,9 +582,10 @@ void by_type(int type, const F& f) {
     else f(std::integral_constant<int, kF32>{});
 }
 template <class F>
-void by_even(int64_t K, const F& f) {
-    if (K % 8 == 0) f(std::true_type{});
-    else f(std::false_type{});
+void by_cut(int64_t K, const F& f) {
+    if (K % 8 == 0) f(std::integral_constant<int, kWhole>{});
+    else if (K > 8) f(std::integral_constant<int, kOverlap>{});
+    else f(std::integral_constant<int, kShort>{});
 }
 template <int A, int B>
 struct Shape {
@@ -571,16 +619,18 @@ unsigned blocks_for(int64_t M, int rows, int64_t most) {
 
 template <bool INT8>
 hipError_t launch_norm(hipStream_t st, int type, const NormArgs& a) {
-    by_type(type, [&](auto t) { by_even(a.K, [&](auto e) {
+    by_type(type, [&](auto t) { by_cut(a.K, [&](auto e) {
         constexpr int T = decltype(t)::value;
-        constexpr bool EVEN = decltype(e)::value;
+        constexpr int CUT = decltype(e)::value;
         const bool done = by_length(a.K, [&](auto s) {
             constexpr int TPR = decltype(s)::tpr, P = decltype(s)::p, N = kThreads<TPR>;
-            hipLaunchKernelGGL((norm_kernel<T, TPR, P, INT8, EVEN>),
+            if constexpr (CUT != kShort || TPR == 8)
+                hipLaunchKernelGGL((norm_kernel<T, TPR, P, INT8, CUT>),
                                dim3(blocks_for(a.M, N / TPR, kRowBlocks)), dim3(N), 0, st, a);
         });
-        if (!done)
-            hipLaunchKernelGGL((norm_long_kernel<T, INT8, EVEN>),
+        if constexpr (CUT != kShort)
+            if (!done)
+                hipLaunchKernelGGL((norm_long_kernel<T, INT8, CUT>),
                                dim3(blocks_for(a.M, 1, kRowBlocks)), dim3(1024), 0, st, a);
     }); });
     return hipGetLastError();
@@ -642,16 +692,17 @@ hipError_t rms_norm_grad(hipStream_t st, const void* dy, int type, const Lines& 
     const GradArgs a{dy, h, weight, dh, dx, dweight ? part : nullptr, ldy, lh, ldh, M, K,
                      uint32_t(inner), weight_type, eps};
     const unsigned blocks = blocks_for(M, grad_rows(K), kGradBlocks);
-    by_type(type, [&](auto t) { by_even(K, [&](auto e) {
+    by_type(type, [&](auto t) { by_cut(K, [&](auto e) {
         constexpr int T = decltype(t)::value;
-        constexpr bool EVEN = decltype(e)::value;
+        constexpr int CUT = decltype(e)::value;
         const bool done = K <= 16384 && by_length(K, [&](auto s) {
             constexpr int TPR = decltype(s)::tpr, P = decltype(s)::p, N = kThreads<TPR>;
-            if constexpr (TPR * P <= 2048)
-                hipLaunchKernelGGL((norm_grad_kernel<T, TPR, P, EVEN>), dim3(blocks), dim3(N), 0, st, a);
+            if constexpr (TPR * P <= 2048 && (CUT != kShort || TPR == 8))
+                hipLaunchKernelGGL((norm_grad_kernel<T, TPR, P, CUT>), dim3(blocks), dim3(N), 0, st, a);
         });
-        if (!done)
-            hipLaunchKernelGGL((norm_grad_long_kernel<T, EVEN>), dim3(blocks), dim3(1024), 0, st, a);
+        if constexpr (CUT != kShort)
+            if (!done)
+                hipLaunchKernelGGL((norm_grad_long_kernel<T, CUT>), dim3(blocks), dim3(1024), 0, st, a);
     }); });
     if (!dweight) return hipGetLastError();
     by_type(weight_type, [&](auto t) {

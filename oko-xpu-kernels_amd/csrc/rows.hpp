@@ -25,18 +25,48 @@ struct __attribute__((packed, aligned(T == kF32 ? 4 : 2))) Loose8 {
     uint32_t w[T == kF32 ? 8 : 4];
 };
 
-// the piece at d < n of a row of n; EVEN: n is a multiple of 8, no piece is cut
+// The piece at d < n of a row of n.  EVEN: n is a multiple of 8, no piece is cut.  A cut one
+// is read with what lies before it (its row has at least 8 values, or goes one by one) and
+// shifted to its place, zeros past its end; it is written in runs of 4, 2 and 1.
 template <int T, bool EVEN>
 __device__ __forceinline__ Piece8<T> piece_load(const void* row, int64_t d, int64_t n) {
+    constexpr int W = int(sizeof(Piece8<T>::w) / 4);
     Piece8<T> p;
     if (EVEN || d + 8 <= n) {
         const auto* q = reinterpret_cast<const Loose8<T>*>(static_cast<const char*>(row) + d * kElem<T>);
 #pragma unroll
-        for (int i = 0; i < int(sizeof(p.w) / 4); ++i) p.w[i] = q->w[i];
+        for (int i = 0; i < W; ++i) p.w[i] = q->w[i];
+        return p;
+    }
+    if (n >= 8) {
+        const auto* q = reinterpret_cast<const Loose8<T>*>(static_cast<const char*>(row) + (n - 8) * kElem<T>);
+#pragma unroll
+        for (int i = 0; i < W; ++i) p.w[i] = q->w[i];
+        const int s = int(d + 8 - n);                 // 1..7 values too early
+        if constexpr (T == kF32) {
+#pragma unroll
+            for (int b = 4; b; b /= 2)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    p.w[i] = s & b ? (i + b < 8 ? p.w[i + b < 8 ? i + b : 0] : 0u) : p.w[i];
+        } else {
+            uint64_t lo = p.w[0] | uint64_t(p.w[1]) << 32, hi = p.w[2] | uint64_t(p.w[3]) << 32;
+            if (s >= 4) {
+                lo = hi >> (16 * (s - 4));
+                hi = 0;
+            } else {
+                lo = lo >> (16 * s) | hi << (64 - 16 * s);
+                hi >>= 16 * s;
+            }
+            p.w[0] = uint32_t(lo);
+            p.w[1] = uint32_t(lo >> 32);
+            p.w[2] = uint32_t(hi);
+            p.w[3] = uint32_t(hi >> 32);
+        }
         return p;
     }
 #pragma unroll
-    for (int i = 0; i < int(sizeof(p.w) / 4); ++i) p.w[i] = 0;
+    for (int i = 0; i < W; ++i) p.w[i] = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         if (d + i >= n) continue;
@@ -48,17 +78,35 @@ __device__ __forceinline__ Piece8<T> piece_load(const void* row, int64_t d, int6
 
 template <int T, bool EVEN>
 __device__ __forceinline__ void piece_store(void* row, int64_t d, int64_t n, const Piece8<T>& p) {
+    constexpr int W = int(sizeof(Piece8<T>::w) / 4);
+    struct __attribute__((packed, aligned(kElem<T>))) Four { uint32_t w[kElem<T>]; };
+    struct __attribute__((packed, aligned(kElem<T>))) Two { uint32_t w[kElem<T> / 2]; };
+    char* at = static_cast<char*>(row) + d * kElem<T>;
     if (EVEN || d + 8 <= n) {
-        auto* q = reinterpret_cast<Loose8<T>*>(static_cast<char*>(row) + d * kElem<T>);
+        auto* q = reinterpret_cast<Loose8<T>*>(at);
 #pragma unroll
-        for (int i = 0; i < int(sizeof(p.w) / 4); ++i) q->w[i] = p.w[i];
+        for (int i = 0; i < W; ++i) q->w[i] = p.w[i];
         return;
     }
+    const int c = int(n - d);                         // 1..7 values
+    if (c & 4) {
+        Four f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (d + i >= n) continue;
-        if constexpr (T == kF32) static_cast<uint32_t*>(row)[d + i] = p.w[i];
-        else static_cast<uint16_t*>(row)[d + i] = uint16_t(p.w[i / 2] >> (16 * (i & 1)));
+        for (int i = 0; i < W / 2; ++i) f.w[i] = p.w[i];
+        *reinterpret_cast<Four*>(at) = f;
+    }
+    const bool second = c & 4;                        // where the rest begins
+    if (c & 2) {
+        Two t;
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) t.w[i] = second ? p.w[W / 2 + i] : p.w[i];
+        *reinterpret_cast<Two*>(at + (c & 4) * kElem<T>) = t;
+    }
+    if (c & 1) {                                      // value c - 1, of an even place
+        const uint32_t a = second ? p.w[W / 2] : p.w[0], b = second ? p.w[W / 2 + W / 4] : p.w[W / 4];
+        const uint32_t v = c & 2 ? b : a;
+        if constexpr (T == kF32) *reinterpret_cast<uint32_t*>(at + (c - 1) * 4) = v;
+        else *reinterpret_cast<uint16_t*>(at + (c - 1) * 2) = uint16_t(v);
     }
 }
 
