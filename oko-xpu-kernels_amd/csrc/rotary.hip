@@ -155,7 +155,7 @@ hipError_t rope_axes(hipStream_t st, const Heads& q, const Heads& k, int type,
         constexpr int T = decltype(t)::value;
         constexpr bool SPLIT = decltype(split)::value;
         auto launch = [&](auto even) {
-            in_launches(B * S, kMaxBlocks * a.each, [&](int64_t at, int64_t m) {
+            in_launches(B * S, kMaxBlocks / 2 * a.each, [&](int64_t at, int64_t m) {
                 a.first = uint32_t(at);
                 hipLaunchKernelGGL((rotary_kernel<T, SPLIT, decltype(even)::value>),
                                    dim3(unsigned((m + a.each - 1) / a.each)), dim3(threads),

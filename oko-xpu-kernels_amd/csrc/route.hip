@@ -187,12 +187,20 @@ __global__ __launch_bounds__(256) void route_exact_kernel(RouteArgs a) {
 // A token has L lanes of V experts, 64 / L tokens a wave.  Keys are made in fp32 first, to
 // a known error; of each the 32 bits that order like it, with the expert's place in the low
 // ones, are sorted in every lane and merged across the lanes down to the token's highest 16,
-// all in integer minima and maxima.  These 16 candidates, one a lane, then get their keys in
-// 64 bits, and each counts the ones above its own: its slot.  The choice is sure when the
-// last chosen key is above anything that the 17th could be; a token for which that does not
-// hold (more keys than 16 within 2^-13 to 2^-15 of the last one chosen, a NaN, scores that
-// underflow) goes through route_token.  Groups whose fp32 values are too near, and softmax
-// keys nearer than the sum's error, are looked at again in 64 bits.
+// all in integer minima and maxima.  The first of these candidates, one a lane, get their
+// keys in 64 bits.  The choice is sure when these are in order and the last one chosen is
+// above anything that the next candidate (with 16 lanes: the 17th key) could be; if not, all
+// 16 candidates are counted against each other in 64 bits, which 16 keys within 2^-13 to
+// 2^-15 of the last one chosen, a NaN, or scores that underflow leave open still: such a
+// token goes through route_token.  Groups whose fp32 values are too near, and softmax keys
+// nearer than the fp32 sum's error, are looked at again in 64 bits too.
+//
+// Bound by instructions (half of them the sort's and the merges'), so few lanes a token: 8 for
+// up to 8 slots and 256 experts (65536 tokens, 8 of 64 experts in bf16 10 us and 17 with 16 lanes;
+// of 128 by biased sigmoids in fp32 17 and 22; 32768 of 256 in bf16 10 and 13).  Groups take 16
+// lanes below 65536 tokens, whose waves are too few to hide what the groups add (8192 tokens of
+// 256 in 8 groups 10 us and 13 with 8 lanes, 65536 34 and 34).  16381 of these take 16 us (with a
+// wave a token and all keys in 64 bits 103), 4 tokens of 64 experts 2.5.
 constexpr int kCandidates = 16;
 constexpr uint32_t kNothing = 0x00800000u;           // ordered(-inf) and the bits of a place are below
 
@@ -201,6 +209,27 @@ __device__ __forceinline__ double dpp64(double x) {
     const uint64_t b = __builtin_bit_cast(uint64_t, x);
     const uint32_t lo = dppu<CTRL>(uint32_t(b)), hi = dppu<CTRL>(uint32_t(b >> 32));
     return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_any(float x) { return dpp<CTRL>(x); }
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_any(uint32_t x) { return dppu<CTRL>(x); }
+template <int CTRL>
+__device__ __forceinline__ double dpp_any(double x) { return dpp64<CTRL>(x); }
+
+// x of another lane of a row of ROW lanes, every lane of it once over K = 1 .. ROW - 1: of 16
+// by rotation, of 8 of lane ^ K
+template <int ROW, int K, class X>
+__device__ __forceinline__ X other_lane(X x) {
+    constexpr int kXor3 = 0x1B;                       // quad_perm [3,2,1,0]
+    if constexpr (ROW == 16) return dpp_any<0x120 + K>(x);
+    else if constexpr (K == 1) return dpp_any<kDppXor1>(x);
+    else if constexpr (K == 2) return dpp_any<kDppXor2>(x);
+    else if constexpr (K == 3) return dpp_any<kXor3>(x);
+    else if constexpr (K == 7) return dpp_any<kDppXor7>(x);
+    else if constexpr (K == 4) return dpp_any<kXor3>(dpp_any<kDppXor7>(x));
+    else if constexpr (K == 5) return dpp_any<kDppXor2>(dpp_any<kDppXor7>(x));
+    else return dpp_any<kDppXor1>(dpp_any<kDppXor7>(x));
 }
 // x of a lane on the other side of D, where the lanes of each side hold the same: lane ^ 1,
 // ^ 2, ^ 7, ^ 15 by DPP, then ^ 16 and ^ 32
@@ -249,9 +278,23 @@ __device__ __forceinline__ void sort_odd_even(uint32_t (&a)[M]) {
         merge_odd_even<N, AT, 1>(a);
     }
 }
+// a lane's own V keys sorted, the 16 highest of 32
+template <int V, int M>
+__device__ __forceinline__ void sort_lane(uint32_t (&a)[M]) {
+    if constexpr (V <= kCandidates) {
+        sort_odd_even<V, 0>(a);
+    } else {
+        static_assert(V == 2 * kCandidates);
+        sort_odd_even<kCandidates, 0>(a);
+        sort_odd_even<kCandidates, kCandidates>(a);
+#pragma unroll
+        for (int i = 0; i < kCandidates; ++i) a[i] = max(a[i], a[V - 1 - i]);
+        sort_bitonic<kCandidates, 0>(a);
+    }
+}
 // The sorted N values of this side of D and of the other, of which the 16 highest: in both.
-template <int N, int D>
-__device__ __forceinline__ void merge_lanes(uint32_t (&a)[kCandidates]) {
+template <int N, int D, int M>
+__device__ __forceinline__ void merge_lanes(uint32_t (&a)[M]) {
     uint32_t b[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) b[i] = other_side<D>(a[i]);
@@ -270,8 +313,8 @@ __device__ __forceinline__ void merge_lanes(uint32_t (&a)[kCandidates]) {
         sort_bitonic<N, 0>(a);
     }
 }
-template <int L, int N, int D = 1>
-__device__ __forceinline__ void merge_token(uint32_t (&a)[kCandidates]) {
+template <int L, int N, int D = 1, int M>
+__device__ __forceinline__ void merge_token(uint32_t (&a)[M]) {
     if constexpr (D < L) {
         merge_lanes<N, D>(a);
         merge_token<L, (2 * N < kCandidates ? 2 * N : kCandidates), 2 * D>(a);
@@ -283,54 +326,12 @@ template <int L>
 __device__ __forceinline__ float token_max(float x) { return lanes_max<L>(x); }
 template <int L>
 __device__ __forceinline__ float token_sum(float x) { return lanes_sum<L>(x); }
-
-// bits that order like the float (no NaN), and back
-__device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t b = __float_as_uint(x);
-    return b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
-}
-__device__ __forceinline__ float unordered(uint32_t k) {
-    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
-}
-
-// the other groups of 2^bits lanes in a row of 16 whose range of values is above this one's,
-// and those that are not below it (groups that are not there are -inf)
-template <int K>
-__device__ __forceinline__ void count_groups(int bits, float low, float high, int& above, int& maybe) {
-    if constexpr (K < 16) {
-        if ((K & ((1 << bits) - 1)) == 0) {
-            const float ol = dpp<0x120 + K>(low), oh = dpp<0x120 + K>(high);
-            above += ol > high;
-            maybe += !(oh < low);
-        }
-        count_groups<K + 1>(bits, low, high, above, maybe);
-    }
-}
-// Whether a key of a row of 16 is above the next one by more than tol, or the same at a lower
-// expert (`place` falls along the experts); what is not to be chosen comes last in any order.
-__device__ __forceinline__ bool in_order(double key, uint32_t place, int r, double tol) {
-    const double next = dpp64<0x101>(key);            // row_shl: lane r gets r + 1's
-    const uint32_t next_place = dppu<0x101>(place);
-    return r == 15 || next == kNone || key > next + tol || (key == next && place > next_place);
-}
-template <int K>
-__device__ __forceinline__ void count_above(double key, uint32_t place, int& rank) {
-    if constexpr (K < 16) {
-        const double other = dpp64<0x120 + K>(key);   // row_ror, as far as all have been seen
-        rank += other > key || (other == key && dppu<0x120 + K>(place) > place);
-        count_above<K + 1>(key, place, rank);
-    }
-}
-__device__ __forceinline__ double row_sum(double x) {
+template <int L>
+__device__ __forceinline__ double token_total(double x) {
     x += dpp64<kDppXor1>(x);
     x += dpp64<kDppXor2>(x);
     x += dpp64<kDppXor7>(x);
-    x += dpp64<kDppXor15>(x);
-    return x;
-}
-template <int L>
-__device__ __forceinline__ double token_total(double x) {
-    x = row_sum(x);
+    if constexpr (L >= 16) x += dpp64<kDppXor15>(x);
 #pragma unroll
     for (int d = 16; d < L; d *= 2) x += __shfl_xor(x, d);
     return x;
@@ -342,12 +343,65 @@ __device__ __forceinline__ bool token_any(bool x) {
     else return (m >> (threadIdx.x & (64 - L)) & ((uint64_t(1) << L) - 1)) != 0;
 }
 
+// bits that order like the float (no NaN), and back
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// the other groups of 2^bits lanes in a row whose range of values is above this one's, and
+// those that are not below it (groups that are not there are -inf)
+template <int ROW, int K = 1>
+__device__ __forceinline__ void count_groups(int bits, float low, float high, int& above, int& maybe) {
+    if constexpr (K < ROW) {
+        if ((K & ((1 << bits) - 1)) == 0) {
+            const float ol = other_lane<ROW, K>(low), oh = other_lane<ROW, K>(high);
+            above += ol > high;
+            maybe += !(oh < low);
+        }
+        count_groups<ROW, K + 1>(bits, low, high, above, maybe);
+    }
+}
+// A candidate: its packed key, expert, score, key and how many candidates are above it
+struct Candidate {
+    uint32_t packed;
+    int e, rank;
+    double s, k;
+};
+// Whether a key of a row is above the next lane's by more than tol, or the same at a lower
+// expert (`place` falls along the experts); what is not to be chosen comes last in any order.
+template <int ROW>
+__device__ __forceinline__ bool in_order(double key, uint32_t place, int r, double tol) {
+    const double next = dpp64<0x101>(key);            // row_shl: lane r gets r + 1's
+    const uint32_t next_place = dppu<0x101>(place);
+    return r == ROW - 1 || next == kNone || key > next + tol || (key == next && place > next_place);
+}
+__device__ __forceinline__ bool goes_before(double ka, uint32_t pa, double kb, uint32_t pb) {
+    return ka > kb || (ka == kb && pa > pb);
+}
+template <int ROW, int Q, int K = 1>
+__device__ __forceinline__ void count_above(Candidate (&c)[Q], uint32_t places) {
+    if constexpr (K < ROW) {
+#pragma unroll
+        for (int o = 0; o < Q; ++o) {
+            const double k = other_lane<ROW, K>(c[o].k);
+            const uint32_t p = other_lane<ROW, K>(c[o].packed & places);
+#pragma unroll
+            for (int q = 0; q < Q; ++q) c[q].rank += goes_before(k, p, c[q].k, c[q].packed & places);
+        }
+        count_above<ROW, Q, K + 1>(c, places);
+    }
+}
+
 // how the experts of a token lie: group g in the 2^bits lanes from g * 2^bits on, `each` a lane
 struct Spread {
     int bits, each;
 };
 
-// V consecutive logits from `first` on (-inf past `count`), in one load if they are whole
+// V consecutive logits from `at` on (-inf past `count`), in one load if they are whole
 template <int T, int V>
 __device__ __forceinline__ void logits_load(const void* logits, int64_t at, int count, float (&l)[V]) {
     constexpr int W = V * kElem<T> / 4;
@@ -377,8 +431,9 @@ __device__ __forceinline__ void logits_load(const void* logits, int64_t at, int 
 template <int T, int L, int V, int THREADS>
 __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, int64_t first_token) {
     constexpr int PER = 64 / L, WAVES = THREADS / 64;
+    constexpr int ROW = L < 16 ? L : 16, Q = kCandidates / ROW;      // candidates a lane, in all
     constexpr uint32_t kPlace = L * V - 1;            // the bits of an expert's place
-    const int lane = threadIdx.x & 63, in = lane & (L - 1), r = lane & 15;
+    const int lane = threadIdx.x & 63, in = lane & (L - 1), r = lane & (ROW - 1);
     const int n = a.E / a.how.groups;
     const int group = in >> sp.bits, part = in & ((1 << sp.bits) - 1);
     const int first = group * n + part * sp.each;     // this lane's experts
@@ -387,73 +442,80 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
     const int64_t t0 = first_token + (int64_t(blockIdx.x) * WAVES + (threadIdx.x >> 6)) * PER;
     if (t0 >= a.T) return;
     const int64_t t = min(t0 + lane / L, a.T - 1);
-    float l[V], b[V];
-    logits_load<T>(a.logits, t * a.ld + first, count, l);
-    if (a.bias) logits_load<kF32>(a.bias, first, count, b);
-    float most = -INFINITY, all = 0.f;
+    float key[V], most = -INFINITY, sum = 1.f;        // key: the logits, then scores, then keys
+    bool bad = false, odd = false;
+    constexpr float kLog2e = 1.4426950408889634f;
+    logits_load<T>(a.logits, t * a.ld + first, count, key);
+    {
+        float all = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        all += l[i];
-        most = fmaxf(most, l[i]);
-    }
-    // a NaN or infinity anywhere (or a sum that overflows): looked for one by one
-    bool bad = false;
-    const bool odd = __builtin_amdgcn_ballot_w64(!(fabsf(all) < INFINITY)) != 0;
-    if (odd) {
+        for (int i = 0; i < V; ++i) {
+            all += key[i];
+            most = fmaxf(most, key[i]);
+        }
+        // a NaN or infinity anywhere (or a sum that overflows): looked for one by one
+        odd = __builtin_amdgcn_ballot_w64(!(fabsf(all) < INFINITY)) != 0;
+        if (odd) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) bad |= __builtin_isnan(l[i]) || (!a.how.sigmoid && l[i] == INFINITY);
+            for (int i = 0; i < V; ++i)
+                bad |= __builtin_isnan(key[i]) || (!a.how.sigmoid && key[i] == INFINITY);
+        }
     }
+    if (!a.how.sigmoid) most = token_max<L>(most);
     // fp32 scores.  A sigmoid s: its exponential off by 2 units (2^-24) and |l| of its
     // argument's rounding, of which s (1 - s) < 1/4 (times |l| < 1/4) counts, the sum's and
     // the reciprocal's 3: under 2^-21.  A softmax's: 2 and the argument's |x|, where
-    // |x| e^-|x| < 0.4, the sum's 22 additions of such terms and the reciprocal: under 2^-19
+    // |x| e^-|x| < 0.4, the sum's 38 additions of such terms and the reciprocal: under 2^-18
     // of the highest score.
-    float key[V], sum = 1.f;
-    constexpr float kLog2e = 1.4426950408889634f;
-    if (!a.how.sigmoid) {
-        most = token_max<L>(most);
-        const float ref = most == -INFINITY ? 0.f : most;
-        sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            key[i] = __builtin_amdgcn_exp2f((l[i] - ref) * kLog2e);
-            sum += key[i];
-        }
-        sum = token_sum<L>(sum);
-    }
-    if (plain) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = l[i];
-    } else {
-        const float share = __builtin_amdgcn_rcpf(sum);
+    const bool scores = !plain || (!a.how.sigmoid && !a.how.renormalize);
+    if (scores) {
+        float e[V];
         if (a.how.sigmoid) {
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                key[i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-l[i] * kLog2e));
+                e[i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-key[i] * kLog2e));
         } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) key[i] *= share;
-        }
-        float check = 0.f;
-        if (a.bias) {
+            const float ref = most == -INFINITY ? 0.f : most;
+            sum = 0.f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                key[i] += b[i];
-                check += key[i];
+                e[i] = __builtin_amdgcn_exp2f((key[i] - ref) * kLog2e);
+                sum += e[i];
             }
-        }
-        if (odd || __builtin_amdgcn_ballot_w64(!(fabsf(check) < INFINITY))) {
+            sum = token_sum<L>(sum);
+            const float share = __builtin_amdgcn_rcpf(sum);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                if (l[i] == -INFINITY) key[i] = -INFINITY;
-                bad |= __builtin_isnan(key[i]);
+            for (int i = 0; i < V; ++i) e[i] *= share;
+        }
+        if (!plain) {
+            float check = 0.f;
+            if (odd) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) e[i] = key[i] == -INFINITY ? -INFINITY : e[i];
             }
+            if (a.bias) {
+                float b[V];
+                logits_load<kF32>(a.bias, first, count, b);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    e[i] += b[i];
+                    check += e[i];
+                }
+                if (__builtin_amdgcn_ballot_w64(!(fabsf(check) < INFINITY))) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) bad |= __builtin_isnan(e[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) key[i] = e[i];
         }
     }
-    const float off = plain ? 0.f : a.how.sigmoid ? 0x1p-21f : 0x1p-19f * __builtin_amdgcn_rcpf(sum);
-    double sum64 = sum;                           // the softmax's, exact once asked for
+    const float off = plain ? 0.f : a.how.sigmoid ? 0x1p-21f : 0x1p-18f * __builtin_amdgcn_rcpf(sum);
+    double sum64 = sum;                               // the softmax's, exact once asked for
     bool sum_exact = false;
     auto exact_sum = [&] {
+        float l[V];
+        logits_load<T>(a.logits, t * a.ld + first, count, l);
         double u = 0.0;
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -479,10 +541,10 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
         }
         const float value = two == -INFINITY ? one : one + two;
         const float e = one == -INFINITY ? 0.f : 2.f * off + 0x1p-22f * (fabsf(one) + fabsf(value));
-        int above = 0, maybe = 0;                 // groups surely above, and perhaps
+        int above = 0, maybe = 0;                     // groups surely above, and perhaps
         const float low = value - e, high = value + e;
-        if constexpr (L == 16) {
-            count_groups<1>(sp.bits, low, high, above, maybe);
+        if constexpr (L <= 16) {
+            count_groups<L>(sp.bits, low, high, above, maybe);
         } else {
             for (int g = 0; g < a.how.groups; ++g) {
                 const int from = (lane & ~(L - 1)) + (g << sp.bits);
@@ -495,13 +557,15 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
         // (a group with nothing to choose from is as good in as out)
         dropped = one == -INFINITY || above >= a.how.top_groups;
         const bool open = group < a.how.groups && !dropped && maybe >= a.how.top_groups;
-        if (__builtin_amdgcn_ballot_w64(open)) {  // values too near: in 64 bits
+        if (__builtin_amdgcn_ballot_w64(open)) {      // values too near: in 64 bits
             if (!a.how.sigmoid) exact_sum();
             double first64 = kNone, second64 = kNone;
+            float l[V];
+            logits_load<T>(a.logits, t * a.ld + first, count, l);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                if (key[i] == -INFINITY) continue;
-                const double k = score64(l[i]) + (a.bias ? double(b[i]) : 0.0);
+                if (l[i] == -INFINITY) continue;
+                const double k = score64(l[i]) + (a.bias ? double(a.bias[first + i]) : 0.0);
                 second64 = fmax(second64, fmin(first64, k));
                 first64 = fmax(first64, k);
             }
@@ -520,58 +584,80 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
         }
     }
     // (-inf orders below kNothing, and so does what is dropped)
-    uint32_t c[kCandidates];
+    uint32_t c[V > kCandidates ? V : kCandidates];
     const uint32_t keep = dropped ? 0u : ~kPlace;
 #pragma unroll
     for (int i = 0; i < V; ++i) c[i] = (ordered(key[i]) & keep) | (kPlace - uint32_t(in * V + i));
-    sort_odd_even<V, 0>(c);
-    merge_token<L, V>(c);
-    uint32_t mine = c[0];
+    sort_lane<V>(c);
+    merge_token<L, (V < kCandidates ? V : kCandidates)>(c);
+    Candidate mine[Q];
+    double tol = 0.0;
+    // the candidates Q ROW + r, in 64 bits
+    auto look = [&](int q) {
+        Candidate& m = mine[q];
+        m.packed = c[q * ROW];
 #pragma unroll
-    for (int i = 1; i < kCandidates; ++i) mine = r == i ? c[i] : mine;
-    // this lane's candidate, in 64 bits
-    const bool is = mine >= kNothing;
-    const int place = int(kPlace - (mine & kPlace)), at = place / V;
-    const int e = (at >> sp.bits) * n + (at & ((1 << sp.bits) - 1)) * sp.each + place % V;
-    const float x = is ? logit_at<T>(a.logits, t, a.ld, e) : -INFINITY;
-    double s = 0.0, k = kNone, tol = 0.0;
-    auto look = [&] {
-        if (!is) return;
-        s = plain && a.how.renormalize && !a.how.sigmoid ? exp(double(x) - double(most)) : score64(x);
-        k = plain ? double(x) : s + (a.bias ? double(a.bias[e]) : 0.0);
+        for (int i = 1; i < ROW; ++i) m.packed = r == i ? c[q * ROW + i] : m.packed;
+        const int at = int(kPlace - (m.packed & kPlace)) / V, i = int(kPlace - (m.packed & kPlace)) % V;
+        m.e = m.packed >= kNothing ? (at >> sp.bits) * n + (at & ((1 << sp.bits) - 1)) * sp.each + i : -1;
+        m.s = 0.0;
+        m.k = kNone;
+        m.rank = q * ROW + r;
+        if (m.e < 0) return;
+        const float x = logit_at<T>(a.logits, t, a.ld, m.e);
+        m.s = plain && a.how.renormalize && !a.how.sigmoid ? exp(double(x) - double(most)) : score64(x);
+        m.k = plain ? double(x) : m.s + (a.bias ? double(a.bias[m.e]) : 0.0);
         // keys nearer than the fp32 sum's error are looked at again with the exact one
-        tol = plain || a.how.sigmoid || sum_exact ? 0.0 : 0x1p-17 * s;
+        if (!plain && !a.how.sigmoid && !sum_exact) tol = fmax(tol, 0x1p-16 * m.s);
     };
-    look();
-    // the candidates lie in the order of their fp32 keys' upper bits, mostly the right one:
-    // otherwise each counts those above it, with the exact sum
-    int rank = r;
-    if (__builtin_amdgcn_ballot_w64(!in_order(k, mine & kPlace, r, tol))) {
-        if (!plain && !a.how.sigmoid && !sum_exact) {
-            exact_sum();
-            look();
+    // whether a chosen candidate is above all that order behind `next`
+    auto sure = [&](const Candidate& m, uint32_t next) {
+        if (m.e < 0 || m.rank >= a.top || next < kNothing) return true;
+        // (16-bit logits are whole in the upper bits: equal ones are in order)
+        if (plain && T != kF32) return true;
+        const float highest = unordered(next | kPlace);
+        return m.k > double(highest) + 2.0 * off + (plain ? 0.0 : 0x1p-22 * fabs(double(highest)));
+    };
+    look(0);
+#pragma unroll
+    for (int q = 1; q < Q; ++q) mine[q] = Candidate{0, -1, kCandidates, 0.0, kNone};
+    bool ordered_now = in_order<ROW>(mine[0].k, mine[0].packed & kPlace, r, tol);
+    ordered_now &= sure(mine[0], c[Q > 1 ? ROW : kCandidates - 1]);
+    if (__builtin_amdgcn_ballot_w64(!ordered_now)) {
+        if (!plain && !a.how.sigmoid && !sum_exact) exact_sum();
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            look(q);
+            mine[q].rank = 0;
         }
-        rank = 0;
-        count_above<1>(k, mine & kPlace, rank);
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int o = 0; o < Q; ++o)
+                if (o != q)
+                    mine[q].rank += goes_before(mine[o].k, mine[o].packed & kPlace, mine[q].k,
+                                                mine[q].packed & kPlace);
+        count_above<ROW, Q>(mine, kPlace);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) bad |= !sure(mine[q], c[kCandidates - 1]);
     }
-    const bool chosen = is && rank < a.top;
-    if (c[kCandidates - 1] >= kNothing) {             // there may be a 17th
-        const uint32_t last = c[kCandidates - 1];
-        const float highest = unordered(last | kPlace);
-        if (plain && T != kF32) {
-            // 16-bit logits are whole in the upper bits: equal ones are in order
-        } else if (plain) {
-            bad |= chosen && !(k > double(highest));
-        } else {
-            bad |= chosen && !(k > double(highest) + 2.0 * off + 0x1p-22 * fabs(double(highest)));
-        }
+    double total = 1.0;
+    if (a.how.renormalize) {
+        total = 0.0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) total += mine[q].rank < a.top ? mine[q].s : 0.0;
+        total = token_total<ROW>(total);
     }
-    const double total = a.how.renormalize ? row_sum(chosen ? s : 0.0) : 1.0;
-    bad |= chosen && !(total > 1e-200);
+    bad |= mine[0].e >= 0 && !(total > 1e-200);
     const bool again = token_any<L>(bad);
-    if (!again && in < 16 && rank < a.top && t0 + lane / L < a.T) {
-        a.ids[t * a.top + rank] = is ? e : -1;
-        a.weights[t * a.top + rank] = is ? float(double(a.how.scale) * s / total) : 0.f;
+    if (!again && in < ROW && t0 + lane / L < a.T) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            if (mine[q].rank >= a.top) continue;
+            a.ids[t * a.top + mine[q].rank] = mine[q].e;
+            a.weights[t * a.top + mine[q].rank] =
+                mine[q].e >= 0 ? float(double(a.how.scale) * mine[q].s / total) : 0.f;
+        }
     }
     uint64_t left = __builtin_amdgcn_ballot_w64(again && in == 0 && t0 + lane / L < a.T);
     while (left) {
@@ -830,7 +916,7 @@ hipError_t moe_route(hipStream_t st, const void* logits, int type, int64_t ld, c
     bool done = false;
     auto go = [&](auto t, auto lanes, auto v) {
         constexpr int L = decltype(lanes)::value, V = decltype(v)::value, TY = decltype(t)::value;
-        if (done || padded > L || top > kCandidates) return;
+        if (done || padded > L || top > (L < kCandidates ? L : kCandidates)) return;
         int bits = 0;
         while (padded << (bits + 1) <= L) ++bits;
         const Spread sp{bits, (n + (1 << bits) - 1) >> bits};
@@ -848,6 +934,11 @@ hipError_t moe_route(hipStream_t st, const void* logits, int type, int64_t ld, c
                                0, st, a, sp, int64_t(0));
     };
     auto by = [&](auto t) {
+        if (how.groups == 1 || T >= 65536) {          // (see above)
+            go(t, std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
+            go(t, std::integral_constant<int, 8>{}, std::integral_constant<int, 16>{});
+            go(t, std::integral_constant<int, 8>{}, std::integral_constant<int, 32>{});
+        }
         go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
         go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{});
         go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 16>{});

@@ -272,3 +272,29 @@ def test_feeds_the_int8_linear(dev, m):
     acc = q.cpu().double() @ wq.cpu().double().t()
     scale = (wsr[None] * s[:, None]).cpu().double()
     within(int8.linear_quantized(q, s, wq, wsr), acc * scale, 2 * U * acc.abs() * scale)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 16, 16), (5, 48, 80), (17, 16, 2064), (64, 320, 1296), (257, 1040, 528),
+                                   (3, 4112, 4096), (1000, 64, 272)])
+def test_linear_of_quantized_rows(dev, m, n, k):
+    """Multiples of 16, any strides, scalar scales, no rows."""
+    g = torch.Generator().manual_seed(m)
+    q, w8 = (torch.randint(-127, 128, (r, k), generator=g, dtype=torch.int8) for r in (m, n))
+    s, ws, b = (torch.rand(r, generator=g) + 0.5 for r in (m, n, n))
+    acc = q.double() @ w8.double().t()
+    for bias in (None, b, b.bfloat16()):
+        want = acc * (ws[None] * s[:, None]).double() + (0 if bias is None else bias.double())
+        error = 3 * U * (acc.abs() * (ws[None] * s[:, None]).double() + (0 if bias is None else bias.double().abs()))
+        bd = None if bias is None else bias.to(dev)
+        y = int8.linear_quantized(q.to(dev), s.to(dev), w8.to(dev), ws.to(dev), bd)
+        within(y, want, error)
+        wide = torch.zeros(m, k + 16, dtype=torch.int8, device=dev)
+        wide[:, 3:k + 3] = q.to(dev)
+        assert torch.equal(int8.linear_quantized(wide[:, 3:k + 3], s.to(dev)[:, None], w8.to(dev).t().contiguous().t(),
+                                                 ws.to(dev)[:, None], bd), y)
+        assert torch.equal(int8.linear_quantized(q.to(dev)[None], s.to(dev)[None], w8.to(dev), ws.to(dev), bd), y[None])
+    one = int8.linear_quantized(q.to(dev), s.to(dev), w8.to(dev), 0.25)
+    within(one, acc * 0.25 * s[:, None].double(), 3 * U * acc.abs() * s[:, None].double())
+    assert int8.linear_quantized(q.to(dev)[:0], s.to(dev)[:0], w8.to(dev), 0.25).shape == (0, n)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        int8.linear_quantized(q.to(dev), s.to(dev).requires_grad_(), w8.to(dev), 0.25)

@@ -25,8 +25,8 @@ def weight_error(how):
     """Scores are 64 bits until their one rounding, but that a softmax's sum over all experts
     (which drops out of renormalised weights) may be fp32: of exponentials off by 2 units and
     by their argument's two roundings, |x| units each (their mean over the sum, e^-|x| |x| /
-    e^-|x|, is under 8), 16 in a lane and 6 across lanes: 2 + 2 * 8 + 22 units."""
-    return 40 * U if how.get("scores", "softmax") == "softmax" and not how.get("renormalize", True) else 1e-12
+    e^-|x|, is under 8), 32 in a lane and 6 across lanes: 2 + 2 * 8 + 38 units."""
+    return 56 * U if how.get("scores", "softmax") == "softmax" and not how.get("renormalize", True) else 1e-12
 
 
 def check(dev, logits, top, dweights=None, **how):
