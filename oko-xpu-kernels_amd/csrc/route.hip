@@ -800,7 +800,8 @@ __device__ __forceinline__ void four_store(void* row, int e, int E, const float 
 // The same with several tokens a wave, up to 16 slots each: slots in the 16 lanes of a row,
 // a token's experts in fours over its L lanes.  The whole row of logits is read, beside the
 // ids, not after them (its chosen few lie in as many lines); they are looked up in LDS, and
-// gradients go through it to where they are written.
+// gradients go through it to where they are written.  HBM-bound: 16381 tokens of 256 experts in
+// fp32 9.9 us (3.4 TB/s; 11.3 to 12.7 with a wave a token and the chosen logits after the ids).
 template <int T, int L, int V>
 __global__ __launch_bounds__(256) void route_grad_rows_kernel(RouteGradArgs a, int64_t first_token) {
     constexpr int PER = 64 / L, F = V / 4;

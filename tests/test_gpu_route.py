@@ -209,3 +209,24 @@ def test_gradient_against_differences(dev):
             diff = ((up[1].double() - down[1].double()) * dw).sum() / (2 * step)
             # step^2 / 6 of a third derivative of at most 6 |g|, and the weights' roundings
             assert abs(diff - d[1, e]) < 2e-4
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("e,groups,top_groups", [(64, 8, 4), (60, 4, 2), (256, 8, 4), (256, 2, 1), (200, 1, 1)])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_many_tokens_as_few_at_a_time(dev, dtype, e, groups, top_groups, scores):
+    """The lanes that a token has depend on the number of tokens; its experts do not."""
+    t = 66000
+    lg = logits_of(t, e, dtype).to(dev)
+    lg[::1000, : e // 2] = -math.inf
+    lg[5::2000] = -math.inf
+    lg[7, 3] = math.nan
+    for bias in (torch.zeros(e, device=dev), (randn(e, seed=5) * 0.05).to(dev)):
+        how = dict(scores=scores, bias=bias, groups=groups, top_groups=top_groups)
+        ids, w = moe.route(lg, 8, **how)
+        parts = [moe.route(lg[i:i + 3000], 8, **how) for i in range(0, t, 3000)]
+        assert torch.equal(ids, torch.cat([p[0] for p in parts]))
+        # renormalised weights are of 64-bit scores, to whose factor both sums are the same
+        want = torch.cat([p[1] for p in parts])
+        assert torch.equal(w.isnan(), want.isnan())
+        assert ((w - want).abs() <= 2 * U * want.abs()).logical_or(w.isnan()).all()
