@@ -7,7 +7,7 @@
 //
 // An expert whose logit or key is -inf is never chosen; slots left over have id -1 and
 // weight 0.  A row with a NaN logit (for softmax +inf too) has NaN weights; its experts are
-// chosen by the logits, NaNs last.
+// chosen by the logits, NaNs last.  A NaN key (of a NaN bias) counts as the lowest.
 //
 // Which experts are chosen hangs on keys that may be next to each other, so the ones that
 // matter are compared in 64 bits.
@@ -586,8 +586,9 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
     // (-inf orders below kNothing, and so does what is dropped)
     uint32_t c[V > kCandidates ? V : kCandidates];
     const uint32_t keep = dropped ? 0u : ~kPlace;
+    // (a sum with 0 has no negative zero, which would order below the zero that it equals)
 #pragma unroll
-    for (int i = 0; i < V; ++i) c[i] = (ordered(key[i]) & keep) | (kPlace - uint32_t(in * V + i));
+    for (int i = 0; i < V; ++i) c[i] = (ordered(key[i] + 0.f) & keep) | (kPlace - uint32_t(in * V + i));
     sort_lane<V>(c);
     merge_token<L, (V < kCandidates ? V : kCandidates)>(c);
     Candidate mine[Q];

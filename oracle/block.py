@@ -71,7 +71,7 @@ def route(logits, top, scores="softmax", bias=None, groups=1, top_groups=1, reno
             b = [0.0] * e if bias is None else bias.double().tolist()
             # without a bias scores rise with their logits
             key = {j: row[j] if bias is None and groups == 1 else s[j] + b[j] for j in live}
-        key = {j: v for j, v in key.items() if v != -math.inf}
+        key = {j: -1e308 if math.isnan(v) else v for j, v in key.items() if v != -math.inf}
         if groups > 1:
             best = [sorted((key[j] for j in range(g * n, (g + 1) * n) if j in key), reverse=True)[:2]
                     for g in range(groups)]

@@ -230,3 +230,31 @@ def test_many_tokens_as_few_at_a_time(dev, dtype, e, groups, top_groups, scores)
         want = torch.cat([p[1] for p in parts])
         assert torch.equal(w.isnan(), want.isnan())
         assert ((w - want).abs() <= 2 * U * want.abs()).logical_or(w.isnan()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e", [24, 64, 100, 256, 600])
+def test_signed_zeros_are_equal(dev, dtype, scores, e):
+    g = torch.Generator().manual_seed(e)
+    lg = torch.where(torch.rand(40, e, generator=g) < 0.5, -0.0, 0.0).to(dtype)
+    lg[20:, ::7] = -1.0
+    lg[30:, 5::9] = 1.0
+    for bias in (None, torch.zeros(e), -torch.zeros(e)):
+        check(dev, lg, 8, scores=scores, bias=bias)
+        check(dev, lg, 8, scores=scores, bias=bias, groups=2, top_groups=1)
+
+
+@pytest.mark.parametrize("how", range(len(HOWS)))
+@pytest.mark.parametrize("groups,top_groups", [(1, 1), (4, 2)])
+def test_biases_that_are_not_finite(dev, how, groups, top_groups):
+    """+inf is chosen first, -inf never, NaN last; weights are of the scores alone."""
+    t, e = 9, 32
+    for value in (math.inf, -math.inf, math.nan):
+        bias = randn(e, seed=5) * 0.05
+        bias[[3, 9, 30]] = value
+        check(dev, logits_of(t, e, torch.float32), 6, randn(t, 6, seed=7), **HOWS[how], bias=bias,
+              groups=groups, top_groups=top_groups)
+        bias[:] = value
+        check(dev, logits_of(t, e, torch.float32), 6, **HOWS[how], bias=bias, groups=groups,
+              top_groups=top_groups)
