@@ -995,22 +995,31 @@ const Tensor* lines_arg(PyObject* o, Lines& l) {
 
 // The gradient of a leaf ends in a node that lives as long as any graph of the leaf and
 // belongs to the stream that was current when it was made.  A backward pass that is captured
-// makes that stream wait for the capturing one, which, if it is not captured too, ends the
-// capture and with it the process; a call that would lead there is refused (in Python, which
-// knows the streams, _capture.refuse_foreign_leaf).
+// makes that stream wait for the capturing one; the default stream cannot, and that ends the
+// process: a captured call that would lead there, at once or through views and other nodes of
+// one input, is refused (_capture.py knows the captures).
 void check_leaf(const Tensor* t) {
-    if (!t || !t->requires_grad() || t->grad_fn()) return;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-    if (!node) return;
-    const auto made = node->stream();
-    if (!made || c10::impl::VirtualGuardImpl(t->device().type()).getStream(t->device()) == *made) return;
-    PyObject* module = PyImport_ImportModule("xpu_kernels._capture");
-    PyObject* r = module ? PyObject_CallMethod(module, "refuse_foreign_leaf", "LiL", (long long)made->id(),
-                                               int(made->device_index()), (long long)made->device_type())
-                         : nullptr;
-    Py_XDECREF(module);
-    if (!r) throw python_error();
-    Py_DECREF(r);
+    if (!t || !t->requires_grad()) return;
+    if (c10::impl::VirtualGuardImpl(t->device().type()).getStream(t->device()).id() == 0) return;
+    std::shared_ptr<torch::autograd::Node> node = t->grad_fn();
+    if (!node) node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    for (int far = 0; node && far < 16; ++far) {
+        const auto made = node->stream();
+        if (made && made->id() == 0) {
+            PyObject* module = PyImport_ImportModule("xpu_kernels._capture");
+            PyObject* r =
+                module ? PyObject_CallMethod(module, "refuse_default_stream_leaf", nullptr) : nullptr;
+            Py_XDECREF(module);
+            if (!r) throw python_error();
+            Py_DECREF(r);
+            return;
+        }
+        std::shared_ptr<torch::autograd::Node> next;
+        int inputs = 0;
+        for (const auto& edge : node->next_edges())
+            if (edge.is_valid() && inputs++ == 0) next = edge.function;
+        node = inputs == 1 ? next : nullptr;
+    }
 }
 
 // x, weight or None, eps, residual or None of a norm

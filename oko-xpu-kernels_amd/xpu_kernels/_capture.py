@@ -15,22 +15,13 @@ def is_capturing() -> bool:
         return False
 
 
-def _is_captured(stream) -> bool:
-    with torch.cuda.stream(stream):
-        return is_capturing()
-
-
-def refuse_foreign_leaf(stream_id: int, device_index: int, device_type: int) -> None:
-    """Raise if the current stream is being captured and the given one, to which the gradient
-    of a leaf belongs, is not: the backward pass would make it wait for the capturing stream,
-    which breaks the capture and ends the process."""
-    if not is_capturing():
-        return
-    # (the default stream, id 0, is never captured, and asking it disturbs a capture)
-    if stream_id != 0 and _is_captured(torch.cuda.Stream(
-            stream_id=stream_id, device_index=device_index, device_type=device_type)):
-        return
-    raise RuntimeError(
-        "a leaf that needs a gradient has one of a graph that was made on a stream outside of this "
-        "capture and is still alive; its backward pass cannot be captured. Delete what holds that "
-        "graph (a loss, an output) before capturing, or make it on the capturing stream")
+def refuse_default_stream_leaf() -> None:
+    """Raise if the current stream is being captured.  Called for a tensor whose gradient goes
+    to a graph of the default stream: the backward pass would make that stream wait for the
+    capturing one, which no capture allows and which ends the process.  (A stream that can be
+    captured joins the capture and is joined to it again.)"""
+    if is_capturing():
+        raise RuntimeError(
+            "a tensor that needs a gradient is part of a graph that was made on the default stream "
+            "and is still alive; its backward pass cannot be captured. Delete what holds that graph "
+            "(a loss, an output) before capturing, or make it on a stream of its own")

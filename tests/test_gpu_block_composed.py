@@ -122,8 +122,8 @@ def test_experts_of_a_block_in_a_graph(dev, dtype):
 
 @pytest.mark.parametrize("native", [True, False])
 def test_a_leaf_of_an_eager_graph_is_refused_in_a_capture(dev, monkeypatch, native):
-    """While an eager graph of a leaf lives, the leaf's gradient belongs to that graph's stream,
-    and a captured backward pass, which would make that stream wait for the capturing one,
+    """While an eager graph of a leaf on the default stream lives, the leaf's gradient belongs to
+    that stream, and a captured backward pass, which would make it wait for the capturing one,
     ends the process: the forward call is refused.  Without the graph it is captured."""
     if not native:                                 # every call through the Python code
         check = L.HOST.check_leaves
@@ -134,6 +134,7 @@ def test_a_leaf_of_an_eager_graph_is_refused_in_a_capture(dev, monkeypatch, nati
     x, w, r = randn(6, 64, seed=1).to(dev), randn(64, seed=2).to(dev), randn(6, 64, seed=3).to(dev)
     q, k = randn(1, 6, 2, 16, seed=4).to(dev), randn(1, 6, 1, 16, seed=5).to(dev)
     calls = {"norm x": (x, lambda v: norm.rms_norm(v, w)), "norm weight": (w, lambda v: norm.rms_norm(x, v)),
+             "view": (x, lambda v: norm.rms_norm(v.view(2, 3, 64)[:1], w)),
              "residual": (r, lambda v: norm.rms_norm(x, w, residual=v)[0]),
              "route": (x, lambda v: moe.route(v, 4)[1]), "q": (q, lambda v: rope.rotate_axes(v, k, pos, f)[0]),
              "k": (k, lambda v: rope.rotate_axes(q, v, pos, f)[1])}
@@ -165,6 +166,46 @@ def test_a_leaf_of_an_eager_graph_is_refused_in_a_capture(dev, monkeypatch, nati
         torch.cuda.synchronize()
         y2 = call(leaf)
         assert torch.equal(y, y2) and torch.equal(g, torch.autograd.grad(y2, leaf, y2.detach())[0]), name
+
+
+def test_a_step_whose_warm_up_is_alive_is_captured(dev):
+    """The usual order of a captured training step: warmed up on a side stream, whose last
+    loss is still there at the capture.  That stream joins the capture and is joined to it."""
+    x = randn(9, 64, seed=1).to(dev)
+    w, v = (1 + 0.1 * randn(64, seed=2)).to(dev).requires_grad_(), randn(16, 64, seed=3).to(dev).requires_grad_()
+
+    def step():
+        y = norm.rms_norm(x, w)
+        weights = moe.route(torch.mm(y, v.t()), 4, scores="sigmoid")[1]
+        loss = (weights * weights).sum() + (y * y).sum()
+        loss.backward()
+        return loss
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            w.grad = v.grad = None
+            loss = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    w.grad = v.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step()                              # (the warm-up's loss lives until this one is there)
+    gw, gv = w.grad, v.grad
+    for seed in (5, 6, 7):
+        x.copy_(randn(9, 64, seed=seed))
+        gw.zero_()
+        gv.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [gw.clone(), gv.clone()]
+        w.grad = v.grad = None
+        step()
+        torch.cuda.synchronize()
+        assert w.grad.any() and v.grad.any()
+        assert torch.equal(got[0], w.grad) and torch.equal(got[1], v.grad)
 
 
 def test_a_leaf_of_a_captured_stream_is_not_refused(dev):
