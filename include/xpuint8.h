@@ -639,8 +639,8 @@ int xpuint8_moe_combine_grad_stream(const void *stream, const void *dy, int32_t 
  * sigmoid = 1, sigmoid(logits); keys are s + bias (fp32 [E], NULL: none).  E / groups
  * consecutive experts are a group, its value the sum of its two highest keys; of the
  * experts in the top_groups groups of highest value the `top` highest keys are chosen, ties
- * to the lower index, in the order of their keys.  weights = scale * s, with renormalize = 1
- * divided by the sum of the chosen s.  An expert whose logit or key is -inf is never chosen;
+ * to the lower index, in the order of their keys (a NaN key counts as the lowest).
+ * weights = scale * s, with renormalize = 1 divided by the sum of the chosen s.  An expert whose logit or key is -inf is never chosen;
  * slots left over have id -1 and weight 0.  A row with a NaN logit, for softmax also with
  * one of +inf, has NaN weights.  top <= 64, groups <= 64.  No counterpart in the reference. */
 int xpuint8_moe_route_stream(const void *stream, const void *logits, int32_t type, int64_t ld,
@@ -660,7 +660,8 @@ int xpuint8_moe_route_grad_stream(const void *stream, const void *logits, int32_
  * `inner` rows (a divisor of M, 1 for evenly spaced rows; the heads of a position, say): rows
  * ld elements apart in a run, runs outer apart (inner 1: rows are outer apart, ld is not
  * read).  Inputs may have the alignment of their elements; outputs and work are contiguous
- * and 16-byte aligned.  Statistics are fp32.  K <= 2^24.  No counterpart in the reference.
+ * and 16-byte aligned, and overlap no input nor each other.  Statistics are fp32.
+ * K <= 2^24.  No counterpart in the reference.
  *
  * h = x + residual rounded to the type (residual and h NULL: h is x);
  * y = h / sqrt(mean(h^2) + eps) * weight (fp32 until y's rounding; weight [K] of its own
@@ -686,7 +687,8 @@ int64_t xpuint8_rms_norm_grad_workspace_size(int64_t M, int64_t K);
 int xpuint8_rms_norm_grad_stream(const void *stream, const void *dy, int32_t type, int64_t ldy,
                                  int64_t outer_dy, const void *h, int64_t ldh, int64_t outer_h,
                                  const void *weight, int32_t weight_type, const void *dh,
-                                 int64_t lddh, int64_t outer_dh, int64_t inner, float eps, void *dx, void *dweight, int64_t M, int64_t K, void *work,
+                                 int64_t lddh, int64_t outer_dh, int64_t inner, float eps,
+                                 void *dx, void *dweight, int64_t M, int64_t K, void *work,
                                  int64_t work_bytes);
 
 /* ---- rotary positions on several axes -----------------------------------
@@ -697,7 +699,7 @@ int xpuint8_rms_norm_grad_stream(const void *stream, const void *dy, int32_t typ
  * are fp32.  q_strides = {b, s, head} of q, then of q_out, in elements, the last dimensions
  * contiguous; position_strides = {axis, b, s}; positions int32, int64 or fp32 (position_type
  * 0, 1, 2); an axis outside [0, axes) does not turn.  Buffers have the alignment of their
- * elements.  pairs <= 512, D <= 4096.  Strides are read on the host.  No counterpart in the
+ * elements; q_out and k_out overlap no input.  pairs <= 512, D <= 4096.  Strides are read on the host.  No counterpart in the
  * reference. */
 int xpuint8_rope_axes_stream(const void *stream, const void *q, void *q_out,
                              const int64_t *q_strides, int64_t q_heads, const void *k, void *k_out,

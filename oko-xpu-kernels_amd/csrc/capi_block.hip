@@ -121,7 +121,8 @@ int64_t xpuint8_rms_norm_grad_workspace_size(int64_t M, int64_t K) {
 int xpuint8_rms_norm_grad_stream(const void* stream, const void* dy, int32_t type, int64_t ldy,
                                  int64_t outer_dy, const void* h, int64_t ldh, int64_t outer_h,
                                  const void* weight, int32_t weight_type, const void* dh,
-                                 int64_t lddh, int64_t outer_dh, int64_t inner, float eps, void* dx, void* dweight, int64_t M, int64_t K, void* work,
+                                 int64_t lddh, int64_t outer_dh, int64_t inner, float eps,
+                                 void* dx, void* dweight, int64_t M, int64_t K, void* work,
                                  int64_t work_bytes) {
     XPU_TRY(check_rows(M, K));
     XPU_TRY(check_type(type, "type"));
@@ -148,7 +149,8 @@ int xpuint8_rms_norm_grad_stream(const void* stream, const void* dy, int32_t typ
     }
     XPU_TRY(ensure_device());
     return launched(rms_norm_grad(as_stream(stream), dy, type, dy_lines, h, h_lines, weight,
-                                  weight_type, dh, dh_lines, inner, eps, dx, dweight, M, K, static_cast<float*>(work)),
+                                  weight_type, dh, dh_lines, inner, eps, dx, dweight, M, K,
+                                  static_cast<float*>(work)),
                     "rms_norm_grad");
 }
 

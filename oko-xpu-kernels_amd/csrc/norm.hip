@@ -4,7 +4,8 @@
 //   h = x + residual, rounded to the stream's type (h = x without one): what the next
 //       layer adds to, so the norm is of that value and not of the unrounded sum
 //   r = 1 / sqrt(mean(h^2) + eps),  y = h r weight
-//   backward, g = dy weight:  dx = r g - h r^3 mean(g h) + dh,  dweight = sum_rows dy h r
+//   backward, g = dy weight, n = h r:  dx = r (g - n mean(g n)) + dh,  dweight = sum_rows dy n
+//       (r^3 by itself would leave fp32's range long before the formula does)
 //   int8: v = h weight, rotated by 256s or not; m = max(|v|, 1e-30);
 //         q = rint(v (127 / m)), scale = r m / 127
 //
@@ -458,7 +459,7 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_grad_kernel(GradArgs a) {
         row_reduce<TPR, false>(sum, along, slots);
         if (!live) continue;
         const float r = inverse_rms(sum, a.K, a.eps);
-        const float back = r * r * r * (along / float(a.K));
+        const float back = along * r / float(a.K);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             int64_t d = 8 * (int64_t(i) * TPR + t);
@@ -471,8 +472,9 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_grad_kernel(GradArgs a) {
             piece_expand(dh[i], o);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (!(CUT == kOverlap && j < skip)) dw[i][j] = __builtin_fmaf(g[j], u[j] * r, dw[i][j]);
-                o[j] += __builtin_fmaf(g[j] * w[i][j], r, -(u[j] * back));
+                const float n = u[j] * r;
+                if (!(CUT == kOverlap && j < skip)) dw[i][j] = __builtin_fmaf(g[j], n, dw[i][j]);
+                o[j] += r * __builtin_fmaf(-n, back, g[j] * w[i][j]);
             }
             piece_store<T, whole(CUT)>(row_of<T>(a.dx, row, a.K), d, a.K, piece_round<T>(o));
         }
@@ -536,7 +538,7 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(GradArgs a) {
         }
         row_reduce<1024, false>(sum, along, slots);
         const float r = inverse_rms(sum, a.K, a.eps);
-        const float back = r * r * r * (along / float(a.K));
+        const float back = along * r / float(a.K);
         for (int64_t d = 8 * int64_t(threadIdx.x); d < a.K; d += 8 * 1024) {
             const int64_t at = place<CUT>(d, a.K);
             const int skip = int(d - at);
@@ -548,10 +550,10 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(GradArgs a) {
                 piece_expand(piece_load<T, whole(CUT)>(line_of<T>(a.dh, row, a.inner, a.ldh), at, a.K), o);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float term = g[j] * (u[j] * r);
+                const float n = u[j] * r, term = g[j] * n;
                 if (part && j >= skip && at + j < a.K)
                     part[at + j] = row == int64_t(blockIdx.x) ? term : part[at + j] + term;
-                o[j] += __builtin_fmaf(g[j] * w[j], r, -(u[j] * back));
+                o[j] += r * __builtin_fmaf(-n, back, g[j] * w[j]);
             }
             piece_store<T, whole(CUT)>(row_of<T>(a.dx, row, a.K), at, a.K, piece_round<T>(o));
         }
@@ -660,8 +662,8 @@ hipError_t rms_norm(hipStream_t st, const void* x, int type, const Lines& lx,
 
 hipError_t rms_norm_int8(hipStream_t st, const void* x, int type, const Lines& lx,
                          const void* residual, const Lines& lr, int64_t inner,
-                         const void* weight, int weight_type, float eps, void* h, int8_t* q, float* scale, bool rotate, int64_t M,
-                         int64_t K) {
+                         const void* weight, int weight_type, float eps, void* h, int8_t* q,
+                         float* scale, bool rotate, int64_t M, int64_t K) {
     const NormArgs a{x, residual, weight, h, q, scale, lx, lr, M, K, uint32_t(inner), weight_type, eps};
     if (!rotate) return launch_norm<true>(st, type, a);
     by_type(type, [&](auto t) {
@@ -670,10 +672,11 @@ hipError_t rms_norm_int8(hipStream_t st, const void* x, int type, const Lines& l
             // rows of few groups share a block of 16
             const int S = int(K / 256), R = S >= 16 ? 1 : 16 / S;
             const int threads = (S * R * 16 + 63) / 64 * 64;
-            // Blocks that together request 40 KB a CU, 60 without a residual (no fewer than one, no more than its 16
-            // waves): more rows under way at once are slower.  16381 x 5120 bf16 with a
-            // residual (40 KB: 2 blocks): 118 us with 1, 111 with 2, 131 with 3, 123 with 6;
-            // 8192 x 8192 85 with 1, 91 with 2; 20000 x 4096 without one 64 with 2, 52 with 4.
+            // Blocks that together request 40 KB a CU, 60 without a residual (no fewer than
+            // one, no more than its 16 waves): more rows under way at once are slower.
+            // 16381 x 5120 bf16 with a residual (40 KB: 2 blocks): 118 us with 1, 111 with 2,
+            // 131 with 3, 123 with 6; 8192 x 8192 85 with 1, 91 with 2; 20000 x 4096 without
+            // one 64 with 2, 52 with 4.
             const int bytes = threads * 16 * kElem<T> * (residual ? 2 : 1);
             const int each = std::max(1, std::min((residual ? 40960 : 61440) / bytes, 1024 / threads));
             const dim3 grid(blocks_for(M, R, int64_t(each) * device_cus()));
@@ -695,8 +698,8 @@ int64_t rms_norm_grad_work_bytes(int64_t M, int64_t K) {
 
 hipError_t rms_norm_grad(hipStream_t st, const void* dy, int type, const Lines& ldy,
                          const void* h, const Lines& lh, const void* weight, int weight_type,
-                         const void* dh, const Lines& ldh, int64_t inner, float eps, void* dx, void* dweight, int64_t M, int64_t K,
-                         float* part) {
+                         const void* dh, const Lines& ldh, int64_t inner, float eps, void* dx,
+                         void* dweight, int64_t M, int64_t K, float* part) {
     const GradArgs a{dy, h, weight, dh, dx, dweight ? part : nullptr, ldy, lh, ldh, M, K,
                      uint32_t(inner), weight_type, eps};
     const unsigned blocks = blocks_for(M, grad_rows(K), kGradBlocks);

@@ -70,6 +70,24 @@ def test_gradient(dev, dtype, m, k):
         within(got[1], dw, terms * (e + (2 + -(-m // 512) + 32 + 16 + 32) * U))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size", [1e-15, 1e15])
+@pytest.mark.parametrize("k", [7, 100, 1280, 5120, 16390])
+def test_gradient_of_rows_whose_cube_is_out_of_range(dev, dtype, size, k):
+    """r ** 3 is 10 ** 45 or 10 ** -45; what the formula makes of it is not."""
+    x, w = (randn(5, k, seed=1) * size).to(dtype), (1 + 0.2 * randn(k, seed=3)).to(dtype)
+    dy = (randn(5, k, seed=4) + 0.5 * torch.sign(x.float())).to(dtype)
+    leaves = [x.to(dev).requires_grad_(), w.to(dev).requires_grad_()]
+    got = torch.autograd.grad(norm.rms_norm(*leaves, 0.0), leaves, dy.to(dev))
+    _, h, rr = O.rms_norm(x, w, 0.0)
+    dx, dw = O.rms_norm_grad(dy, h, w, 0.0)
+    g, hd = (dy.double() * w.double()).abs(), h.double().abs()
+    e = norm_error(k)
+    within(got[0], dx, rr * g * (e + 4 * U) + hd * rr ** 3 * (g * hd).mean(-1, keepdim=True) * (
+        3 * e + (chain(k) + 8) * U))
+    within(got[1], dw, (dy.double() * h.double() * rr).abs().sum(0) * (e + 90 * U))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,k,rotate", [(m, k, rotate) for m, k in [
     (1, 256), (3, 512), (5, 768), (7, 1280), (2, 2304), (4, 4096), (3, 5120), (2, 16384), (2, 16640),
