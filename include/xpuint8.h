@@ -640,16 +640,17 @@ int xpuint8_moe_combine_grad_stream(const void *stream, const void *dy, int32_t 
  * consecutive experts are a group, its value the sum of its two highest keys; of the
  * experts in the top_groups groups of highest value the `top` highest keys are chosen, ties
  * to the lower index, in the order of their keys (a NaN key counts as the lowest).
- * weights = scale * s, with renormalize = 1 divided by the sum of the chosen s.  An expert whose logit or key is -inf is never chosen;
- * slots left over have id -1 and weight 0.  A row with a NaN logit, for softmax also with
- * one of +inf, has NaN weights.  top <= 64, groups <= 64.  No counterpart in the reference. */
+ * weights = scale * s, with renormalize = 1 divided by the sum of the chosen s.  An expert
+ * whose logit or key is -inf is never chosen; slots left over have id -1 and weight 0.  A
+ * row with a NaN logit, for softmax also with one of +inf, has NaN weights.  top <= 64,
+ * groups <= 64.  No counterpart in the reference. */
 int xpuint8_moe_route_stream(const void *stream, const void *logits, int32_t type, int64_t ld,
                              const float *bias, int32_t sigmoid, int64_t groups,
                              int64_t top_groups, int32_t renormalize, float scale, int32_t *ids,
                              float *weights, int64_t T, int64_t E, int64_t top);
 
 /* dlogits [T, E] (contiguous, the logits' type) of the weights' gradient dweights [T, top];
- * slots without an expert have none */
+ * slots without an expert have none, and no two of a token the same */
 int xpuint8_moe_route_grad_stream(const void *stream, const void *logits, int32_t type, int64_t ld,
                                   const int32_t *ids, const float *dweights, int32_t sigmoid,
                                   int32_t renormalize, float scale, void *dlogits, int64_t T,

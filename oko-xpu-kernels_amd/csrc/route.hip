@@ -189,7 +189,8 @@ __global__ __launch_bounds__(256) void route_exact_kernel(RouteArgs a) {
 // ones, are sorted in every lane and merged across the lanes down to the token's highest 16,
 // all in integer minima and maxima.  The first of these candidates, one a lane, get their
 // keys in 64 bits.  The choice is sure when these are in order and the last one chosen is
-// above anything that the next candidate (with 16 lanes: the 17th key) could be; if not, all
+// above anything that the next candidate (with 16 lanes: the last one, or for 15 and 16 slots
+// the key behind it) could be; if not, all
 // 16 candidates are counted against each other in 64 bits, which 16 keys within 2^-13 to
 // 2^-15 of the last one chosen, a NaN, or scores that underflow leave open still: such a
 // token goes through route_token.  Groups whose fp32 values are too near, and softmax keys
@@ -293,8 +294,9 @@ __device__ __forceinline__ void sort_lane(uint32_t (&a)[M]) {
     }
 }
 // The sorted N values of this side of D and of the other, of which the 16 highest: in both.
+// deep: `rest` becomes the highest of those left out.
 template <int N, int D, int M>
-__device__ __forceinline__ void merge_lanes(uint32_t (&a)[M]) {
+__device__ __forceinline__ void merge_lanes(uint32_t (&a)[M], bool deep, uint32_t& rest) {
     uint32_t b[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) b[i] = other_side<D>(a[i]);
@@ -308,16 +310,21 @@ __device__ __forceinline__ void merge_lanes(uint32_t (&a)[M]) {
         sort_bitonic<N, 0>(a);
         sort_bitonic<N, N>(a);
     } else {
+        if (deep) {
+            rest = max(rest, other_side<D>(rest));
+#pragma unroll
+            for (int i = 0; i < N; ++i) rest = max(rest, min(a[i], b[N - 1 - i]));
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) a[i] = max(a[i], b[N - 1 - i]);
         sort_bitonic<N, 0>(a);
     }
 }
 template <int L, int N, int D = 1, int M>
-__device__ __forceinline__ void merge_token(uint32_t (&a)[M]) {
+__device__ __forceinline__ void merge_token(uint32_t (&a)[M], bool deep, uint32_t& rest) {
     if constexpr (D < L) {
-        merge_lanes<N, D>(a);
-        merge_token<L, (2 * N < kCandidates ? 2 * N : kCandidates), 2 * D>(a);
+        merge_lanes<N, D>(a, deep, rest);
+        merge_token<L, (2 * N < kCandidates ? 2 * N : kCandidates), 2 * D>(a, deep, rest);
     }
 }
 
@@ -590,7 +597,12 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
 #pragma unroll
     for (int i = 0; i < V; ++i) c[i] = (ordered(key[i] + 0.f) & keep) | (kPlace - uint32_t(in * V + i));
     sort_lane<V>(c);
-    merge_token<L, (V < kCandidates ? V : kCandidates)>(c);
+    // the key behind the candidates where it counts: 65536 tokens of 128 experts in fp32, 16
+    // slots 31 us (without it all of them went through route_token: 235)
+    const bool deep = L >= kCandidates && a.top >= kCandidates - 1 && (T == kF32 || !plain);
+    uint32_t last = 0;
+    merge_token<L, (V < kCandidates ? V : kCandidates)>(c, deep, last);
+    if (!deep) last = c[kCandidates - 1];
     Candidate mine[Q];
     double tol = 0.0;
     // the candidates Q ROW + r, in 64 bits
@@ -623,7 +635,7 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
 #pragma unroll
     for (int q = 1; q < Q; ++q) mine[q] = Candidate{0, -1, kCandidates, 0.0, kNone};
     bool ordered_now = in_order<ROW>(mine[0].k, mine[0].packed & kPlace, r, tol);
-    ordered_now &= sure(mine[0], c[Q > 1 ? ROW : kCandidates - 1]);
+    ordered_now &= sure(mine[0], Q > 1 ? c[ROW % kCandidates] : last);
     if (__builtin_amdgcn_ballot_w64(!ordered_now)) {
         if (!plain && !a.how.sigmoid && !sum_exact) exact_sum();
 #pragma unroll
@@ -640,7 +652,7 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
                                                 mine[q].packed & kPlace);
         count_above<ROW, Q>(mine, kPlace);
 #pragma unroll
-        for (int q = 0; q < Q; ++q) bad |= !sure(mine[q], c[kCandidates - 1]);
+        for (int q = 0; q < Q; ++q) bad |= !sure(mine[q], last);
     }
     double total = 1.0;
     if (a.how.renormalize) {

@@ -258,3 +258,23 @@ def test_biases_that_are_not_finite(dev, how, groups, top_groups):
         bias[:] = value
         check(dev, logits_of(t, e, torch.float32), 6, **HOWS[how], bias=bias, groups=groups,
               top_groups=top_groups)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("how", range(len(HOWS)))
+@pytest.mark.parametrize("e", [16, 17, 40, 128, 256, 512, 1000])
+def test_as_many_slots_as_candidates(dev, dtype, how, e):
+    """9 to 16 slots; with keys that are a unit apart, or the same, around the last one."""
+    logits = logits_of(25, e, dtype)
+    order = logits.float().argsort(-1, descending=True)
+    for j in range(8, min(e, 22)):                 # rows 10 to 19: the 9th key on is a cluster
+        step = torch.tensor(float(j % 3)) * (2.0 ** -22 if dtype == torch.float32 else 0.0)
+        rows = torch.arange(10, 20)
+        logits[rows, order[rows, j]] = (logits[rows, order[rows, 8]].float() * (1 - step)).to(dtype)
+    logits[20:] = logits[20:, :1]                  # all the same
+    for top in (9, 14, 15, 16):
+        check(dev, logits, top, randn(25, top, seed=7), **HOWS[how])
+        check(dev, logits, top, **HOWS[how], bias=randn(e, seed=5) * 0.05)
+        check(dev, logits, top, **HOWS[how], bias=torch.zeros(e))
+        if e % 4 == 0 and e // 2 >= top:
+            check(dev, logits, top, **HOWS[how], bias=torch.zeros(e), groups=4, top_groups=2)
