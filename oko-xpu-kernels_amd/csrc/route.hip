@@ -201,7 +201,11 @@ __global__ __launch_bounds__(256) void route_exact_kernel(RouteArgs a) {
 // of 128 by biased sigmoids in fp32 17 and 22; 32768 of 256 in bf16 10 and 13).  Groups take 16
 // lanes below 65536 tokens, whose waves are too few to hide what the groups add (8192 tokens of
 // 256 in 8 groups 10 us and 13 with 8 lanes, 65536 34 and 34).  16381 of these take 16 us (with a
-// wave a token and all keys in 64 bits 103), 4 tokens of 64 experts 2.5.
+// wave a token and all keys in 64 bits 103), 4 tokens of 64 experts 2.5.  More than 256 experts
+// take 16 or 32 lanes from 8192 tokens on (8 of 512 in bf16: 8192 tokens 6.9 us and 9.0 with
+// twice the lanes, 65536 33 and 52; 8 of 1024: 81 and 130), below that twice as many (2048
+// tokens of 512 4.5 us and 4.8).
+constexpr int64_t kManyTokens = 8192;
 constexpr int kCandidates = 16;
 constexpr uint32_t kNothing = 0x00800000u;           // ordered(-inf) and the bits of a place are below
 
@@ -279,15 +283,19 @@ __device__ __forceinline__ void sort_odd_even(uint32_t (&a)[M]) {
         merge_odd_even<N, AT, 1>(a);
     }
 }
-// a lane's own V keys sorted, the 16 highest of 32
+// a lane's own V keys sorted, the 16 highest of 32; deep: `rest` becomes the highest other one
 template <int V, int M>
-__device__ __forceinline__ void sort_lane(uint32_t (&a)[M]) {
+__device__ __forceinline__ void sort_lane(uint32_t (&a)[M], bool deep, uint32_t& rest) {
     if constexpr (V <= kCandidates) {
         sort_odd_even<V, 0>(a);
     } else {
         static_assert(V == 2 * kCandidates);
         sort_odd_even<kCandidates, 0>(a);
         sort_odd_even<kCandidates, kCandidates>(a);
+        if (deep) {
+#pragma unroll
+            for (int i = 0; i < kCandidates; ++i) rest = max(rest, min(a[i], a[V - 1 - i]));
+        }
 #pragma unroll
         for (int i = 0; i < kCandidates; ++i) a[i] = max(a[i], a[V - 1 - i]);
         sort_bitonic<kCandidates, 0>(a);
@@ -403,9 +411,13 @@ __device__ __forceinline__ void count_above(Candidate (&c)[Q], uint32_t places) 
     }
 }
 
-// how the experts of a token lie: group g in the 2^bits lanes from g * 2^bits on, `each` a lane
+// How the experts of a token lie: group g in the 2^bits lanes from g * 2^bits on, `each` a lane.
+// A lane reads V logits from its first one on or, where there are fewer, the last V of its
+// group, and masks those that the lanes before have (all of them, if none are left for it).
+// Groups of fewer than V are read one by one.
 struct Spread {
     int bits, each;
+    int last;                                         // where a lane's logits begin at most
 };
 
 // V consecutive logits from `at` on (-inf past `count`), in one load if they are whole
@@ -443,8 +455,17 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
     const int lane = threadIdx.x & 63, in = lane & (L - 1), r = lane & (ROW - 1);
     const int n = a.E / a.how.groups;
     const int group = in >> sp.bits, part = in & ((1 << sp.bits) - 1);
-    const int first = group * n + part * sp.each;     // this lane's experts
-    const int count = group < a.how.groups ? max(0, min(sp.each, n - part * sp.each)) : 0;
+    const bool there = group < a.how.groups;
+    const int first = (there ? group * n : 0) + min(part * sp.each, sp.last);
+    const int count = n >= V ? V : there ? max(0, min(sp.each, n - part * sp.each)) : 0;
+    const int skip = n < V ? 0 : there ? min(V, max(0, part * sp.each - sp.last)) : V;
+    const bool skips = __builtin_amdgcn_ballot_w64(skip != 0) != 0;
+    auto mask = [&](float (&l)[V]) {
+        if (skips) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) l[i] = i < skip ? -INFINITY : l[i];
+        }
+    };
     const bool plain = !a.bias && a.how.groups == 1;  // keys are the logits
     const int64_t t0 = first_token + (int64_t(blockIdx.x) * WAVES + (threadIdx.x >> 6)) * PER;
     if (t0 >= a.T) return;
@@ -467,6 +488,7 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
             for (int i = 0; i < V; ++i)
                 bad |= __builtin_isnan(key[i]) || (!a.how.sigmoid && key[i] == INFINITY);
         }
+        mask(key);
     }
     if (!a.how.sigmoid) most = token_max<L>(most);
     // fp32 scores.  A sigmoid s: its exponential off by 2 units (2^-24) and |l| of its
@@ -513,6 +535,7 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
                     for (int i = 0; i < V; ++i) bad |= __builtin_isnan(e[i]);
                 }
             }
+            if (!odd) mask(e);
 #pragma unroll
             for (int i = 0; i < V; ++i) key[i] = e[i];
         }
@@ -523,6 +546,7 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
     auto exact_sum = [&] {
         float l[V];
         logits_load<T>(a.logits, t * a.ld + first, count, l);
+        mask(l);
         double u = 0.0;
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -569,6 +593,7 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
             double first64 = kNone, second64 = kNone;
             float l[V];
             logits_load<T>(a.logits, t * a.ld + first, count, l);
+            mask(l);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 if (l[i] == -INFINITY) continue;
@@ -596,11 +621,11 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
     // (a sum with 0 has no negative zero, which would order below the zero that it equals)
 #pragma unroll
     for (int i = 0; i < V; ++i) c[i] = (ordered(key[i] + 0.f) & keep) | (kPlace - uint32_t(in * V + i));
-    sort_lane<V>(c);
     // the key behind the candidates where it counts: 65536 tokens of 128 experts in fp32, 16
     // slots 31 us (without it all of them went through route_token: 235)
     const bool deep = L >= kCandidates && a.top >= kCandidates - 1 && (T == kF32 || !plain);
     uint32_t last = 0;
+    sort_lane<V>(c, deep, last);
     merge_token<L, (V < kCandidates ? V : kCandidates)>(c, deep, last);
     if (!deep) last = c[kCandidates - 1];
     Candidate mine[Q];
@@ -612,7 +637,8 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
 #pragma unroll
         for (int i = 1; i < ROW; ++i) m.packed = r == i ? c[q * ROW + i] : m.packed;
         const int at = int(kPlace - (m.packed & kPlace)) / V, i = int(kPlace - (m.packed & kPlace)) % V;
-        m.e = m.packed >= kNothing ? (at >> sp.bits) * n + (at & ((1 << sp.bits) - 1)) * sp.each + i : -1;
+        const int from = min((at & ((1 << sp.bits) - 1)) * sp.each, sp.last);
+        m.e = m.packed >= kNothing ? (at >> sp.bits) * n + from + i : -1;
         m.s = 0.0;
         m.k = kNone;
         m.rank = q * ROW + r;
@@ -933,17 +959,19 @@ hipError_t moe_route(hipStream_t st, const void* logits, int type, int64_t ld, c
         if (done || padded > L || top > (L < kCandidates ? L : kCandidates)) return;
         int bits = 0;
         while (padded << (bits + 1) <= L) ++bits;
-        const Spread sp{bits, (n + (1 << bits) - 1) >> bits};
-        if (sp.each > V) return;
+        if (n > V << bits) return;
+        const Spread sp = n < V ? Spread{bits, (n + (1 << bits) - 1) >> bits, n} : Spread{bits, V, n - V};
         done = true;
         // small calls in blocks of one wave, which spread over more of the chip
-        const int64_t per = 64 / L;
-        if (T >= 2048 * per)
+        constexpr int64_t per = 64 / L;
+        constexpr bool many = L >= 16 && V == 32;     // (for these alone)
+        static_assert(!many || kManyTokens >= 2048 * per);
+        if (many || T >= 2048 * per)
             in_launches(T, kMaxBlocks * 4 * per, [&](int64_t at, int64_t m) {
                 hipLaunchKernelGGL((route_kernel<TY, L, V, 256>), dim3(unsigned((m + 4 * per - 1) / (4 * per))),
                                    dim3(256), 0, st, a, sp, at);
             });
-        else
+        else if constexpr (!many)
             hipLaunchKernelGGL((route_kernel<TY, L, V, 64>), dim3(unsigned((T + per - 1) / per)), dim3(64),
                                0, st, a, sp, int64_t(0));
     };
@@ -956,6 +984,10 @@ hipError_t moe_route(hipStream_t st, const void* logits, int type, int64_t ld, c
         go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
         go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{});
         go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 16>{});
+        if (T >= kManyTokens) {
+            go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 32>{});
+            go(t, std::integral_constant<int, 32>{}, std::integral_constant<int, 32>{});
+        }
         go(t, std::integral_constant<int, 32>{}, std::integral_constant<int, 16>{});
         go(t, std::integral_constant<int, 64>{}, std::integral_constant<int, 16>{});
     };

@@ -278,3 +278,53 @@ def test_as_many_slots_as_candidates(dev, dtype, how, e):
         check(dev, logits, top, **HOWS[how], bias=torch.zeros(e))
         if e % 4 == 0 and e // 2 >= top:
             check(dev, logits, top, **HOWS[how], bias=torch.zeros(e), groups=4, top_groups=2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("how", range(len(HOWS)))
+@pytest.mark.parametrize("e,groups,top_groups", [
+    (9, 1, 1), (23, 1, 1), (33, 3, 2), (60, 4, 2), (65, 5, 3), (72, 8, 4), (100, 1, 1), (130, 1, 1), (144, 12, 4), (257, 1, 1),
+    (264, 8, 3), (384, 1, 1), (385, 5, 2), (513, 1, 1), (768, 8, 4), (1023, 1, 1), (1023, 31, 7)])
+def test_experts_that_do_not_fill_their_lanes(dev, dtype, how, e, groups, top_groups):
+    """Masked, infinite and equal logits where lanes overlap and at the rows' ends."""
+    t, top = 21, min(8, e // groups * top_groups)
+    logits = logits_of(t, e, dtype)
+    logits[3:6, -9:] = 4.0                          # the last ones, all the same
+    logits[6:9, -7:] = -math.inf
+    logits[9:12, : e - 5] = -math.inf
+    logits[12, -1] = logits[13, -8] = math.inf
+    logits[14, -2] = math.nan
+    logits[15] = logits[15, 0]
+    logits[16:18] = -math.inf
+    logits[17, -1] = -1.0
+    wide = torch.full((t, e + 40), 50.0, dtype=dtype, device=dev)      # what lies beside is higher
+    wide[:, 20:e + 20] = logits.to(dev)
+    for bias in (None, torch.zeros(e), randn(e, seed=5) * 0.05):
+        call = dict(HOWS[how], bias=bias, groups=groups, top_groups=top_groups)
+        ids, w = check(dev, logits, top, **call)
+        call["bias"] = None if bias is None else bias.to(dev)
+        ids2, w2 = moe.route(wide[:, 20:e + 20], top, **call)
+        assert torch.equal(ids, ids2) and torch.equal(w.nan_to_num(7.0), w2.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("e,groups,top_groups", [(300, 1, 1), (512, 8, 4), (520, 1, 1), (1000, 20, 4), (1024, 1, 1),
+                                                 (1024, 32, 9)])
+@pytest.mark.parametrize("how", [0, 1, 2])
+def test_many_tokens_of_many_experts(dev, dtype, e, groups, top_groups, how):
+    """As a few tokens at a time, which have more lanes."""
+    t = 8200
+    lg = logits_of(t, e, dtype).to(dev)
+    lg[::1000, : e // 2] = -math.inf
+    lg[5::2000] = -math.inf
+    lg[7, 3] = math.nan
+    lg[20:40, ::3] = 2.5
+    for top, bias in ((8, None), (15, torch.zeros(e, device=dev)), (16, (randn(e, seed=5) * 0.05).to(dev))):
+        call = dict(HOWS[how], bias=bias, groups=groups, top_groups=top_groups)
+        ids, w = moe.route(lg, top, **call)
+        parts = [moe.route(lg[i:i + 3000], top, **call) for i in range(0, t, 3000)]
+        assert torch.equal(ids, torch.cat([p[0] for p in parts]))
+        want = torch.cat([p[1] for p in parts])
+        assert torch.equal(w.isnan(), want.isnan())
+        error = 2 * weight_error(HOWS[how]) + 2 * U
+        assert ((w - want).abs() <= error * want.abs()).logical_or(w.isnan()).all()
