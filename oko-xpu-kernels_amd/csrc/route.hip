@@ -36,39 +36,106 @@ __device__ __forceinline__ float logit_at(const void* logits, int64_t row, int64
     else return float(static_cast<const _Float16*>(logits)[i]);
 }
 
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = dppu<CTRL>(uint32_t(b)), hi = dppu<CTRL>(uint32_t(b >> 32));
+    return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_any(float x) { return dpp<CTRL>(x); }
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_any(uint32_t x) { return dppu<CTRL>(x); }
+template <int CTRL>
+__device__ __forceinline__ int dpp_any(int x) { return int(dppu<CTRL>(uint32_t(x))); }
+template <int CTRL>
+__device__ __forceinline__ double dpp_any(double x) { return dpp64<CTRL>(x); }
+
+// the values of two lanes D (16 or 32) apart, in both of them, without a trip through LDS
+template <class V>
+struct Both {
+    V lo, hi;
+};
+template <int D>
+__device__ __forceinline__ Both<uint32_t> both_sides(uint32_t x) {
+    if constexpr (D == 16) {
+        const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return {p[0], p[1]};
+    } else {
+        const auto p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return {p[0], p[1]};
+    }
+}
+template <int D>
+__device__ __forceinline__ Both<int> both_sides(int x) {
+    const auto p = both_sides<D>(uint32_t(x));
+    return {int(p.lo), int(p.hi)};
+}
+template <int D>
+__device__ __forceinline__ Both<float> both_sides(float x) {
+    const auto p = both_sides<D>(__float_as_uint(x));
+    return {__uint_as_float(p.lo), __uint_as_float(p.hi)};
+}
+template <int D>
+__device__ __forceinline__ Both<double> both_sides(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const auto l = both_sides<D>(uint32_t(b)), h = both_sides<D>(uint32_t(b >> 32));
+    return {__builtin_bit_cast(double, uint64_t(h.lo) << 32 | l.lo),
+            __builtin_bit_cast(double, uint64_t(h.hi) << 32 | l.hi)};
+}
+
 template <class V>
 __device__ __forceinline__ V wave_total(V x) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
-    return x;
+    x += dpp_any<kDppXor1>(x);
+    x += dpp_any<kDppXor2>(x);
+    x += dpp_any<kDppXor7>(x);
+    x += dpp_any<kDppXor15>(x);
+    const auto p = both_sides<16>(x);
+    const auto q = both_sides<32>(p.lo + p.hi);
+    return q.lo + q.hi;
 }
 template <class V>
+__device__ __forceinline__ V greater_of(V x, V y) { return y > x ? y : x; }
+template <class V>
 __device__ __forceinline__ V wave_most(V x) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const V y = __shfl_xor(x, d);
-        x = y > x ? y : x;
-    }
-    return x;
+    x = greater_of(x, dpp_any<kDppXor1>(x));
+    x = greater_of(x, dpp_any<kDppXor2>(x));
+    x = greater_of(x, dpp_any<kDppXor7>(x));
+    x = greater_of(x, dpp_any<kDppXor15>(x));
+    const auto p = both_sides<16>(x);
+    const auto q = both_sides<32>(greater_of(p.lo, p.hi));
+    return greater_of(q.lo, q.hi);
 }
 
 // the highest key of the wave and its expert (the lowest of equal ones), in every lane
-__device__ __forceinline__ void wave_best(double& key, int& e) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double k = __shfl_xor(key, d);
-        const int o = __shfl_xor(e, d);
-        if (k > key || (k == key && o < e)) {
-            key = k;
-            e = o;
-        }
+__device__ __forceinline__ void take_best(double& key, int& e, double k, int o) {
+    if (k > key || (k == key && o < e)) {
+        key = k;
+        e = o;
     }
+}
+__device__ __forceinline__ void wave_best(double& key, int& e) {
+    take_best(key, e, dpp_any<kDppXor1>(key), dpp_any<kDppXor1>(e));
+    take_best(key, e, dpp_any<kDppXor2>(key), dpp_any<kDppXor2>(e));
+    take_best(key, e, dpp_any<kDppXor7>(key), dpp_any<kDppXor7>(e));
+    take_best(key, e, dpp_any<kDppXor15>(key), dpp_any<kDppXor15>(e));
+    const auto k16 = both_sides<16>(key);
+    const auto e16 = both_sides<16>(e);
+    key = k16.lo;
+    e = e16.lo;
+    take_best(key, e, k16.hi, e16.hi);
+    const auto k32 = both_sides<32>(key);
+    const auto e32 = both_sides<32>(e);
+    key = k32.lo;
+    e = e32.lo;
+    take_best(key, e, k32.hi, e32.hi);
 }
 
 constexpr double kNone = -__builtin_huge_val();      // not to be chosen
 constexpr double kLowest = -1.7976931348623157e308;
 
-// A token by a whole wave, lane l holding the experts l, l + 64, ..; keys are 64 bits.
+// A token by a whole wave, lane l holding the experts l, l + 64, ..; keys are 64 bits.  A round a
+// slot: 4 tokens, 24 of 256 experts 13.6 us (20 with all exchanges through LDS), 65536 284.
 template <int T, int V>
 __device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t) {
     const int lane = threadIdx.x & 63;
@@ -203,24 +270,11 @@ __global__ __launch_bounds__(256) void route_exact_kernel(RouteArgs a) {
 // 256 in 8 groups 10 us and 13 with 8 lanes, 65536 34 and 34).  16381 of these take 16 us (with a
 // wave a token and all keys in 64 bits 103), 4 tokens of 64 experts 2.5.  More than 256 experts
 // take 16 or 32 lanes from 8192 tokens on (8 of 512 in bf16: 8192 tokens 6.9 us and 9.0 with
-// twice the lanes, 65536 33 and 52; 8 of 1024: 81 and 130), below that twice as many (2048
-// tokens of 512 4.5 us and 4.8).
+// twice the lanes, 65536 33 and 52; 8 of 1024: 81 and 130, 73 since lanes 16 and 32 apart meet
+// without LDS), below that twice as many (2048 tokens of 512 4.5 us and 4.8).
 constexpr int64_t kManyTokens = 8192;
 constexpr int kCandidates = 16;
 constexpr uint32_t kNothing = 0x00800000u;           // ordered(-inf) and the bits of a place are below
-
-template <int CTRL>
-__device__ __forceinline__ double dpp64(double x) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, x);
-    const uint32_t lo = dppu<CTRL>(uint32_t(b)), hi = dppu<CTRL>(uint32_t(b >> 32));
-    return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
-}
-template <int CTRL>
-__device__ __forceinline__ float dpp_any(float x) { return dpp<CTRL>(x); }
-template <int CTRL>
-__device__ __forceinline__ uint32_t dpp_any(uint32_t x) { return dppu<CTRL>(x); }
-template <int CTRL>
-__device__ __forceinline__ double dpp_any(double x) { return dpp64<CTRL>(x); }
 
 // x of another lane of a row of ROW lanes, every lane of it once over K = 1 .. ROW - 1: of 16
 // by rotation, of 8 of lane ^ K
@@ -236,15 +290,15 @@ __device__ __forceinline__ X other_lane(X x) {
     else if constexpr (K == 5) return dpp_any<kDppXor2>(dpp_any<kDppXor7>(x));
     else return dpp_any<kDppXor1>(dpp_any<kDppXor7>(x));
 }
-// x of a lane on the other side of D, where the lanes of each side hold the same: lane ^ 1,
-// ^ 2, ^ 7, ^ 15 by DPP, then ^ 16 and ^ 32
+// x and that of a lane on the other side of D, where the lanes of each side hold the same: lane
+// ^ 1, ^ 2, ^ 7, ^ 15 by DPP, then the same two of D = 16 and 32 in both
 template <int D>
-__device__ __forceinline__ uint32_t other_side(uint32_t x) {
-    if constexpr (D == 1) return dppu<kDppXor1>(x);
-    else if constexpr (D == 2) return dppu<kDppXor2>(x);
-    else if constexpr (D == 4) return dppu<kDppXor7>(x);
-    else if constexpr (D == 8) return dppu<kDppXor15>(x);
-    else return uint32_t(__shfl_xor(int(x), D));
+__device__ __forceinline__ Both<uint32_t> sides(uint32_t x) {
+    if constexpr (D == 1) return {x, dppu<kDppXor1>(x)};
+    else if constexpr (D == 2) return {x, dppu<kDppXor2>(x)};
+    else if constexpr (D == 4) return {x, dppu<kDppXor7>(x)};
+    else if constexpr (D == 8) return {x, dppu<kDppXor15>(x)};
+    else return both_sides<D>(x);
 }
 
 // a falls along i: compare and exchange
@@ -307,7 +361,11 @@ template <int N, int D, int M>
 __device__ __forceinline__ void merge_lanes(uint32_t (&a)[M], bool deep, uint32_t& rest) {
     uint32_t b[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) b[i] = other_side<D>(a[i]);
+    for (int i = 0; i < N; ++i) {
+        const auto p = sides<D>(a[i]);
+        a[i] = p.lo;
+        b[i] = p.hi;
+    }
     if constexpr (N < kCandidates) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -319,7 +377,8 @@ __device__ __forceinline__ void merge_lanes(uint32_t (&a)[M], bool deep, uint32_
         sort_bitonic<N, N>(a);
     } else {
         if (deep) {
-            rest = max(rest, other_side<D>(rest));
+            const auto p = sides<D>(rest);
+            rest = max(p.lo, p.hi);
 #pragma unroll
             for (int i = 0; i < N; ++i) rest = max(rest, min(a[i], b[N - 1 - i]));
         }
@@ -347,8 +406,14 @@ __device__ __forceinline__ double token_total(double x) {
     x += dpp64<kDppXor2>(x);
     x += dpp64<kDppXor7>(x);
     if constexpr (L >= 16) x += dpp64<kDppXor15>(x);
-#pragma unroll
-    for (int d = 16; d < L; d *= 2) x += __shfl_xor(x, d);
+    if constexpr (L >= 32) {
+        const auto p = both_sides<16>(x);
+        x = p.lo + p.hi;
+    }
+    if constexpr (L >= 64) {
+        const auto p = both_sides<32>(x);
+        x = p.lo + p.hi;
+    }
     return x;
 }
 template <int L>
