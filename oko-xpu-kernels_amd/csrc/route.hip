@@ -135,7 +135,8 @@ constexpr double kNone = -__builtin_huge_val();      // not to be chosen
 constexpr double kLowest = -1.7976931348623157e308;
 
 // A token by a whole wave, lane l holding the experts l, l + 64, ..; keys are 64 bits.  A round a
-// slot: 4 tokens, 24 of 256 experts 13.6 us (20 with all exchanges through LDS), 65536 284.
+// slot: 4 tokens, 24 of 256 experts 13.6 us (20 with all exchanges through LDS; 5.9 by 32
+// candidates), 65536 284 (47).
 template <int T, int V>
 __device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t) {
     const int lane = threadIdx.x & 63;
@@ -253,8 +254,9 @@ __global__ __launch_bounds__(256) void route_exact_kernel(RouteArgs a) {
 // ------------------------------------------------------------ several tokens a wave
 // A token has L lanes of V experts, 64 / L tokens a wave.  Keys are made in fp32 first, to
 // a known error; of each the 32 bits that order like it, with the expert's place in the low
-// ones, are sorted in every lane and merged across the lanes down to the token's highest 16,
-// all in integer minima and maxima.  The first of these candidates, one a lane, get their
+// ones, are sorted in every lane and merged across the lanes down to the token's highest 16
+// (32 for 17 to 32 slots, which begin with the counting below), all in integer minima and
+// maxima.  The first of these candidates, one a lane, get their
 // keys in 64 bits.  The choice is sure when these are in order and the last one chosen is
 // above anything that the next candidate (with 16 lanes: the last one, or for 15 and 16 slots
 // the key behind it) could be; if not, all
@@ -273,7 +275,6 @@ __global__ __launch_bounds__(256) void route_exact_kernel(RouteArgs a) {
 // twice the lanes, 65536 33 and 52; 8 of 1024: 81 and 130, 73 since lanes 16 and 32 apart meet
 // without LDS), below that twice as many (2048 tokens of 512 4.5 us and 4.8).
 constexpr int64_t kManyTokens = 8192;
-constexpr int kCandidates = 16;
 constexpr uint32_t kNothing = 0x00800000u;           // ordered(-inf) and the bits of a place are below
 
 // x of another lane of a row of ROW lanes, every lane of it once over K = 1 .. ROW - 1: of 16
@@ -337,27 +338,27 @@ __device__ __forceinline__ void sort_odd_even(uint32_t (&a)[M]) {
         merge_odd_even<N, AT, 1>(a);
     }
 }
-// a lane's own V keys sorted, the 16 highest of 32; deep: `rest` becomes the highest other one
-template <int V, int M>
+// a lane's own V keys sorted, the C highest of 2 C; deep: `rest` becomes the highest other one
+template <int V, int C, int M>
 __device__ __forceinline__ void sort_lane(uint32_t (&a)[M], bool deep, uint32_t& rest) {
-    if constexpr (V <= kCandidates) {
+    if constexpr (V <= C) {
         sort_odd_even<V, 0>(a);
     } else {
-        static_assert(V == 2 * kCandidates);
-        sort_odd_even<kCandidates, 0>(a);
-        sort_odd_even<kCandidates, kCandidates>(a);
+        static_assert(V == 2 * C);
+        sort_odd_even<C, 0>(a);
+        sort_odd_even<C, C>(a);
         if (deep) {
 #pragma unroll
-            for (int i = 0; i < kCandidates; ++i) rest = max(rest, min(a[i], a[V - 1 - i]));
+            for (int i = 0; i < C; ++i) rest = max(rest, min(a[i], a[V - 1 - i]));
         }
 #pragma unroll
-        for (int i = 0; i < kCandidates; ++i) a[i] = max(a[i], a[V - 1 - i]);
-        sort_bitonic<kCandidates, 0>(a);
+        for (int i = 0; i < C; ++i) a[i] = max(a[i], a[V - 1 - i]);
+        sort_bitonic<C, 0>(a);
     }
 }
-// The sorted N values of this side of D and of the other, of which the 16 highest: in both.
+// The sorted N values of this side of D and of the other, of which the C highest: in both.
 // deep: `rest` becomes the highest of those left out.
-template <int N, int D, int M>
+template <int N, int C, int D, int M>
 __device__ __forceinline__ void merge_lanes(uint32_t (&a)[M], bool deep, uint32_t& rest) {
     uint32_t b[N];
 #pragma unroll
@@ -366,7 +367,7 @@ __device__ __forceinline__ void merge_lanes(uint32_t (&a)[M], bool deep, uint32_
         a[i] = p.lo;
         b[i] = p.hi;
     }
-    if constexpr (N < kCandidates) {
+    if constexpr (N < C) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t u = a[i], v = b[N - 1 - i];
@@ -387,11 +388,11 @@ __device__ __forceinline__ void merge_lanes(uint32_t (&a)[M], bool deep, uint32_
         sort_bitonic<N, 0>(a);
     }
 }
-template <int L, int N, int D = 1, int M>
+template <int L, int N, int C, int D = 1, int M>
 __device__ __forceinline__ void merge_token(uint32_t (&a)[M], bool deep, uint32_t& rest) {
     if constexpr (D < L) {
-        merge_lanes<N, D>(a, deep, rest);
-        merge_token<L, (2 * N < kCandidates ? 2 * N : kCandidates), 2 * D>(a, deep, rest);
+        merge_lanes<N, C, D>(a, deep, rest);
+        merge_token<L, (2 * N < C ? 2 * N : C), C, 2 * D>(a, deep, rest);
     }
 }
 
@@ -512,10 +513,10 @@ __device__ __forceinline__ void logits_load(const void* logits, int64_t at, int 
     for (int i = 0; i < V; ++i) l[i] = i < count ? logit_at<T>(p, 0, 0, i) : -INFINITY;
 }
 
-template <int T, int L, int V, int THREADS>
+template <int T, int L, int V, int C, int THREADS>
 __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, int64_t first_token) {
     constexpr int PER = 64 / L, WAVES = THREADS / 64;
-    constexpr int ROW = L < 16 ? L : 16, Q = kCandidates / ROW;      // candidates a lane, in all
+    constexpr int ROW = L < 16 ? L : 16, Q = C / ROW;  // lanes with candidates, and of each
     constexpr uint32_t kPlace = L * V - 1;            // the bits of an expert's place
     const int lane = threadIdx.x & 63, in = lane & (L - 1), r = lane & (ROW - 1);
     const int n = a.E / a.how.groups;
@@ -681,18 +682,18 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
         }
     }
     // (-inf orders below kNothing, and so does what is dropped)
-    uint32_t c[V > kCandidates ? V : kCandidates];
+    uint32_t c[V > C ? V : C];
     const uint32_t keep = dropped ? 0u : ~kPlace;
     // (a sum with 0 has no negative zero, which would order below the zero that it equals)
 #pragma unroll
     for (int i = 0; i < V; ++i) c[i] = (ordered(key[i] + 0.f) & keep) | (kPlace - uint32_t(in * V + i));
     // the key behind the candidates where it counts: 65536 tokens of 128 experts in fp32, 16
     // slots 31 us (without it all of them went through route_token: 235)
-    const bool deep = L >= kCandidates && a.top >= kCandidates - 1 && (T == kF32 || !plain);
+    const bool deep = L >= 16 && a.top >= C - 1 && (T == kF32 || !plain);
     uint32_t last = 0;
-    sort_lane<V>(c, deep, last);
-    merge_token<L, (V < kCandidates ? V : kCandidates)>(c, deep, last);
-    if (!deep) last = c[kCandidates - 1];
+    sort_lane<V, C>(c, deep, last);
+    merge_token<L, (V < C ? V : C), C>(c, deep, last);
+    if (!deep) last = c[C - 1];
     Candidate mine[Q];
     double tol = 0.0;
     // the candidates Q ROW + r, in 64 bits
@@ -722,11 +723,15 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
         const float highest = unordered(next | kPlace);
         return m.k > double(highest) + 2.0 * off + (plain ? 0.0 : 0x1p-22 * fabs(double(highest)));
     };
-    look(0);
+    // (32 candidates are for slots that the first of a lane are too few for)
+    bool ordered_now = false;
+    if constexpr (C <= 16) {
+        look(0);
 #pragma unroll
-    for (int q = 1; q < Q; ++q) mine[q] = Candidate{0, -1, kCandidates, 0.0, kNone};
-    bool ordered_now = in_order<ROW>(mine[0].k, mine[0].packed & kPlace, r, tol);
-    ordered_now &= sure(mine[0], Q > 1 ? c[ROW % kCandidates] : last);
+        for (int q = 1; q < Q; ++q) mine[q] = Candidate{0, -1, C, 0.0, kNone};
+        ordered_now = in_order<ROW>(mine[0].k, mine[0].packed & kPlace, r, tol);
+        ordered_now &= sure(mine[0], Q > 1 ? c[ROW % C] : last);
+    }
     if (__builtin_amdgcn_ballot_w64(!ordered_now)) {
         if (!plain && !a.how.sigmoid && !sum_exact) exact_sum();
 #pragma unroll
@@ -1019,42 +1024,56 @@ hipError_t moe_route(hipStream_t st, const void* logits, int type, int64_t ld, c
     while (padded < how.groups) padded *= 2;
     const int n = E / how.groups;
     bool done = false;
-    auto go = [&](auto t, auto lanes, auto v) {
+    auto go = [&](auto t, auto lanes, auto v, auto candidates) {
         constexpr int L = decltype(lanes)::value, V = decltype(v)::value, TY = decltype(t)::value;
-        if (done || padded > L || top > (L < kCandidates ? L : kCandidates)) return;
+        constexpr int C = decltype(candidates)::value;
+        if (done || padded > L || top > (L < 16 ? L : C)) return;
         int bits = 0;
         while (padded << (bits + 1) <= L) ++bits;
         if (n > V << bits) return;
         const Spread sp = n < V ? Spread{bits, (n + (1 << bits) - 1) >> bits, n} : Spread{bits, V, n - V};
         done = true;
-        // small calls in blocks of one wave, which spread over more of the chip
         constexpr int64_t per = 64 / L;
-        constexpr bool many = L >= 16 && V == 32;     // (for these alone)
-        static_assert(!many || kManyTokens >= 2048 * per);
-        if (many || T >= 2048 * per)
-            in_launches(T, kMaxBlocks * 4 * per, [&](int64_t at, int64_t m) {
-                hipLaunchKernelGGL((route_kernel<TY, L, V, 256>), dim3(unsigned((m + 4 * per - 1) / (4 * per))),
-                                   dim3(256), 0, st, a, sp, at);
+        auto launch = [&](auto threads) {
+            constexpr int N = decltype(threads)::value;
+            constexpr int64_t tokens = N / 64 * per;  // a block
+            in_launches(T, kMaxBlocks * tokens, [&](int64_t at, int64_t m) {
+                hipLaunchKernelGGL((route_kernel<TY, L, V, C, N>), dim3(unsigned((m + tokens - 1) / tokens)),
+                                   dim3(N), 0, st, a, sp, at);
             });
-        else if constexpr (!many)
-            hipLaunchKernelGGL((route_kernel<TY, L, V, 64>), dim3(unsigned((T + per - 1) / per)), dim3(64),
-                               0, st, a, sp, int64_t(0));
+        };
+        // small calls in blocks of one wave, which spread over more of the chip, and all with
+        // more than 16 slots
+        constexpr bool many = L >= 16 && V == 32;     // (for these alone, with up to 16)
+        static_assert(!many || kManyTokens >= 2048 * per);
+        if constexpr (C > 16) launch(std::integral_constant<int, 64>{});
+        else if (many || T >= 2048 * per) launch(std::integral_constant<int, 256>{});
+        else if constexpr (!many) launch(std::integral_constant<int, 64>{});
     };
     auto by = [&](auto t) {
+        constexpr std::integral_constant<int, 4> k4;
+        constexpr std::integral_constant<int, 8> k8;
+        constexpr std::integral_constant<int, 16> k16;
+        constexpr std::integral_constant<int, 32> k32;
+        constexpr std::integral_constant<int, 64> k64;
         if (how.groups == 1 || T >= 65536) {          // (see above)
-            go(t, std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
-            go(t, std::integral_constant<int, 8>{}, std::integral_constant<int, 16>{});
-            go(t, std::integral_constant<int, 8>{}, std::integral_constant<int, 32>{});
+            go(t, k8, k8, k16);
+            go(t, k8, k16, k16);
+            go(t, k8, k32, k16);
         }
-        go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
-        go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{});
-        go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 16>{});
+        go(t, k16, k4, k16);
+        go(t, k16, k8, k16);
+        go(t, k16, k16, k16);
         if (T >= kManyTokens) {
-            go(t, std::integral_constant<int, 16>{}, std::integral_constant<int, 32>{});
-            go(t, std::integral_constant<int, 32>{}, std::integral_constant<int, 32>{});
+            go(t, k16, k32, k16);
+            go(t, k32, k32, k16);
         }
-        go(t, std::integral_constant<int, 32>{}, std::integral_constant<int, 16>{});
-        go(t, std::integral_constant<int, 64>{}, std::integral_constant<int, 16>{});
+        go(t, k32, k16, k16);
+        go(t, k64, k16, k16);
+        go(t, k16, k4, k32);
+        go(t, k16, k16, k32);
+        go(t, k16, k32, k32);
+        go(t, k32, k32, k32);
     };
     if (type == kBf16) by(std::integral_constant<int, kBf16>{});
     else if (type == kF16) by(std::integral_constant<int, kF16>{});

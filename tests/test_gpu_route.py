@@ -328,3 +328,26 @@ def test_many_tokens_of_many_experts(dev, dtype, e, groups, top_groups, how):
         assert torch.equal(w.isnan(), want.isnan())
         error = 2 * weight_error(HOWS[how]) + 2 * U
         assert ((w - want).abs() <= error * want.abs()).logical_or(w.isnan()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("how", range(len(HOWS)))
+@pytest.mark.parametrize("e", [32, 33, 64, 100, 256, 384, 1000])
+def test_seventeen_to_thirty_three_slots(dev, dtype, how, e):
+    """With keys that are a unit apart, or the same, around the last one."""
+    t = 17
+    logits = logits_of(t, e, dtype)
+    order = logits.float().argsort(-1, descending=True)
+    for j in range(16, min(e, 40)):                # rows 8 to 13: the 17th key on is a cluster
+        step = torch.tensor(float(j % 3)) * (2.0 ** -22 if dtype == torch.float32 else 0.0)
+        rows = torch.arange(8, 14)
+        logits[rows, order[rows, j]] = (logits[rows, order[rows, 16]].float() * (1 - step)).to(dtype)
+    logits[14] = logits[14, 0]                     # all the same
+    logits[15, 20:] = -math.inf
+    logits[16] = -math.inf
+    for top in (17, 24, 31, 32) + ((33,) if e > 32 else ()):
+        check(dev, logits, top, randn(t, top, seed=7), **HOWS[how])
+        check(dev, logits, top, **HOWS[how], bias=randn(e, seed=5) * 0.05)
+        check(dev, logits, top, **HOWS[how], bias=torch.zeros(e))
+        if e % 4 == 0 and e // 2 >= top:
+            check(dev, logits, top, **HOWS[how], bias=torch.zeros(e), groups=4, top_groups=2)
