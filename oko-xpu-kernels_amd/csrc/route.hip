@@ -51,39 +51,6 @@ __device__ __forceinline__ int dpp_any(int x) { return int(dppu<CTRL>(uint32_t(x
 template <int CTRL>
 __device__ __forceinline__ double dpp_any(double x) { return dpp64<CTRL>(x); }
 
-// the values of two lanes D (16 or 32) apart, in both of them, without a trip through LDS
-template <class V>
-struct Both {
-    V lo, hi;
-};
-template <int D>
-__device__ __forceinline__ Both<uint32_t> both_sides(uint32_t x) {
-    if constexpr (D == 16) {
-        const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-        return {p[0], p[1]};
-    } else {
-        const auto p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-        return {p[0], p[1]};
-    }
-}
-template <int D>
-__device__ __forceinline__ Both<int> both_sides(int x) {
-    const auto p = both_sides<D>(uint32_t(x));
-    return {int(p.lo), int(p.hi)};
-}
-template <int D>
-__device__ __forceinline__ Both<float> both_sides(float x) {
-    const auto p = both_sides<D>(__float_as_uint(x));
-    return {__uint_as_float(p.lo), __uint_as_float(p.hi)};
-}
-template <int D>
-__device__ __forceinline__ Both<double> both_sides(double x) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, x);
-    const auto l = both_sides<D>(uint32_t(b)), h = both_sides<D>(uint32_t(b >> 32));
-    return {__builtin_bit_cast(double, uint64_t(h.lo) << 32 | l.lo),
-            __builtin_bit_cast(double, uint64_t(h.hi) << 32 | l.hi)};
-}
-
 template <class V>
 __device__ __forceinline__ V wave_total(V x) {
     x += dpp_any<kDppXor1>(x);

@@ -159,6 +159,39 @@ __device__ __forceinline__ void vector_load(const void* w, int type, int64_t d, 
     }
 }
 
+// the values of two lanes D (16 or 32) apart, in both of them, without a trip through LDS
+template <class V>
+struct Both {
+    V lo, hi;
+};
+template <int D>
+__device__ __forceinline__ Both<uint32_t> both_sides(uint32_t x) {
+    if constexpr (D == 16) {
+        const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return {p[0], p[1]};
+    } else {
+        const auto p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return {p[0], p[1]};
+    }
+}
+template <int D>
+__device__ __forceinline__ Both<float> both_sides(float x) {
+    const auto p = both_sides<D>(__float_as_uint(x));
+    return {__uint_as_float(p.lo), __uint_as_float(p.hi)};
+}
+template <int D>
+__device__ __forceinline__ Both<int> both_sides(int x) {
+    const auto p = both_sides<D>(uint32_t(x));
+    return {int(p.lo), int(p.hi)};
+}
+template <int D>
+__device__ __forceinline__ Both<double> both_sides(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const auto l = both_sides<D>(uint32_t(b)), h = both_sides<D>(uint32_t(b >> 32));
+    return {__builtin_bit_cast(double, uint64_t(h.lo) << 32 | l.lo),
+            __builtin_bit_cast(double, uint64_t(h.hi) << 32 | l.hi)};
+}
+
 // The sum over N (8, 16, 32 or 64) consecutive lanes, in every one of them: DPP inside
 // a row of 16 lanes, whose steps each add two disjoint groups of equal partial sums,
 // then across rows.  The order is fixed.
@@ -168,8 +201,14 @@ __device__ __forceinline__ float lanes_sum(float x) {
     x += dpp<kDppXor2>(x);
     x += dpp<kDppXor7>(x);
     if constexpr (N >= 16) x += dpp<kDppXor15>(x);
-    if constexpr (N >= 32) x += swz_xor<16>(x);
-    if constexpr (N >= 64) x += __shfl_xor(x, 32);
+    if constexpr (N >= 32) {
+        const auto p = both_sides<16>(x);
+        x = p.lo + p.hi;
+    }
+    if constexpr (N >= 64) {
+        const auto p = both_sides<32>(x);
+        x = p.lo + p.hi;
+    }
     return x;
 }
 template <int N>
@@ -178,8 +217,14 @@ __device__ __forceinline__ float lanes_max(float x) {
     x = fmaxf(x, dpp<kDppXor2>(x));
     x = fmaxf(x, dpp<kDppXor7>(x));
     if constexpr (N >= 16) x = fmaxf(x, dpp<kDppXor15>(x));
-    if constexpr (N >= 32) x = fmaxf(x, swz_xor<16>(x));
-    if constexpr (N >= 64) x = fmaxf(x, __shfl_xor(x, 32));
+    if constexpr (N >= 32) {
+        const auto p = both_sides<16>(x);
+        x = fmaxf(p.lo, p.hi);
+    }
+    if constexpr (N >= 64) {
+        const auto p = both_sides<32>(x);
+        x = fmaxf(p.lo, p.hi);
+    }
     return x;
 }
 
