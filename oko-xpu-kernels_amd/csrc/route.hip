@@ -651,9 +651,12 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
     // (-inf orders below kNothing, and so does what is dropped)
     uint32_t c[V > C ? V : C];
     const uint32_t keep = dropped ? 0u : ~kPlace;
-    // (a sum with 0 has no negative zero, which would order below the zero that it equals)
+    if (plain) {                                      // a negative zero would order below zero
+#pragma unroll                                        // (sums of scores are never one)
+        for (int i = 0; i < V; ++i) key[i] += 0.f;
+    }
 #pragma unroll
-    for (int i = 0; i < V; ++i) c[i] = (ordered(key[i] + 0.f) & keep) | (kPlace - uint32_t(in * V + i));
+    for (int i = 0; i < V; ++i) c[i] = (ordered(key[i]) & keep) | (kPlace - uint32_t(in * V + i));
     // the key behind the candidates where it counts: 65536 tokens of 128 experts in fp32, 16
     // slots 31 us (without it all of them went through route_token: 235)
     const bool deep = L >= 16 && a.top >= C - 1 && (T == kF32 || !plain);
