@@ -419,13 +419,24 @@ struct Candidate {
     int e, rank;
     double s, k;
 };
-// Whether a key of a row is above the next lane's by more than tol, or the same at a lower
-// expert (`place` falls along the experts); what is not to be chosen comes last in any order.
+// Whether a candidate of a row surely comes before the next lane's: its key is above, or the
+// same at a lower expert (the place in `packed` falls along the experts); what is not to be
+// chosen comes last in any order.  off: the scores' common relative error (0: none), which moves
+// each key by its own score and so their difference by as much of the greater one, and makes a
+// tie only where it moves both alike.
 template <int ROW>
-__device__ __forceinline__ bool in_order(double key, uint32_t place, int r, double tol) {
-    const double next = dpp64<0x101>(key);            // row_shl: lane r gets r + 1's
-    const uint32_t next_place = dppu<0x101>(place);
-    return r == ROW - 1 || next == kNone || key > next + tol || (key == next && place > next_place);
+__device__ __forceinline__ bool in_order(const Candidate& c, uint32_t places, int r, double off) {
+    const double next = dpp64<0x101>(c.k);            // row_shl: lane r gets r + 1's
+    const uint32_t place = c.packed & places, next_place = dppu<0x101>(place);
+    double tol = 0.0;
+    bool alike = true;
+    if (off != 0.0) {                                 // (the same in all lanes)
+        const double next_s = dpp64<0x101>(c.s);
+        tol = off * fmax(c.s, next_s);
+        alike = c.s == next_s;
+    }
+    return r == ROW - 1 || next == kNone || c.k > next + tol ||
+           (c.k == next && alike && place > next_place);
 }
 __device__ __forceinline__ bool goes_before(double ka, uint32_t pa, double kb, uint32_t pb) {
     return ka > kb || (ka == kb && pa > pb);
@@ -665,7 +676,6 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
     merge_token<L, (V < C ? V : C), C>(c, deep, last);
     if (!deep) last = c[C - 1];
     Candidate mine[Q];
-    double tol = 0.0;
     // the candidates Q ROW + r, in 64 bits
     auto look = [&](int q) {
         Candidate& m = mine[q];
@@ -682,8 +692,6 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
         const float x = logit_at<T>(a.logits, t, a.ld, m.e);
         m.s = plain && a.how.renormalize && !a.how.sigmoid ? exp(double(x) - double(most)) : score64(x);
         m.k = plain ? double(x) : m.s + (a.bias ? double(a.bias[m.e]) : 0.0);
-        // keys nearer than the fp32 sum's error are looked at again with the exact one
-        if (!plain && !a.how.sigmoid && !sum_exact) tol = fmax(tol, 0x1p-16 * m.s);
     };
     // whether a chosen candidate is above all that order behind `next`
     auto sure = [&](const Candidate& m, uint32_t next) {
@@ -699,7 +707,10 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
         look(0);
 #pragma unroll
         for (int q = 1; q < Q; ++q) mine[q] = Candidate{0, -1, C, 0.0, kNone};
-        ordered_now = in_order<ROW>(mine[0].k, mine[0].packed & kPlace, r, tol);
+        // keys nearer than the fp32 sum's error (2^-18 of a score, see above) are looked at again
+        // with the exact one
+        const bool rough = !plain && !a.how.sigmoid && !sum_exact;
+        ordered_now = in_order<ROW>(mine[0], kPlace, r, rough ? 0x1p-16 : 0.0);
         ordered_now &= sure(mine[0], Q > 1 ? c[ROW % C] : last);
     }
     if (__builtin_amdgcn_ballot_w64(!ordered_now)) {
