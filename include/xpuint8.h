@@ -674,7 +674,8 @@ int xpuint8_rms_norm_stream(const void *stream, const void *x, int32_t type, int
 
 /* the same in int8 with a scale a row, for the int8 linears: v = h * weight in fp32, with
  * rotate = 1 (K % 256 == 0) rotated as xpuint8_convrot_quantize_stream rotates;
- * m = max(|v|, 1e-30), q = rint(v * (127 / m)), scale = m / 127 / sqrt(mean(h^2) + eps) */
+ * m = max(|v|, 1e-30), q = rint(v * (127 / m)), scale = m / 127 / sqrt(mean(h^2) + eps), NaN
+ * where h has an infinity or NaN */
 int xpuint8_rms_norm_int8_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
                                  int64_t outer_x, const void *residual, int64_t ldr,
                                  int64_t outer_r, int64_t inner, const void *weight,

@@ -6,8 +6,10 @@
 //   r = 1 / sqrt(mean(h^2) + eps),  y = h r weight
 //   backward, g = dy weight, n = h r:  dx = r (g - n mean(g n)) + dh,  dweight = sum_rows dy n
 //       (r^3 by itself would leave fp32's range long before the formula does)
-//   int8: v = h weight, rotated by 256s or not; m = max(|v|, 1e-30);
+//   int8: v = h weight, rotated by 256s or not; m = max(|v|, 1e-30), NaN if a v is;
 //         q = rint(v (127 / m)), scale = r m / 127
+//       (an infinity or NaN in the row makes a v infinite or NaN, whatever the weight and the
+//       rotation do to it, and r 0 or NaN: the scale is NaN)
 //
 // Sums are fp32.  A row's codes do not depend on r, so the int8 form needs its sum and its
 // maximum at once, in one exchange between the waves.
@@ -78,13 +80,13 @@ __device__ __forceinline__ float inverse_rms(float sum, int64_t K, float eps) {
     return 1.0f / sqrtf(sum / float(K) + eps);
 }
 
-// Two numbers of each lane to their sum and, MAX, their maximum (else both sums) over the
-// TPR threads of a row.  Above a wave through LDS: one slot a wave, read by all.
+// Two numbers of each lane to their sum and, MAX, their maximum (NaN if one is; else both sums)
+// over the TPR threads of a row.  Above a wave through LDS: one slot a wave, read by all.
 template <int TPR, bool MAX>
 __device__ __forceinline__ void row_reduce(float& a, float& b, float2* slots) {
     constexpr int N = TPR < 64 ? TPR : 64;
     a = lanes_sum<N>(a);
-    b = MAX ? lanes_max<N>(b) : lanes_sum<N>(b);
+    b = MAX ? lanes_max_or_nan<N>(b) : lanes_sum<N>(b);
     if constexpr (TPR > 64) {
         const int wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0) slots[wave] = make_float2(a, b);
@@ -94,7 +96,7 @@ __device__ __forceinline__ void row_reduce(float& a, float& b, float2* slots) {
 #pragma unroll
         for (int w = 1; w < TPR / 64; ++w) {
             a += slots[w].x;
-            b = MAX ? fmaxf(b, slots[w].y) : b + slots[w].y;
+            b = MAX ? greater_or_nan(b, slots[w].y) : b + slots[w].y;
         }
         lds_barrier();                 // the slots are read before the next row's are written
     }
@@ -166,13 +168,13 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_kernel(NormArgs a) {
             for (int j = 0; j < 8; ++j) {
                 if (CUT == kOverlap && j < skip) continue;
                 sum = __builtin_fmaf(v[j], v[j], sum);
-                if constexpr (INT8) most = fmaxf(most, fabsf(v[j] * w[i][j]));
+                if constexpr (INT8) most = greater_or_nan(most, fabsf(v[j] * w[i][j]));
             }
         }
-        row_reduce<TPR, true>(sum, most, slots);
+        row_reduce<TPR, INT8>(sum, most, slots);
         const float r = inverse_rms(sum, a.K, a.eps);
         if (!live) continue;
-        const float m = fmaxf(most, 1e-30f), inv = 127.0f / m;
+        const float m = greater_or_nan(most, 1e-30f), inv = 127.0f / m;
         if (INT8 && t == 0) a.scale[row] = r * m / 127.0f;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
@@ -210,12 +212,12 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
             for (int j = 0; j < 8; ++j) {
                 if (CUT == kOverlap && j < skip) continue;
                 sum = __builtin_fmaf(v[j], v[j], sum);
-                if constexpr (INT8) most = fmaxf(most, fabsf(v[j] * w[j]));
+                if constexpr (INT8) most = greater_or_nan(most, fabsf(v[j] * w[j]));
             }
         }
-        row_reduce<1024, true>(sum, most, slots);
+        row_reduce<1024, INT8>(sum, most, slots);
         const float r = inverse_rms(sum, a.K, a.eps);
-        const float m = fmaxf(most, 1e-30f), inv = 127.0f / m;
+        const float m = greater_or_nan(most, 1e-30f), inv = 127.0f / m;
         if (INT8 && threadIdx.x == 0) a.scale[row] = r * m / 127.0f;
         // each thread reads what it has written itself (an overlapping piece too)
         const char* from = a.residual ? row_of<T>(a.h, row, a.K)
@@ -261,6 +263,14 @@ __device__ __forceinline__ void rotated_input(const NormArgs& a, int64_t row, in
             v[8 * i + j] = h[j] * w[j];
         }
     }
+}
+
+// the greatest |v|, NaN if one is
+__device__ __forceinline__ float magnitude(const float (&v)[16]) {
+    float m = fabsf(v[0]);
+#pragma unroll
+    for (int j = 1; j < 16; ++j) m = greater_or_nan(m, fabsf(v[j]));
+    return m;
 }
 
 __device__ __forceinline__ void rotated_store(int8_t* row, int64_t d, float (&v)[16], float k) {
@@ -325,7 +335,7 @@ __global__ __launch_bounds__(1024) void norm_rotated_kernel(NormArgs a, int S, i
         }
         request(row + step);
         const float dom = rotate_groups<1>(v, sgn);
-        const float most = lanes_max<16 * G>(absmax16(v[0], 0.f) * dom);
+        const float most = lanes_max_or_nan<16 * G>(magnitude(v[0]) * dom);
         sum = lanes_sum<16 * G>(sum);
         // (the slots of two rows in turn: one barrier a row)
         if ((threadIdx.x & (16 * G - 1)) == 0) slots[turn][seg / G] = make_float2(sum, most);
@@ -335,7 +345,7 @@ __global__ __launch_bounds__(1024) void norm_rotated_kernel(NormArgs a, int S, i
         for (int i = 0; i < S / G; ++i) {
             const float2 u = slots[turn][r * (S / G) + i];
             total += u.x;
-            m = fmaxf(m, u.y);
+            m = greater_or_nan(m, u.y);
         }
         if (sg == 0 && sl == 0) a.scale[row] = inverse_rms(total, a.K, a.eps) * m / 127.0f;
         rotated_store(static_cast<int8_t*>(a.y) + row * a.K, sg * 256 + lane_w_rot(sl) * 16, v[0],
@@ -358,9 +368,9 @@ __global__ __launch_bounds__(1024) void norm_rotated_long_kernel(NormArgs a) {
             for (int j = 0; j < 16; ++j) v[0][j] = 0.f;
             if (g0 + seg < groups) rotated_input<T>(a, row, (g0 + seg) * 256 + lane_w(sl) * 16, v[0], sum);
             const float dom = rotate_groups<1>(v, sgn);
-            most = fmaxf(most, absmax16(v[0], 0.f) * dom);
+            most = greater_or_nan(most, magnitude(v[0]) * dom);
         }
-        most = lanes_max<16>(most);
+        most = lanes_max_or_nan<16>(most);
         sum = lanes_sum<16>(sum);
         if (sl == 0) slots[seg] = make_float2(sum, most);
         lds_barrier();
@@ -368,7 +378,7 @@ __global__ __launch_bounds__(1024) void norm_rotated_long_kernel(NormArgs a) {
         for (int i = 0; i < kMaxSegs; ++i) {
             const float2 u = slots[i];
             total += u.x;
-            m = fmaxf(m, u.y);
+            m = greater_or_nan(m, u.y);
         }
         lds_barrier();
         if (threadIdx.x == 0) a.scale[row] = inverse_rms(total, a.K, a.eps) * m / 127.0f;

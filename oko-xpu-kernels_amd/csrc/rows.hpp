@@ -228,4 +228,26 @@ __device__ __forceinline__ float lanes_max(float x) {
     return x;
 }
 
+
+// the greater of two numbers, NaN if either is one (fmaxf gives the other one)
+__device__ __forceinline__ float greater_or_nan(float a, float b) {
+    return __builtin_elementwise_maximum(a, b);
+}
+template <int N>
+__device__ __forceinline__ float lanes_max_or_nan(float x) {
+    x = greater_or_nan(x, dpp<kDppXor1>(x));
+    x = greater_or_nan(x, dpp<kDppXor2>(x));
+    x = greater_or_nan(x, dpp<kDppXor7>(x));
+    if constexpr (N >= 16) x = greater_or_nan(x, dpp<kDppXor15>(x));
+    if constexpr (N >= 32) {
+        const auto p = both_sides<16>(x);
+        x = greater_or_nan(p.lo, p.hi);
+    }
+    if constexpr (N >= 64) {
+        const auto p = both_sides<32>(x);
+        x = greater_or_nan(p.lo, p.hi);
+    }
+    return x;
+}
+
 }  // namespace xpuint8
