@@ -99,7 +99,8 @@ __device__ __forceinline__ void wave_best(double& key, int& e) {
 }
 
 constexpr double kNone = -__builtin_huge_val();      // not to be chosen
-constexpr double kLowest = -1.7976931348623157e308;
+// a NaN key: below all others (fp32 biases and scores), and so that the sum of two is above kNone
+constexpr double kLowest = -1e300;
 
 // A token by a whole wave, lane l holding the experts l, l + 64, ..; keys are 64 bits.  A round a
 // slot: 4 tokens, 24 of 256 experts 13.6 us (20 with all exchanges through LDS; 5.9 by 32

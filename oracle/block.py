@@ -48,6 +48,9 @@ def rms_norm_int8(x, weight, eps, residual=None, rotate=True):
 
 
 # ------------------------------------------------------------- the choice of experts
+LOWEST = -1e300       # a NaN key; a group of two has a finite value
+
+
 def route(logits, top, scores="softmax", bias=None, groups=1, top_groups=1, renormalize=True,
           scale=1.0):
     """(ids, weights in 64 bits), a token at a time."""
@@ -59,7 +62,7 @@ def route(logits, top, scores="softmax", bias=None, groups=1, top_groups=1, reno
         spoilt = any(math.isnan(v) or (scores == "softmax" and v == math.inf) for v in row)
         live = [j for j in range(e) if row[j] != -math.inf]
         if spoilt:
-            key = {j: -1e308 if math.isnan(row[j]) else row[j] for j in live}
+            key = {j: LOWEST if math.isnan(row[j]) else row[j] for j in live}
             s = {j: math.nan for j in live}
         elif scores == "softmax":
             most = max((row[j] for j in live), default=0.0)
@@ -71,7 +74,7 @@ def route(logits, top, scores="softmax", bias=None, groups=1, top_groups=1, reno
             b = [0.0] * e if bias is None else bias.double().tolist()
             # without a bias scores rise with their logits
             key = {j: row[j] if bias is None and groups == 1 else s[j] + b[j] for j in live}
-        key = {j: -1e308 if math.isnan(v) else v for j, v in key.items() if v != -math.inf}
+        key = {j: LOWEST if math.isnan(v) else v for j, v in key.items() if v != -math.inf}
         if groups > 1:
             best = [sorted((key[j] for j in range(g * n, (g + 1) * n) if j in key), reverse=True)[:2]
                     for g in range(groups)]
