@@ -228,9 +228,10 @@ __global__ __launch_bounds__(256) void route_exact_kernel(RouteArgs a) {
 // keys in 64 bits.  The choice is sure when these are in order and the last one chosen is
 // above anything that the next candidate (with 16 lanes: the last one, or for 15 and 16 slots
 // the key behind it) could be; if not, all
-// 16 candidates are counted against each other in 64 bits, which 16 keys within 2^-13 to
-// 2^-15 of the last one chosen, a NaN, or scores that underflow leave open still: such a
-// token goes through route_token.  Groups whose fp32 values are too near, and softmax keys
+// 16 candidates are counted against each other in 64 bits, which 16 keys that agree with the last
+// one chosen in all bits that the place leaves (23 of the mantissa less the place's 6 to 10, so
+// within 2^-17 of it for 64 experts and 2^-13 for 1024), a NaN, or scores that underflow leave
+// open still: such a token goes through route_token.  Groups whose fp32 values are too near, and softmax keys
 // nearer than the fp32 sum's error, are looked at again in 64 bits too.
 //
 // Bound by instructions (half of them the sort's and the merges'), so few lanes a token: 8 for
