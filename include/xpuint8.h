@@ -650,7 +650,8 @@ int xpuint8_moe_route_stream(const void *stream, const void *logits, int32_t typ
                              float *weights, int64_t T, int64_t E, int64_t top);
 
 /* dlogits [T, E] (contiguous, the logits' type) of the weights' gradient dweights [T, top];
- * slots without an expert have none, and no two of a token the same */
+ * slots without an expert have none, and no two of a token the same.  A token with NaN weights
+ * has NaNs throughout. */
 int xpuint8_moe_route_grad_stream(const void *stream, const void *logits, int32_t type, int64_t ld,
                                   const int32_t *ids, const float *dweights, int32_t sigmoid,
                                   int32_t renormalize, float scale, void *dlogits, int64_t T,

@@ -763,7 +763,8 @@ __global__ __launch_bounds__(THREADS) void route_kernel(RouteArgs a, Spread sp, 
 //   renormalised:  dl_j = scale w_j (g_j - sum_i g_i w_i) [(1 - s_j) for sigmoid]
 //   softmax:       dl_e = scale s_e ([e chosen] g_e - sum_j g_j s_j)
 //   sigmoid:       dl_j = scale s_j (1 - s_j) g_j
-// zeros elsewhere.  A wave a token, the chosen experts in the first lanes.
+// zeros elsewhere.  A token with NaN weights (a NaN logit, for softmax also one of +inf, chosen or
+// not) has NaNs throughout.  A wave a token, the chosen experts in the first lanes.
 struct RouteGradArgs {
     const void* logits;
     const int* ids;
@@ -773,6 +774,11 @@ struct RouteGradArgs {
     int E, top;
     RouteHow how;
 };
+
+// whether a logit makes its token's weights NaN
+__device__ __forceinline__ bool spoils(float l, bool sigmoid) {
+    return sigmoid ? __builtin_isnan(l) : !(l < INFINITY);
+}
 
 template <int T, int V>
 __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
@@ -784,16 +790,18 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
         const float mine = id >= 0 ? logit_at<T>(a.logits, t, a.ld, id) : -INFINITY;
         const bool dense = !a.how.sigmoid && !a.how.renormalize;
         float d = 0.f, p[V], along = 0.f;             // d: the chosen expert's
+        bool bad = false;
 #pragma unroll
-        for (int i = 0; i < V; ++i) p[i] = 0.f;
+        for (int i = 0; i < V; ++i) {
+            const int e = 64 * i + lane;
+            p[i] = e < a.E ? logit_at<T>(a.logits, t, a.ld, e) : -INFINITY;
+            bad |= spoils(p[i], a.how.sigmoid);
+        }
+        const bool spoilt = __builtin_amdgcn_ballot_w64(bad) != 0;
         if (dense) {
             float most = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int e = 64 * i + lane;
-                p[i] = e < a.E ? logit_at<T>(a.logits, t, a.ld, e) : -INFINITY;
-                most = fmaxf(most, p[i]);
-            }
+            for (int i = 0; i < V; ++i) most = fmaxf(most, p[i]);
             most = wave_most(most);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -840,6 +848,7 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a) {
         for (int i = 0; i < V; ++i) {
             const int e = 64 * i + lane;
             if (e >= a.E) continue;
+            if (spoilt) out[i] = NAN;
             const int64_t at = t * a.E + e;
             if constexpr (T == kF32) static_cast<float*>(a.dlogits)[at] = out[i];
             else static_cast<uint16_t*>(a.dlogits)[at] = uint16_t(pack2<T>(out[i], 0.f));
@@ -893,7 +902,7 @@ __device__ __forceinline__ void four_store(void* row, int e, int E, const float 
 // a token's experts in fours over its L lanes.  The whole row of logits is read, beside the
 // ids, not after them (its chosen few lie in as many lines); they are looked up in LDS, and
 // gradients go through it to where they are written.  HBM-bound: 16381 tokens of 256 experts in
-// fp32 9.9 us (3.4 TB/s; 11.3 to 12.7 with a wave a token and the chosen logits after the ids).
+// fp32 10.1 us (3.3 TB/s; 11.3 to 12.7 with a wave a token and the chosen logits after the ids).
 template <int T, int L, int V>
 __global__ __launch_bounds__(256) void route_grad_rows_kernel(RouteGradArgs a, int64_t first_token) {
     constexpr int PER = 64 / L, F = V / 4;
@@ -908,9 +917,12 @@ __global__ __launch_bounds__(256) void route_grad_rows_kernel(RouteGradArgs a, i
     const float weight = r < a.top ? a.dweights[t * a.top + r] : 0.f;
     const char* from = static_cast<const char*>(a.logits) + t * a.ld * kElem<T>;
     float out[F][4], d;                               // d: the chosen expert's
+    bool bad = false;
 #pragma unroll
     for (int i = 0; i < F; ++i) {
         four_load<T>(from, 4 * (i * L + in), a.E, out[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= spoils(out[i][j], a.how.sigmoid);
         *reinterpret_cast<float4*>(row + 4 * (i * L + in)) =
             make_float4(out[i][0], out[i][1], out[i][2], out[i][3]);
     }
@@ -961,6 +973,11 @@ __global__ __launch_bounds__(256) void route_grad_rows_kernel(RouteGradArgs a, i
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) out[i / 4][i % 4] = 0.f;
+    }
+    if (token_any<L>(bad)) {
+        d = NAN;
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i / 4][i % 4] = NAN;
     }
 #pragma unroll
     for (int i = 0; i < F; ++i)

@@ -122,8 +122,8 @@ def route(logits, top, *, scores="softmax", bias=None, groups=1, top_groups=1, r
 
     An expert whose logit or key is -inf is never chosen (a mask); slots that are left over
     have id -1, which :func:`sort` gives to no expert, and weight 0.  A NaN logit, for the
-    softmax +inf too, makes the token's weights NaN; a NaN in the bias counts as the lowest
-    key.  The gradient of the weights reaches the logits."""
+    softmax +inf too, makes the token's weights NaN, and all of its logits' gradients; a NaN
+    in the bias counts as the lowest key.  The gradient of the weights reaches the logits."""
     if L.HOST is not None:
         r = L.HOST.moe_route(logits, top, scores, bias, groups, top_groups, renormalize, scale)
         if r is not None:

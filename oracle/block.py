@@ -104,7 +104,7 @@ def route(logits, top, scores="softmax", bias=None, groups=1, top_groups=1, reno
 
 def route_grad(logits, ids, dweights, scores="softmax", renormalize=True, scale=1.0):
     """dlogits in 64 bits of the weights' gradient, the choice held fixed: by torch's
-    differentiation of the weights' formula."""
+    differentiation of the weights' formula.  NaNs for a token whose weights are."""
     lg = logits.double().clone().requires_grad_()
     live = ids >= 0
     at = ids.clamp(min=0).long()
@@ -119,6 +119,8 @@ def route_grad(logits, ids, dweights, scores="softmax", renormalize=True, scale=
     if some.any():
         d, = torch.autograd.grad((torch.where(live, w, 0.0) * g)[some].sum(), lg)
         out[some] = d[some]
+    spoilt = logits.isnan() if scores == "sigmoid" else logits.isnan() | (logits == math.inf)
+    out[spoilt.any(-1)] = math.nan
     return out
 
 
