@@ -1359,7 +1359,8 @@ PyObject* host_rotate_axes(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const Tensor* axis = on(plain(PyTuple_GET_ITEM(a[3], 1), at::kInt), *q);
         if (!positions || !inv_freq || !axis || inv_freq->dim() != 1 || axis->dim() != 1 ||
             axis->numel() != inv_freq->numel() || axis->numel() > 512 || 2 * axis->numel() > q->size(3) ||
-            q->size(2) + (k ? k->size(2) : 0) > 65536 || has_tangent(*q, k) || has_tangent(*positions))
+            q->size(2) + (k ? k->size(2) : 0) > 65536 || has_tangent(*q, k) || has_tangent(*positions) ||
+            has_tangent(*inv_freq) || wants_grad(*inv_freq))
             Py_RETURN_NONE;
         const int split = PyObject_IsTrue(a[4]);
         if (split < 0) throw python_error();

@@ -200,7 +200,8 @@ def rotate_axes(q, k, positions, frequencies, *, split_half=True):
     pairs (:func:`axis_frequencies`); a pair whose axis is not in 0..A-1 is not turned.
     Pairs are the elements j and j + P with ``split_half``, else 2j and 2j + 1; those past
     2 P stay as they are.  Strides are free but for a contiguous head dimension (others are
-    copied): a [B, H, S, D] tensor goes in as ``x.transpose(1, 2)``."""
+    copied): a [B, H, S, D] tensor goes in as ``x.transpose(1, 2)``.  Positions and
+    frequencies have no gradient, and ones that need one are refused."""
     if L.HOST is not None and type(frequencies) is AxisFrequencies:
         r = L.HOST.rotate_axes(q, k, positions, frequencies, split_half)
         if r is not None:
@@ -240,10 +241,12 @@ def rotate_axes(q, k, positions, frequencies, *, split_half=True):
             or positions.shape[1:] not in (q.shape[:2], q.shape[1:2])):
         raise ValueError(f"positions must be [A, {q.shape[0]}, {q.shape[1]}] or [A, {q.shape[1]}] "
                          f"with 1..{MAX_AXES} axes, got {tuple(positions.shape)}")
-    if positions.requires_grad and torch.is_grad_enabled():
-        raise ValueError("positions get no gradient")
+    if torch.is_grad_enabled() and (positions.requires_grad or frequencies.inv_freq.requires_grad):
+        raise ValueError("positions and frequencies get no gradient")
+    wanted = _wants_grad(q, k, positions, frequencies.inv_freq)
     positions = positions.detach().resolve_neg()
-    if _wants_grad(q, k):
+    frequencies = AxisFrequencies(*(t.detach() for t in frequencies))
+    if wanted:
         _check_leaves(q, k)
         r = _TurnFn.apply(q, k, positions, *frequencies, bool(split_half))
         return (r, None) if k is None else r
