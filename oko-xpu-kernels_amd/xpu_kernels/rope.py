@@ -245,7 +245,7 @@ def rotate_axes(q, k, positions, frequencies, *, split_half=True):
         raise ValueError("positions and frequencies get no gradient")
     wanted = _wants_grad(q, k, positions, frequencies.inv_freq)
     positions = positions.detach().resolve_neg()
-    frequencies = AxisFrequencies(*(t.detach() for t in frequencies))
+    frequencies = AxisFrequencies(*(t.detach().resolve_neg() for t in frequencies))
     if wanted:
         _check_leaves(q, k)
         r = _TurnFn.apply(q, k, positions, *frequencies, bool(split_half))

@@ -1,5 +1,5 @@
-"""Derivatives that the operators between a block's projections do not have are refused, not
-left out."""
+"""The inputs beside the heads, rows and logits of the operators between a block's projections:
+derivatives that these do not have are refused, not left out, and signs are applied."""
 
 import pytest
 import torch
@@ -30,3 +30,17 @@ def test_frequencies_and_positions(dev, monkeypatch, native, both):
                           (p, rope.AxisFrequencies(fwad.make_dual(f.inv_freq, torch.ones_like(f.inv_freq)), f.axis))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 rope.rotate_axes(q, None, pos, freq)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_lazily_negated_frequencies(dev, monkeypatch, native):
+    """A sign that is a flag of the view is applied."""
+    if not native:
+        monkeypatch.setattr(L, "HOST", None)
+    q, p = randn(1, 3, 2, 16, seed=4).to(dev), torch.arange(3, device=dev)[None]
+    f = rope.axis_frequencies((4, 4), device=dev)
+    for i in range(2):
+        view = [torch._neg_view(t) if i == j else t for j, t in enumerate(f)]
+        made = [-t if i == j else t for j, t in enumerate(f)]
+        assert torch.equal(rope.rotate_axes(q, None, p, rope.AxisFrequencies(*view))[0],
+                           rope.rotate_axes(q, None, p, rope.AxisFrequencies(*made))[0])
