@@ -304,7 +304,10 @@ def _fp32(t):
 
 def _c(t):
     """``t`` contiguous with a 16-byte aligned start (the library reads and
-    writes every buffer with 16-byte vector accesses); copies only if needed."""
+    writes every buffer with 16-byte vector accesses) and the sign applied that
+    may be a flag of the view; copies only if needed."""
+    if t.is_neg():
+        t = t.resolve_neg()
     if not t.is_contiguous():
         t = t.contiguous()
     if t.data_ptr() % 16:

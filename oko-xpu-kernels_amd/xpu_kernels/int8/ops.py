@@ -62,11 +62,11 @@ def _opt(t):
 def _pack_key(w8):
     """The registry key of a weight that can carry a packed copy, else None:
     a CUDA int8 [N, K] tensor (N, K multiples of 16) that starts its storage,
-    is contiguous and 16-byte aligned, and has a version counter (not an
-    inference tensor)."""
+    is contiguous and 16-byte aligned, not lazily negated, and has a version
+    counter (not an inference tensor)."""
     if not isinstance(w8, torch.Tensor) or w8.dtype != torch.int8 or w8.dim() != 2:
         return None
-    if not w8.is_cuda or w8.is_inference() or w8.storage_offset() != 0:
+    if not w8.is_cuda or w8.is_inference() or w8.storage_offset() != 0 or w8.is_neg():
         return None
     n, k = w8.shape
     if n == 0 or n % 16 or k == 0 or k % 16 or not w8.is_contiguous() or w8.data_ptr() % 16:
@@ -570,7 +570,7 @@ def expand_scale(scale, n, device=None):
         return torch.full((n,), float(scale), device=device, dtype=torch.float32)
     if (scale.dtype == torch.float32 and scale.dim() == 1 and scale.numel() == n
             and scale.is_contiguous() and (device is None or scale.device == device)
-            and scale.data_ptr() % 16 == 0):
+            and scale.data_ptr() % 16 == 0 and not scale.is_neg()):
         return scale
     s = scale.reshape(-1).to(device=device or scale.device, dtype=torch.float32)
     if s.numel() == 1 and n != 1:
@@ -587,7 +587,7 @@ def _bias_arg(bias, n, device):
         return None, 0
     if (isinstance(bias, torch.Tensor) and bias.dtype == torch.bfloat16 and bias.dim() == 1
             and bias.numel() == n and bias.is_contiguous() and bias.device == device
-            and bias.data_ptr() % 16 == 0):
+            and bias.data_ptr() % 16 == 0 and not bias.is_neg()):
         return bias, 1
     return expand_scale(bias, n, device), 0
 
@@ -656,7 +656,7 @@ def int_mm(a, b):
     if b.shape[0] != k:
         raise ValueError(f"K mismatch: a has {k} columns, b has {b.shape[0]} rows")
     n = b.shape[1]
-    a = _c(a)
+    a, b = _c(a), b.resolve_neg()
     c = torch.empty((m, n), device=a.device, dtype=torch.int32)
     st = _stream(a.device)
     if b.t().is_contiguous() and b.data_ptr() % 16 == 0:
@@ -693,6 +693,7 @@ def dequant_slice(acc, x_scale, w_scale, bias=None):
     lib = _lib()
     if acc.dim() != 2 or acc.dtype != torch.int32:
         raise TypeError("acc must be an int32 [M, N] tensor")
+    acc = acc.resolve_neg()
     if acc.stride(1) != 1 or acc.stride(0) % 4 or acc.data_ptr() % 16:
         acc = acc.contiguous() if acc.stride(1) != 1 else acc
         if acc.stride(0) % 4 or acc.data_ptr() % 16:
@@ -835,8 +836,7 @@ def linear(x, w8, w_scale, bias=None, act: Optional[str] = None, residual=None,
     x2 = x.reshape(m, -1)
     if x2.dtype != torch.bfloat16:
         x2 = x2.to(dtype=torch.bfloat16)
-    if not x2.is_contiguous():
-        x2 = x2.contiguous()
+    x2 = x2.resolve_neg().contiguous()
 
     lib = _lib()
     w8c = _c(w8)
@@ -1055,8 +1055,7 @@ def ffn(x, up_w8, up_scale, down_w8, down_scale, down_bias=None, act="situ"):
     x2 = x.reshape(m, k)
     if x2.dtype != torch.bfloat16:
         x2 = x2.to(dtype=torch.bfloat16)
-    if not x2.is_contiguous():
-        x2 = x2.contiguous()
+    x2 = x2.resolve_neg().contiguous()
 
     lib = _lib()
     uw8 = _c(up_w8)
