@@ -22,6 +22,7 @@ import weakref
 from typing import Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .._capture import is_capturing
 from . import _lib as _L
@@ -942,8 +943,10 @@ def linear_quantized(q, scale, w8, w_scale, bias=None):
     for t, name in ((scale, "scale"), (w8, "w8"), (w_scale, "w_scale"), (bias, "bias")):
         if isinstance(t, torch.Tensor) and t.device != q.device:
             raise TypeError(f"{name} is on {t.device} but q is on {q.device}")
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                       for t in (scale, w_scale, bias)):
+    floats = [t for t in (scale, w_scale, bias) if isinstance(t, torch.Tensor)]
+    if any(unpack_dual(t).tangent is not None for t in floats):
+        raise NotImplementedError("linear_quantized has no forward-mode derivative")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in floats):
         raise RuntimeError("linear_quantized has no gradient; call it under torch.no_grad(), or "
                            "int8_linear for one")
     out = torch.empty((*q.shape[:-1], n), device=q.device, dtype=torch.bfloat16)

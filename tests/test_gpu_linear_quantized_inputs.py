@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from mx_util import randn
 from xpu_kernels import int8
@@ -45,3 +46,12 @@ def test_lazily_negated_beside_it(dev, which, packed):
         for a, b in zip(int8.prepare_weight(negated[0][:, None].expand(5, 16, 256).reshape(80, 256)),
                         int8.prepare_weight(args[0][:, None].expand(5, 16, 256).reshape(80, 256))):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", [1, 3, 4])
+def test_tangents(dev, which):
+    args = inputs(dev)
+    with fwad.dual_level():
+        args[which] = fwad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            int8.linear_quantized(*args)
