@@ -22,6 +22,7 @@
 #include <torch/csrc/Storage.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -32,6 +33,8 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <unordered_map>
+#include <unordered_set>
 #include <vector>
 
 #include "xpuint8.h"
@@ -90,6 +93,7 @@ static_assert(sizeof(Library) == kEntries * sizeof(void*), "one address per entr
 
 Library g_lib;
 PyObject* g_raw_stream = nullptr;   // device index -> current stream's handle
+PyObject* g_capturing = nullptr;    // () -> whether the current stream is being captured
 PyObject* g_packed = nullptr;       // the packed-weight registry (ops._PACKED)
 
 // ----------------------------------------------------------- arguments
@@ -642,17 +646,22 @@ Tensor run_combine(const Tensor& z, const Tensor* w, const Tensor& position,
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-const void* stream_of(const Tensor& t) {
+// f() with the GIL, a Python error carried to where the engine reports it
+template <class F>
+auto with_gil(const F& f) {
     struct Gil {
         PyGILState_STATE s = PyGILState_Ensure();
         ~Gil() { PyGILState_Release(s); }
     } gil;
     try {
-        return current_stream(t);
+        return f();
     } catch (python_error& e) {
         e.persist();
         throw;
     }
+}
+const void* stream_of(const Tensor& t) {
+    return with_gil([&] { return current_stream(t); });
 }
 void check(int rc, const char* what) {
     if (rc != 0) throw std::runtime_error(std::string(what) + ": " + g_lib.last_error());
@@ -668,10 +677,65 @@ Rows rows_of(const Tensor& x) {
     if (t.stride(1) != 1 || (many && t.stride(0) < t.size(1))) t = t.contiguous();
     return {t, t.size(0) > 1 ? t.stride(0) : t.size(1)};
 }
+bool on_default_stream(const Tensor& t) {
+    return c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device()).id() == 0;
+}
+// whether the current stream is being captured (with the GIL)
+bool capturing() {
+    if (!g_capturing) return false;
+    PyObject* r = PyObject_CallNoArgs(g_capturing);
+    if (!r) throw python_error();
+    const bool yes = r == Py_True;
+    Py_DECREF(r);
+    return yes;
+}
+void refuse_if_capturing() {
+    PyObject* module = PyImport_ImportModule("xpu_kernels._capture");
+    PyObject* r = module ? PyObject_CallMethod(module, "refuse_default_stream_leaf", nullptr) : nullptr;
+    Py_XDECREF(module);
+    if (!r) throw python_error();
+    Py_DECREF(r);
+}
+
+// The gradient of a leaf ends in a node that lives as long as any graph of the leaf and
+// belongs to the stream that was current when it was made.  A backward pass that is captured
+// makes that stream wait for the capturing one; the default stream cannot, and that ends the
+// process.  So a node here, before it gives its gradients to the engine in a capture, looks at
+// all nodes that the pass takes them to, and refuses to go on if one is of the default stream.
+void check_backward(const variable_list& in) {
+    const Tensor* some = nullptr;
+    for (const Tensor& g : in)
+        if (g.defined()) some = &g;
+    if (!some || !some->is_cuda() || on_default_stream(*some)) return;
+    if (!with_gil([] { return capturing(); })) return;
+    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
+    if (!node) return;
+    // (empty: the pass goes to all of them)
+    const auto* pass = torch::autograd::get_current_graph_task_exec_info();
+    std::vector<torch::autograd::Node*> left{node.get()};
+    std::unordered_set<torch::autograd::Node*> seen{node.get()};
+    while (!left.empty()) {
+        torch::autograd::Node* from = left.back();
+        left.pop_back();
+        for (const auto& edge : from->next_edges()) {
+            torch::autograd::Node* to = edge.function.get();
+            if (!to || !seen.insert(to).second) continue;
+            if (pass && !pass->empty()) {
+                const auto it = pass->find(to);
+                if (it == pass->end() || !it->second.should_execute()) continue;
+            }
+            const auto made = to->stream();
+            if (made && made->id() == 0) return with_gil([] { refuse_if_capturing(); });
+            left.push_back(to);
+        }
+    }
+}
+
 // the gradients that f() gives, which have no derivative themselves: an error where one is
 // asked for
 template <class F>
 variable_list once(const variable_list& in, const F& f) {
+    check_backward(in);
     variable_list grads;
     {
         at::NoGradGuard no_grad;
@@ -993,27 +1057,18 @@ const Tensor* lines_arg(PyObject* o, Lines& l) {
     return &t;
 }
 
-// The gradient of a leaf ends in a node that lives as long as any graph of the leaf and
-// belongs to the stream that was current when it was made.  A backward pass that is captured
-// makes that stream wait for the capturing one; the default stream cannot, and that ends the
-// process: a captured call that would lead there, at once or through views and other nodes of
-// one input, is refused (_capture.py knows the captures).
+// A forward call of a capture whose gradient would lead to a graph of the default stream (see
+// check_backward), at once or through up to 16 views and other nodes of one input, is refused:
+// most captured steps are stopped before their backward pass.  (Also where no backward pass
+// follows: without gradient mode nothing is refused.)
 void check_leaf(const Tensor* t) {
     if (!t || !t->requires_grad()) return;
-    if (c10::impl::VirtualGuardImpl(t->device().type()).getStream(t->device()).id() == 0) return;
+    if (on_default_stream(*t)) return;
     std::shared_ptr<torch::autograd::Node> node = t->grad_fn();
     if (!node) node = torch::autograd::impl::try_get_grad_accumulator(*t);
     for (int far = 0; node && far < 16; ++far) {
         const auto made = node->stream();
-        if (made && made->id() == 0) {
-            PyObject* module = PyImport_ImportModule("xpu_kernels._capture");
-            PyObject* r =
-                module ? PyObject_CallMethod(module, "refuse_default_stream_leaf", nullptr) : nullptr;
-            Py_XDECREF(module);
-            if (!r) throw python_error();
-            Py_DECREF(r);
-            return;
-        }
+        if (made && made->id() == 0) return refuse_if_capturing();
         std::shared_ptr<torch::autograd::Node> next;
         int inputs = 0;
         for (const auto& edge : node->next_edges())
@@ -1382,7 +1437,18 @@ PyObject* host_rotate_axes(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
-// check_leaves(tensors or Nones ..): the same for calls that go through Python
+// check_backward(gradients or Nones ..): for nodes of Python
+PyObject* host_check_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded(n_args, n_args, [&]() -> PyObject* {
+        variable_list in;
+        for (Py_ssize_t i = 0; i < n_args; ++i)
+            if (THPVariable_Check(a[i])) in.push_back(THPVariable_Unpack(a[i]));
+        check_backward(in);
+        Py_RETURN_NONE;
+    });
+}
+
+// check_leaves(tensors or Nones ..): check_leaf for calls that go through Python
 PyObject* host_check_leaves(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded(n_args, n_args, [&]() -> PyObject* {
         for (Py_ssize_t i = 0; i < n_args; ++i)
@@ -1410,6 +1476,11 @@ PyObject* host_bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     std::memcpy(static_cast<void*>(&g_lib), p.data(), sizeof(g_lib));
     Py_XSETREF(g_raw_stream, Py_NewRef(a[1]));
     Py_XSETREF(g_packed, Py_NewRef(a[2]));
+    PyObject* torch_c = PyImport_ImportModule("torch._C");
+    PyObject* asks = torch_c ? PyObject_GetAttrString(torch_c, "_cuda_isCurrentStreamCapturing") : nullptr;
+    Py_XDECREF(torch_c);
+    if (!asks) PyErr_Clear();                        // (torch without a device: nothing is captured)
+    Py_XSETREF(g_capturing, asks);
     Py_RETURN_NONE;
 }
 
@@ -1436,6 +1507,7 @@ PyMethodDef kMethods[] = {XPU_HOST("bind", host_bind),
                           XPU_HOST("moe_route", host_moe_route),
                           XPU_HOST("rotate_axes", host_rotate_axes),
                           XPU_HOST("check_leaves", host_check_leaves),
+                          XPU_HOST("check_backward", host_check_backward),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host",
                        "The int8 API's hot calls in native code (see host_ops.cpp).", -1, kMethods};

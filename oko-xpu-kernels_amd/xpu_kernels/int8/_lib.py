@@ -284,6 +284,13 @@ def _stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def check_backward(*grads):
+    """Refuse, in a capture, a backward pass that goes on to a graph of the default stream
+    (called by a node with the gradients that it gets)."""
+    if HOST is not None:
+        HOST.check_backward(*grads)
+
+
 _STAY = contextlib.nullcontext()
 
 

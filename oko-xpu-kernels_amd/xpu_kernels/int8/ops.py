@@ -464,6 +464,7 @@ class _Int8LinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        _L.check_backward(dy)
         w8, w_scale = ctx.saved_tensors
         if ctx.mode in ("int8", "dense") and _backward_one_call(dy, w8) and \
                 w_scale.numel() in (1, w8.shape[0]):
@@ -1135,6 +1136,7 @@ class _TrainableInt8LinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        _L.check_backward(dy)
         x, weight, w8, ws = ctx.saved_tensors
         dy = dy.reshape(-1, dy.shape[-1])
         x2 = x.reshape(-1, x.shape[-1])

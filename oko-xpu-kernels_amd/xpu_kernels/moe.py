@@ -102,6 +102,7 @@ class _RouteFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, _, dweights):
+        L.check_backward(dweights)
         logits, ids = ctx.saved_tensors
         if dweights is None:
             return None, None, None, None
@@ -239,6 +240,7 @@ class _DispatchFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dxs):
+        L.check_backward(dxs)
         return _combine(dxs, Routing(*ctx.saved_tensors), None, dxs.dtype), None
 
 
@@ -251,6 +253,7 @@ class _CombineFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        L.check_backward(dy)
         z, weights, *routing = ctx.saved_tensors
         routing = Routing(*routing)
         t, top = routing.position.shape

@@ -239,6 +239,7 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        L.check_backward(dy)
         codes, scales = ctx.saved_tensors
         dx = dbias = None
         if ctx.needs_input_grad[0]:
@@ -302,6 +303,7 @@ class _GroupedFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         from . import moe
+        L.check_backward(dy)
         codes, scales, *routing = ctx.saved_tensors
         routing = moe.Routing(*routing)
         if not ctx.gather:

@@ -150,6 +150,7 @@ class _NormFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh=None):
+        L.check_backward(dy, dh)
         h, weight = ctx.saved_tensors
         want = ctx.needs_input_grad[1]
         if dy is None:                       # only h went on

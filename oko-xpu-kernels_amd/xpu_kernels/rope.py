@@ -177,6 +177,7 @@ class _TurnFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk=None):
+        L.check_backward(dq, dk)
         positions, *frequencies = ctx.saved_tensors
         frequencies = AxisFrequencies(*frequencies)
         dq = dq if ctx.needs_input_grad[0] else None
