@@ -698,8 +698,8 @@ int xpuint8_rms_norm_grad_stream(const void *stream, const void *dy, int32_t typ
  * q [B, S, q_heads, D] and k [B, S, k_heads, D] (NULL: q alone) to q_out and k_out: pair j <
  * pairs of each head turned by positions[axis[j], b, s] * inv_freq[j] radians (inverse = 1:
  * by the opposite angle, the gradient); pairs are elements j and j + pairs (split_half = 1)
- * or 2j and 2j + 1; elements past 2 * pairs are copied.  Angles are reduced in fp64, products
- * are fp32.  q_strides = {b, s, head} of q, then of q_out, in elements, the last dimensions
+ * or 2j and 2j + 1; elements past 2 * pairs are copied.  Angles are reduced in fp64 (to 2^-51 of
+ * themselves), products are fp32.  q_strides = {b, s, head} of q, then of q_out, in elements, the last dimensions
  * contiguous; position_strides = {axis, b, s}; positions int32, int64 or fp32 (position_type
  * 0, 1, 2); an axis outside [0, axes) does not turn.  Buffers have the alignment of their
  * elements; q_out and k_out overlap no input.  pairs <= 512, D <= 4096.  Strides are read on the host.  No counterpart in the

@@ -901,8 +901,10 @@ __device__ __forceinline__ void four_store(void* row, int e, int E, const float 
 // The same with several tokens a wave, up to 16 slots each: slots in the 16 lanes of a row,
 // a token's experts in fours over its L lanes.  The whole row of logits is read, beside the
 // ids, not after them (its chosen few lie in as many lines); they are looked up in LDS, and
-// gradients go through it to where they are written.  HBM-bound: 16381 tokens of 256 experts in
-// fp32 10.1 us (3.3 TB/s; 11.3 to 12.7 with a wave a token and the chosen logits after the ids).
+// gradients go through it to where they are written.  16381 tokens of 256 experts in fp32 10.1 us
+// (11.3 to 12.7 with a wave a token and the chosen logits after the ids); the bytes take 6.6 at a
+// copy's rate, and the waves wait for 64% of their cycles: loads, LDS, exponentials and stores follow
+// one another.  65536 tokens 29 (4.6 TB/s).
 template <int T, int L, int V>
 __global__ __launch_bounds__(256) void route_grad_rows_kernel(RouteGradArgs a, int64_t first_token) {
     constexpr int PER = 64 / L, F = V / 4;

@@ -918,7 +918,14 @@ def linear_quantized(q, scale, w8, w_scale, bias=None):
     ``norm.rms_norm_int8`` (or, against a weight that is not rotated, row by row without
     the rotation): int8 q [.., K] and its scales [..] -> bf16 [.., N],
     ``float(q @ w8.T) * (w_scale * scale) + bias``.  K and N multiples of 16.  No
-    counterpart in the reference, whose linear quantizes its input itself."""
+    counterpart in the reference, whose linear quantizes its input itself.
+
+    It reads ``w8`` itself, not the packed copy, and does not split K, as :func:`linear`
+    does: ``norm.rms_norm_int8`` and this are the faster pair where rows and columns are
+    many (4096 x 5120 -> 5120 106 us, ``norm.rms_norm`` and :func:`linear` 114; 16381 rows
+    435 and 465), the slower one where either is few (1024 x 5120 -> 1280 57 and 31, 128 x
+    4096 -> 4096 42 and 14, 16 rows 18 and 14), and about even between (4096 x 1280 ->
+    10240 66 and 65)."""
     if not isinstance(q, torch.Tensor) or q.dtype != torch.int8 or q.dim() < 1:
         raise TypeError(f"q must be an int8 [.., K] tensor, got "
                         f"{getattr(q, 'dtype', type(q).__name__)}")

@@ -4,7 +4,8 @@ output for the int8 linears.
     y = norm.rms_norm(x, weight)                          # [.., K] in x's type
     y, h = norm.rms_norm(x, weight, residual=r)           # h = x + r, y the norm of h
     q, scale, h = norm.rms_norm_int8(x, weight, residual=r)
-    out = int8.linear_quantized(q, scale, w8, w_scale)    # of prepare_weight's w8
+    out = int8.linear_quantized(q, scale, w8, w_scale)    # of prepare_weight's w8 (many rows:
+                                                          # see there)
 
 ``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, in fp32 from the
 values of ``h`` in its type (bf16, fp16 or fp32) to the one rounding of ``y``; a sum of

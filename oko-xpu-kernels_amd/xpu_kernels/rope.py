@@ -196,8 +196,9 @@ def rotate_axes(q, k, positions, frequencies, *, split_half=True):
     b cos + a sin).  Returns (q, k) in their type (bf16, fp16 or fp32) and layout (a layout
     with gaps: contiguous), with gradients to both.
 
-    ``positions`` [A, B, S], or [A, S] for all of the batch: int32, int64 or fp32, of any
-    size (angles are reduced in fp64).  ``frequencies`` is an :class:`AxisFrequencies` of P
+    ``positions`` [A, B, S], or [A, S] for all of the batch: int32, int64 or fp32.  Angles
+    are reduced in fp64, to 2^-51 of themselves: closer than fp32 tells apart up to 10^8
+    radians, less beyond.  ``frequencies`` is an :class:`AxisFrequencies` of P
     pairs (:func:`axis_frequencies`); a pair whose axis is not in 0..A-1 is not turned.
     Pairs are the elements j and j + P with ``split_half``, else 2j and 2j + 1; those past
     2 P stay as they are.  Strides are free but for a contiguous head dimension (others are
