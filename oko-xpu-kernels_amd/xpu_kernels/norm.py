@@ -190,7 +190,8 @@ def rms_norm_int8(x, weight=None, eps=1e-6, residual=None, rotate=True):
     ``v = h * weight`` (rotated) in fp32, ``m = max(|v|, 1e-30)``,
     ``q = rint(v * (127 / m))`` and ``scale = m / 127 / sqrt(mean(h^2) + eps)``: the norm
     is not rounded between, and a row with an infinity or NaN has a NaN scale (as every row
-    has with a NaN in the weight; finite rows whose squares overflow have a scale of 0).
+    has with a NaN in the weight; finite rows whose squares overflow have a scale of 0, or
+    NaN where ``v`` overflows too).
     Whole numbers have no gradient: inputs that need one are refused outside of
     ``torch.no_grad()``."""
     if L.HOST is not None:
